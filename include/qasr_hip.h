@@ -177,6 +177,86 @@ int qasr_hip_bidirectional_attention(qasr_hip *h, float *out, const float *q, co
                                      const float *v, int64_t seq, int64_t n_heads, int64_t head_dim,
                                      float scale, int64_t window_tokens);
 
+/* ---- an 8-bit decoder layer over many rows and many sequences ------------
+ * No counterpart in the reference (whose int8 path takes one row at a time and
+ * whose KV cache is f32): int8 activation rows, the int8 x int8 product, a KV
+ * cache in int8 and the attention over it.  Calls take device pointers, are
+ * ordered on the handle's stream, allocate nothing and may be captured into a
+ * graph from that stream.
+ *
+ * int8 rounding, here: to the nearest value, halves away from zero, decided
+ * exactly (qasr_hip_quantize_act forms a product in f32 first and can differ by
+ * one next to a half). */
+/* s = x + res; n = s / sqrt(mean(s^2) + eps) * norm_w; q = n rounded to int8
+ * with one scale a row, max|n| / 127 (1 for a row of zeros).  x, res and sum hold
+ * rows of hidden values, ld elements apart, f32 or (bf16 != 0) bf16; q is
+ * [rows][hidden], scales [rows].  res null: s = x.  norm_w null: n = s, the rows
+ * are quantized as they are (eps unused).  sum (nullable) receives s; it may be x
+ * or res itself.  Sums and rounding decisions are formed in f64 from the sum
+ * before it is rounded to its type.  A row that holds a value that is not finite
+ * gets q = 0 and a NaN scale.  hidden <= 16384. */
+int qasr_hip_add_rms_norm_int8(qasr_hip *h, int8_t *q, float *scales, void *sum, const void *x, const void *res,
+                               const float *norm_w, int64_t rows, int64_t hidden, int64_t ld, float eps, int bf16);
+/* y[m, n] = (sum_k a[m, k] w[n, k]) * a_scales[m] * w_scales[n] (+ bias[n],
+ * nullable): int8 rows a [M][K] and w [N][K], exact int32 sums, y f32 or
+ * (y_bf16 != 0) bf16, K < 131072.  A product is ((float)sum * a_scale) *
+ * w_scale in f32, as in the int8 matvecs above.  mode:
+ *   QASR_GEMM_PLAIN   y [M][N]
+ *   QASR_GEMM_ADDTO   y = (y + bias) + product
+ *   QASR_GEMM_SWIGLU  w holds interleaved gate / up rows, N even: y [M][N / 2] =
+ *                     silu(gate) * up */
+#define QASR_GEMM_PLAIN 0
+#define QASR_GEMM_ADDTO 1
+#define QASR_GEMM_SWIGLU 2
+int qasr_hip_gemm_w8a8(qasr_hip *h, void *y, const int8_t *a, const float *a_scales, const int8_t *w,
+                       const float *w_scales, const float *bias, int64_t M, int64_t N, int64_t K, int mode, int y_bf16);
+/* The int8 KV cache of n_seq sequences: capacity positions each (a multiple of
+ * QASR_KV8_BLOCK), n_kv_heads heads of head_dim 64 or 128, one scale for the
+ * QASR_KV8_BLOCK positions of a block and head; a value is int8 * scale.
+ *   k8 [n_seq][n_kv_heads][capacity][head_dim]
+ *   v8 [n_seq][n_kv_heads][capacity / 64][head_dim][64]: of a dim's 64 bytes byte
+ *      16 g + 4 t + r is position 16 t + 4 g + r of the block (g, t, r in 0..3)
+ *   k_scales, v_scales f32 [n_seq][n_kv_heads][capacity / 64]
+ * k8 and v8 16-byte aligned.  Rows of all sequences follow one another: sequence
+ * j's are row_start[j] .. row_start[j + 1] (device int32 [n_seq + 1]; null: max_rows
+ * each), at most max_rows of them (those past max_rows are left out); its row i is
+ * at position pos[j] + i (device int32 [n_seq]).  Positions outside [0, capacity)
+ * do not exist: a negative pos switches a sequence's first rows off.
+ * row_start is held to [0, n_rows], so no value in it or in pos leads outside the
+ * buffers. */
+#define QASR_KV8_BLOCK 64
+/* Rows k, v (f32 or bf16, head h of a row at h * head_dim, rows ld elements
+ * apart) into the cache.  The rows written end their sequence: positions behind
+ * them lose their meaning.  A block's scale is max|value| / 127 over its finite
+ * values; where a block holds earlier positions of the sequence, their scale is
+ * kept, or raised to the new values' and the earlier positions rounded again at
+ * the new scale (at most half a new step each time it rises).  NaN is stored as
+ * 0, infinities as +-127. */
+int qasr_hip_kv8_write(qasr_hip *h, int8_t *k8, int8_t *v8, float *k_scales, float *v_scales, const void *k,
+                       const void *v, int64_t ld, const int32_t *row_start, const int32_t *pos, int64_t n_rows,
+                       int64_t n_seq, int64_t max_rows, int64_t n_kv_heads, int64_t head_dim, int64_t capacity,
+                       int bf16);
+/* The way back: the cache's values at those positions into rows k, v (layout as
+ * for the write).  Rows whose position does not exist, and rows behind the last
+ * sequence, are left as they were. */
+int qasr_hip_kv8_read(qasr_hip *h, void *k, void *v, int64_t ld, const int8_t *k8, const int8_t *v8,
+                      const float *k_scales, const float *v_scales, const int32_t *row_start, const int32_t *pos,
+                      int64_t n_rows, int64_t n_seq, int64_t max_rows, int64_t n_kv_heads, int64_t head_dim,
+                      int64_t capacity, int bf16);
+/* Attention of rows q (f32 or bf16, rows ldq elements apart, n_heads heads, a
+ * multiple of n_kv_heads; query head h reads KV head h / (n_heads / n_kv_heads))
+ * over the cache: out [n_rows][n_heads * head_dim] of q's type = softmax(scale *
+ * q . k) v.  Row i of sequence j sees the positions up to pos[j] + i; with window
+ * > 0 only the last window of those and the first sinks.  A row that sees nothing
+ * gives zeros; rows behind the last sequence are left as they were.  max_len (0:
+ * capacity): about the longest pos + rows, by which the work is split; results do
+ * not depend on it beyond f32 rounding.  Uses the handle's scratch area. */
+int qasr_hip_attention_kv8(qasr_hip *h, void *out, const void *q, int64_t ldq, const int8_t *k8, const int8_t *v8,
+                           const float *k_scales, const float *v_scales, const int32_t *row_start, const int32_t *pos,
+                           int64_t n_rows, int64_t n_seq, int64_t max_rows, int64_t max_len, int64_t n_heads,
+                           int64_t n_kv_heads, int64_t head_dim, int64_t capacity, float scale, int64_t window,
+                           int64_t sinks, int bf16);
+
 /* ---- checkpoints: safetensors (safetensors.rs) ---------------------------
  * A read-only mapping of one checkpoint file or of a directory's shards.
  * Tensor data stays in the mapping (no host copy); the *_load_st loaders

@@ -17,6 +17,10 @@ QASR_ERR_HIP = -2
 QASR_ERR_NOMEM = -3
 QASR_ROUND_HALF_AWAY = 0
 QASR_TRUNC = 1
+QASR_GEMM_PLAIN = 0
+QASR_GEMM_ADDTO = 1
+QASR_GEMM_SWIGLU = 2
+QASR_KV8_BLOCK = 64
 
 P = C.c_void_p
 I64 = C.c_int64
@@ -142,6 +146,12 @@ _SIGS = {
     "qasr_hip_gemm_w8_bf16": (C.c_int, [P, P, P, P, P, I64, I64, I64]),
     "qasr_hip_layer_norm": (C.c_int, [P, P, P, P, P, I64, I64, F32]),
     "qasr_hip_bidirectional_attention": (C.c_int, [P, P, P, P, P, I64, I64, I64, F32, I64]),
+    "qasr_hip_add_rms_norm_int8": (C.c_int, [P, P, P, P, P, P, P, I64, I64, I64, F32, C.c_int]),
+    "qasr_hip_gemm_w8a8": (C.c_int, [P, P, P, P, P, P, P, I64, I64, I64, C.c_int, C.c_int]),
+    "qasr_hip_kv8_write": (C.c_int, [P, P, P, P, P, P, P, I64, P, P, I64, I64, I64, I64, I64, I64, C.c_int]),
+    "qasr_hip_kv8_read": (C.c_int, [P, P, P, I64, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, C.c_int]),
+    "qasr_hip_attention_kv8": (C.c_int, [P, P, P, I64, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, F32,
+                                         I64, I64, C.c_int]),
     "qasr_hip_encoder_load": (C.c_int, [P, C.POINTER(EncConfig), C.POINTER(EncWeights), C.POINTER(P)]),
     "qasr_hip_encoder_load_st": (C.c_int, [P, P, C.POINTER(EncConfig), C.POINTER(P)]),
     "qasr_hip_encoder_free": (None, [P]),

@@ -340,3 +340,69 @@ hipError_t launch_head_norm_rope_strided(float *x, int64_t row_stride, const flo
                                          const float *sin_t, int64_t seq, int heads, float eps, int do_norm,
                                          int do_rope, hipStream_t st);
 }  // namespace qasr
+
+namespace qasr {
+// ---- an 8-bit layer over many rows (k_rows8.hip, k_gemm8.hip, k_kv8.hip) ------
+// |x| / s to the nearest whole number, halves up, at most 127: exact for f32
+// values in f64 (254 |x| and (2 k + 1) s have at most 32 bits); inv about 1 / s
+__device__ __forceinline__ int round_ratio(double ax, double s, double inv) {
+    const int k = (int)fmin(floor(ax * inv), 127.0);
+    return min(127, k + (2.0 * ax >= (double)(2 * k + 1) * s ? 1 : 0));
+}
+
+#define QASR_ROWS8_MAX_HIDDEN 16384
+struct Rows8Args {
+    const void *x, *res;      // [rows][ld] f32 or bf16; res nullable
+    void *sum;                // [rows][ld], nullable; may be x or res
+    const float *norm_w;      // [H], nullable: no norm
+    int8_t *q;                // [rows][H]
+    float *scales;            // [rows]
+    int64_t rows, ld;
+    int H;
+    float eps;
+};
+hipError_t launch_add_rms_norm_int8(const Rows8Args &a, bool bf16, hipStream_t st);
+
+struct Gemm8Args {
+    const int8_t *a;          // [M][K]
+    const float *as;          // [M]
+    const int8_t *w;          // [N][K]
+    const float *ws;          // [N]
+    const float *bias;        // [N] or null
+    void *y;                  // [M][N] f32 or bf16 (SWIGLU: [M][N / 2])
+    int64_t M, N, K;
+};
+enum { G8_PLAIN = 0, G8_ADDTO = 1, G8_SWIGLU = 2 };
+hipError_t launch_gemm_w8a8(const Gemm8Args &g, int mode, bool y_bf16, hipStream_t st);
+
+#define QASR_KV8_TILE 64      // positions of a block: one scale, and the K of one int8 MFMA
+struct Kv8Args {
+    int8_t *k8;               // [n_seq][Hkv][cap][hd]
+    int8_t *v8;               // [n_seq][Hkv][cap / 64][hd][64], positions permuted (kv8_slot)
+    float *ks, *vs;           // [n_seq][Hkv][cap / 64]
+    const int32_t *row_start; // [n_seq + 1] or null: max_rows each
+    const int32_t *pos;       // [n_seq]
+    int64_t n_rows, max_rows;
+    int n_seq, Hkv, hd, cap;
+    void *k, *v;              // rows of Hkv * hd values, ld apart (write: read only)
+    int64_t ld;
+    int vec;                  // rows 16-byte aligned (set by the launcher)
+};
+hipError_t launch_kv8_write(const Kv8Args &a, bool bf16, hipStream_t st);
+hipError_t launch_kv8_read(const Kv8Args &a, bool bf16, hipStream_t st);
+
+struct AttnKv8Args {
+    Kv8Args c;                // k, v, ld unused
+    const void *q;            // [n_rows][ldq] f32 or bf16
+    int64_t ldq;
+    void *out;                // [n_rows][Hq * hd] of q's type
+    int Hq, G;
+    float scale;
+    int window, sinks;        // window 0: every position up to the row's own
+    int max_len;              // about the longest sequence: the split's measure
+    float *part;              // partial results (QASR_SCRATCH_BYTES)
+    unsigned *counters;       // QASR_CTR_ATTN_N, zero between kernels
+    int vec_q, vec_o;         // set by the launcher
+};
+hipError_t launch_attention_kv8(const AttnKv8Args &a, bool bf16, hipStream_t st);
+}  // namespace qasr

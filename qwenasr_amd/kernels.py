@@ -7,7 +7,7 @@ every call runs the HIP kernels of libqasr_hip.so on the array's device
 """
 import ctypes as C
 
-from ._lib import QASR_ROUND_HALF_AWAY, P, check, lib
+from ._lib import QASR_GEMM_ADDTO, QASR_GEMM_PLAIN, QASR_GEMM_SWIGLU, QASR_ROUND_HALF_AWAY, P, check, lib
 
 
 def _h(a):
@@ -128,3 +128,61 @@ def bidirectional_attention(out, q, k, v, seq, n_heads, head_dim, scale, window_
     """kernels/mod.rs:1386 with windows of window_tokens positions."""
     check(lib().qasr_hip_bidirectional_attention(_h(q), out.ptr, q.ptr, k.ptr, v.ptr, seq, n_heads, head_dim,
                                                  scale, window_tokens))
+
+
+# ---------------------------------------------------------------------------
+# an 8-bit decoder layer over many rows and sequences (no counterpart in the
+# reference): include/qasr_hip.h holds the definitions and the cache's layout
+# ---------------------------------------------------------------------------
+
+def _p(a):
+    return a.ptr if a is not None else None
+
+
+def add_rms_norm_int8(q, scales, x, norm_w, rows, hidden, res=None, sum_out=None, ld=None, eps=1e-6, bf16=False):
+    """int8 rows q [rows][hidden] and scales [rows] of RMSNorm(x + res) * norm_w.
+
+    res None: no addition; norm_w None: no norm.  sum_out receives x + res and
+    may be x or res.  x, res, sum_out: f32 (or bf16) rows ld elements apart."""
+    check(lib().qasr_hip_add_rms_norm_int8(_h(x), q.ptr, scales.ptr, _p(sum_out), x.ptr, _p(res), _p(norm_w), rows, hidden,
+                                           hidden if ld is None else ld, eps, 1 if bf16 else 0))
+
+
+def gemm_w8a8(y, a, a_scales, w, w_scales, M, N, K, bias=None, accumulate=False, swiglu=False, bf16=False):
+    """y[M, N] = (a_int8 [M, K] . w_int8 [N, K]^T) * a_scales[M] * w_scales[N] (+ bias); y f32 or bf16.
+
+    accumulate: y = (y + bias) + product; swiglu: interleaved gate / up rows,
+    y [M, N / 2] = silu(gate) * up."""
+    if accumulate and swiglu:
+        raise ValueError("gemm_w8a8: accumulate and swiglu exclude each other")
+    mode = QASR_GEMM_ADDTO if accumulate else QASR_GEMM_SWIGLU if swiglu else QASR_GEMM_PLAIN
+    check(lib().qasr_hip_gemm_w8a8(_h(a), y.ptr, a.ptr, a_scales.ptr, w.ptr, w_scales.ptr, _p(bias), M, N, K, mode,
+                                   1 if bf16 else 0))
+
+
+def kv8_write(k8, v8, k_scales, v_scales, k, v, pos, n_rows, n_seq, max_rows, n_kv_heads, head_dim, capacity,
+              row_start=None, ld=None, bf16=False):
+    """Rows k, v of n_seq sequences into the int8 cache: row i of sequence j at position pos[j] + i.
+
+    row_start (int32 [n_seq + 1]): the sequences' rows; None: max_rows each.
+    ld: elements between rows (default n_kv_heads * head_dim)."""
+    check(lib().qasr_hip_kv8_write(_h(k8), k8.ptr, v8.ptr, k_scales.ptr, v_scales.ptr, k.ptr, v.ptr,
+                                   n_kv_heads * head_dim if ld is None else ld, _p(row_start), pos.ptr, n_rows, n_seq,
+                                   max_rows, n_kv_heads, head_dim, capacity, 1 if bf16 else 0))
+
+
+def kv8_read(k, v, k8, v8, k_scales, v_scales, pos, n_rows, n_seq, max_rows, n_kv_heads, head_dim, capacity,
+             row_start=None, ld=None, bf16=False):
+    """The int8 cache's values back into f32 (or bf16) rows k, v; arguments as kv8_write."""
+    check(lib().qasr_hip_kv8_read(_h(k8), k.ptr, v.ptr, n_kv_heads * head_dim if ld is None else ld, k8.ptr, v8.ptr,
+                                  k_scales.ptr, v_scales.ptr, _p(row_start), pos.ptr, n_rows, n_seq, max_rows, n_kv_heads,
+                                  head_dim, capacity, 1 if bf16 else 0))
+
+
+def attention_kv8(out, q, k8, v8, k_scales, v_scales, pos, n_rows, n_seq, max_rows, n_heads, n_kv_heads, head_dim,
+                  capacity, scale, row_start=None, ldq=None, max_len=0, window=0, sinks=0, bf16=False):
+    """softmax(scale q k) v over the int8 cache: row i of sequence j sees the positions up to pos[j] + i,
+    with window > 0 the last `window` of those and the first `sinks`."""
+    check(lib().qasr_hip_attention_kv8(_h(q), out.ptr, q.ptr, n_heads * head_dim if ldq is None else ldq, k8.ptr, v8.ptr,
+                                       k_scales.ptr, v_scales.ptr, _p(row_start), pos.ptr, n_rows, n_seq, max_rows, max_len,
+                                       n_heads, n_kv_heads, head_dim, capacity, scale, window, sinks, 1 if bf16 else 0))
