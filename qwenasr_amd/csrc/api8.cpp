@@ -112,6 +112,7 @@ extern "C" int qasr_hip_attention_kv8(qasr_hip *h, void *out, const void *q, int
     if (!out || !q) return bad("attention_kv8: null pointer");
     if (n_heads <= 0 || n_heads % n_kv_heads != 0 || n_heads > 65536)
         return bad("attention_kv8: n_heads must be a positive multiple of n_kv_heads");
+    if (max_rows * (n_heads / n_kv_heads) > (1 << 30)) return bad("attention_kv8: max_rows x heads of a group out of range");
     if (ldq < n_heads * head_dim || ldq > INT32_MAX) return bad("attention_kv8: row stride out of range");
     if (window < 0 || sinks < 0 || max_len < 0) return bad("attention_kv8: window, sinks and max_len must not be negative");
     CHECK_H(h);
@@ -122,7 +123,6 @@ extern "C" int qasr_hip_attention_kv8(qasr_hip *h, void *out, const void *q, int
     a.sinks = (int)std::min<int64_t>(sinks, capacity);
     a.max_len = (int)(max_len > 0 ? std::min<int64_t>(max_len, capacity) : capacity);
     a.part = reinterpret_cast<float *>(h->scratch);
-    a.counters = h->counters + QASR_CTR_ATTN;
     LAUNCHCHK(launch_attention_kv8(a, bf16 != 0, h->stream), "attention_kv8");
     return QASR_OK;
 }

@@ -9,6 +9,7 @@
 // the bytes of a dim of V stand in the order (g, t, r): V is stored so, a block
 // [dim][64], and no value crosses lanes or goes through LDS between the products.
 #include "kernels.h"
+#include "gemm_common.h"
 
 namespace qasr {
 
@@ -268,47 +269,189 @@ hipError_t launch_kv8_read(const Kv8Args &a0, bool bf16, hipStream_t st) {
 // Per tile of 16 query rows (row = query row x heads of the group, flattened) and
 // KV head: S = scale q.k over blocks of 64 positions with the running maximum and
 // sum of the softmax, O += P V.  Everything is exact integer products:
-//   q: round(q c) with c = 8e6 / max|q| of the row, three signed base-256 digits
-//      (24 bits: a row's error is 6e-8 of its largest value), three MFMAs a product
-//   p: round(2^30 p), p = 2^(s - max) in [0, 1], four digits.  30 bits and not 24:
-//      a sink that holds the maximum leaves every other p small, and what a long
-//      context loses by rounding them grows with its length
-// The digits of a value n come out together: the bytes of (n + 0x80808080) ^
-// 0x80808080 are its signed base-256 digits.
-// A block's scale is the same for all of its 64 positions: it joins the score's
-// factor (K) and the product's (V).
+//   q: round(q c), c = N / max|q| of the row, in D signed base-256 digits, one MFMA
+//      a digit
+//   p: round(N p), p = 2^(s - the block's own maximum) in [0, 1], the same digits
+// with N = 8e6 and D = 3 for f32 rows (a value is off by at most 6e-8 of the largest
+// of its row or block) and N = 32000, D = 2 for bf16 rows (1.6e-5; their output is
+// rounded to 2^-8 of itself).  p is counted from the block's maximum and not the
+// running one: where one position far back holds the maximum (a sink), what is left
+// of every other block would otherwise vanish in the rounding, and the loss would
+// grow with the context.  A block's scale is the same for all of its 64 positions:
+// it joins the score's factor (K) and the product's (V).
+//
+// The sums (O and the weights') count from a reference that moves only when a
+// block's maximum is 2^16 above it: in f32 they lose nothing by that, and most
+// blocks rescale nothing.
+//
+// What bounds it: the HBM reads where every sequence has one row; vector
+// instructions where rows share the positions (a score's way from the integer sums
+// to the digits is about 14 instructions, a product's value 5; three in bf16).
+//
+// A block takes CG tiles (CG x 16 flattened rows) with CG x PG waves: PG groups of
+// waves take every PG-th block of positions each, the CG waves of a group one tile
+// each.  SHARED: a group's K and V blocks come through one slot each in LDS, direct
+// from memory (global_load_lds_dwordx4), K while the block before is multiplied by
+// its weights, V during the scores.  (Operands loaded straight into registers leave
+// the four lanes of a quad in four rows: a 64-byte run is then asked for four times
+// over, and 16 KB a tile and block at 5.3 TB/s was the end, cached or not.  Two slots
+// each, a whole block ahead: 36 us for 29 at 1337 rows; the waves that the LDS then
+// keeps out are worth more.)  With `splits` > 1 several blocks share a tile's
+// positions; a second launch merges their parts.
 // ---------------------------------------------------------------------------
 
-// 4 values' digit dwords -> digit d of the 4 values in one dword (a 4 x 4 byte transpose)
-__device__ __forceinline__ void digits4(uint32_t n0, uint32_t n1, uint32_t n2, uint32_t n3, uint32_t *d) {
-    const uint32_t a = __builtin_amdgcn_perm(n1, n0, 0x05010400), b = __builtin_amdgcn_perm(n1, n0, 0x07030602);
-    const uint32_t c = __builtin_amdgcn_perm(n3, n2, 0x05010400), e = __builtin_amdgcn_perm(n3, n2, 0x07030602);
-    d[0] = __builtin_amdgcn_perm(c, a, 0x05040100);
-    d[1] = __builtin_amdgcn_perm(c, a, 0x07060302);
-    d[2] = __builtin_amdgcn_perm(e, b, 0x05040100);
-    d[3] = __builtin_amdgcn_perm(e, b, 0x07060302);
+// Digit dwords: digit d of 4 values in one dword, a byte each.  Signed base-256
+// digits are the bytes of (n + 0x..8080) ^ 0x..8080; the highest of a value that is
+// not negative needs no offset.  v holds the sums in its low bytes.
+template <int D, bool SIGNED>
+__device__ __forceinline__ void digits4(const uint32_t *v, uint32_t *d) {
+    const uint32_t a = __builtin_amdgcn_perm(v[1], v[0], 0x05010400), b = __builtin_amdgcn_perm(v[3], v[2], 0x05010400);
+    d[0] = __builtin_amdgcn_perm(b, a, 0x05040100) ^ 0x80808080u;
+    d[1] = __builtin_amdgcn_perm(b, a, 0x07060302);
+    if (D == 3 || SIGNED) d[1] ^= 0x80808080u;
+    if (D == 3) {
+        const uint32_t e = __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0602), f = __builtin_amdgcn_perm(v[3], v[2], 0x06020c0c);
+        d[D - 1] = e | f;
+        if (SIGNED) d[D - 1] ^= 0x80808080u;
+    }
 }
-__device__ __forceinline__ uint32_t signed_digits(int n) { return ((uint32_t)n + 0x80808080u) ^ 0x80808080u; }
+// the value of a product's digit sums
+template <int D>
+__device__ __forceinline__ float digit_sum(const i32x4 *acc, int r) {
+    if (D == 2) return (float)(acc[1][r] * 256 + acc[0][r]);
+    return fmaf((float)(acc[D - 1][r] * 256 + acc[1][r]), 256.0f, (float)acc[0][r]);
+}
 
-#define QASR_KV8_WAVES 4
+// 4 output values of flattened row f, dims d .. d + 3, from O and the weights' sum
 template <bool BF16, int HD>
-__global__ __launch_bounds__(64 * QASR_KV8_WAVES) void k_attn_kv8(AttnKv8Args a) {
-    constexpr int KS = HD / 64, DT = HD / 16, W = QASR_KV8_WAVES;
-    __shared__ float o_l[W][16][HD + 4];
-    __shared__ float ml_l[W][2][16];
+__device__ __forceinline__ void kv8_put(const AttnKv8Args &a, const Kv8Seq &sq, int h, unsigned f, int d, f32x4 v, float l) {
+#pragma unroll
+    for (int r = 0; r < 4; r++) v[r] = l == 0.0f ? 0.0f : __fdiv_rn(v[r], l);
+    const unsigned qi = f / (unsigned)a.G, qg = f - qi * (unsigned)a.G;
+    const int64_t at = ((sq.r0 + qi) * a.Hq + (int64_t)h * a.G + qg) * HD + d;
+    if (BF16) {
+        typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+        u16x4 u;
+#pragma unroll
+        for (int r = 0; r < 4; r++) u[r] = __builtin_bit_cast(uint16_t, (__bf16)v[r]);
+        uint16_t *p = reinterpret_cast<uint16_t *>(a.out) + at;
+        if (a.vec_o) {
+            *reinterpret_cast<u16x4 *>(p) = u;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; r++) p[r] = u[r];
+        }
+    } else {
+        float *p = reinterpret_cast<float *>(a.out) + at;
+        if (a.vec_o) {
+            *reinterpret_cast<f32x4 *>(p) = v;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; r++) p[r] = v[r];
+        }
+    }
+}
+
+// one split's part of a tile in the scratch area: maxima and sums [2][16], then O [16][HD]
+template <int HD> constexpr int kv8_part = 32 + 16 * HD;
+
+// LDS placement of a row's 16-byte slots (rows of 64 and of 128 bytes): the 16 rows
+// that the lanes of one operand read start on different banks
+template <int RB>
+__device__ __forceinline__ int kv8_swz(int row) { return RB == 64 ? (row >> 2) & 3 : (row >> 1) & 7; }
+
+template <bool BF16, int HD, int CG, int PG, bool SHARED>
+__global__ __launch_bounds__(64 * CG * PG, SHARED ? 4 : 2) void k_attn_kv8(AttnKv8Args a) {
+    constexpr int KS = HD / 64, DT = HD / 16, D = BF16 ? 2 : 3, TB = 64 * HD, LD = HD / 8 / CG;   // bytes of a block; a wave's loads of K and V
+    constexpr float N = BF16 ? 32000.0f : 8.0e6f;
+    static_assert(SHARED || CG == 1, "waves that share a block's positions share its bytes in LDS");
+    constexpr int MERGE = PG > 1 ? CG * PG * 16 * (HD + 4) * 4 : 16, SLOTS = SHARED ? PG * 2 * TB : 0;
+    __shared__ __attribute__((aligned(16))) char smem[MERGE > SLOTS ? MERGE : SLOTS];
+    __shared__ float ml_l[CG * PG][2][16];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int cg = wid % CG, pg = wid / CG;
     const int c = lane & 15, g = lane >> 4;
-    const int h = blockIdx.y, j = blockIdx.z;
+    // heads fastest: with 8 of them each XCD (blocks go to the 8 in turn) has one head's
+    // cache in its L2, and every head's longest rows come first
+    const int j = blockIdx.y, S = a.splits;
+    const unsigned rest = blockIdx.x / (unsigned)a.c.Hkv;
+    const int h = blockIdx.x - rest * a.c.Hkv, tx = rest / (unsigned)S, split = rest - tx * S;
+    const int tile0 = (a.tiles - 1 - tx) * CG, tile = tile0 + cg;
     const Kv8Seq sq = kv8_seq(a.c, j);
-    const int64_t n_flat = (int64_t)sq.n * a.G, f0 = (int64_t)blockIdx.x * 16;
-    if (f0 >= n_flat) return;
-    const int64_t fr = min(f0 + c, n_flat - 1);
-    const int qi = (int)(fr / a.G), qg = (int)(fr % a.G);
-    const int i_lo = (int)(f0 / a.G), i_hi = (int)(min(f0 + 15, n_flat - 1) / a.G);
-    const int last = sq.p0 + qi;                               // this column's own position
+    // flattened rows: fewer than 2^30 (the entry point)
+    const unsigned n_flat = (unsigned)sq.n * (unsigned)a.G;
+    if ((unsigned)tile0 * 16 >= n_flat) return;
+    const unsigned f0 = (unsigned)tile * 16, f1 = n_flat - 1;      // a tile past the last row repeats it
+    const unsigned fr = min(f0 + c, f1);
+    const int qi = (int)(fr / (unsigned)a.G), qg = (int)(fr - (unsigned)qi * (unsigned)a.G);
+    const int i_lo = (int)(min(f0, f1) / (unsigned)a.G), i_hi = (int)(min(f0 + 15, f1) / (unsigned)a.G);
+    const int last = sq.p0 + qi;                               // this column's own position, and its window's first
+    const int low = a.window > 0 ? last - a.window + 1 : INT32_MIN;
+
+    // the blocks that some row of the block's tiles sees: the sinks' and the window's; this split's run of them
+    const int hi_pos = min(sq.p0 + (int)(min((unsigned)(tile0 + CG) * 16 - 1, f1) / (unsigned)a.G), a.c.cap - 1);
+    int lo_pos = 0, n_sink = 0;
+    if (a.window > 0) {
+        lo_pos = max(0, sq.p0 + (int)((unsigned)tile0 * 16 / (unsigned)a.G) - a.window + 1);
+        n_sink = min((a.sinks + 63) / 64, lo_pos / 64);
+    }
+    const int lo_blk = lo_pos / 64;
+    const int n_blk = hi_pos < 0 ? 0 : n_sink + max(0, hi_pos / 64 - lo_blk + 1);
+    const int per = n_blk / S, more = n_blk - per * S;         // the first `more` splits take one block more
+    const int u0 = split * per + min(split, more), u1 = u0 + per + (split < more ? 1 : 0);
+    auto block_of = [&](int u) { return u < n_sink ? u : lo_blk + u - n_sink; };
+
+    const int64_t head = (int64_t)j * a.c.Hkv + h;
+    const int8_t *kb = a.c.k8 + head * a.c.cap * HD, *vb = a.c.v8 + head * a.c.cap * HD;
+    const float *ks = a.c.ks + head * (a.c.cap / 64), *vs = a.c.vs + head * (a.c.cap / 64);
+    int u = u0 + pg;
+    // SHARED: this lane's bytes of the wave's loads
+    char *kt = smem + pg * 2 * TB, *vt = kt + TB;
+    // a load fills 64 slots: 8 rows of 128 bytes (the swizzle repeats every 16 rows) or 16 of 64
+    const uint32_t v_src = (lane >> 2) * 64 + 16 * ((lane & 3) ^ kv8_swz<64>(lane >> 2));
+    const uint32_t k_src[2] = {HD == 64 ? v_src : (lane >> 3) * 128 + 16 * ((lane & 7) ^ kv8_swz<128>(lane >> 3)),
+                               HD == 64 ? v_src : (lane >> 3) * 128 + 16 * ((lane & 7) ^ kv8_swz<128>(8 + (lane >> 3)))};
+    static_assert(LD % 4 == 0 || HD == 64, "pairs of loads a wave");
+    auto issue_k = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < LD / 2; i++) {
+            const int at = 1024 * (cg * (LD / 2) + i);
+            lds_dma16_s(kb + (int64_t)b * TB + at, k_src[i & 1], kt + at);
+        }
+    };
+    auto issue_v = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < LD / 2; i++) {
+            const int at = 1024 * (cg * (LD / 2) + i);
+            lds_dma16_s(vb + (int64_t)b * TB + at, v_src, vt + at);
+        }
+    };
+    // otherwise the operands themselves, loaded again as soon as the products have read them
+    i32x4 kr[4][KS], vr[DT];
+    auto load_k = [&](int b) {
+        const int8_t *p = kb + (int64_t)b * TB + c * HD + 16 * g;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int k = 0; k < KS; k++) kr[t][k] = *reinterpret_cast<const i32x4 *>(p + 16 * t * HD + 64 * k);
+    };
+    auto load_v = [&](int b) {
+        const int8_t *p = vb + (int64_t)b * TB + c * 64 + 16 * g;
+#pragma unroll
+        for (int d = 0; d < DT; d++) vr[d] = *reinterpret_cast<const i32x4 *>(p + 16 * d * 64);
+    };
+    if (u < u1) {
+        if constexpr (SHARED) {
+            issue_k(block_of(u));
+        } else {
+            load_k(block_of(u));
+            load_v(block_of(u));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
 
     // the column's row in signed digits: dims 64 s + 16 g + 0..15 of product s
-    i32x4 qd[KS][3];
+    i32x4 qd[KS][D];
     float qf;                                                  // score = integer sum x qf x the block's scale
     {
         const int64_t at = (sq.r0 + qi) * a.ldq + (int64_t)(h * a.G + qg) * HD;
@@ -318,149 +461,297 @@ __global__ __launch_bounds__(64 * QASR_KV8_WAVES) void k_attn_kv8(AttnKv8Args a)
         for (int s = 0; s < KS; s++) {
             kv8_load16<BF16>(a.q, at + 64 * s + 16 * g, a.vec_q, x[s]);
 #pragma unroll
+            for (int e = 0; e < 16; e++) x[s][e] = a.scale < 0.0f ? -x[s][e] : x[s][e];   // the scores' factor is not negative
+#pragma unroll
             for (int e = 0; e < 16; e++) { m = fmaxf(m, fabsf(x[s][e])); bad |= !kv8_finite(x[s][e]); }
         }
         m = xhalf_max(xrow16_max(m));
         float nf = bad ? 1.0f : 0.0f;
         nf = xhalf_max(xrow16_max(nf));
         // a row below 1e-30 multiplies by the largest factor that stays finite with it
-        const float f = __fdiv_rn(8.0e6f, fmaxf(m, 1e-30f));
+        const float f = __fdiv_rn(N, fmaxf(m, 1e-30f));
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                uint32_t d[4];
-                digits4(signed_digits((int)rintf(x[s][4 * e] * f)), signed_digits((int)rintf(x[s][4 * e + 1] * f)),
-                        signed_digits((int)rintf(x[s][4 * e + 2] * f)), signed_digits((int)rintf(x[s][4 * e + 3] * f)), d);
-                qd[s][0][e] = (int)d[0];
-                qd[s][1][e] = (int)d[1];
-                qd[s][2][e] = (int)d[2];
+                uint32_t n[4], d[D];
+#pragma unroll
+                for (int i = 0; i < 4; i++) n[i] = (uint32_t)(int)rintf(x[s][4 * e + i] * f) + 0x80808080u;
+                digits4<D, true>(n, d);
+#pragma unroll
+                for (int i = 0; i < D; i++) qd[s][i][e] = (int)d[i];
             }
-        qf = nf > 0.0f ? __builtin_nanf("") : a.scale * 1.4426950408889634f * __fdiv_rn(1.0f, f);
+        qf = nf > 0.0f ? __builtin_nanf("") : fabsf(a.scale) * 1.4426950408889634f * __fdiv_rn(1.0f, f);
     }
 
-    // the blocks that some row of the tile sees: the sinks' and the window's
-    const int hi_pos = min(sq.p0 + i_hi, a.c.cap - 1);
-    int lo_pos = 0, n_sink = 0;
-    if (a.window > 0) {
-        lo_pos = max(0, sq.p0 + i_lo - a.window + 1);
-        n_sink = min((min(a.sinks, a.c.cap) + 63) / 64, lo_pos / 64);
-    }
-    const int lo_blk = lo_pos / 64;
-    const int n_blk = hi_pos < 0 ? 0 : n_sink + max(0, hi_pos / 64 - lo_blk + 1);
-
-    const int64_t head = (int64_t)j * a.c.Hkv + h;
-    const int8_t *kb = a.c.k8 + head * a.c.cap * HD, *vb = a.c.v8 + head * a.c.cap * HD;
-    const float *ks = a.c.ks + head * (a.c.cap / 64), *vs = a.c.vs + head * (a.c.cap / 64);
-    float m = -__builtin_inff(), l = 0.0f;
+    float m = -__builtin_inff(), l = 0.0f;                     // m: what O and l count from
     f32x4 o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    for (int u = wid; u < n_blk; u += W) {
-        const int b = u < n_sink ? u : lo_blk + u - n_sink;
-        const int8_t *kt = kb + (int64_t)b * 64 * HD, *vt = vb + (int64_t)b * 64 * HD;
-        const float kf = ks[b] * qf;
+    float ksl = 0.0f, vsl = 0.0f;                              // lane i: the scales of this group's block `it` + i
+    const int n_it = (u1 - u0 + PG - 1) / PG;
+    for (int it = 0; it < n_it; it++, u += PG) {
+        if ((it & 63) == 0) {
+            const int ul = u + lane * PG;
+            ksl = ul < u1 ? ks[block_of(ul)] : 0.0f;
+            vsl = ul < u1 ? vs[block_of(ul)] : 0.0f;
+            // waited for here: a wait at their use would drain the loads in flight in every turn
+            asm volatile("" : "+v"(ksl), "+v"(vsl));
+        }
+        const bool live = u < u1;
+        const int b = block_of(u), bn = block_of(min(u + PG, u1 - 1));
+        if constexpr (SHARED) {
+            wait_vmcnt<0>();                                   // this wave's part of the block's K has landed
+            __syncthreads();                                   // ... and every wave's; V of the block before has been read
+            if (live) issue_v(b);
+        }
+        if (!live) {                                           // the other groups' last block
+            if (SHARED) __syncthreads();
+            continue;
+        }
+        const float ksb = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ksl), it & 63));
+        const float vsb = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vsl), it & 63));
+        // a product's sums are read behind the next product's issue
         float s[16];
-        float mx = -__builtin_inff();
+        {
+            i32x4 acc[2][D];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            i32x4 acc[3] = {};
+            for (int t = 0; t <= 4; t++) {
+                if (t < 4) {
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const i32x4 ka = *reinterpret_cast<const i32x4 *>(kt + (16 * t + c) * HD + 64 * k + 16 * g);
+                    for (int d = 0; d < D; d++) acc[t & 1][d] = i32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int d = 0; d < 3; d++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(ka, qd[k][d], acc[d], 0, 0, 0);
-            }
+                    for (int k = 0; k < KS; k++) {
+                        const int r = 16 * t + c;
+                        if (SHARED) kr[t][k] = *reinterpret_cast<const i32x4 *>(kt + r * HD + 16 * ((4 * k + g) ^ kv8_swz<HD>(r)));
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int p = b * 64 + 16 * t + 4 * g + r;
-                const float v = fmaf((float)(acc[2][r] * 256 + acc[1][r]), 256.0f, (float)acc[0][r]) * kf;
-                const bool seen = p <= last && (a.window == 0 || p > last - a.window || p < a.sinks);
-                s[4 * t + r] = seen ? v : -__builtin_inff();
-                mx = fmaxf(mx, s[4 * t + r]);
+                        for (int d = 0; d < D; d++)
+                            acc[t & 1][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[t][k], qd[k][d], acc[t & 1][d], 0, 0, 0);
+                    }
+                }
+                if (t > 0) {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) s[4 * (t - 1) + r] = digit_sum<D>(acc[(t - 1) & 1], r);
+                }
             }
         }
-        mx = xhalf_max(xrow16_max(mx));
-        const float mn = fmaxf(m, mx), ms = mn == -__builtin_inff() ? 0.0f : mn;
-        const float al = __builtin_amdgcn_exp2f(m - ms);
-        m = mn;
+        if constexpr (!SHARED) {
+            __builtin_amdgcn_sched_barrier(0);
+            load_k(bn);                                        // a whole block ahead of their use
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // p from the integer sums; mb: the block's maximum
+        const float kf = ksb * qf;
+        float mb, p[16];
+        if (ksb >= 0.0f && b * 64 + 63 <= sq.p0 + i_lo &&
+            (a.window == 0 || b * 64 > sq.p0 + i_hi - a.window || b * 64 + 63 < a.sinks)) {
+            // every row of the tile sees the whole block
+            mb = s[0];
+#pragma unroll
+            for (int i = 1; i < 16; i++) mb = fmaxf(mb, s[i]);
+            mb = xhalf_max(xrow16_max(mb)) * kf;
+#pragma unroll
+            for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], kf, -mb));
+        } else {
+            mb = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int at = b * 64 + 16 * (i >> 2) + 4 * g + (i & 3);
+                const bool seen = (at <= last) & ((at >= low) | (at < a.sinks));
+                s[i] = seen ? s[i] * kf : -__builtin_inff();
+                mb = fmaxf(mb, s[i]);
+            }
+            mb = xhalf_max(xrow16_max(mb));
+            const float ref = mb == -__builtin_inff() ? 0.0f : mb;
+#pragma unroll
+            for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(s[i] - ref);
+        }
+        const bool up = mb > m + 16.0f;
+        if (__any(up)) {
+            const float al = up ? __builtin_amdgcn_exp2f(m - mb) : 1.0f;
+            m = up ? mb : m;
+            l *= al;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) o[dt][r] *= al;
+        }
         // a column that sees none of this block takes nothing of it, its scale neither
-        const float vf = mx == -__builtin_inff() ? 0.0f : vs[b] * 0x1p-30f;
-        i32x4 pd[4];
+        const float eb = mb == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mb - m);
+        const float vf = mb == -__builtin_inff() ? 0.0f : vsb * eb * (1.0f / N);
+        i32x4 pd[D];
         float sum = 0.0f;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            uint32_t n[4], d[4];
+            uint32_t n[4], d[D];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const float p = __builtin_amdgcn_exp2f(s[4 * t + r] - ms);
-                sum += p;
-                n[r] = signed_digits((int)rintf(p * 0x1p30f));
+                sum += p[4 * t + r];
+                // 2^23 + the lower digits' offset: the sum's low bytes are round(N p) + that offset
+                n[r] = __float_as_uint(fmaf(p[4 * t + r], N, 8388608.0f + (D == 2 ? 128.0f : 32896.0f)));
             }
-            digits4(n[0], n[1], n[2], n[3], d);
+            digits4<D, false>(n, d);
 #pragma unroll
-            for (int e = 0; e < 4; e++) pd[e][t] = (int)d[e];
+            for (int e = 0; e < D; e++) pd[e][t] = (int)d[e];
         }
-        l = fmaf(l, al, sum);
+        l = fmaf(sum, eb, l);
+        if constexpr (SHARED) {
+            wait_vmcnt<0>();                                   // V has landed, and every wave has read K
+            __syncthreads();
+            if (u + PG < u1) issue_k(bn);
+        }
+        {
+            i32x4 acc[2][D];
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++) {
-            const i32x4 va = *reinterpret_cast<const i32x4 *>(vt + (16 * dt + c) * 64 + 16 * g);
-            i32x4 acc[4];
+            for (int dt = 0; dt <= DT; dt++) {
+                if (dt < DT) {
+                    const int vrow = 16 * dt + c;
+                    if (SHARED) vr[dt] = *reinterpret_cast<const i32x4 *>(vt + vrow * 64 + 16 * (g ^ kv8_swz<64>(vrow)));
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const i32x4 z = {0, 0, 0, 0};
-                acc[e] = __builtin_amdgcn_mfma_i32_16x16x64_i8(va, pd[e], z, 0, 0, 0);
+                    for (int e = 0; e < D; e++) {
+                        const i32x4 z = {0, 0, 0, 0};
+                        acc[dt & 1][e] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vr[dt], pd[e], z, 0, 0, 0);
+                    }
+                }
+                if (dt > 0) {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) o[dt - 1][r] = fmaf(digit_sum<D>(acc[(dt - 1) & 1], r), vf, o[dt - 1][r]);
+                }
+                // one product, then its share of the last one's vector instructions: the two run side by side
+                if (dt > 0 && dt < DT) {
+#pragma unroll
+                    for (int e = 0; e < D; e++) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, D == 3 ? 7 : 6, 0);
+                    }
+                }
             }
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float pv = fmaf((float)(acc[3][r] * 256 + acc[2][r]), 65536.0f, (float)(acc[1][r] * 256 + acc[0][r]));
-                o[dt][r] = fmaf(o[dt][r], al, pv * vf);
-            }
+        }
+        if constexpr (!SHARED) {
+            __builtin_amdgcn_sched_barrier(0);
+            load_v(bn);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     l = xhalf_sum(xrow16_sum(l));
 
-    // the waves' parts
+    const int cols = f0 < n_flat ? (int)min(16u, n_flat - f0) : 0;
+    float *part = a.part + ((((int64_t)j * a.c.Hkv + h) * a.tiles * CG + tile) * S + split) * kv8_part<HD>;
+    if constexpr (PG == 1) {
+        if (c >= cols) return;
+        if (S > 1 && g == 0) { part[c] = m; part[16 + c] = l; }
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) {
+            if (S > 1) *reinterpret_cast<f32x4 *>(part + 32 + c * HD + 16 * dt + 4 * g) = o[dt];
+            else kv8_put<BF16, HD>(a, sq, h, f0 + c, 16 * dt + 4 * g, o[dt], l);
+        }
+        return;
+    }
+    // the groups' parts of each tile, through the ring's LDS (every load into it has landed and been read)
+    float (*o_l)[16][HD + 4] = reinterpret_cast<float (*)[16][HD + 4]>(smem);
+    __syncthreads();
     if (g == 0) { ml_l[wid][0][c] = m; ml_l[wid][1][c] = l; }
 #pragma unroll
     for (int dt = 0; dt < DT; dt++) *reinterpret_cast<f32x4 *>(&o_l[wid][c][16 * dt + 4 * g]) = o[dt];
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * (HD / 4); i += 64 * W) {
+    for (int i = lane + 64 * pg; i < cols * (HD / 4); i += 64 * PG) {
         const int col = i / (HD / 4), d = 4 * (i % (HD / 4));
-        const int64_t f = f0 + col;
-        if (f >= n_flat) continue;
         float mm = -__builtin_inff();
 #pragma unroll
-        for (int w = 0; w < W; w++) mm = fmaxf(mm, ml_l[w][0][col]);
+        for (int w = 0; w < PG; w++) mm = fmaxf(mm, ml_l[w * CG + cg][0][col]);
         const float ms = mm == -__builtin_inff() ? 0.0f : mm;
         float ll = 0.0f;
         f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < W; w++) {
-            const float e = __builtin_amdgcn_exp2f(ml_l[w][0][col] - ms);
-            ll = fmaf(ml_l[w][1][col], e, ll);
-            const f32x4 ow = *reinterpret_cast<const f32x4 *>(&o_l[w][col][d]);
+        for (int w = 0; w < PG; w++) {
+            const float e = __builtin_amdgcn_exp2f(ml_l[w * CG + cg][0][col] - ms);
+            ll = fmaf(ml_l[w * CG + cg][1][col], e, ll);
+            const f32x4 ow = *reinterpret_cast<const f32x4 *>(&o_l[w * CG + cg][col][d]);
 #pragma unroll
             for (int r = 0; r < 4; r++) v[r] = fmaf(ow[r], e, v[r]);
         }
-#pragma unroll
-        for (int r = 0; r < 4; r++) v[r] = ll == 0.0f ? 0.0f : __fdiv_rn(v[r], ll);
-        const int64_t at = ((sq.r0 + f / a.G) * a.Hq + (int64_t)h * a.G + f % a.G) * HD + d;
-        if (BF16) {
-            uint16_t *p = reinterpret_cast<uint16_t *>(a.out) + at;
-#pragma unroll
-            for (int r = 0; r < 4; r++) p[r] = __builtin_bit_cast(uint16_t, (__bf16)v[r]);
+        if (S > 1) {
+            if (d == 0) { part[col] = mm; part[16 + col] = ll; }
+            *reinterpret_cast<f32x4 *>(part + 32 + col * HD + d) = v;
         } else {
-            float *p = reinterpret_cast<float *>(a.out) + at;
-            if (a.vec_o) {
-                *reinterpret_cast<f32x4 *>(p) = v;
-            } else {
-#pragma unroll
-                for (int r = 0; r < 4; r++) p[r] = v[r];
-            }
+            kv8_put<BF16, HD>(a, sq, h, f0 + col, d, v, ll);
         }
     }
+}
+
+// The splits' parts of a tile, in split order; one block a tile: the parts' weights
+// first, then sums whose loads do not wait for one another.  A launch of its own:
+// handing the parts over inside the first one (a counter, the last block merging)
+// cost 45 us at 512 blocks, each block's release writing its whole L2 back.
+template <bool BF16, int HD>
+__global__ __launch_bounds__(256) void k_attn_kv8_merge(AttnKv8Args a) {
+    __shared__ float w_l[64][17], l_l[16];
+    const int tile = blockIdx.x, h = blockIdx.y, j = blockIdx.z, S = a.splits;
+    const Kv8Seq sq = kv8_seq(a.c, j);
+    const unsigned n_flat = (unsigned)sq.n * (unsigned)a.G, f0 = (unsigned)tile * 16;
+    if (f0 >= n_flat) return;
+    const int cols = (int)min(16u, n_flat - f0);
+    const float *part = a.part + (((int64_t)j * a.c.Hkv + h) * gridDim.x + tile) * S * kv8_part<HD>;
+    // 16 lanes a column, each with the splits w, w + 16, ... (at most 4)
+    const int col = threadIdx.x >> 4, w0 = threadIdx.x & 15;
+    if (col < cols) {
+        float mw[4], lw[4], mm = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int w = w0 + 16 * i;
+            mw[i] = w < S ? part[w * kv8_part<HD> + col] : -__builtin_inff();
+            lw[i] = w < S ? part[w * kv8_part<HD> + 16 + col] : 0.0f;
+            mm = fmaxf(mm, mw[i]);
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));
+        const float ms = mm == -__builtin_inff() ? 0.0f : mm;
+        float ll = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float e = __builtin_amdgcn_exp2f(mw[i] - ms);
+            ll = fmaf(lw[i], e, ll);
+            if (w0 + 16 * i < S) w_l[w0 + 16 * i][col] = e;
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) ll += __shfl_xor(ll, o, 64);
+        if (w0 == 0) l_l[col] = ll;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < cols * (HD / 4); i += 256) {
+        const int cc = i / (HD / 4), d = 4 * (i % (HD / 4));
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+        for (int w = 0; w < S; w++) {
+            const f32x4 ow = *reinterpret_cast<const f32x4 *>(part + w * kv8_part<HD> + 32 + cc * HD + d);
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[r] = fmaf(ow[r], w_l[w][cc], v[r]);
+        }
+        kv8_put<BF16, HD>(a, sq, h, f0 + cc, d, v, l_l[cc]);
+    }
+}
+
+template <bool BF16, int HD, int CG, int PG, bool SHARED>
+static hipError_t go_attn_kv8(const AttnKv8Args &a, hipStream_t st) {
+    const dim3 grid((unsigned)(a.tiles * a.splits * a.c.Hkv), (unsigned)a.c.n_seq);
+    hipLaunchKernelGGL((k_attn_kv8<BF16, HD, CG, PG, SHARED>), grid, dim3(64 * CG * PG), 0, st, a);
+    if (a.splits > 1)
+        hipLaunchKernelGGL((k_attn_kv8_merge<BF16, HD>), dim3((unsigned)a.tiles * CG, (unsigned)a.c.Hkv, (unsigned)a.c.n_seq), dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+template <int CG, int PG, bool SHARED>
+static hipError_t pick_attn_kv8(AttnKv8Args &a, bool bf16, int splits, hipStream_t st) {
+    const int64_t tiles = (a.c.max_rows * a.G + 16 * CG - 1) / (16 * CG), units = tiles * CG * a.c.Hkv * a.c.n_seq;
+    // the splits' parts fit the scratch area
+    int64_t s = std::min<int64_t>(splits, (int64_t)QASR_KV8_PART_BYTES / (units * (32 + 16 * a.c.hd) * 4));
+    s = std::max<int64_t>(1, std::min<int64_t>(s, 64));
+    if (tiles * s * a.c.Hkv > INT32_MAX) return hipErrorInvalidValue;
+    a.tiles = (int)tiles;
+    a.splits = (int)s;
+    if (bf16) return a.c.hd == 128 ? go_attn_kv8<true, 128, CG, PG, SHARED>(a, st) : go_attn_kv8<true, 64, CG, PG, SHARED>(a, st);
+    return a.c.hd == 128 ? go_attn_kv8<false, 128, CG, PG, SHARED>(a, st) : go_attn_kv8<false, 64, CG, PG, SHARED>(a, st);
 }
 
 hipError_t launch_attention_kv8(const AttnKv8Args &a0, bool bf16, hipStream_t st) {
@@ -468,17 +759,29 @@ hipError_t launch_attention_kv8(const AttnKv8Args &a0, bool bf16, hipStream_t st
     if ((a.c.hd != 64 && a.c.hd != 128) || a.c.n_seq > 65535 || a.c.Hkv > 65535) return hipErrorInvalidValue;
     a.vec_q = kv8_vec(a.q, nullptr, a.ldq, bf16 ? 2 : 4);
     a.vec_o = (uintptr_t)a.out % 16 == 0;
-    const int64_t tiles = (a.c.max_rows * a.G + 15) / 16;
-    if (tiles > INT32_MAX) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)tiles, (unsigned)a.c.Hkv, (unsigned)a.c.n_seq), blk(64 * QASR_KV8_WAVES);
-    if (bf16) {
-        if (a.c.hd == 128) hipLaunchKernelGGL((k_attn_kv8<true, 128>), grid, blk, 0, st, a);
-        else hipLaunchKernelGGL((k_attn_kv8<true, 64>), grid, blk, 0, st, a);
-    } else {
-        if (a.c.hd == 128) hipLaunchKernelGGL((k_attn_kv8<false, 128>), grid, blk, 0, st, a);
-        else hipLaunchKernelGGL((k_attn_kv8<false, 64>), grid, blk, 0, st, a);
+    const int64_t rows = a.c.max_rows * a.G;
+    // blocks of positions that the longest sequence's rows see
+    const int64_t seen = a.window > 0 ? std::min<int64_t>(a.max_len, (int64_t)a.window + a.sinks + a.c.max_rows) : a.max_len;
+    const int64_t blocks = (seen + 63) / 64;
+    if (rows <= 16) {
+        // One tile a sequence and head (decoding): the operands straight into registers, as no
+        // second tile shares them.  Positions are split over blocks of 4 waves up to 384 blocks,
+        // a wave left with one block of positions at least; below 25 of them the merge costs what
+        // the split saves.  us, 1 split against these, 8 KV heads x 2 heads of 128, bf16: one
+        // sequence at 4000 positions 25.2 -> 9.9, at 60000 323 -> 30, 4 at 16000 90 -> 24; at 1000
+        // positions 10.9 against 12.2; 32 at 4000 40.3 against 42.5 (2 splits), so one there.
+        const int64_t units = a.c.Hkv * (int64_t)a.c.n_seq;
+        const int splits = blocks <= 24 ? 1 : (int)std::min<int64_t>(384 / units, (blocks + 3) / 4);
+        return pick_attn_kv8<1, 4, false>(a, bf16, splits, st);
     }
-    return hipGetLastError();
+    // Two tiles a block.  2 groups of waves a block where 384 blocks are there, else 4 groups
+    // and splits up to 512 blocks, each wave left with 4 blocks of positions at least.  us, 2
+    // groups against 4: 1337 rows 29.4 / 32.4, with bf16 22.6 / 26.6; 404 rows 12.5 / 12.2; 2 x
+    // 300 rows behind 3000 positions 45 / 41; 4 x 67 rows, window 8192: 87 / 61, with 3 splits
+    // 43 + 5 / 38 + 5.
+    const int64_t units = (rows + 31) / 32 * a.c.Hkv * a.c.n_seq;
+    if (units >= 384) return pick_attn_kv8<2, 2, true>(a, bf16, 1, st);
+    return pick_attn_kv8<2, 4, true>(a, bf16, (int)std::min<int64_t>(512 / units, blocks / 16), st);
 }
 
 }  // namespace qasr

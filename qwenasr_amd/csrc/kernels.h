@@ -400,9 +400,9 @@ struct AttnKv8Args {
     float scale;
     int window, sinks;        // window 0: every position up to the row's own
     int max_len;              // about the longest sequence: the split's measure
-    float *part;              // partial results (QASR_SCRATCH_BYTES)
-    unsigned *counters;       // QASR_CTR_ATTN_N, zero between kernels
-    int vec_q, vec_o;         // set by the launcher
+    float *part;              // the splits' parts (QASR_KV8_PART_BYTES)
+    int vec_q, vec_o, tiles, splits;   // set by the launcher
 };
+#define QASR_KV8_PART_BYTES (32u << 20)
 hipError_t launch_attention_kv8(const AttnKv8Args &a, bool bf16, hipStream_t st);
 }  // namespace qasr

@@ -8,12 +8,13 @@
 #include "kernels.h"
 
 // scratch area of a handle: argmax partials, attention partials
-#define QASR_SCRATCH_BYTES (8u << 20)
+#define QASR_SCRATCH_BYTES (32u << 20)
 #define QASR_ARGMAX_MAX_BLOCKS 4096
 #define QASR_COUNTERS 1024
 #define QASR_CTR_ARGMAX 0
 #define QASR_CTR_ATTN 64
 #define QASR_CTR_ATTN_N 256
+static_assert(QASR_KV8_PART_BYTES <= QASR_SCRATCH_BYTES, "scratch");
 // kernel kinds of qasr_hip_decoder_profile
 #define QASR_PROFILE_KINDS 8
 

@@ -84,14 +84,14 @@ class Cache:
         return self.q["k"].astype(np.int8), v8, self.s["k"], self.s["v"]
 
 
-def attend(q, k, v, pos, scale, window=0, sinks=0):
+def attend(q, k, v, pos, scale, window=0, sinks=0, steps=8.0e6):
     """q [n][G * heads][dim] over k, v [heads][cap][dim]; row i sees positions up to pos + i.
-    Returns (out, spread, bound): spread = sum of weights x |v|, bound the part of it that f32
-    arithmetic may lose (see below)."""
+    steps: the whole numbers that the largest value of a row of q, and the largest weight of a block, count.
+    Returns (out, bound): bound on what the operator's arithmetic may lose (see below)."""
     n, hq, d = q.shape
     heads, cap, _ = k.shape
     g = hq // heads
-    out, spread, bound = np.zeros(q.shape), np.zeros(q.shape), np.zeros((n, hq, 1))
+    out, bound = np.zeros(q.shape), np.zeros(q.shape)
     p = np.arange(cap)
     for i in range(n):
         last = pos + i
@@ -103,13 +103,18 @@ def attend(q, k, v, pos, scale, window=0, sinks=0):
             s = scale * (kk @ q[i, h])
             e = np.exp(s - s.max())
             w = e / e.sum()
-            out[i, h], spread[i, h] = w @ vv, w @ np.abs(vv)
-            # a weight's relative error, twice (the sum has it too).  The score: q in steps of max|q| / 8e6, half a
-            # step off against |k|; six roundings of it (the step's factor and its inverse, scale x log2 e, the block's
+            out[i, h] = w @ vv
+            # a weight's relative error, twice (the sum has it too).  The score: q in whole numbers of max|q| / steps, half
+            # a one off against |k|; six roundings of it (the step's factor and its inverse, scale x log2 e, the block's
             # scale, two of the sum, the product); the difference from the maximum; the exponential's unit in the last
             # place.  Then the block's scale, the rescaling of the sums at each block and their additions
             u = 2.0 ** -24
-            score = scale * np.abs(kk).sum(1) * np.abs(q[i, h]).max() / 1.6e7 + 8 * u * np.abs(s) + u * np.abs(s - s.max())
+            score = scale * np.abs(kk).sum(1) * np.abs(q[i, h]).max() / (2 * steps) + 8 * u * np.abs(s) + u * np.abs(s - s.max())
             blocks = (seen.sum() + 2 * BLOCK) // BLOCK + 1
-            bound[i, h] = 2 * score.max() + (4 * blocks + 24) * u
-    return out, spread, bound
+            # a block's weights are whole numbers of its largest / steps, half a one off against |v|
+            at = p[seen] // BLOCK
+            top = np.zeros(cap // BLOCK)
+            np.maximum.at(top, at, w)
+            whole = (top[at] / (2 * steps)) @ np.abs(vv)
+            bound[i, h] = (2 * score.max() + (4 * blocks + 24) * u) * (w @ np.abs(vv)) + 1.01 * whole
+    return out, bound

@@ -362,8 +362,8 @@ def check_attention(got, ref, q, counts, pos, window=0, sinks=0, is_bf16=False):
     k, v = ref.values("k"), ref.values("v")
     for j, n in enumerate(counts):
         rows = slice(start[j], start[j] + n)
-        want, spread, rel = ref8.attend(q[rows], k[j], v[j], pos[j], dim ** -0.5, window, sinks)
-        err = rel * spread + (BF16 if is_bf16 else F32) * np.abs(want)
+        want, err = ref8.attend(q[rows], k[j], v[j], pos[j], dim ** -0.5, window, sinks, 32000.0 if is_bf16 else 8.0e6)
+        err = err + (BF16 if is_bf16 else F32) * (np.abs(want) + err)
         over = np.abs(got[rows] - want) > err
         assert not over.any(), (j, np.argwhere(over)[:4], np.abs(got[rows] - want).max(), err.max())
 
@@ -374,7 +374,8 @@ ATTN = [([1], [0], 1, 1, 64, 64, 0, 0), ([1], [403], 8, 2, 128, 512, 0, 0), ([1,
         ([5, 9], [60, 126], 1, 7, 64, 128, 0, 0), ([133], [0], 2, 1, 128, 192, 0, 0), ([1, 1], [3000, 1500], 2, 2, 128, 3200, 0, 0),
         ([1, 1], [900, 40], 8, 2, 128, 1024, 100, 4), ([30, 66], [700, 0], 2, 2, 64, 1024, 65, 70), ([33], [512], 2, 2, 128, 1024, 1, 0),
         ([1, 20], [1000, 900], 1, 16, 128, 1024, 64, 0), ([3], [2000], 2, 2, 128, 256, 100, 5), ([130], [0], 1, 2, 128, 256, 1000, 3),
-        ([1], [5000], 4, 33, 64, 5120, 0, 0)]
+        ([1], [5000], 4, 33, 64, 5120, 0, 0), ([260, 259, 100], [0, 1, 60], 16, 1, 64, 320, 0, 0), ([40], [3000], 2, 2, 128, 3136, 1500, 70),
+        ([2, 1], [3000, 2999], 1, 4, 128, 3136, 2500, 100), ([9], [4000], 1, 2, 64, 4096, 0, 0)]
 
 
 @pytest.mark.parametrize("is_bf16", [False, True])
