@@ -355,11 +355,6 @@ __device__ __forceinline__ void kv8_put(const AttnKv8Args &a, const Kv8Seq &sq, 
 // one split's part of a tile in the scratch area: maxima and sums [2][16], then O [16][HD]
 template <int HD> constexpr int kv8_part = 32 + 16 * HD;
 
-// LDS placement of a row's 16-byte slots (rows of 64 and of 128 bytes): the 16 rows
-// that the lanes of one operand read start on different banks
-template <int RB>
-__device__ __forceinline__ int kv8_swz(int row) { return RB == 64 ? (row >> 2) & 3 : (row >> 1) & 7; }
-
 template <bool BF16, int HD, int CG, int PG, bool SHARED>
 __global__ __launch_bounds__(64 * CG * PG, SHARED ? 4 : 2) void k_attn_kv8(AttnKv8Args a) {
     constexpr int KS = HD / 64, DT = HD / 16, D = BF16 ? 2 : 3, TB = 64 * HD, LD = HD / 8 / CG;   // bytes of a block; a wave's loads of K and V
@@ -408,9 +403,9 @@ __global__ __launch_bounds__(64 * CG * PG, SHARED ? 4 : 2) void k_attn_kv8(AttnK
     // SHARED: this lane's bytes of the wave's loads
     char *kt = smem + pg * 2 * TB, *vt = kt + TB;
     // a load fills 64 slots: 8 rows of 128 bytes (the swizzle repeats every 16 rows) or 16 of 64
-    const uint32_t v_src = (lane >> 2) * 64 + 16 * ((lane & 3) ^ kv8_swz<64>(lane >> 2));
-    const uint32_t k_src[2] = {HD == 64 ? v_src : (lane >> 3) * 128 + 16 * ((lane & 7) ^ kv8_swz<128>(lane >> 3)),
-                               HD == 64 ? v_src : (lane >> 3) * 128 + 16 * ((lane & 7) ^ kv8_swz<128>(8 + (lane >> 3)))};
+    const uint32_t v_src = (lane >> 2) * 64 + 16 * ((lane & 3) ^ lds_swz<64>(lane >> 2));
+    const uint32_t k_src[2] = {HD == 64 ? v_src : (lane >> 3) * 128 + 16 * ((lane & 7) ^ lds_swz<128>(lane >> 3)),
+                               HD == 64 ? v_src : (lane >> 3) * 128 + 16 * ((lane & 7) ^ lds_swz<128>(8 + (lane >> 3)))};
     static_assert(LD % 4 == 0 || HD == 64, "pairs of loads a wave");
     auto issue_k = [&](int b) {
 #pragma unroll
@@ -524,7 +519,7 @@ __global__ __launch_bounds__(64 * CG * PG, SHARED ? 4 : 2) void k_attn_kv8(AttnK
 #pragma unroll
                     for (int k = 0; k < KS; k++) {
                         const int r = 16 * t + c;
-                        if (SHARED) kr[t][k] = *reinterpret_cast<const i32x4 *>(kt + r * HD + 16 * ((4 * k + g) ^ kv8_swz<HD>(r)));
+                        if (SHARED) kr[t][k] = *reinterpret_cast<const i32x4 *>(kt + r * HD + 16 * ((4 * k + g) ^ lds_swz<HD>(r)));
 #pragma unroll
                         for (int d = 0; d < D; d++)
                             acc[t & 1][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[t][k], qd[k][d], acc[t & 1][d], 0, 0, 0);
@@ -607,7 +602,7 @@ __global__ __launch_bounds__(64 * CG * PG, SHARED ? 4 : 2) void k_attn_kv8(AttnK
             for (int dt = 0; dt <= DT; dt++) {
                 if (dt < DT) {
                     const int vrow = 16 * dt + c;
-                    if (SHARED) vr[dt] = *reinterpret_cast<const i32x4 *>(vt + vrow * 64 + 16 * (g ^ kv8_swz<64>(vrow)));
+                    if (SHARED) vr[dt] = *reinterpret_cast<const i32x4 *>(vt + vrow * 64 + 16 * (g ^ lds_swz<64>(vrow)));
 #pragma unroll
                     for (int e = 0; e < D; e++) {
                         const i32x4 z = {0, 0, 0, 0};
