@@ -56,7 +56,14 @@ __device__ __forceinline__ void load8(const void *base, int64_t row0, int e, int
 // f32 -> bf16, nearest even, any input
 __device__ __forceinline__ uint16_t to_bf16(float f) { return __builtin_bit_cast(uint16_t, (__bf16)f); }
 
-template <bool BF16, bool VEC>
+// STREAM: past the caches
+template <bool STREAM, typename V>
+__device__ __forceinline__ void put(V *p, V v) {
+    if (STREAM) __builtin_nontemporal_store(v, p);
+    else *p = v;
+}
+
+template <bool BF16, bool VEC, bool STREAM>
 __device__ __forceinline__ void store8(void *base, int64_t row0, int e, int H, const float *v) {
     if (BF16) {
         uint16_t *p = reinterpret_cast<uint16_t *>(base) + row0 + e;
@@ -64,7 +71,7 @@ __device__ __forceinline__ void store8(void *base, int64_t row0, int e, int H, c
             u16x8 u;
 #pragma unroll
             for (int i = 0; i < 8; i++) u[i] = to_bf16(v[i]);
-            *reinterpret_cast<u16x8 *>(p) = u;
+            put<STREAM>(reinterpret_cast<u16x8 *>(p), u);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++)
@@ -73,8 +80,8 @@ __device__ __forceinline__ void store8(void *base, int64_t row0, int e, int H, c
     } else {
         float *p = reinterpret_cast<float *>(base) + row0 + e;
         if (VEC) {
-            reinterpret_cast<f32x4 *>(p)[0] = f32x4{v[0], v[1], v[2], v[3]};
-            reinterpret_cast<f32x4 *>(p)[1] = f32x4{v[4], v[5], v[6], v[7]};
+            put<STREAM>(reinterpret_cast<f32x4 *>(p), f32x4{v[0], v[1], v[2], v[3]});
+            put<STREAM>(reinterpret_cast<f32x4 *>(p) + 1, f32x4{v[4], v[5], v[6], v[7]});
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++)
@@ -85,7 +92,7 @@ __device__ __forceinline__ void store8(void *base, int64_t row0, int e, int H, c
 
 // One block of T threads a row; thread t holds the 8-value chunks t, t + T, ...
 // (C of them).  VEC: H and ld multiples of 8, 16-byte aligned buffers.
-template <bool BF16, bool VEC, int T, int C>
+template <bool BF16, bool VEC, bool STREAM, int T, int C>
 __global__ __launch_bounds__(T) void k_add_rms_norm_int8(Rows8Args a) {
     constexpr int W = T / 64;
     __shared__ double red[2][W];
@@ -118,7 +125,7 @@ __global__ __launch_bounds__(T) void k_add_rms_norm_int8(Rows8Args a) {
             bad |= !(fabs(td) <= 1.7976931348623157e308) || !(fabs(sd) <= 1.7976931348623157e308);
             mx = fmax(mx, fabs(td));
         }
-        if (a.sum) store8<BF16, VEC>(a.sum, r0, e, H, s);
+        if (a.sum) store8<BF16, VEC, STREAM>(a.sum, r0, e, H, s);
     }
     ss = wave_sum_f64(ss);
     mx = wave_max_f64(mx);
@@ -150,7 +157,8 @@ __global__ __launch_bounds__(T) void k_add_rms_norm_int8(Rows8Args a) {
         }
         int8_t *p = a.q + row * H + e;
         if (VEC) {
-            *reinterpret_cast<int2 *>(p) = make_int2(pack4_i8(q[0], q[1], q[2], q[3]), pack4_i8(q[4], q[5], q[6], q[7]));
+            typedef int i32x2 __attribute__((ext_vector_type(2)));
+            put<STREAM>(reinterpret_cast<i32x2 *>(p), i32x2{pack4_i8(q[0], q[1], q[2], q[3]), pack4_i8(q[4], q[5], q[6], q[7])});
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++)
@@ -159,22 +167,38 @@ __global__ __launch_bounds__(T) void k_add_rms_norm_int8(Rows8Args a) {
     }
 }
 
-template <bool BF16, bool VEC>
+// As many threads as the row has chunks, half as many in bf16, whose chunks are 16
+// bytes: a wave then keeps as much in flight (12120 x 2048 bf16 with 256 and 128
+// threads 42.6 and 39.6 us; f32 5000 x 2048 27.5 and 30.7).  From 2^23 values on the
+// results go past the caches, which do not hold them until they are read (that case
+// 45.5 -> 42.6 us with 256 threads).
+template <bool BF16, bool VEC, bool STREAM>
 static hipError_t go_rows8(const Rows8Args &a, hipStream_t st) {
+    constexpr int C = BF16 ? 2 : 1;
     const dim3 grid((unsigned)a.rows);
-    const int chunks = (a.H + 7) / 8;
-    if (chunks <= 256) hipLaunchKernelGGL((k_add_rms_norm_int8<BF16, VEC, 256, 1>), grid, dim3(256), 0, st, a);
-    else if (chunks <= 1024) hipLaunchKernelGGL((k_add_rms_norm_int8<BF16, VEC, 1024, 1>), grid, dim3(1024), 0, st, a);
-    else hipLaunchKernelGGL((k_add_rms_norm_int8<BF16, VEC, 1024, 2>), grid, dim3(1024), 0, st, a);
+    const int n = (a.H + 8 * C - 1) / (8 * C);
+#define QR(T, CC) hipLaunchKernelGGL((k_add_rms_norm_int8<BF16, VEC, STREAM, T, CC>), grid, dim3(T), 0, st, a)
+    if (n <= 64) QR(64, C);
+    else if (n <= 128) QR(128, C);
+    else if (n <= 256) QR(256, C);
+    else if (n <= 512) QR(512, C);
+    else if (n <= 1024) QR(1024, C);
+    else QR(1024, 2);
+#undef QR
     return hipGetLastError();
+}
+
+template <bool BF16, bool VEC>
+static hipError_t pick_rows8(const Rows8Args &a, hipStream_t st) {
+    return a.rows * a.H >= (1 << 23) ? go_rows8<BF16, VEC, true>(a, st) : go_rows8<BF16, VEC, false>(a, st);
 }
 
 hipError_t launch_add_rms_norm_int8(const Rows8Args &a, bool bf16, hipStream_t st) {
     if (a.rows <= 0 || a.rows > INT32_MAX || a.H <= 0 || a.H > QASR_ROWS8_MAX_HIDDEN) return hipErrorInvalidValue;
     const uintptr_t ptrs = (uintptr_t)a.x | (uintptr_t)a.res | (uintptr_t)a.sum | (uintptr_t)a.norm_w;
     const bool vec = a.H % 8 == 0 && a.ld % 8 == 0 && ptrs % 16 == 0 && (uintptr_t)a.q % 8 == 0;
-    if (bf16) return vec ? go_rows8<true, true>(a, st) : go_rows8<true, false>(a, st);
-    return vec ? go_rows8<false, true>(a, st) : go_rows8<false, false>(a, st);
+    if (bf16) return vec ? pick_rows8<true, true>(a, st) : pick_rows8<true, false>(a, st);
+    return vec ? pick_rows8<false, true>(a, st) : pick_rows8<false, false>(a, st);
 }
 
 }  // namespace qasr
