@@ -67,23 +67,126 @@ __device__ __forceinline__ void kv8_load16(const void *base, int64_t at, bool ve
     }
 }
 
+// 16 bytes of a row: 8 bf16 or 4 f32 values
+template <bool BF16>
+__device__ __forceinline__ void kv8_load(const void *base, int64_t at, bool vec, float *v) {
+    if (BF16) {
+        const uint16_t *p = reinterpret_cast<const uint16_t *>(base) + at;
+        u16x8 u;
+        if (vec) {
+            u = *reinterpret_cast<const u16x8 *>(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) u[i] = p[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = bf16_to_f32(u[i]);
+    } else {
+        const float *p = reinterpret_cast<const float *>(base) + at;
+        f32x4 u;
+        if (vec) {
+            u = *reinterpret_cast<const f32x4 *>(p);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) u[i] = p[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = u[i];
+    }
+}
+template <bool BF16>
+__device__ __forceinline__ void kv8_store(void *base, int64_t at, bool vec, const float *v) {
+    if (BF16) {
+        uint16_t *p = reinterpret_cast<uint16_t *>(base) + at;
+        u16x8 u;
+#pragma unroll
+        for (int i = 0; i < 8; i++) u[i] = __builtin_bit_cast(uint16_t, (__bf16)v[i]);
+        if (vec) {
+            *reinterpret_cast<u16x8 *>(p) = u;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) p[i] = u[i];
+        }
+    } else {
+        float *p = reinterpret_cast<float *>(base) + at;
+        if (vec) {
+            *reinterpret_cast<f32x4 *>(p) = f32x4{v[0], v[1], v[2], v[3]};
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[i] = v[i];
+        }
+    }
+}
+
 __device__ __forceinline__ bool kv8_finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
-// x at scale s (inv about 1 / s): NaN 0, infinities +-127, everything 0 at scale 0
-__device__ __forceinline__ int kv8_round(float x, double s, double inv) {
-    if (!(fabsf(x) >= 0.0f) || s == 0.0) return 0;
-    const int k = kv8_finite(x) ? round_ratio((double)fabsf(x), s, inv) : 127;
-    return x < 0.0f ? -k : k;
-}
+// A block's scale as its values meet it.  A multiple x / s is formed in f32, off by at
+// most 2^-23 of itself, and decided exactly in f64 where that could matter: within
+// 1e-4 of a half, and at scales whose inverse f32 does not hold well (every value so:
+// 19 us where this takes 11, 8 prompts of 1337 bf16 rows at most).
+struct Kv8Scale {
+    double s, inv;
+    float inv_f;
+    bool tiny;
+    __device__ __forceinline__ explicit Kv8Scale(float sc)
+        : s((double)sc), inv(sc > 0.0f ? 1.0 / (double)sc : 0.0), inv_f((float)inv), tiny(sc < 1e-30f) {}
+    // 4 values' bytes: NaN 0, infinities +-127, everything 0 at scale 0
+    __device__ __forceinline__ uint32_t round4(float x0, float x1, float x2, float x3) const {
+        const float x[4] = {x0, x1, x2, x3};
+        // 1.5 x 2^23: a sum's low byte is the nearest whole number's
+        const float big = 12582912.0f;
+        uint32_t n[4];
+        bool near = tiny;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float u = x[i] * inv_f, t = u + big;
+            n[i] = __float_as_uint(t);
+            near |= !(fabsf(u - (t - big)) <= 0.4999f);          // also what is not finite
+        }
+        if (near) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int k = s == 0.0 || x[i] != x[i] ? 0 : kv8_finite(x[i]) ? round_ratio((double)fabsf(x[i]), s, inv) : 127;
+                n[i] = (uint32_t)(x[i] < 0.0f ? -k : k);
+            }
+        }
+        const uint32_t a = __builtin_amdgcn_perm(n[1], n[0], 0x0c0c0400), b = __builtin_amdgcn_perm(n[3], n[2], 0x04000c0c);
+        return a | b;
+    }
+    // an earlier value q at scale `old`
+    __device__ __forceinline__ int again(int q, double old) const {
+        const int k = round_ratio((double)abs(q) * old, s, inv);
+        return q < 0 ? -k : k;
+    }
+};
+
+// How a block's 64 x HD values meet its 256 threads, in the write and the read: a
+// thread has E consecutive dims (16 bytes of a row) of 4 consecutive positions 4 m ..
+// 4 m + 3, for IT values of m.  A row is LPR lanes wide, so loads and stores cover whole
+// rows; the 4 positions of one dim are one word of V's block.
+template <bool BF16, int HD>
+struct Kv8Map {
+    static constexpr int E = BF16 ? 8 : 4, LPR = HD / E, RG = 256 / LPR, IT = RG < 16 ? 16 / RG : 1;
+    int d, m0;
+    __device__ __forceinline__ Kv8Map(int t) : d(t % LPR * E), m0(t / LPR) {}
+    __device__ __forceinline__ int m(int i) const { return m0 + i * RG; }      // 16 and more: nothing
+    // word of V's [dim][16 words] that holds positions 4 m .. 4 m + 3
+    __device__ __forceinline__ static int word(int m) { return (m & 3) * 4 + (m >> 2); }
+};
+// V's block in LDS: rows of 17 words, for dims that lie LPR lanes apart
+#define KV8_ROW 17
+
+__device__ __forceinline__ uint32_t pack_bytes(const int *q) { return (uint32_t)pack4_i8(q[0], q[1], q[2], q[3]); }
 
 // ---------------------------------------------------------------------------
 // write: one block of 256 threads per (block of the sequence, head, sequence, K or V)
 // ---------------------------------------------------------------------------
 template <bool BF16, int HD>
 __global__ __launch_bounds__(256) void k_kv8_write(Kv8Args a) {
-    constexpr int CH = HD / 16, RP = 256 / CH, IT = 64 / RP;     // 16-value chunks a row, rows a pass, passes
+    typedef Kv8Map<BF16, HD> Map;
+    constexpr int E = Map::E, IT = Map::IT;
     __shared__ float red[4];
-    __shared__ __attribute__((aligned(16))) int8_t tile[HD][64 + 16];
+    __shared__ uint32_t tile[HD * KV8_ROW];
     const int t = threadIdx.x, lane = t & 63, wid = t >> 6;
     const bool is_v = blockIdx.z & 1;
     const int j = blockIdx.z >> 1, h = blockIdx.y;
@@ -97,69 +200,115 @@ __global__ __launch_bounds__(256) void k_kv8_write(Kv8Args a) {
     float *sp = (is_v ? a.vs : a.ks) + blk;
     int8_t *dst = (is_v ? a.v8 : a.k8) + blk * 64 * HD;
     const int keep = lo - b * 64, upto = hi - b * 64;            // positions held before, and behind the new ones
-    const int ch = t % CH, rr = t / CH;
-    float x[IT][16];
+    const Map map(t);
+    float x[IT][4][E];
     float m = 0.0f;
 #pragma unroll
-    for (int i = 0; i < IT; i++) {
-        const int p = i * RP + rr;
-        if (p < keep || p >= upto) continue;
-        kv8_load16<BF16>(src, (sq.r0 + (b * 64 + p - sq.p0)) * a.ld + h * HD + ch * 16, a.vec, x[i]);
+    for (int i = 0; i < IT; i++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) m = kv8_finite(x[i][e]) ? fmaxf(m, fabsf(x[i][e])) : m;
-    }
+        for (int r = 0; r < 4; r++) {
+            const int p = 4 * map.m(i) + r;
+            if (p < keep || p >= upto) continue;                 // upto <= 64: m past 15 has none
+            kv8_load<BF16>(src, (sq.r0 + (b * 64 + p - sq.p0)) * a.ld + h * HD + map.d, a.vec, x[i][r]);
+#pragma unroll
+            for (int e = 0; e < E; e++) m = fmaxf(m, fabsf(x[i][r][e]));     // NaN does not count
+        }
+    const float s_old = keep > 0 ? *sp : 0.0f;
     m = wave_max_f32(m);
     if (lane == 0) red[wid] = m;
-    const float s_old = keep > 0 ? *sp : 0.0f;
     __syncthreads();
     m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    if (!kv8_finite(m)) {                                        // nor do infinities
+        m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < IT; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int p = 4 * map.m(i) + r;
+                if (p < keep || p >= upto) continue;
+#pragma unroll
+                for (int e = 0; e < E; e++) m = kv8_finite(x[i][r][e]) ? fmaxf(m, fabsf(x[i][r][e])) : m;
+            }
+        m = wave_max_f32(m);
+        __syncthreads();
+        if (lane == 0) red[wid] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    }
     const float s = fmaxf(s_old, __fdiv_rn(m, 127.0f));
-    const double sd = (double)s, inv = s > 0.0f ? 1.0 / sd : 0.0, od = (double)s_old;
+    const Kv8Scale sc(s);
     const bool grow = keep > 0 && s > s_old;
-    auto again = [&](int q) {                                    // an earlier value at the raised scale
-        const int k = round_ratio((double)abs(q) * od, sd, inv);
-        return q < 0 ? -k : k;
-    };
+    auto again = [&](int q) { return sc.again(q, (double)s_old); };
     if (t == 0) *sp = s;
     if (!is_v) {
 #pragma unroll
-        for (int i = 0; i < IT; i++) {
-            const int p = i * RP + rr;
-            i32x4 *o = reinterpret_cast<i32x4 *>(dst + p * HD + ch * 16);
-            if (p >= keep && p < upto) {
-                int q[16];
+        for (int i = 0; i < IT; i++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) q[e] = kv8_round(x[i][e], sd, inv);
-                *o = i32x4{pack4_i8(q[0], q[1], q[2], q[3]), pack4_i8(q[4], q[5], q[6], q[7]),
-                           pack4_i8(q[8], q[9], q[10], q[11]), pack4_i8(q[12], q[13], q[14], q[15])};
-            } else if (p < keep && grow) {
-                i32x4 v = *o;
+            for (int r = 0; r < 4; r++) {
+                const int p = 4 * map.m(i) + r;
+                uint32_t *o = reinterpret_cast<uint32_t *>(dst + p * HD + map.d);
+                if (p >= keep && p < upto) {
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    v[e] = pack4_i8(again((int8_t)v[e]), again((int8_t)(v[e] >> 8)), again((int8_t)(v[e] >> 16)), again(v[e] >> 24));
-                *o = v;
+                    for (int w = 0; w < E / 4; w++)
+                        o[w] = sc.round4(x[i][r][4 * w], x[i][r][4 * w + 1], x[i][r][4 * w + 2], x[i][r][4 * w + 3]);
+                } else if (p < keep && grow) {
+#pragma unroll
+                    for (int w = 0; w < E / 4; w++) {
+                        const int v = (int)o[w], q[4] = {again((int8_t)v), again((int8_t)(v >> 8)), again((int8_t)(v >> 16)), again(v >> 24)};
+                        o[w] = pack_bytes(q);
+                    }
+                }
             }
-        }
         return;
     }
-    // V: the stored block goes through LDS, where rows become bytes of a dim
-    if (keep > 0 || upto < 64) {
-        for (int i = t; i < HD * 4; i += 256) *reinterpret_cast<i32x4 *>(&tile[i >> 2][16 * (i & 3)]) = reinterpret_cast<const i32x4 *>(dst)[i];
+    // V.  A few positions into a block that stays at its scale: their bytes alone
+    if (!grow && upto - keep <= 4) {
+#pragma unroll
+        for (int i = 0; i < IT; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int p = 4 * map.m(i) + r;
+                if (p < keep || p >= upto) continue;
+#pragma unroll
+                for (int w = 0; w < E / 4; w++) {
+                    const uint32_t q = sc.round4(x[i][r][4 * w], x[i][r][4 * w + 1], x[i][r][4 * w + 2], x[i][r][4 * w + 3]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) dst[(map.d + 4 * w + e) * 64 + kv8_slot(p)] = (int8_t)(q >> (8 * e));
+                }
+            }
+        return;
+    }
+    // else the stored block through LDS, where rows become words of a dim
+    const bool part = keep > 0 || upto < 64;
+    if (part) {
+        for (int i = t; i < HD * 16; i += 256) tile[(i >> 4) * KV8_ROW + (i & 15)] = reinterpret_cast<const uint32_t *>(dst)[i];
         __syncthreads();
     }
 #pragma unroll
     for (int i = 0; i < IT; i++) {
-        const int p = i * RP + rr, sl = kv8_slot(p);
-        if (p >= keep && p < upto) {
+        const int mm = map.m(i);
+        if (mm >= 16 || 4 * mm >= upto || (!grow && 4 * mm + 3 < keep)) continue;
 #pragma unroll
-            for (int e = 0; e < 16; e++) tile[ch * 16 + e][sl] = (int8_t)kv8_round(x[i][e], sd, inv);
-        } else if (p < keep && grow) {
+        for (int e = 0; e < E; e++) {
+            uint32_t *w = &tile[(map.d + e) * KV8_ROW + Map::word(mm)];
+            if (4 * mm >= keep && 4 * mm + 3 < upto) {           // all new
+                *w = sc.round4(x[i][0][e], x[i][1][e], x[i][2][e], x[i][3][e]);
+                continue;
+            }
+            const int v = (int)*w;                               // a whole block has none of these
+            int q[4];
 #pragma unroll
-            for (int e = 0; e < 16; e++) tile[ch * 16 + e][sl] = (int8_t)again(tile[ch * 16 + e][sl]);
+            for (int r = 0; r < 4; r++) {
+                const int p = 4 * mm + r, was = (int8_t)(v >> (8 * r));
+                if (p >= upto) q[r] = was;
+                else if (p >= keep) q[r] = (int8_t)sc.round4(x[i][r][e], 0.0f, 0.0f, 0.0f);
+                else q[r] = grow ? again(was) : was;
+            }
+            *w = pack_bytes(q);
         }
     }
     __syncthreads();
-    for (int i = t; i < HD * 4; i += 256) reinterpret_cast<i32x4 *>(dst)[i] = *reinterpret_cast<const i32x4 *>(&tile[i >> 2][16 * (i & 3)]);
+    for (int i = t; i < HD * 16; i += 256) reinterpret_cast<uint32_t *>(dst)[i] = tile[(i >> 4) * KV8_ROW + (i & 15)];
 }
 
 template <bool BF16>
@@ -190,8 +339,9 @@ hipError_t launch_kv8_write(const Kv8Args &a0, bool bf16, hipStream_t st) {
 // ---------------------------------------------------------------------------
 template <bool BF16, int HD>
 __global__ __launch_bounds__(256) void k_kv8_read(Kv8Args a) {
-    constexpr int CH = HD / 16, RP = 256 / CH, IT = 64 / RP;
-    __shared__ __attribute__((aligned(16))) int8_t tile[HD][64 + 16];
+    typedef Kv8Map<BF16, HD> Map;
+    constexpr int E = Map::E, IT = Map::IT;
+    __shared__ uint32_t tile[HD * KV8_ROW];
     const int t = threadIdx.x;
     const bool is_v = blockIdx.z & 1;
     const int j = blockIdx.z >> 1, h = blockIdx.y;
@@ -203,47 +353,42 @@ __global__ __launch_bounds__(256) void k_kv8_read(Kv8Args a) {
     const int64_t head = (int64_t)j * a.Hkv + h, blk = head * (a.cap / 64) + b;
     const int8_t *src = (is_v ? a.v8 : a.k8) + blk * 64 * HD;
     const float s = is_v ? a.vs[blk] : a.ks[blk];
+    const Map map(t);
+    uint32_t k8[IT][4][E / 4];
     if (is_v) {
-        for (int i = t; i < HD * 4; i += 256) *reinterpret_cast<i32x4 *>(&tile[i >> 2][16 * (i & 3)]) = reinterpret_cast<const i32x4 *>(src)[i];
+        for (int i = t; i < HD * 16; i += 256) tile[(i >> 4) * KV8_ROW + (i & 15)] = reinterpret_cast<const uint32_t *>(src)[i];
         __syncthreads();
+    } else {
+#pragma unroll
+        for (int i = 0; i < IT; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int p = 4 * map.m(i) + r;
+                if (p < lo || p >= hi) continue;
+#pragma unroll
+                for (int w = 0; w < E / 4; w++) k8[i][r][w] = reinterpret_cast<const uint32_t *>(src + p * HD + map.d)[w];
+            }
     }
-    const int ch = t % CH, rr = t / CH;
 #pragma unroll
     for (int i = 0; i < IT; i++) {
-        const int p = i * RP + rr;
-        if (p < lo || p >= hi) continue;
-        float x[16];
+        const int mm = map.m(i);
+        if (mm >= 16 || 4 * mm >= hi || 4 * mm + 3 < lo) continue;
+        uint32_t v8[E];
         if (is_v) {
-            const int sl = kv8_slot(p);
 #pragma unroll
-            for (int e = 0; e < 16; e++) x[e] = __fmul_rn((float)tile[ch * 16 + e][sl], s);
-        } else {
-            const i32x4 v = *reinterpret_cast<const i32x4 *>(src + p * HD + ch * 16);
-#pragma unroll
-            for (int e = 0; e < 16; e++) x[e] = __fmul_rn((float)(int8_t)(v[e >> 2] >> (8 * (e & 3))), s);
+            for (int e = 0; e < E; e++) v8[e] = tile[(map.d + e) * KV8_ROW + Map::word(mm)];
         }
-        const int64_t at = (sq.r0 + (b * 64 + p - sq.p0)) * a.ld + h * HD + ch * 16;
-        if (BF16) {
-            uint16_t *o = reinterpret_cast<uint16_t *>(is_v ? a.v : a.k) + at;
-            u16x8 u[2];
 #pragma unroll
-            for (int e = 0; e < 16; e++) u[e >> 3][e & 7] = __builtin_bit_cast(uint16_t, (__bf16)x[e]);
-            if (a.vec) {
-                reinterpret_cast<u16x8 *>(o)[0] = u[0];
-                reinterpret_cast<u16x8 *>(o)[1] = u[1];
-            } else {
+        for (int r = 0; r < 4; r++) {
+            const int p = 4 * mm + r;
+            if (p < lo || p >= hi) continue;
+            float x[E];
 #pragma unroll
-                for (int e = 0; e < 16; e++) o[e] = u[e >> 3][e & 7];
+            for (int e = 0; e < E; e++) {
+                const int q = is_v ? (int8_t)(v8[e] >> (8 * r)) : (int8_t)(k8[i][r][e >> 2] >> (8 * (e & 3)));
+                x[e] = __fmul_rn((float)q, s);
             }
-        } else {
-            float *o = reinterpret_cast<float *>(is_v ? a.v : a.k) + at;
-            if (a.vec) {
-#pragma unroll
-                for (int c = 0; c < 4; c++) reinterpret_cast<f32x4 *>(o)[c] = f32x4{x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; e++) o[e] = x[e];
-            }
+            kv8_store<BF16>(is_v ? a.v : a.k, (sq.r0 + (b * 64 + p - sq.p0)) * a.ld + h * HD + map.d, a.vec, x);
         }
     }
 }
