@@ -194,7 +194,7 @@ int qasr_hip_bidirectional_attention(qasr_hip *h, float *out, const float *q, co
  * are quantized as they are (eps unused).  sum (nullable) receives s; it may be x
  * or res itself.  Sums and rounding decisions are formed in f64 from the sum
  * before it is rounded to its type.  A row that holds a value that is not finite
- * gets q = 0 and a NaN scale.  hidden <= 16384. */
+ * gets q = 0 and a NaN scale.  hidden <= 16384, rows < 2^22. */
 int qasr_hip_add_rms_norm_int8(qasr_hip *h, int8_t *q, float *scales, void *sum, const void *x, const void *res,
                                const float *norm_w, int64_t rows, int64_t hidden, int64_t ld, float eps, int bf16);
 /* y[m, n] = (sum_k a[m, k] w[n, k]) * a_scales[m] * w_scales[n] (+ bias[n],

@@ -15,7 +15,7 @@ extern "C" int qasr_hip_add_rms_norm_int8(qasr_hip *h, int8_t *q, float *scales,
                                           float eps, int bf16) {
     if (!q || !scales || !x) return bad("add_rms_norm_int8: null pointer");
     if (hidden <= 0 || hidden > QASR_ROWS8_MAX_HIDDEN) return bad("add_rms_norm_int8: hidden must be in [1, 16384]");
-    if (rows < 0 || rows > INT32_MAX || ld < hidden || ld > INT32_MAX)
+    if (rows < 0 || rows >= (1 << 22) || ld < hidden || ld > INT32_MAX)
         return bad("add_rms_norm_int8: rows or row stride out of range");
     if (!(eps >= 0.0f)) return bad("add_rms_norm_int8: eps must not be negative");
     CHECK_H(h);

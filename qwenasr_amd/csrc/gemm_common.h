@@ -20,7 +20,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 //   - wait_vmcnt<N> here is right where at least N loads of the wave are younger
 //     than the ones it waits for.  k_gemm_lds and k_gemm_ring: the loads of the
 //     NS - 2 stages behind (their other loads come before the first stage or
-//     after the last wait).  k_gemm_ks: N = 0.  k_attn_mfma and k_attn_bf3: the
+//     after the last wait).  k_gemm_ks, k_gemm8, k_attn_kv8: N = 0.  k_attn_mfma and k_attn_bf3: the
 //     L loads of the next K tile or of the V tile; q is loaded behind the first
 //     two tiles and waited for ahead of the loop.
 // The compiler makes no use of M0 in the kernels of the files that include this

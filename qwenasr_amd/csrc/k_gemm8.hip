@@ -131,21 +131,27 @@ __global__ __launch_bounds__(256) void k_gemm8_any(Gemm8Args g) {
     }
 }
 
-// The fast form: BM x BN tiles fed by direct global -> LDS loads through rings of NS
-// stages, so NS - 1 K-steps of BK bytes are in flight while one is multiplied.  KP
-// groups of WM x WN waves each take every KP-th K-step through a ring of their own
-// and add up in LDS at the end (int32: exact in any order): a short grid or few rows
-// leave a CU few waves otherwise, and a long chain of K-steps for each.
+// The fast form: BM x BN tiles fed by direct global -> LDS loads through rings of two
+// stages of BK = 128 bytes of K, one in flight while one is multiplied.  KP groups of
+// WM x WN waves each take every KP-th K-step through a ring of their own and add up in
+// LDS at the end (int32: exact in any order): a short grid or few rows leave a CU few
+// waves otherwise, and a long chain of K-steps for each.
 //
-// A stage holds the tile's activation rows, then its weight rows, BK bytes each, in
-// 16-byte slots; slot q of row r stands at q ^ lds_swz(r).  A load fills 64 slots in lane order.  K-steps
-// past the end load zeros, so every wait counts the same.  Needs K % 16 == 0 and
-// 16-byte aligned operands.
+// What bounds it is the way from the caches into LDS.  Such loads, with nothing else
+// running, bring 34 TB/s when a row gives 128 bytes and lies in the XCD's L2, 20 when it
+// gives 64, 7-8 when it comes from the cache behind the L2s (375 x 151936 x 1024, 192 x
+// 128 tiles: 142 us with 64-byte steps and three stages, 109 with these; more stages or
+// larger tiles leave too few waves on a CU).  Hence also the order of the tiles, below.
+//
+// A stage holds the tile's activation rows, then its weight rows, in 16-byte slots;
+// slot q of row r stands at q ^ lds_swz(r).  A load fills 64 slots in lane order.
+// K-steps past the end load zeros, so every wait counts the same.  Needs K % 16 == 0
+// and 16-byte aligned operands.
 __device__ __attribute__((aligned(256))) int4 g_gemm8_zero16[16];
 
-template <int MODE, typename YT, int BM, int BN, int WM, int WN, int KP, int BK, int NS>
+template <int MODE, typename YT, int BM, int BN, int WM, int WN, int KP>
 __global__ __launch_bounds__(64 * WM * WN * KP, WM * WN * KP > 8 ? 4 : 2) void k_gemm8(Gemm8Args g, int vec) {
-    constexpr int W = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, RPL = 1024 / BK, SPR = BK / 16;
+    constexpr int BK = 128, NS = 2, W = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, RPL = 1024 / BK, SPR = BK / 16;
     constexpr int LA = BM / RPL / W, LB = BN / RPL / W, STG = (BM + BN) * BK;
     static_assert(BM % (RPL * W) == 0 && BN % (RPL * W) == 0 && BM % (16 * WM) == 0 && BN % (16 * WN) == 0, "tile");
     // after the K loop: the groups' partial sums, then 16 rows of each wave's results
@@ -296,12 +302,12 @@ __global__ __launch_bounds__(64 * WM * WN * KP, WM * WN * KP > 8 ? 4 : 2) void k
     }
 }
 
-template <int MODE, typename YT, int BM, int BN, int WM, int WN, int KP, int BK, int NS>
+template <int MODE, typename YT, int BM, int BN, int WM, int WN, int KP>
 static hipError_t go_gemm8_tile(const Gemm8Args &g, int vec, hipStream_t st) {
     const int64_t gx = (g.N + BN - 1) / BN, gy = (g.M + BM - 1) / BM;
     const int64_t blocks = (gx + 7) / 8 * 8 * gy;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_gemm8<MODE, YT, BM, BN, WM, WN, KP, BK, NS>), dim3((unsigned)blocks), dim3(64 * WM * WN * KP), 0, st, g, vec);
+    if (blocks * 64 * WM * WN * KP > UINT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_gemm8<MODE, YT, BM, BN, WM, WN, KP>), dim3((unsigned)blocks), dim3(64 * WM * WN * KP), 0, st, g, vec);
     return hipGetLastError();
 }
 
@@ -313,37 +319,33 @@ static hipError_t go_gemm8(const Gemm8Args &g, hipStream_t st) {
     if (vec_k) {
         // The form with the least estimated time: ns for the first round of tiles over the 256
         // CUs (fixed, and for each 64 of K), and for each further round, halfway between the
-        // whole and the fractional count of rounds, as several blocks share a CU.  Fits to 115
-        // shapes, M 1 ... 2000, N 512 ... 151936, K 320 ... 6144; the choice is 3% behind the best
-        // of ten forms there on average and 27% at worst (1337 x 5000 x 4096).  us, in the order
-        // of the list: 1 x 4096 x 1024 5.1, 5.5, 7.7, 11.2, 10.4; 404 x 4096 x 1024 16.7, 8.9,
-        // 8.8, 12.6, 13.0; 1337 x 12288 x 2048 173, 80, 62, 61, 60; 375 x 151936 x 1024 -, 214,
-        // 153, 120, 126.
-        static const struct { int bm, bn, one, one_k, more, more_k; } f[] = {
-                                   {32, 64, 3795, 94, 2415, 114},
-                                   {64, 64, 3603, 135, 1858, 92},
-                                   {64, 128, 4460, 248, 2331, 131},
-                                   {128, 128, 5557, 397, 2960, 289},
-                                   {128, 128, 5806, 344, 3262, 292}};
+        // whole and the fractional count of rounds, as several blocks share a CU.  Fits to 215
+        // shapes, M 1 ... 2000, N 512 ... 151936, K 320 ... 6144; the choice is 2% behind the best
+        // of seven forms there on average and 22% at worst (1337 x 4096 x 320).  us, in the order
+        // of the list: 1 x 4096 x 1024 5.0, 5.4, 7.9, 13.1; 404 x 4096 x 1024 16.9, 8.8, 10.1,
+        // 14.2; 1337 x 12288 x 2048 173, 78, 57, 54; 375 x 151936 x 1024 484, 215, 121, 110.
+        static const struct { int bm, bn, one, one_k, more, more_k; } f[] = {{32, 64, 3877, 98, 2461, 118},
+                                                                             {64, 64, 3743, 142, 1930, 92},
+                                                                             {128, 128, 4472, 319, 3526, 253},
+                                                                             {192, 128, 6957, 458, 5072, 298}};
         const int64_t nk = (g.K + 63) / 64;
         int best = 0;
         int64_t best_ns = INT64_MAX;
-        for (int i = 0; i < 5; i++) {
+        for (int i = 0; i < 4; i++) {
             const int64_t tiles = (g.M + f[i].bm - 1) / f[i].bm * ((g.N + f[i].bn - 1) / f[i].bn), rounds = (tiles + 255) / 256;
             const int64_t over = rounds > 1 ? tiles + 256 * rounds - 512 : 0;         // further rounds, in 1 / 512
             const int64_t ns = f[i].one + f[i].one_k * nk + over * (f[i].more + f[i].more_k * nk) / 512;
             if (ns < best_ns) { best_ns = ns; best = i; }
         }
         switch (best) {
-            case 0: return go_gemm8_tile<MODE, YT, 32, 64, 1, 2, 4, 128, 2>(g, vec, st);
-            case 1: return go_gemm8_tile<MODE, YT, 64, 64, 2, 2, 2, 128, 2>(g, vec, st);
-            case 2: return go_gemm8_tile<MODE, YT, 64, 128, 1, 4, 1, 128, 2>(g, vec, st);
-            case 3: return go_gemm8_tile<MODE, YT, 128, 128, 2, 2, 1, 64, 3>(g, vec, st);
-            default: return go_gemm8_tile<MODE, YT, 128, 128, 2, 2, 1, 128, 2>(g, vec, st);
+            case 0: return go_gemm8_tile<MODE, YT, 32, 64, 1, 2, 4>(g, vec, st);
+            case 1: return go_gemm8_tile<MODE, YT, 64, 64, 2, 2, 2>(g, vec, st);
+            case 2: return go_gemm8_tile<MODE, YT, 128, 128, 2, 4, 1>(g, vec, st);
+            default: return go_gemm8_tile<MODE, YT, 192, 128, 2, 2, 1>(g, vec, st);
         }
     }
     const int64_t gx = (g.N + 63) / 64, gy = (g.M + 63) / 64;
-    if (gx * gy > INT32_MAX) return hipErrorInvalidValue;
+    if (gx * gy * 256 > UINT32_MAX) return hipErrorInvalidValue;
     hipLaunchKernelGGL((k_gemm8_any<MODE, YT>), dim3((unsigned)(gx * gy)), dim3(256), 0, st, g);
     return hipGetLastError();
 }

@@ -887,7 +887,7 @@ static hipError_t pick_attn_kv8(AttnKv8Args &a, bool bf16, int splits, hipStream
     // the splits' parts fit the scratch area
     int64_t s = std::min<int64_t>(splits, (int64_t)QASR_KV8_PART_BYTES / (units * (32 + 16 * a.c.hd) * 4));
     s = std::max<int64_t>(1, std::min<int64_t>(s, 64));
-    if (tiles * s * a.c.Hkv > INT32_MAX) return hipErrorInvalidValue;
+    if (tiles * s * a.c.Hkv * 64 * CG * PG > UINT32_MAX || tiles * CG * 256 > UINT32_MAX) return hipErrorInvalidValue;   // the grid's limit
     a.tiles = (int)tiles;
     a.splits = (int)s;
     if (bf16) return a.c.hd == 128 ? go_attn_kv8<true, 128, CG, PG, SHARED>(a, st) : go_attn_kv8<true, 64, CG, PG, SHARED>(a, st);

@@ -194,7 +194,7 @@ static hipError_t pick_rows8(const Rows8Args &a, hipStream_t st) {
 }
 
 hipError_t launch_add_rms_norm_int8(const Rows8Args &a, bool bf16, hipStream_t st) {
-    if (a.rows <= 0 || a.rows > INT32_MAX || a.H <= 0 || a.H > QASR_ROWS8_MAX_HIDDEN) return hipErrorInvalidValue;
+    if (a.rows <= 0 || a.rows >= (1 << 22) || a.H <= 0 || a.H > QASR_ROWS8_MAX_HIDDEN) return hipErrorInvalidValue;
     const uintptr_t ptrs = (uintptr_t)a.x | (uintptr_t)a.res | (uintptr_t)a.sum | (uintptr_t)a.norm_w;
     const bool vec = a.H % 8 == 0 && a.ld % 8 == 0 && ptrs % 16 == 0 && (uintptr_t)a.q % 8 == 0;
     if (bf16) return vec ? pick_rows8<true, true>(a, st) : pick_rows8<true, false>(a, st);
