@@ -230,8 +230,9 @@ int qasr_hip_gemm_w8a8(qasr_hip *h, void *y, const int8_t *a, const float *a_sca
  * them lose their meaning.  A block's scale is max|value| / 127 over its finite
  * values; where a block holds earlier positions of the sequence, their scale is
  * kept, or raised to the new values' and the earlier positions rounded again at
- * the new scale (at most half a new step each time it rises).  NaN is stored as
- * 0, infinities as +-127. */
+ * the new scale (at most half a new step each time it rises): rows that begin
+ * inside a block nothing was written to need its scales to be 0 there.  NaN is
+ * stored as 0, infinities as +-127. */
 int qasr_hip_kv8_write(qasr_hip *h, int8_t *k8, int8_t *v8, float *k_scales, float *v_scales, const void *k,
                        const void *v, int64_t ld, const int32_t *row_start, const int32_t *pos, int64_t n_rows,
                        int64_t n_seq, int64_t max_rows, int64_t n_kv_heads, int64_t head_dim, int64_t capacity,
@@ -250,7 +251,9 @@ int qasr_hip_kv8_read(qasr_hip *h, void *k, void *v, int64_t ld, const int8_t *k
  * > 0 only the last window of those and the first sinks.  A row that sees nothing
  * gives zeros; rows behind the last sequence are left as they were.  max_len (0:
  * capacity): about the longest pos + rows, by which the work is split; results do
- * not depend on it beyond f32 rounding.  Uses the handle's scratch area. */
+ * not depend on it beyond f32 rounding.  Uses the handle's scratch area, and so
+ * does a graph that holds the call: launch it on the handle's stream, or in
+ * order with that stream's work. */
 int qasr_hip_attention_kv8(qasr_hip *h, void *out, const void *q, int64_t ldq, const int8_t *k8, const int8_t *v8,
                            const float *k_scales, const float *v_scales, const int32_t *row_start, const int32_t *pos,
                            int64_t n_rows, int64_t n_seq, int64_t max_rows, int64_t max_len, int64_t n_heads,

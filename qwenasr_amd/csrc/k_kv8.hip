@@ -122,8 +122,9 @@ __device__ __forceinline__ bool kv8_finite(float x) { return fabsf(x) <= 3.40282
 
 // A block's scale as its values meet it.  A multiple x / s is formed in f32, off by at
 // most 2^-23 of itself, and decided exactly in f64 where that could matter: within
-// 1e-4 of a half, and at scales whose inverse f32 does not hold well (every value so:
-// 19 us where this takes 11, 8 prompts of 1337 bf16 rows at most).
+// 1e-4 of a half, and at scales whose inverse f32 does not hold well.  (The write of 8
+// ragged prompts of up to 1337 bf16 rows, 8 heads of 128: 15 - 17 us, 17 - 20 with every
+// value decided in f64.)
 struct Kv8Scale {
     double s, inv;
     float inv_f;
@@ -505,7 +506,7 @@ __global__ __launch_bounds__(64 * CG * PG, SHARED ? 4 : 2) void k_attn_kv8(AttnK
     constexpr int KS = HD / 64, DT = HD / 16, D = BF16 ? 2 : 3, TB = 64 * HD, LD = HD / 8 / CG;   // bytes of a block; a wave's loads of K and V
     constexpr float N = BF16 ? 32000.0f : 8.0e6f;
     static_assert(SHARED || CG == 1, "waves that share a block's positions share its bytes in LDS");
-    constexpr int MERGE = PG > 1 ? CG * PG * 16 * (HD + 4) * 4 : 16, SLOTS = SHARED ? PG * 2 * TB : 0;
+    constexpr int MERGE = CG * PG * 16 * (HD + 4) * 4, SLOTS = SHARED ? PG * 2 * TB : 0;
     __shared__ __attribute__((aligned(16))) char smem[MERGE > SLOTS ? MERGE : SLOTS];
     __shared__ float ml_l[CG * PG][2][16];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -778,16 +779,6 @@ __global__ __launch_bounds__(64 * CG * PG, SHARED ? 4 : 2) void k_attn_kv8(AttnK
 
     const int cols = f0 < n_flat ? (int)min(16u, n_flat - f0) : 0;
     float *part = a.part + ((((int64_t)j * a.c.Hkv + h) * a.tiles * CG + tile) * S + split) * kv8_part<HD>;
-    if constexpr (PG == 1) {
-        if (c >= cols) return;
-        if (S > 1 && g == 0) { part[c] = m; part[16 + c] = l; }
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++) {
-            if (S > 1) *reinterpret_cast<f32x4 *>(part + 32 + c * HD + 16 * dt + 4 * g) = o[dt];
-            else kv8_put<BF16, HD>(a, sq, h, f0 + c, 16 * dt + 4 * g, o[dt], l);
-        }
-        return;
-    }
     // the groups' parts of each tile, through the ring's LDS (every load into it has landed and been read)
     float (*o_l)[16][HD + 4] = reinterpret_cast<float (*)[16][HD + 4]>(smem);
     __syncthreads();

@@ -190,7 +190,9 @@ static hipError_t go_rows8(const Rows8Args &a, hipStream_t st) {
 
 template <bool BF16, bool VEC>
 static hipError_t pick_rows8(const Rows8Args &a, hipStream_t st) {
-    return a.rows * a.H >= (1 << 23) ? go_rows8<BF16, VEC, true>(a, st) : go_rows8<BF16, VEC, false>(a, st);
+    if constexpr (VEC)
+        if (a.rows * a.H >= (1 << 23)) return go_rows8<BF16, VEC, true>(a, st);
+    return go_rows8<BF16, VEC, false>(a, st);
 }
 
 hipError_t launch_add_rms_norm_int8(const Rows8Args &a, bool bf16, hipStream_t st) {

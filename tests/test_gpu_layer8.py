@@ -34,7 +34,8 @@ def values(d, is_bf16):
 # rows, hidden, padding of the row stride, residual, norm
 ROWS = [(1, 1024, 0, True, True), (3, 1, 0, True, True), (5, 7, 2, True, True), (2, 63, 0, False, True), (33, 1000, 24, True, True),
         (4, 2048, 8, False, False), (1, 2049, 0, True, True), (2, 4096, 0, True, True), (3, 8192, 0, True, True), (2, 8200, 1, True, False),
-        (2, 16384, 0, True, True), (301, 1024, 0, True, True), (700, 136, 0, True, True)]
+        (2, 16384, 0, True, True), (301, 1024, 0, True, True), (700, 136, 0, True, True),
+        (4100, 2048, 0, True, True), (4193, 2001, 0, False, True), (513, 16384, 8, True, False)]        # and from 2^23 values on
 
 
 @pytest.mark.parametrize("is_bf16", [False, True])
@@ -168,6 +169,16 @@ def test_gemm(dev, M, N, Kd, mode, with_bias, is_bf16):
     acc, _ = ref8.gemm8(a, sa, w, sw)
     check_gemm(got[:M], acc, sa, sw, None if bias is None else bias.astype(np.float64), was[:M], mode, is_bf16)
     assert (got[M] == was[M]).all()                           # nothing past the last row
+
+
+# what the larger tiles are chosen for: edges inside a tile, rows of y of every alignment, K-steps that end inside 128
+LARGE = [(1500, 4102, 336), (900, 5004, 2000), (1337, 6001, 80), (641, 12290, 464), (1153, 4100, 1104), (1700, 4999, 1040)]
+
+
+@pytest.mark.parametrize("mode,with_bias,is_bf16", [("plain", True, False), ("add", True, True), ("swiglu", True, True)])
+@pytest.mark.parametrize("M,N,Kd", LARGE)
+def test_gemm_large(dev, M, N, Kd, mode, with_bias, is_bf16):
+    test_gemm(dev, M, N, Kd, mode, with_bias, is_bf16)
 
 
 @pytest.mark.parametrize("off_a,off_w", [(1, 0), (0, 1), (4, 8), (15, 15)])
@@ -436,6 +447,69 @@ def test_attention_not_finite(dev):
     assert (got[keep] == want[keep]).all()
 
 
+def test_rows_past_max_rows(dev):
+    """A sequence's rows past max_rows are left out: of the cache, of what is read back and of the attention's output."""
+    from qwenasr_amd import kernels as K
+    r = rng(16)
+    heads, dim, cap, counts, most = 2, 64, 128, [5, 2, 40], 3
+    start, n, total = prefix(counts), len(counts), sum(counts)
+    ref = ref8.Cache(n, heads, cap, dim).fill(r)
+    d = DevCache(dev, ref)
+    dpos, dstart = dev.upload(np.array([60, 0, 7], np.int32)), dev.upload(start)
+    rows, q = r.normal(0, 1, (total, heads * dim)), r.normal(0, 1, (total, 4 * dim))
+    dr, back = up(dev, rows, False), up(dev, np.full(rows.shape, 3.0), False)
+    out = up(dev, np.full((total, 4 * dim), 3.0), False)
+    K.kv8_write(*d.buf, dr, dr, dpos, total, n, most, *d.geometry(), row_start=dstart)
+    K.kv8_read(back, dev.zeros(rows.shape, np.float32), *d.buf, dpos, total, n, most, *d.geometry(), row_start=dstart)
+    K.attention_kv8(out, up(dev, q, False), *d.buf, dpos, total, n, most, 4, heads, dim, cap, dim ** -0.5, row_start=dstart)
+    keep = [min(c, most) for c in counts]
+    for j in range(n):
+        x = held(rows, False)[start[j]:start[j] + keep[j]].reshape(-1, heads, dim)
+        ref.write(j, [60, 0, 7][j], {"k": x, "v": x})
+    d.check()
+    taken = np.concatenate([np.arange(start[j], start[j] + keep[j]) for j in range(n)])
+    left = np.setdiff1d(np.arange(total), taken)
+    assert (back.numpy()[left] == 3.0).all() and (out.numpy()[left] == 3.0).all() and (back.numpy()[taken] != 3.0).all()
+    check_attention(values(out, False)[taken].reshape(-1, 4, dim), ref, held(q, False)[taken].reshape(-1, 4, dim), keep, [60, 0, 7])
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows", [2, 40])
+def test_long_cache(dev, rows, is_bf16):
+    """Positions whose bytes lie past 2^31 in the cache: with a window, the bits of a short cache that holds the same
+    positions; without, against the formula (positions never written have scale 0: their scores and values are 0)."""
+    from qwenasr_amd import kernels as K
+    r = rng(17 + rows)
+    n, heads, group, dim, cap, short, pos = 3, 8, 2, 128, 1 << 20, 512, 400
+    hq, base, total = heads * group, cap - short, n * rows
+    k, v = r.normal(0, 1, (n * (pos + rows), heads * dim)), r.normal(0, 1, (n * (pos + rows), heads * dim))
+    q = up(dev, r.normal(0, 1, (total, hq * dim)), is_bf16)
+    dk, dv = up(dev, k, False), up(dev, v, False)
+    out = {}
+    for name, c, b in (("short", short, 0), ("long", cap, base)):
+        buf = [dev.zeros((n, heads, c, dim), np.int8), dev.zeros((n, heads, c // 64, dim, 64), np.int8),
+               dev.zeros((n, heads, c // 64), np.float32), dev.zeros((n, heads, c // 64), np.float32)]
+        K.kv8_write(*buf, dk, dv, dev.upload(np.full(n, b, np.int32)), len(k), n, pos + rows, heads, dim, c)
+        back = [dev.zeros((len(k), heads * dim), np.float32) for _ in range(2)]
+        K.kv8_read(*back, *buf, dev.upload(np.full(n, b, np.int32)), len(k), n, pos + rows, heads, dim, c)
+        o, dp = up(dev, np.zeros((total, hq * dim)), is_bf16), dev.upload(np.full(n, b + pos, np.int32))
+        K.attention_kv8(o, q, *buf, dp, total, n, rows, hq, heads, dim, c, dim ** -0.5, window=200, bf16=is_bf16)
+        out[name] = [o.numpy()] + [a.numpy() for a in back]
+        if name == "long":
+            K.attention_kv8(o, q, *buf, dp, total, n, rows, hq, heads, dim, c, dim ** -0.5, bf16=is_bf16)
+            full = values(o, is_bf16).reshape(n, rows, hq, dim)
+    assert all((a == b).all() for a, b in zip(out["short"], out["long"]))
+    back_k, back_v = (a.astype(np.float64).reshape(n, pos + rows, heads, dim) for a in out["long"][1:])
+    qh = values(q, is_bf16).reshape(n, rows, hq, dim)
+    for j, i, h in ((2, 0, 15), (2, rows - 1, 14), (1, 1, 0)):
+        kk, vv = np.zeros((1, cap, dim)), np.zeros((1, cap, dim))
+        kk[0, base:base + pos + rows], vv[0, base:base + pos + rows] = back_k[j, :, h // group], back_v[j, :, h // group]
+        want, err = ref8.attend(qh[j, i:i + 1, h:h + 1], kk, vv, base + pos + i, dim ** -0.5, 0, 0, 32000.0 if is_bf16 else 8.0e6)
+        # back_k and back_v are the cache's values rounded once to f32
+        err = err + (BF16 if is_bf16 else F32) * (np.abs(want) + err) + 2 * F32 * np.abs(vv).max()
+        assert (np.abs(full[j, i, h] - want[0, 0]) <= err[0, 0]).all()
+
+
 def test_attention_uniform_rows(dev):
     """row_start None: max_rows rows a sequence, the same bits as with it."""
     from qwenasr_amd import kernels as K
@@ -572,6 +646,53 @@ def test_captured(dev):
     finally:
         hip.hipGraphExecDestroy(exe)
         hip.hipGraphDestroy(graph)
+
+
+@pytest.mark.parametrize("rows", [1, 20])
+def test_two_handles(dev, rows):
+    """Calls in turn on two handles, nothing waited for in between, and a graph of one of them: each handle splits the
+    positions through its own scratch area, so every result is that of the call alone."""
+    from qwenasr_amd import Device
+    from qwenasr_amd import kernels as K
+    from qwenasr_amd._lib import lib
+    hip = C.CDLL("libamdhip64.so.7")     # the HIP runtime the library already loaded
+    r = rng(23 + rows)
+    heads, group, dim, cap = 2, 2, 128, 4096
+    hq, other, sides = heads * group, Device(0), []
+    try:
+        for side in (dev, other):
+            d = DevCache(side, ref8.Cache(1, heads, cap, dim).fill(r))
+            q, pos = up(side, r.normal(0, 1, (rows, hq * dim)), False), side.upload(np.array([cap - rows], np.int32))
+            outs = [side.zeros((rows, hq * dim), np.float32) for _ in range(6)]
+
+            def run(o, d=d, q=q, pos=pos):
+                K.attention_kv8(o, q, *d.buf, pos, rows, 1, rows, hq, heads, dim, cap, dim ** -0.5)
+            run(outs[0])
+            sides.append((run, outs, outs[0].numpy()))
+        stream = C.c_void_p(lib().qasr_hip_stream(dev.h))
+        graph, exe = C.c_void_p(), C.c_void_p()
+        captured = dev.zeros((rows, hq * dim), np.float32)
+        assert hip.hipStreamBeginCapture(stream, 2) == 0
+        try:
+            sides[0][0](captured)
+        finally:
+            assert hip.hipStreamEndCapture(stream, C.byref(graph)) == 0
+        assert hip.hipGraphInstantiate(C.byref(exe), graph, None, None, C.c_size_t(0)) == 0
+        try:
+            for i in range(1, 6):
+                for run, outs, _ in sides:
+                    run(outs[i])
+                assert hip.hipGraphLaunch(exe, stream) == 0
+            for _, outs, want in sides:
+                assert all((o.numpy() == want).all() for o in outs)
+            assert (captured.numpy() == sides[0][2]).all() and np.abs(sides[0][2]).max() > 0
+        finally:
+            hip.hipGraphExecDestroy(exe)
+            hip.hipGraphDestroy(graph)
+        del d, q, pos, outs, run
+        sides.clear()
+    finally:
+        other.close()
 
 
 def test_nothing_to_do(dev):
