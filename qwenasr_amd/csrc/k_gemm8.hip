@@ -158,7 +158,7 @@ __global__ __launch_bounds__(256) void k_gemm8_any(Gemm8Args g) {
 __device__ __attribute__((aligned(256))) int4 g_gemm8_zero16[16];
 
 template <int MODE, typename YT, int BM, int BN, int WM, int WN, int KP, bool STREAM>
-__global__ __launch_bounds__(64 * WM * WN * KP, WM * WN * KP > 8 ? 4 : 2) void k_gemm8(Gemm8Args g) {
+__global__ __launch_bounds__(64 * WM * WN * KP, KP == 1 ? 4 : 2) void k_gemm8(Gemm8Args g) {
     constexpr int BK = 128, NS = 2, W = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, RPL = 1024 / BK, SPR = BK / 16;
     constexpr int LA = BM / RPL / W, LB = BN / RPL / W, STG = (BM + BN) * BK;
     static_assert(BM % (RPL * W) == 0 && BN % (RPL * W) == 0 && BM % (16 * WM) == 0 && BN % (16 * WN) == 0, "tile");
@@ -335,14 +335,14 @@ static hipError_t go_gemm8(const Gemm8Args &g, hipStream_t st) {
         // The form with the least estimated time: ns for the first round of tiles over the 256
         // CUs (fixed, and for each 64 of K), and for each further round, halfway between the
         // whole and the fractional count of rounds, as several blocks share a CU.  Fits to 215
-        // shapes, M 1 ... 2000, N 512 ... 151936, K 320 ... 6144; the choice is 2% behind the best
-        // of seven forms there on average and 22% at worst (1337 x 4096 x 320).  us, in the order
-        // of the list: 1 x 4096 x 1024 5.0, 5.4, 7.9, 13.1; 404 x 4096 x 1024 16.9, 8.8, 10.1,
-        // 14.2; 1337 x 12288 x 2048 173, 78, 57, 54; 375 x 151936 x 1024 484, 215, 121, 110.
-        static const struct { int bm, bn, one, one_k, more, more_k; } f[] = {{32, 64, 3877, 98, 2461, 118},
-                                                                             {64, 64, 3743, 142, 1930, 92},
-                                                                             {128, 128, 4472, 319, 3526, 253},
-                                                                             {192, 128, 6957, 458, 5072, 298}};
+        // shapes, M 1 ... 2000, N 512 ... 151936, K 320 ... 6144; the choice is 0.2% behind the
+        // best form there on average and 13% at worst (1600 x 12288 x 2048).  us, in the order of
+        // the list: 1 x 4096 x 1024 4.9, 5.2, 7.8, 9.9; 404 x 4096 x 1024 16.6, 8.2, 9.7, 12.4;
+        // 1337 x 12288 x 2048 171, 80, 54, 51; 375 x 151936 x 1024 481, 215, 121, 107.
+        static const struct { int bm, bn, one, one_k, more, more_k; } f[] = {{32, 64, 3775, 97, 2486, 114},
+                                                                             {64, 64, 3592, 137, 1887, 91},
+                                                                             {128, 128, 4485, 312, 3021, 269},
+                                                                             {192, 128, 5924, 379, 2420, 427}};
         const int64_t nk = (g.K + 63) / 64;
         int best = 0;
         int64_t best_ns = INT64_MAX;
@@ -352,16 +352,20 @@ static hipError_t go_gemm8(const Gemm8Args &g, hipStream_t st) {
             const int64_t ns = f[i].one + f[i].one_k * nk + over * (f[i].more + f[i].more_k * nk) / 512;
             if (ns < best_ns) { best_ns = ns; best = i; }
         }
+        // Results of 32 MB and more whose rows are whole 64-byte pieces go past the caches: f32,
+        // 1337 x 12288 x 2048 50.0 -> 43.0 us, 404 x 60000 x 512 43 -> 32, 1000 x 60000 x 512 90 -> 64,
+        // 375 x 151936 x 1024 110 -> 107.  A smaller result is better left for its reader (a layer of
+        // 404 rows 77.0 us in all, 78.3 with every result past the caches); rows in odd pieces have to
+        // meet in a cache (2021 x 4999 bf16 18.8 us, 24.5).
+        constexpr bool CAN = MODE != G8_ADDTO;      // which gains nothing: its result was read just before
+        const int64_t row = (MODE == G8_SWIGLU ? g.N / 2 : g.N) * (int64_t)sizeof(YT);
+        const bool stream = g.M * row >= (1 << 25) && row % 64 == 0 && (uintptr_t)g.y % 64 == 0;
         switch (best) {
             case 0: return go_gemm8_tile<MODE, YT, 32, 64, 1, 2, 4>(g, st);
             case 1: return go_gemm8_tile<MODE, YT, 64, 64, 2, 2, 2>(g, st);
-            case 2: return go_gemm8_tile<MODE, YT, 128, 128, 2, 4, 1>(g, st);
-            default: break;
+            case 2: return stream ? go_gemm8_tile<MODE, YT, 128, 128, 2, 4, 1, CAN>(g, st) : go_gemm8_tile<MODE, YT, 128, 128, 2, 4, 1>(g, st);
+            default: return stream ? go_gemm8_tile<MODE, YT, 192, 128, 2, 4, 1, CAN>(g, st) : go_gemm8_tile<MODE, YT, 192, 128, 2, 4, 1>(g, st);
         }
-        // results that the cache behind the L2s (256 MB) holds no large part of go past the caches:
-        // 375 x 151936 x 1024 in f32 109.2 -> 107.9 us
-        return g.M * (MODE == G8_SWIGLU ? g.N / 2 : g.N) < (1 << 25) ? go_gemm8_tile<MODE, YT, 192, 128, 2, 2, 1>(g, st)
-                                                                    : go_gemm8_tile<MODE, YT, 192, 128, 2, 2, 1, true>(g, st);
     }
     const int64_t gx = (g.N + 63) / 64, gy = (g.M + 63) / 64;
     if (gx * gy * 256 > UINT32_MAX) return hipErrorInvalidValue;
