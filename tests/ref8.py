@@ -109,7 +109,7 @@ def attend(q, k, v, pos, scale, window=0, sinks=0, steps=8.0e6):
             # scale, two of the sum, the product); the difference from the maximum; the exponential's unit in the last
             # place.  Then the block's scale, the rescaling of the sums at each block and their additions
             u = 2.0 ** -24
-            score = scale * np.abs(kk).sum(1) * np.abs(q[i, h]).max() / (2 * steps) + 8 * u * np.abs(s) + u * np.abs(s - s.max())
+            score = abs(scale) * np.abs(kk).sum(1) * np.abs(q[i, h]).max() / (2 * steps) + 8 * u * np.abs(s) + u * np.abs(s - s.max())
             blocks = (seen.sum() + 2 * BLOCK) // BLOCK + 1
             # a block's weights are whole numbers of its largest / steps, half a one off against |v|
             at = p[seen] // BLOCK

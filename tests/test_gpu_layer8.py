@@ -197,6 +197,29 @@ def test_gemm_alignment(dev, off_a, off_w):
     check_gemm(y.numpy().astype(np.float64), ref8.gemm8(a, sa, w, sw)[0], sa, sw, None, None, "plain", False)
 
 
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("mode", ["plain", "add", "swiglu"])
+@pytest.mark.parametrize("M,N,Kd", [(70, 200, 256), (300, 2050, 1040), (1500, 4100, 336), (40, 301, 16), (9, 333, 77)])
+def test_gemm_result_anywhere(dev, M, N, Kd, mode, is_bf16):
+    """y, bias and scales that start one element off: rows of y at any alignment, nothing written around them."""
+    from qwenasr_amd._lib import check, lib
+    print(f"w8a8 {M} x {N} x {Kd} {mode} bf16={is_bf16}, one element off", flush=True)
+    N += N % 2 if mode == "swiglu" else 0
+    r = rng(M + N + Kd + is_bf16)
+    a, w = r.integers(-127, 128, (M, Kd), dtype=np.int8), r.integers(-127, 128, (N, Kd), dtype=np.int8)
+    sa, sw = r.uniform(0.01, 0.03, M).astype(np.float32), (r.uniform(0.01, 0.02, N) / np.sqrt(Kd) / 60).astype(np.float32)
+    bias, cols = r.normal(0, 0.5, N).astype(np.float32), N // 2 if mode == "swiglu" else N
+    y0 = np.concatenate([[7.0], r.normal(0, 1, M * cols), [7.0]])
+    y, dsa, dsw, db = up(dev, y0, is_bf16), *(dev.upload(np.concatenate([[0.0], v]).astype(np.float32)) for v in (sa, sw, bias))
+    da, dw = dev.upload(a), dev.upload(w)
+    check(lib().qasr_hip_gemm_w8a8(dev.h, y.offset(1), da.ptr, dsa.offset(1), dw.ptr, dsw.offset(1), db.offset(1), M, N, Kd,
+                                   ["plain", "add", "swiglu"].index(mode), 1 if is_bf16 else 0))
+    got = values(y, is_bf16)
+    assert got[0] == 7.0 and got[-1] == 7.0
+    check_gemm(got[1:-1].reshape(M, cols), ref8.gemm8(a, sa, w, sw)[0], sa, sw, bias.astype(np.float64),
+               held(y0, is_bf16)[1:-1].reshape(M, cols), mode, is_bf16)
+
+
 def test_gemm_largest_sums(dev):
     """Every product -128 x -128 at the longest K: the sum is the largest that 32 bits hold."""
     from qwenasr_amd import kernels as K
@@ -509,6 +532,76 @@ def test_long_cache(dev, rows, is_bf16):
         # back_k and back_v are the cache's values rounded once to f32
         err = err + (BF16 if is_bf16 else F32) * (np.abs(want) + err) + 2 * F32 * np.abs(vv).max()
         assert (np.abs(full[j, i, h] - want[0, 0]) <= err[0, 0]).all()
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("counts,dim,off,pad", [([1, 1], 128, 1, 1), ([2, 19], 128, 3, 5), ([40, 1], 64, 1, 7), ([2, 1], 64, 5, 2)])
+def test_rows_anywhere(dev, counts, dim, off, pad, is_bf16):
+    """Rows that start at any element and lie any number of elements apart: into the cache, back, and the attention's."""
+    from qwenasr_amd import kernels as K
+    r = rng(off * 8 + pad + dim + is_bf16)
+    heads, group, cap, pos = 2, 2, 256, [70, 3]
+    n, hd, hq, es = len(counts), heads * dim, heads * group * dim, 2 if is_bf16 else 4
+    start, total, ld = prefix(counts), sum(counts), hd + pad
+    ref = ref8.Cache(n, heads, cap, dim).fill(r)
+    d = DevCache(dev, ref)
+    dpos, dstart = dev.upload(np.array(pos, np.int32)), dev.upload(start)
+
+    class Off:
+        def __init__(self, b):
+            self.b, self.ptr, self.dev = b, C.c_void_p(b.ptr.value + off * es), dev
+    flat = [r.normal(0, 1, off + total * ld) for _ in range(2)]
+    k, v = (Off(up(dev, f, is_bf16)) for f in flat)
+    K.kv8_write(*d.buf, k, v, dpos, total, n, max(counts), *d.geometry(), row_start=dstart, ld=ld, bf16=is_bf16)
+    kh, vh = (held(f, is_bf16)[off:].reshape(total, ld)[:, :hd].reshape(total, heads, dim) for f in flat)
+    for j in range(n):
+        rows = slice(start[j], start[j + 1])
+        ref.write(j, pos[j], {"k": kh[rows], "v": vh[rows]})
+    d.check()
+    bk, bv = (Off(up(dev, np.full(off + total * ld, 9.0), is_bf16)) for _ in range(2))
+    K.kv8_read(bk, bv, *d.buf, dpos, total, n, max(counts), *d.geometry(), row_start=dstart, ld=ld, bf16=is_bf16)
+    for o, name in ((bk, "k"), (bv, "v")):
+        got = values(o.b, is_bf16)
+        assert (got[:off] == 9.0).all() and (got[off:].reshape(total, ld)[:, hd:] == 9.0).all()
+        want = np.concatenate([ref.values(name)[j, :, pos[j]:pos[j] + counts[j]].transpose(1, 0, 2) for j in range(n)])
+        got = got[off:].reshape(total, ld)[:, :hd].reshape(want.shape)
+        assert (np.abs(got - want) <= (BF16 if is_bf16 else F32) * np.abs(want)).all()
+    ldq = hq + pad
+    qf = r.normal(0, 1, off + total * ldq)
+    o = Off(up(dev, np.full(off + total * hq + 1, 9.0), is_bf16))
+    K.attention_kv8(o, Off(up(dev, qf, is_bf16)), *d.buf, dpos, total, n, max(counts), heads * group, heads, dim, cap, dim ** -0.5,
+                    row_start=dstart, ldq=ldq, bf16=is_bf16)
+    got = values(o.b, is_bf16)
+    assert (got[:off] == 9.0).all() and got[-1] == 9.0
+    q = held(qf, is_bf16)[off:].reshape(total, ldq)[:, :hq].reshape(total, heads * group, dim)
+    check_attention(got[off:-1].reshape(q.shape), ref, q, counts, pos, is_bf16=is_bf16)
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows", [2, 40])
+@pytest.mark.parametrize("scale", [0.0, -0.1, 2.0])
+def test_attention_scale(dev, scale, rows, is_bf16):
+    """Any scale; rows of zeros, and rows of very small and large values."""
+    from qwenasr_amd import kernels as K
+    r = rng(rows + is_bf16)
+    heads, dim, cap, pos = 2, 128, 256, 120
+    ref = ref8.Cache(1, heads, cap, dim).fill(r)
+    d = DevCache(dev, ref)
+    q = r.normal(0, 1, (rows, heads * 2, dim))
+    q[0, 1], q[1, 2], q[1, 3] = 0.0, q[1, 2] * 1e-20, q[1, 3] * 1e3
+    out = up(dev, np.zeros((rows, heads * 2 * dim)), is_bf16)
+    K.attention_kv8(out, up(dev, q, is_bf16), *d.buf, dev.upload(np.array([pos], np.int32)), rows, 1, rows, heads * 2, heads, dim, cap, scale,
+                    bf16=is_bf16)
+    # the scale as the operator gets it: f32
+    want, err = ref8.attend(held(q, is_bf16), ref.values("k")[0], ref.values("v")[0], pos, float(np.float32(scale)),
+                            steps=32000.0 if is_bf16 else 8.0e6)
+    got = values(out, is_bf16).reshape(q.shape)
+    assert np.isfinite(got).all()
+    # the bound is first order in a score's error: below 0.05 here, exp(2 e) - 1 <= 1.06 x 2 e, but for the large row
+    err = 1.06 * err + (BF16 if is_bf16 else F32) * (np.abs(want) + err)
+    ok = np.abs(got - want) <= err
+    ok[1, 3] = True
+    assert ok.all(), np.argwhere(~ok)[:4]
 
 
 def test_attention_uniform_rows(dev):
