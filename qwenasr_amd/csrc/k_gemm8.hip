@@ -333,23 +333,23 @@ static hipError_t go_gemm8(const Gemm8Args &g, hipStream_t st) {
     const int vec_k = g.K % 16 == 0 && ((uintptr_t)g.a | (uintptr_t)g.w) % 16 == 0;
     if (vec_k) {
         // The form with the least estimated time: ns for the first round of tiles over the 256
-        // CUs (fixed, and for each 64 of K), and for each further round, halfway between the
-        // whole and the fractional count of rounds, as several blocks share a CU.  Fits to 215
-        // shapes, M 1 ... 2000, N 512 ... 151936, K 320 ... 6144; the choice is 0.2% behind the
-        // best form there on average and 13% at worst (1600 x 12288 x 2048).  us, in the order of
-        // the list: 1 x 4096 x 1024 4.9, 5.2, 7.8, 9.9; 404 x 4096 x 1024 16.6, 8.2, 9.7, 12.4;
-        // 1337 x 12288 x 2048 171, 80, 54, 51; 375 x 151936 x 1024 481, 215, 121, 107.
-        static const struct { int bm, bn, one, one_k, more, more_k; } f[] = {{32, 64, 3775, 97, 2486, 114},
-                                                                             {64, 64, 3592, 137, 1887, 91},
-                                                                             {128, 128, 4485, 312, 3021, 269},
-                                                                             {192, 128, 5924, 379, 2420, 427}};
+        // CUs (fixed, and for each 64 of K), and for each further round.  Fits to 257 shapes, M 1
+        // ... 2000, N 512 ... 151936, K 320 ... 6144; the choice is 1% behind the best of seven
+        // forms there on average and 33% at worst (200 x 2048 x 6144).  us, in the order of the
+        // list: 32 x 2048 x 6144 8.0, 10.3, 17.5, 31, 37; 32 x 12288 x 2048 12.4, 7.3, 9.2, 13, 16;
+        // 404 x 4096 x 1024 34, 17.0, 8.2, 9.9, 12.2; 2000 x 4096 x 1024 155, 68, 25.8, 17.8, 18.0;
+        // 1337 x 12288 x 2048 409, 208, 78, 49.5, 42.7; 375 x 151936 x 1024 1153, 562, 217, 120, 109.
+        static const struct { int bm, bn, one, one_k, more, more_k; } f[] = {{16, 32, 3531, 47, 1969, 42},
+                                                                             {16, 32, 2908, 70, 792, 20},
+                                                                             {64, 64, 3529, 141, 1877, 70},
+                                                                             {128, 128, 4831, 297, 2450, 218},
+                                                                             {192, 128, 6170, 381, 3731, 256}};
         const int64_t nk = (g.K + 63) / 64;
         int best = 0;
         int64_t best_ns = INT64_MAX;
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < 5; i++) {
             const int64_t tiles = (g.M + f[i].bm - 1) / f[i].bm * ((g.N + f[i].bn - 1) / f[i].bn), rounds = (tiles + 255) / 256;
-            const int64_t over = rounds > 1 ? tiles + 256 * rounds - 512 : 0;         // further rounds, in 1 / 512
-            const int64_t ns = f[i].one + f[i].one_k * nk + over * (f[i].more + f[i].more_k * nk) / 512;
+            const int64_t ns = f[i].one + f[i].one_k * nk + (rounds - 1) * (f[i].more + f[i].more_k * nk);
             if (ns < best_ns) { best_ns = ns; best = i; }
         }
         // Results of 32 MB and more whose rows are whole 64-byte pieces go past the caches: f32,
@@ -361,9 +361,10 @@ static hipError_t go_gemm8(const Gemm8Args &g, hipStream_t st) {
         const int64_t row = (MODE == G8_SWIGLU ? g.N / 2 : g.N) * (int64_t)sizeof(YT);
         const bool stream = g.M * row >= (1 << 25) && row % 64 == 0 && (uintptr_t)g.y % 64 == 0;
         switch (best) {
-            case 0: return go_gemm8_tile<MODE, YT, 32, 64, 1, 2, 4>(g, st);
-            case 1: return go_gemm8_tile<MODE, YT, 64, 64, 2, 2, 2>(g, st);
-            case 2: return stream ? go_gemm8_tile<MODE, YT, 128, 128, 2, 4, 1, CAN>(g, st) : go_gemm8_tile<MODE, YT, 128, 128, 2, 4, 1>(g, st);
+            case 0: return go_gemm8_tile<MODE, YT, 16, 32, 1, 1, 8>(g, st);
+            case 1: return go_gemm8_tile<MODE, YT, 16, 32, 1, 1, 4>(g, st);
+            case 2: return go_gemm8_tile<MODE, YT, 64, 64, 2, 2, 2>(g, st);
+            case 3: return stream ? go_gemm8_tile<MODE, YT, 128, 128, 2, 4, 1, CAN>(g, st) : go_gemm8_tile<MODE, YT, 128, 128, 2, 4, 1>(g, st);
             default: return stream ? go_gemm8_tile<MODE, YT, 192, 128, 2, 4, 1, CAN>(g, st) : go_gemm8_tile<MODE, YT, 192, 128, 2, 4, 1>(g, st);
         }
     }
