@@ -334,9 +334,9 @@ static hipError_t go_gemm8(const Gemm8Args &g, hipStream_t st) {
     if (vec_k) {
         // The form with the least estimated time: ns for the first round of tiles over the 256
         // CUs (fixed, and for each 64 of K), and for each further round.  Fits to 257 shapes, M 1
-        // ... 2000, N 512 ... 151936, K 320 ... 6144; the choice is 1% behind the best of seven
-        // forms there on average and 33% at worst (200 x 2048 x 6144).  us, in the order of the
-        // list: 32 x 2048 x 6144 8.0, 10.3, 17.5, 31, 37; 32 x 12288 x 2048 12.4, 7.3, 9.2, 13, 16;
+        // ... 2000, N 512 ... 151936, K 320 ... 6144; of nine forms and 290 shapes the choice is
+        // 2.5% behind the best on average, 50% at worst (1 x 60000 x 512: 12.4 us, 8.1 with 64 x
+        // 128 tiles, which elsewhere gain too little to be told apart).  us, in the order of the list: 32 x 2048 x 6144 8.0, 10.3, 17.5, 31, 37; 32 x 12288 x 2048 12.4, 7.3, 9.2, 13, 16;
         // 404 x 4096 x 1024 34, 17.0, 8.2, 9.9, 12.2; 2000 x 4096 x 1024 155, 68, 25.8, 17.8, 18.0;
         // 1337 x 12288 x 2048 409, 208, 78, 49.5, 42.7; 375 x 151936 x 1024 1153, 562, 217, 120, 109.
         static const struct { int bm, bn, one, one_k, more, more_k; } f[] = {{16, 32, 3531, 47, 1969, 42},

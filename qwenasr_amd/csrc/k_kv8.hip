@@ -584,6 +584,12 @@ __global__ __launch_bounds__(64 * CG * PG, SHARED ? 4 : 2) void k_attn_kv8(AttnK
 #pragma unroll
         for (int d = 0; d < DT; d++) vr[d] = *reinterpret_cast<const i32x4 *>(p + 16 * d * 64);
     };
+    // the column's row, ahead of the first block: it is turned into digits while that is on its way
+    float x[KS][16];
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+        kv8_load16<BF16>(a.q, (sq.r0 + qi) * a.ldq + (int64_t)(h * a.G + qg) * HD + 64 * s + 16 * g, a.vec_q, x[s]);
+    __builtin_amdgcn_sched_barrier(0);
     if (u < u1) {
         if constexpr (SHARED) {
             issue_k(block_of(u));
@@ -598,12 +604,10 @@ __global__ __launch_bounds__(64 * CG * PG, SHARED ? 4 : 2) void k_attn_kv8(AttnK
     i32x4 qd[KS][D];
     float qf;                                                  // score = integer sum x qf x the block's scale
     {
-        const int64_t at = (sq.r0 + qi) * a.ldq + (int64_t)(h * a.G + qg) * HD;
-        float x[KS][16], m = 0.0f;
+        float m = 0.0f;
         bool bad = false;
 #pragma unroll
         for (int s = 0; s < KS; s++) {
-            kv8_load16<BF16>(a.q, at + 64 * s + 16 * g, a.vec_q, x[s]);
 #pragma unroll
             for (int e = 0; e < 16; e++) x[s][e] = a.scale < 0.0f ? -x[s][e] : x[s][e];   // the scores' factor is not negative
 #pragma unroll
