@@ -917,7 +917,11 @@ hipError_t launch_attention_kv8(const AttnKv8Args &a0, bool bf16, hipStream_t st
     // groups against 4: 1337 rows 29.4 / 32.4, with bf16 22.6 / 26.6; 404 rows 12.5 / 12.2; 2 x
     // 300 rows behind 3000 positions 45 / 41; 4 x 67 rows, window 8192: 87 / 61, with 3 splits
     // 43 + 5 / 38 + 5.
-    const int64_t units = (rows + 31) / 32 * a.c.Hkv * a.c.n_seq;
+    // Sequences shorter than max_rows leave their last tiles' blocks empty: counted are the tiles
+    // that n_rows rows fill, and half a tile a sequence (up to 67 rows each, window 8192: 40.2 + 5.3
+    // -> 30.7 + 6.5; 6 sequences of up to 100 f32 rows behind 6000 positions 85.7 -> 51 + 5.4).
+    const int64_t tiles = std::min((rows + 31) / 32 * a.c.n_seq, (a.c.n_rows * a.G / 16 + a.c.n_seq) / 2 + 1);
+    const int64_t units = tiles * a.c.Hkv;
     if (units >= 384) return pick_attn_kv8<2, 2, true>(a, bf16, 1, st);
     return pick_attn_kv8<2, 4, true>(a, bf16, (int)std::min<int64_t>(512 / units, blocks / 16), st);
 }
