@@ -148,7 +148,7 @@ __global__ __launch_bounds__(256) void k_gemm8_any(Gemm8Args g) {
 // What bounds it is the way from the caches into LDS.  Such loads, with nothing else
 // running, bring 34 TB/s when a row gives 128 bytes and lies in the XCD's L2, 20 when it
 // gives 64, 7-8 when it comes from the cache behind the L2s (375 x 151936 x 1024, 192 x
-// 128 tiles: 142 us with 64-byte steps and three stages, 109 with these; more stages or
+// 128 tiles: 142 us with 64-byte steps and three stages, 107 with these; more stages or
 // larger tiles leave too few waves on a CU).  Hence also the order of the tiles, below.
 //
 // A stage holds the tile's activation rows, then its weight rows, in 16-byte slots;
@@ -174,10 +174,17 @@ __global__ __launch_bounds__(64 * WM * WN * KP, KP == 1 ? 4 : 2) void k_gemm8(Ge
     // another on one XCD, whose L2 then holds the strip once
     const unsigned rows = (unsigned)((M + BM - 1) / BM), xcd = blockIdx.x & 7, q = blockIdx.x >> 3;
     const unsigned strip = q / rows * 8 + xcd;
-    const int64_t m0 = (int64_t)(q - q / rows * rows) * BM, n0 = (int64_t)strip * BN;
+    const unsigned row = q - q / rows * rows;
+    const int64_t m0 = (int64_t)row * BM, n0 = (int64_t)strip * BN;
     if (n0 >= N) return;
     char *ring = smem + grp * NS * STG;
     const int nk = (int)((K + BK - 1) / BK), nit = (nk + KP - 1) / KP;
+    // The K-step that this row tile begins with.  Weights that come from HBM (80 MB and more: the
+    // cache behind the L2s has let go of them) are fetched by a strip's row tiles at different
+    // places then, twice the bytes in flight with two tiles: 375 x 151936 x 1024 106 -> 100 us,
+    // 2000 x 40000 x 2048 206 -> 192.  Weights that a cache holds are better met by all at once:
+    // 1337 x 12288 x 6144 118 us, 121.5 in turn; 32 x 12288 x 2048 7.6, 9.7.
+    const int turn = N * K >= 80000000 ? (int)((int64_t)row * nk / rows) : 0;
     // the epilogue's operands, ahead of the ring's loads
     f32x4 ws[NT], bias[NT];
     float as[MT];
@@ -205,7 +212,7 @@ __global__ __launch_bounds__(64 * WM * WN * KP, KP == 1 ? 4 : 2) void k_gemm8(Ge
     auto issue = [&](int stage, int it) {
         char *st = ring + stage * STG;
         const int kt = grp + KP * it;
-        const int k0 = kt < nk ? kt * BK : (int)K;          // past the end: nothing but zeros
+        const int k0 = kt < nk ? (kt + turn < nk ? kt + turn : kt + turn - nk) * BK : (int)K;   // past the end: nothing but zeros
         const bool whole = k0 + BK <= K;
 #pragma unroll
         for (int u = 0; u < LA + LB; u++) {
