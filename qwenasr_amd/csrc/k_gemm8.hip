@@ -66,80 +66,28 @@ __device__ __forceinline__ f32x4 gemm8_value(i32x4 acc, float as, f32x4 ws, f32x
     return v;
 }
 
-// The form for rows that are not 16-byte aligned: 64 x 64 tiles, four waves of 32 x
-// 32, K-steps of 64 through registers and a pair of LDS buffers (the direct loads into
-// LDS want aligned addresses).
-template <int MODE, typename YT>
-__global__ __launch_bounds__(256) void k_gemm8_any(Gemm8Args g) {
-    constexpr int BK = 64, LDK = BK + 16;
-    __shared__ __attribute__((aligned(16))) int8_t As[2][64][LDK], Ws[2][64][LDK];
-    const int t = threadIdx.x, lane = t & 63;
-    const int wid = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int wm = (wid & 1) * 32, wn = (wid >> 1) * 32;
-    const unsigned strips = (unsigned)((g.N + 63) / 64), by = blockIdx.x / strips;
-    const int64_t m0 = (int64_t)by * 64, n0 = (int64_t)(blockIdx.x - by * strips) * 64;
-    const int64_t K = g.K;
-    const int lr = t >> 2, lk = (t & 3) * 16;        // this thread's 16 bytes of a 64 x 64 tile
-    const int8_t *ap = g.a + min(m0 + lr, g.M - 1) * K, *wp = g.w + min(n0 + lr, g.N - 1) * K;
-    i32x4 ar, wr;
-    auto load16 = [&](const int8_t *p, int64_t k) {
-        typedef int i32x4_any __attribute__((ext_vector_type(4), aligned(1)));   // the hardware takes any address
-        if (k + 16 <= K) return (i32x4)*reinterpret_cast<const i32x4_any *>(p + k);
-        i32x4 v = {0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-            if (k + i < K) v[i >> 2] |= (int)(uint8_t)p[k + i] << (8 * (i & 3));
-        return v;
-    };
-    ar = load16(ap, lk);
-    wr = load16(wp, lk);
-    i32x4 acc[2][2] = {};
-    const int fr = lane & 15, fg = lane >> 4;
-    const int64_t nk = (K + BK - 1) / BK;
-    for (int64_t kt = 0; kt < nk; kt++) {
-        const int b = kt & 1;
-        *reinterpret_cast<i32x4 *>(&As[b][lr][lk]) = ar;
-        *reinterpret_cast<i32x4 *>(&Ws[b][lr][lk]) = wr;
-        __syncthreads();
-        if (kt + 1 < nk) {
-            ar = load16(ap, (kt + 1) * BK + lk);
-            wr = load16(wp, (kt + 1) * BK + lk);
-        }
-        i32x4 af[2], wf[2];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            af[i] = *reinterpret_cast<const i32x4 *>(&As[b][wm + 16 * i + fr][16 * fg]);
-            wf[i] = *reinterpret_cast<const i32x4 *>(&Ws[b][wn + 16 * i + fr][16 * fg]);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], af[i], acc[i][j], 0, 0, 0);
+// 16 bytes of a row from byte k on, `left` of them before the row's end (K bytes), zeros
+// behind it; rows begin at any address, which the hardware's vector loads take
+__device__ __forceinline__ i32x4 gemm8_row16(const int8_t *p, int left, int K) {
+    typedef int Any __attribute__((ext_vector_type(4), aligned(1)));
+    if (left >= 16) return *reinterpret_cast<const Any *>(p);
+    i32x4 v = {0, 0, 0, 0};
+    if (left <= 0) return v;
+    if (K >= 16) {                                           // the row's last 16, moved down
+        v = *reinterpret_cast<const Any *>(p + left - 16);
+        const int sh = 8 * (16 - left);
+        uint64_t lo = (uint32_t)v[0] | (uint64_t)(uint32_t)v[1] << 32, hi = (uint32_t)v[2] | (uint64_t)(uint32_t)v[3] << 32;
+        lo = sh < 64 ? lo >> sh | hi << (64 - sh) : hi >> (sh - 64);
+        hi = sh < 64 ? hi >> sh : 0;
+        return i32x4{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
     }
-    const int64_t cols = MODE == G8_SWIGLU ? g.N >> 1 : g.N;
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-        const int64_t n = n0 + wn + 16 * j + 4 * fg;
-        if (n >= g.N) continue;
-        const f32x4 ws = gemm_load4(g.ws, (int)n, (int)g.N, false);
-        const f32x4 bias = g.bias ? gemm_load4(g.bias, (int)n, (int)g.N, false) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        const int64_t c0 = MODE == G8_SWIGLU ? n >> 1 : n;
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int64_t m = m0 + wm + 16 * i + fr;
-            if (m >= g.M) continue;
-            const f32x4 v = gemm8_value<MODE>(acc[i][j], g.as[m], ws, bias);
-            YT *p = reinterpret_cast<YT *>(g.y) + m * cols + c0;
-#pragma unroll
-            for (int r = 0; r < (MODE == G8_SWIGLU ? 2 : 4); r++) {
-                if (c0 + r >= cols) continue;
-                Gemm8Io<YT>::out(p + r, MODE == G8_ADDTO ? __fadd_rn(__fadd_rn(Gemm8Io<YT>::in(p + r), bias[r]), v[r]) : v[r]);
-            }
-        }
-    }
+    for (int i = 0; i < 15; i++)
+        if (i < left) v[i >> 2] |= (int)(uint8_t)p[i] << (8 * (i & 3));
+    return v;
 }
 
-// The fast form: BM x BN tiles fed by direct global -> LDS loads through rings of two
+// BM x BN tiles fed by direct global -> LDS loads through rings of two
 // stages of BK = 128 bytes of K, one in flight while one is multiplied.  KP groups of
 // WM x WN waves each take every KP-th K-step through a ring of their own and add up in
 // LDS at the end (int32: exact in any order): a short grid or few rows leave a CU few
@@ -153,11 +101,13 @@ __global__ __launch_bounds__(256) void k_gemm8_any(Gemm8Args g) {
 //
 // A stage holds the tile's activation rows, then its weight rows, in 16-byte slots;
 // slot q of row r stands at q ^ lds_swz(r).  A load fills 64 slots in lane order.
-// K-steps past the end load zeros, so every wait counts the same.  Needs K % 16 == 0
-// and 16-byte aligned operands.
+// K-steps past the end load zeros, so every wait counts the same.
+//
+// ANY: K % 16 != 0 or operands that are not 16-byte aligned, which the direct loads do
+// not take: the same slots through registers, a step ahead.
 __device__ __attribute__((aligned(256))) int4 g_gemm8_zero16[16];
 
-template <int MODE, typename YT, int BM, int BN, int WM, int WN, int KP, bool STREAM>
+template <int MODE, typename YT, int BM, int BN, int WM, int WN, int KP, bool STREAM, bool ANY>
 __global__ __launch_bounds__(64 * WM * WN * KP, KP == 1 ? 4 : 2) void k_gemm8(Gemm8Args g) {
     constexpr int BK = 128, NS = 2, W = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, RPL = 1024 / BK, SPR = BK / 16;
     constexpr int LA = BM / RPL / W, LB = BN / RPL / W, STG = (BM + BN) * BK;
@@ -209,10 +159,14 @@ __global__ __launch_bounds__(64 * WM * WN * KP, KP == 1 ? 4 : 2) void k_gemm8(Ge
         src[u] = (u < LA ? g.a + min(m0 + r, M - 1) * K : g.w + min(n0 + r, N - 1) * K) + sq[u];
     }
     const int8_t *zero = reinterpret_cast<const int8_t *>(g_gemm8_zero16);
+    // the byte of K that this group's step begins with; past the end: K, nothing but zeros
+    auto step = [&](int it) {
+        const int kt = grp + KP * it;
+        return kt < nk ? (kt + turn < nk ? kt + turn : kt + turn - nk) * BK : (int)K;
+    };
     auto issue = [&](int stage, int it) {
         char *st = ring + stage * STG;
-        const int kt = grp + KP * it;
-        const int k0 = kt < nk ? (kt + turn < nk ? kt + turn : kt + turn - nk) * BK : (int)K;   // past the end: nothing but zeros
+        const int k0 = step(it);
         const bool whole = k0 + BK <= K;
 #pragma unroll
         for (int u = 0; u < LA + LB; u++) {
@@ -220,13 +174,35 @@ __global__ __launch_bounds__(64 * WM * WN * KP, KP == 1 ? 4 : 2) void k_gemm8(Ge
             lds_dma16(whole || k0 + sq[u] < K ? src[u] + k0 : zero, to);
         }
     };
-    i32x4 acc[NT][MT] = {};
+    // ANY: the step's slots into registers, and from there into a stage
+    i32x4 held[LA + LB];
+    auto load = [&](int it) {
+        const int k0 = step(it);
 #pragma unroll
-    for (int s = 0; s < NS - 1; s++) issue(s, s);
+        for (int u = 0; u < LA + LB; u++) {
+            typedef int Any __attribute__((ext_vector_type(4), aligned(1)));
+            if (k0 + BK <= K) held[u] = *reinterpret_cast<const Any *>(src[u] + k0);
+            else held[u] = gemm8_row16(src[u] + k0, (int)K - k0 - sq[u], (int)K);
+        }
+    };
+    auto store = [&](int stage) {
+        char *st = ring + stage * STG + 16 * lane;
+#pragma unroll
+        for (int u = 0; u < LA + LB; u++)
+            *reinterpret_cast<i32x4 *>(st + (u < LA ? 1024 * (w * LA + u) : BM * BK + 1024 * (w * LB + u - LA))) = held[u];
+    };
+    i32x4 acc[NT][MT] = {};
+    if constexpr (ANY) {
+        load(0);
+        store(0);
+        load(1);
+    } else {
+        issue(0, 0);
+    }
     for (int it = 0; it < nit; it++) {
-        wait_vmcnt<(LA + LB) * (NS - 2)>();                  // this wave's loads of the stage have landed
+        if constexpr (!ANY) wait_vmcnt<0>();                 // this wave's loads of the stage have landed
         __syncthreads();                                     // ... and every wave's; the stage before is free
-        issue((it + NS - 1) % NS, it + NS - 1);
+        if constexpr (!ANY) issue((it + 1) % NS, it + 1);
         const char *at = ring + (it % NS) * STG, *wt = at + BM * BK;
 #pragma unroll
         for (int s = 0; s < BK / 64; s++) {
@@ -245,6 +221,10 @@ __global__ __launch_bounds__(64 * WM * WN * KP, KP == 1 ? 4 : 2) void k_gemm8(Ge
             for (int j = 0; j < NT; j++)
 #pragma unroll
                 for (int i = 0; i < MT; i++) acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], af[i], acc[j][i], 0, 0, 0);
+        }
+        if constexpr (ANY) {
+            store((it + 1) % NS);
+            load(it + 2);
         }
     }
     wait_vmcnt<0>();                                         // no load may land in LDS after the block ends
@@ -326,59 +306,73 @@ __global__ __launch_bounds__(64 * WM * WN * KP, KP == 1 ? 4 : 2) void k_gemm8(Ge
     }
 }
 
-template <int MODE, typename YT, int BM, int BN, int WM, int WN, int KP, bool STREAM = false>
+template <int MODE, typename YT, int BM, int BN, int WM, int WN, int KP, bool STREAM = false, bool ANY = false>
 static hipError_t go_gemm8_tile(const Gemm8Args &g, hipStream_t st) {
     const int64_t gx = (g.N + BN - 1) / BN, gy = (g.M + BM - 1) / BM;
     const int64_t blocks = (gx + 7) / 8 * 8 * gy;
     if (blocks * 64 * WM * WN * KP > UINT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_gemm8<MODE, YT, BM, BN, WM, WN, KP, STREAM>), dim3((unsigned)blocks), dim3(64 * WM * WN * KP), 0, st, g);
+    hipLaunchKernelGGL((k_gemm8<MODE, YT, BM, BN, WM, WN, KP, STREAM, ANY>), dim3((unsigned)blocks), dim3(64 * WM * WN * KP), 0, st, g);
     return hipGetLastError();
+}
+
+// The form with the least estimated time: ns for the first round of tiles over the 256 CUs
+// (fixed, and for each 64 of K), and for each further round.  Fits to 257 shapes, M 1 ...
+// 2000, N 512 ... 151936, K 320 ... 6144; of nine forms and 290 shapes the choice is 2.5%
+// behind the best on average, 50% at worst (1 x 60000 x 512: 12.4 us, 8.1 with 64 x 128
+// tiles, which elsewhere gain too little to be told apart).  us, in the order of the list:
+// 32 x 2048 x 6144 8.0, 10.3, 17.5, 31, 37; 32 x 12288 x 2048 12.4, 7.3, 9.2, 13, 16; 404 x
+// 4096 x 1024 34, 17.0, 8.2, 9.9, 12.2; 2000 x 4096 x 1024 155, 68, 25.8, 17.8, 18.0; 1337 x
+// 12288 x 2048 409, 208, 78, 49.5, 42.7; 375 x 151936 x 1024 1153, 562, 217, 120, 109.
+struct Gemm8Form { int bm, bn, one, one_k, more, more_k; };
+static const Gemm8Form g8_forms[] = {{16, 32, 3531, 47, 1969, 42},
+                                     {16, 32, 2908, 70, 792, 20},
+                                     {64, 64, 3529, 141, 1877, 70},
+                                     {128, 128, 4831, 297, 2450, 218},
+                                     {192, 128, 6170, 381, 3731, 256}};
+// the same where operands come through registers; 169 shapes, K 319 ... 6143: 1% behind the
+// best of the four on average, 11% at worst (64 x 4096 x 319).  16 x 2048 x 6143 12.6, 13.4,
+// 23.5, 44; 404 x 4096 x 1023 71, 38, 12.8, 12.8; 2000 x 4999 x 1023 420, 195, 55, 34.5
+static const Gemm8Form g8_any_forms[] = {{16, 32, 5771, 73, 4046, 78},
+                                         {16, 32, 5320, 84, 1037, 60},
+                                         {64, 64, 5453, 169, 1625, 195},
+                                         {128, 128, 5859, 401, 3659, 428}};
+static int gemm8_form(const Gemm8Form *f, int n, const Gemm8Args &g) {
+    const int64_t nk = (g.K + 63) / 64;
+    int best = 0;
+    int64_t best_ns = INT64_MAX;
+    for (int i = 0; i < n; i++) {
+        const int64_t tiles = (g.M + f[i].bm - 1) / f[i].bm * ((g.N + f[i].bn - 1) / f[i].bn), rounds = (tiles + 255) / 256;
+        const int64_t ns = f[i].one + f[i].one_k * nk + (rounds - 1) * (f[i].more + f[i].more_k * nk);
+        if (ns < best_ns) { best_ns = ns; best = i; }
+    }
+    return best;
 }
 
 template <int MODE, typename YT>
 static hipError_t go_gemm8(const Gemm8Args &g, hipStream_t st) {
-    const int vec_k = g.K % 16 == 0 && ((uintptr_t)g.a | (uintptr_t)g.w) % 16 == 0;
-    if (vec_k) {
-        // The form with the least estimated time: ns for the first round of tiles over the 256
-        // CUs (fixed, and for each 64 of K), and for each further round.  Fits to 257 shapes, M 1
-        // ... 2000, N 512 ... 151936, K 320 ... 6144; of nine forms and 290 shapes the choice is
-        // 2.5% behind the best on average, 50% at worst (1 x 60000 x 512: 12.4 us, 8.1 with 64 x
-        // 128 tiles, which elsewhere gain too little to be told apart).  us, in the order of the list: 32 x 2048 x 6144 8.0, 10.3, 17.5, 31, 37; 32 x 12288 x 2048 12.4, 7.3, 9.2, 13, 16;
-        // 404 x 4096 x 1024 34, 17.0, 8.2, 9.9, 12.2; 2000 x 4096 x 1024 155, 68, 25.8, 17.8, 18.0;
-        // 1337 x 12288 x 2048 409, 208, 78, 49.5, 42.7; 375 x 151936 x 1024 1153, 562, 217, 120, 109.
-        static const struct { int bm, bn, one, one_k, more, more_k; } f[] = {{16, 32, 3531, 47, 1969, 42},
-                                                                             {16, 32, 2908, 70, 792, 20},
-                                                                             {64, 64, 3529, 141, 1877, 70},
-                                                                             {128, 128, 4831, 297, 2450, 218},
-                                                                             {192, 128, 6170, 381, 3731, 256}};
-        const int64_t nk = (g.K + 63) / 64;
-        int best = 0;
-        int64_t best_ns = INT64_MAX;
-        for (int i = 0; i < 5; i++) {
-            const int64_t tiles = (g.M + f[i].bm - 1) / f[i].bm * ((g.N + f[i].bn - 1) / f[i].bn), rounds = (tiles + 255) / 256;
-            const int64_t ns = f[i].one + f[i].one_k * nk + (rounds - 1) * (f[i].more + f[i].more_k * nk);
-            if (ns < best_ns) { best_ns = ns; best = i; }
-        }
-        // Results of 32 MB and more whose rows are whole 64-byte pieces go past the caches: f32,
-        // 1337 x 12288 x 2048 50.0 -> 43.0 us, 404 x 60000 x 512 43 -> 32, 1000 x 60000 x 512 90 -> 64,
-        // 375 x 151936 x 1024 110 -> 107.  A smaller result is better left for its reader (a layer of
-        // 404 rows 77.0 us in all, 78.3 with every result past the caches); rows in odd pieces have to
-        // meet in a cache (2021 x 4999 bf16 18.8 us, 24.5).
-        constexpr bool CAN = MODE != G8_ADDTO;      // which gains nothing: its result was read just before
-        const int64_t row = (MODE == G8_SWIGLU ? g.N / 2 : g.N) * (int64_t)sizeof(YT);
-        const bool stream = g.M * row >= (1 << 25) && row % 64 == 0 && (uintptr_t)g.y % 64 == 0;
-        switch (best) {
-            case 0: return go_gemm8_tile<MODE, YT, 16, 32, 1, 1, 8>(g, st);
-            case 1: return go_gemm8_tile<MODE, YT, 16, 32, 1, 1, 4>(g, st);
-            case 2: return go_gemm8_tile<MODE, YT, 64, 64, 2, 2, 2>(g, st);
-            case 3: return stream ? go_gemm8_tile<MODE, YT, 128, 128, 2, 4, 1, CAN>(g, st) : go_gemm8_tile<MODE, YT, 128, 128, 2, 4, 1>(g, st);
-            default: return stream ? go_gemm8_tile<MODE, YT, 192, 128, 2, 4, 1, CAN>(g, st) : go_gemm8_tile<MODE, YT, 192, 128, 2, 4, 1>(g, st);
+    if (g.K % 16 != 0 || ((uintptr_t)g.a | (uintptr_t)g.w) % 16 != 0) {
+        switch (gemm8_form(g8_any_forms, 4, g)) {
+            case 0: return go_gemm8_tile<MODE, YT, 16, 32, 1, 1, 8, false, true>(g, st);
+            case 1: return go_gemm8_tile<MODE, YT, 16, 32, 1, 1, 4, false, true>(g, st);
+            case 2: return go_gemm8_tile<MODE, YT, 64, 64, 2, 2, 2, false, true>(g, st);
+            default: return go_gemm8_tile<MODE, YT, 128, 128, 2, 4, 1, false, true>(g, st);
         }
     }
-    const int64_t gx = (g.N + 63) / 64, gy = (g.M + 63) / 64;
-    if (gx * gy * 256 > UINT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_gemm8_any<MODE, YT>), dim3((unsigned)(gx * gy)), dim3(256), 0, st, g);
-    return hipGetLastError();
+    // Results of 32 MB and more whose rows are whole 64-byte pieces go past the caches: f32,
+    // 1337 x 12288 x 2048 50.0 -> 43.0 us, 404 x 60000 x 512 43 -> 32, 1000 x 60000 x 512 90 -> 64,
+    // 375 x 151936 x 1024 110 -> 107.  A smaller result is better left for its reader (a layer of
+    // 404 rows 77.0 us in all, 78.3 with every result past the caches); rows in odd pieces have to
+    // meet in a cache (2021 x 4999 bf16 18.8 us, 24.5).
+    constexpr bool CAN = MODE != G8_ADDTO;      // which gains nothing: its result was read just before
+    const int64_t row = (MODE == G8_SWIGLU ? g.N / 2 : g.N) * (int64_t)sizeof(YT);
+    const bool stream = g.M * row >= (1 << 25) && row % 64 == 0 && (uintptr_t)g.y % 64 == 0;
+    switch (gemm8_form(g8_forms, 5, g)) {
+        case 0: return go_gemm8_tile<MODE, YT, 16, 32, 1, 1, 8>(g, st);
+        case 1: return go_gemm8_tile<MODE, YT, 16, 32, 1, 1, 4>(g, st);
+        case 2: return go_gemm8_tile<MODE, YT, 64, 64, 2, 2, 2>(g, st);
+        case 3: return stream ? go_gemm8_tile<MODE, YT, 128, 128, 2, 4, 1, CAN>(g, st) : go_gemm8_tile<MODE, YT, 128, 128, 2, 4, 1>(g, st);
+        default: return stream ? go_gemm8_tile<MODE, YT, 192, 128, 2, 4, 1, CAN>(g, st) : go_gemm8_tile<MODE, YT, 192, 128, 2, 4, 1>(g, st);
+    }
 }
 
 hipError_t launch_gemm_w8a8(const Gemm8Args &g, int mode, bool y_bf16, hipStream_t st) {

@@ -174,7 +174,7 @@ def test_gemm(dev, M, N, Kd, mode, with_bias, is_bf16):
 # what the larger tiles, and long K-steps in eight groups, are chosen for: edges inside a tile, rows of y of every alignment, K-steps that end inside 128
 LARGE = [(1500, 4102, 336), (900, 5004, 2000), (1337, 6001, 80), (641, 12290, 464), (1153, 4100, 1104), (1700, 4999, 1040),
          (2100, 8192, 272), (2100, 4032, 1040), (2000, 6144, 1024), (40, 1003, 6000), (17, 515, 2000),
-         (400, 20004, 4016)]                            # the last: weights past the caches
+         (2000, 2501, 1023), (40, 1003, 6001), (33, 6001, 1030), (130, 4099, 519), (400, 20004, 4016)]                            # the last: weights past the caches
 
 
 @pytest.mark.parametrize("mode,with_bias,is_bf16", [("plain", True, False), ("add", True, True), ("swiglu", True, True)])
