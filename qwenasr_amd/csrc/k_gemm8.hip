@@ -131,8 +131,8 @@ __global__ __launch_bounds__(64 * WM * WN * KP, KP == 1 ? 4 : 2) void k_gemm8(Ge
     const int nk = (int)((K + BK - 1) / BK), nit = (nk + KP - 1) / KP;
     // The K-step that this row tile begins with.  Weights that come from HBM (80 MB and more: the
     // cache behind the L2s has let go of them) are fetched by a strip's row tiles at different
-    // places then, twice the bytes in flight with two tiles: 375 x 151936 x 1024 106 -> 100 us,
-    // 2000 x 40000 x 2048 206 -> 192.  Weights that a cache holds are better met by all at once:
+    // places then, twice the bytes in flight with two tiles: 375 x 151936 x 1024 106 -> 100 us
+    // (though an L2 lets go of a part and 250 MB are fetched for 161), 2000 x 40000 x 2048 206 -> 192.  Weights that a cache holds are better met by all at once:
     // 1337 x 12288 x 6144 118 us, 121.5 in turn; 32 x 12288 x 2048 7.6, 9.7.
     const int turn = N * K >= 80000000 ? (int)((int64_t)row * nk / rows) : 0;
     // the epilogue's operands, ahead of the ring's loads
