@@ -700,7 +700,7 @@ __global__ __launch_bounds__(64 * CG * PG, SHARED ? 4 : 2) void k_attn_kv8(AttnK
             for (int i = 1; i < 16; i++) mb = fmaxf(mb, s[i]);
             mb = xhalf_max(xrow16_max(mb)) * kf;
 #pragma unroll
-            for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], kf, -mb));
+            for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(s[i] * kf - mb);   // two roundings: at most 1, as the digits hold
         } else {
             mb = -__builtin_inff();
 #pragma unroll
