@@ -249,8 +249,11 @@ int qasr_hip_kv8_read(qasr_hip *h, void *k, void *v, int64_t ld, const int8_t *k
  * over the cache: out [n_rows][n_heads * head_dim] of q's type = softmax(scale *
  * q . k) v.  Row i of sequence j sees the positions up to pos[j] + i; with window
  * > 0 only the last window of those and the first sinks.  A row that sees nothing
- * gives zeros; rows behind the last sequence are left as they were.  Scores are
- * f32: one that f32 does not hold makes its row NaN.  max_len (0:
+ * gives zeros; rows behind the last sequence are left as they were.  Rows of q and
+ * the cache's values enter exactly, sums are f32.  A weight is off by f32 rounding of
+ * itself (bf16 rows: by 2^-17 of itself), however small it is beside its row's
+ * largest.  Scores are f32: where the largest that a row sees among the positions of
+ * a block is one that f32 does not hold, the row becomes NaN.  max_len (0:
  * capacity): about the longest pos + rows, by which the work is split; results do
  * not depend on it beyond f32 rounding.  Uses the handle's scratch area, and so
  * does a graph that holds the call: launch it on the handle's stream, or in

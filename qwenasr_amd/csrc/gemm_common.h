@@ -20,9 +20,11 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 //   - wait_vmcnt<N> here is right where at least N loads of the wave are younger
 //     than the ones it waits for.  k_gemm_lds and k_gemm_ring: the loads of the
 //     NS - 2 stages behind (their other loads come before the first stage or
-//     after the last wait).  k_gemm_ks, k_gemm8, k_attn_kv8: N = 0.  k_attn_mfma and k_attn_bf3: the
+//     after the last wait).  k_gemm_ks, k_gemm8: N = 0.  k_attn_mfma and k_attn_bf3: the
 //     L loads of the next K tile or of the V tile; q is loaded behind the first
-//     two tiles and waited for ahead of the loop.
+//     two tiles and waited for ahead of the loop.  k_attn_kv8: the NL loads of V
+//     behind K's, of the next K behind V's; the last block is loaded once more, so
+//     that they are there in every turn.
 // The compiler makes no use of M0 in the kernels of the files that include this
 // header (every mention of it in their generated code is one of these lines).
 // The s_nop is the wait state GFX9 asks for between a scalar write of M0 and
@@ -52,6 +54,9 @@ __device__ __forceinline__ void wait_vmcnt() {
     static_assert(N >= 0 && N < 64, "vmcnt");
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+
+// every LDS access that the wave has issued is done
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // float pair -> bf16 pair, round to nearest even (v_cvt_pk_bf16_f32)
 __device__ __forceinline__ uint32_t cvt_pk_bf16(float a, float b) {

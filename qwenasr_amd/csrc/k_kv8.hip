@@ -412,60 +412,84 @@ hipError_t launch_kv8_read(const Kv8Args &a0, bool bf16, hipStream_t st) {
 // ---------------------------------------------------------------------------
 // attention
 //
-// Per tile of 16 query rows (row = query row x heads of the group, flattened) and
-// KV head: S = scale q.k over blocks of 64 positions with the running maximum and
-// sum of the softmax, O += P V.  Everything is exact integer products:
-//   q: round(q c), c = N / max|q| of the row, in D signed base-256 digits, one MFMA
-//      a digit
-//   p: round(N p), p = 2^(s - the block's own maximum) in [0, 1], the same digits
-// with N = 8e6 and D = 3 for f32 rows (a value is off by at most 6e-8 of the largest
-// of its row or block) and N = 32000, D = 2 for bf16 rows (1.6e-5; their output is
-// rounded to 2^-8 of itself).  p is counted from the block's maximum and not the
-// running one: where one position far back holds the maximum (a sink), what is left
-// of every other block would otherwise vanish in the rounding, and the loss would
-// grow with the context.  A block's scale is the same for all of its 64 positions:
-// it joins the score's factor (K) and the product's (V).
+// Per tile of R flattened rows (query rows x heads of the group) and KV head:
+// S = scale q.k over blocks of 64 positions with the running maximum and sum of the
+// softmax, O += P V, both products on bf16 MFMA with operands that lose nothing:
+//   K, V: an int8 value is a bf16 value; the block's scale joins the score's factor
+//      (K) and the product's (V)
+//   q: bf16 rows as they are, f32 rows in three bf16 terms, which hold all 24 bits
+//   p: in three terms for f32 rows (a weight is off by 2^-24 of itself), in two for
+//      bf16 rows (2^-17, their output is rounded to 2^-8 of itself)
+// The weights are floating point, so small ones beside a large one keep all of their
+// bits: where a position with next to nothing in V holds the maximum (a sink), the
+// others alone are the result.  (Whole numbers of a block's largest weight, in base-256
+// digits on the int8 MFMA, lose them: at 12 behind such a position 64 bf16 weights were
+// 0, and f32 ones off by 3e-3.  That was faster, two or three products of half the
+// length and no conversion: 1337 f32 rows 26 us, now 35; bf16 21, now 25; 4 x 67
+// bf16 rows in a window of 8192 35, now 39, with the merge; one row a sequence as now.)
 //
 // The sums (O and the weights') count from a reference that moves only when a
 // block's maximum is 2^16 above it: in f32 they lose nothing by that, and most
 // blocks rescale nothing.
 //
-// What bounds it: the HBM reads where every sequence has one row; vector
-// instructions where rows share the positions (a score's way from the integer sums
-// to the digits is about 14 instructions, a product's value 5; three in bf16).
+// What bounds it: the HBM reads where every sequence has one row.  Where rows share
+// the positions, a wave's instructions: 384 vector ones to convert a block's K and V,
+// 300 for 32 columns' weights and their terms, 64 for O; beside them 96 (f32) or 48
+// matrix ones of 33 cycles, which let a vector one through in only 14 of them.
 //
-// A block takes CG tiles (CG x 16 flattened rows) with CG x PG waves: PG groups of
-// waves take every PG-th block of positions each, the CG waves of a group one tile
-// each.  SHARED: a group's K and V blocks come through one slot each in LDS, direct
-// from memory (global_load_lds_dwordx4), K while the block before is multiplied by
-// its weights, V during the scores.  (Operands loaded straight into registers leave
-// the four lanes of a quad in four rows: a 64-byte run is then asked for four times
-// over, and 16 KB a tile and block at 5.3 TB/s was the end, cached or not.  Two slots
-// each, a whole block ahead: 36 us for 29 at 1337 rows; the waves that the LDS then
-// keeps out are worth more.)  With `splits` > 1 several blocks share a tile's
-// positions; a second launch merges their parts.
+// R = 16: one tile a sequence and head, K and V straight into registers.  R = 32: two
+// conversions' worth of tiles share one.  Each of a block's 4 waves takes every 4th
+// block of positions, on its own: no barrier before their parts are joined.  K and V
+// come through a slot each of the wave in LDS, direct from memory
+// (global_load_lds_dwordx4), the next K's loads on their way during the weights and
+// the second product, the next V's during the first one.  (Operands loaded straight
+// into registers leave the four lanes of a quad in four rows: a 64-byte run is then
+// asked for four times over, and 16 KB a tile and block at 5.3 TB/s was the end,
+// cached or not.)  Other forms, 1337 f32 rows / 3 x 100 rows behind 8000: tiles of 16
+// by two waves that share slots, 39 / 85 us; two tiles of 16 by one wave on 16 x 16 x
+// 32 products, which hold vector instructions up longer, 41 / 63; the converted blocks
+// in LDS for two or four tiles 41 / 74 and 42 / 81; q in four base-256 digits on the
+// int8 MFMA, the weights as now, 39 / 67.  With `splits` > 1 several blocks share a
+// tile's positions; a second launch merges their parts.
 // ---------------------------------------------------------------------------
 
-// Digit dwords: digit d of 4 values in one dword, a byte each.  Signed base-256
-// digits are the bytes of (n + 0x..8080) ^ 0x..8080; the highest of a value that is
-// not negative needs no offset.  v holds the sums in its low bytes.
-template <int D, bool SIGNED>
-__device__ __forceinline__ void digits4(const uint32_t *v, uint32_t *d) {
-    const uint32_t a = __builtin_amdgcn_perm(v[1], v[0], 0x05010400), b = __builtin_amdgcn_perm(v[3], v[2], 0x05010400);
-    d[0] = __builtin_amdgcn_perm(b, a, 0x05040100) ^ 0x80808080u;
-    d[1] = __builtin_amdgcn_perm(b, a, 0x07060302);
-    if (D == 3 || SIGNED) d[1] ^= 0x80808080u;
-    if (D == 3) {
-        const uint32_t e = __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0602), f = __builtin_amdgcn_perm(v[3], v[2], 0x06020c0c);
-        d[D - 1] = e | f;
-        if (SIGNED) d[D - 1] ^= 0x80808080u;
-    }
+// 4 int8 values as bf16, which holds each: the upper halves of their floats
+__device__ __forceinline__ void kv8_bf16(int w, uint32_t *o) {
+    const float f0 = (float)(int8_t)w, f1 = (float)(int8_t)(w >> 8), f2 = (float)(int8_t)(w >> 16), f3 = (float)(w >> 24);
+    o[0] = __builtin_amdgcn_perm(__float_as_uint(f1), __float_as_uint(f0), 0x07060302);
+    o[1] = __builtin_amdgcn_perm(__float_as_uint(f3), __float_as_uint(f2), 0x07060302);
 }
-// the value of a product's digit sums
-template <int D>
-__device__ __forceinline__ float digit_sum(const i32x4 *acc, int r) {
-    if (D == 2) return (float)(acc[1][r] * 256 + acc[0][r]);
-    return fmaf((float)(acc[D - 1][r] * 256 + acc[1][r]), 256.0f, (float)acc[0][r]);
+// 16 of them: the operands of two products
+__device__ __forceinline__ void kv8_operand(i32x4 v, bf16x8 *o) {
+    uint32_t d[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) kv8_bf16(v[i], d + 2 * i);
+    o[0] = __builtin_bit_cast(bf16x8, make_uint4(d[0], d[1], d[2], d[3]));
+    o[1] = __builtin_bit_cast(bf16x8, make_uint4(d[4], d[5], d[6], d[7]));
+}
+// 8 values in T bf16 terms, each the nearest to what the ones before it leave
+template <int T>
+__device__ __forceinline__ void kv8_terms(const float *x, bf16x8 *o) {
+    if constexpr (T == 3) {
+        split3(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), o);
+    } else {
+        uint32_t c0, c1, hi[4], lo[4];                         // the residuals as split3 forms them
+        if (T == 2) {
+            asm("s_mov_b32 %0, 0xbf80" : "=s"(c0));
+            asm("s_mov_b32 %0, 0xbf800000" : "=s"(c1));
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            hi[e] = cvt_pk_bf16(x[2 * e], x[2 * e + 1]);
+            if (T == 2) {
+                const bf16x2 h = __builtin_bit_cast(bf16x2, hi[e]);
+                lo[e] = cvt_pk_bf16(__builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, c0), x[2 * e], false),
+                                    __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, c1), x[2 * e + 1], false));
+            }
+        }
+        o[0] = __builtin_bit_cast(bf16x8, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+        if (T == 2) o[T - 1] = __builtin_bit_cast(bf16x8, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+    }
 }
 
 // 4 output values of flattened row f, dims d .. d + 3, from O and the weights' sum
@@ -498,45 +522,58 @@ __device__ __forceinline__ void kv8_put(const AttnKv8Args &a, const Kv8Seq &sq, 
     }
 }
 
-// one split's part of a tile in the scratch area: maxima and sums [2][16], then O [16][HD]
+// one split's part of 16 rows in the scratch area: maxima and sums [2][16], then O [16][HD]
 template <int HD> constexpr int kv8_part = 32 + 16 * HD;
+#define KV8_WAVES 4           // of a block: each takes every 4th block of positions
 
-template <bool BF16, int HD, int CG, int PG, bool SHARED>
-__global__ __launch_bounds__(64 * CG * PG, SHARED ? 4 : 2) void k_attn_kv8(AttnKv8Args a) {
-    constexpr int KS = HD / 64, DT = HD / 16, D = BF16 ? 2 : 3, TB = 64 * HD, LD = HD / 8 / CG;   // bytes of a block; a wave's loads of K and V
-    constexpr float N = BF16 ? 32000.0f : 8.0e6f;
-    static_assert(SHARED || CG == 1, "waves that share a block's positions share its bytes in LDS");
-    constexpr int MERGE = CG * PG * 16 * (HD + 4) * 4, SLOTS = SHARED ? PG * 2 * TB : 0;
+// The products of an R x R tile.  Lane l has column l % R; with g = l / R and NG = 64 / R such groups it gives the 8 values
+// of its group to the K dimension and receives rows 4 NG (i / 4) + 4 g + i % 4.
+template <int R> struct Kv8Mfma;
+template <> struct Kv8Mfma<16> {
+    typedef f32x4 Acc;
+    __device__ __forceinline__ static Acc mul(bf16x8 a, bf16x8 b, Acc c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    __device__ __forceinline__ static float max(float v) { return xhalf_max(xrow16_max(v)); }      // over the groups
+    __device__ __forceinline__ static float sum(float v) { return xhalf_sum(xrow16_sum(v)); }
+};
+template <> struct Kv8Mfma<32> {
+    typedef float Acc __attribute__((ext_vector_type(16)));
+    __device__ __forceinline__ static Acc mul(bf16x8 a, bf16x8 b, Acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    __device__ __forceinline__ static float max(float v) { return xhalf_max(v); }
+    __device__ __forceinline__ static float sum(float v) { return xhalf_sum(v); }
+};
+
+template <bool BF16, int HD, int R>
+__global__ __launch_bounds__(64 * KV8_WAVES, 2) void k_attn_kv8(AttnKv8Args a) {
+    typedef Kv8Mfma<R> Mfma;
+    constexpr bool LDS = R == 32;
+    constexpr int PG = KV8_WAVES, NG = 64 / R, NA = R * R / 64, TB = 64 * HD, NL = TB / 1024;   // TB: bytes of a block; NL: loads of it into LDS
+    constexpr int KT = 64 / R, KM = HD / (16 * NG), VT = HD / R, VM = 4 / NG;   // tiles of positions and dims; 16-byte operands of each
+    constexpr int QT = BF16 ? 1 : 3, PT = BF16 ? 2 : 3;        // terms of q and of the weights
+    constexpr int MERGE = PG * R * (HD + 4) * 4, SLOTS = LDS ? PG * 2 * TB : 0;
     __shared__ __attribute__((aligned(16))) char smem[MERGE > SLOTS ? MERGE : SLOTS];
-    __shared__ float ml_l[CG * PG][2][16];
+    __shared__ float ml_l[PG][2][R];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int cg = wid % CG, pg = wid / CG;
-    const int c = lane & 15, g = lane >> 4;
-    // Heads fastest: with 8 of them each XCD (blocks go to the 8 in turn) has one head's
-    // cache in its L2.  Tiles from the longest on, but every second 256 blocks the other way
-    // round: a CU that has a long tile gets a short one next (1337 rows 29.3 -> 28.2 us).
+    const int c = lane % R, g = lane / R;
+    // Heads fastest: with 8 of them each XCD (blocks go to the 8 in turn) has one head's cache in its L2.  Tiles from
+    // the longest on, but the `first` shortest ahead of all
     const int j = blockIdx.y, S = a.splits;
     const unsigned rest = blockIdx.x / (unsigned)a.c.Hkv;
     const int h = blockIdx.x - rest * a.c.Hkv, tx = rest / (unsigned)S, split = rest - tx * S;
-    const int run = max(1, 256 / (a.c.Hkv * S)), turn = tx / run;
-    const int back = (turn & 1) && (turn + 1) * run <= a.tiles ? (2 * turn + 1) * run - 1 - tx : tx;
-    const int tile0 = (a.tiles - 1 - back) * CG, tile = tile0 + cg;
+    const int tile = tx < a.first ? tx : a.tiles - 1 - (tx - a.first);
     const Kv8Seq sq = kv8_seq(a.c, j);
     // flattened rows: fewer than 2^30 (the entry point)
-    const unsigned n_flat = (unsigned)sq.n * (unsigned)a.G;
-    if ((unsigned)tile0 * 16 >= n_flat) return;
-    const unsigned f0 = (unsigned)tile * 16, f1 = n_flat - 1;      // a tile past the last row repeats it
-    const unsigned fr = min(f0 + c, f1);
-    const int qi = (int)(fr / (unsigned)a.G), qg = (int)(fr - (unsigned)qi * (unsigned)a.G);
-    const int i_lo = (int)(min(f0, f1) / (unsigned)a.G), i_hi = (int)(min(f0 + 15, f1) / (unsigned)a.G);
-    const int last = sq.p0 + qi;                               // this column's own position, and its window's first
+    const unsigned n_flat = (unsigned)sq.n * (unsigned)a.G, f0 = (unsigned)tile * R;
+    if (f0 >= n_flat) return;
+    const unsigned f1 = n_flat - 1, fr = min(f0 + c, f1);      // a column past the last row repeats it
+    const int i_lo = (int)(f0 / (unsigned)a.G), i_hi = (int)(min(f0 + R - 1, f1) / (unsigned)a.G);
+    const int last = sq.p0 + (int)(fr / (unsigned)a.G);        // this column's own position, and its window's first
     const int low = a.window > 0 ? last - a.window + 1 : INT32_MIN;
 
-    // the blocks that some row of the block's tiles sees: the sinks' and the window's; this split's run of them
-    const int hi_pos = min(sq.p0 + (int)(min((unsigned)(tile0 + CG) * 16 - 1, f1) / (unsigned)a.G), a.c.cap - 1);
+    // the blocks that some row of the tile sees: the sinks' and the window's; this split's run of them
+    const int hi_pos = min(sq.p0 + i_hi, a.c.cap - 1);
     int lo_pos = 0, n_sink = 0;
     if (a.window > 0) {
-        lo_pos = max(0, sq.p0 + (int)((unsigned)tile0 * 16 / (unsigned)a.G) - a.window + 1);
+        lo_pos = max(0, sq.p0 + i_lo - a.window + 1);
         n_sink = min((a.sinks + 63) / 64, lo_pos / 64);
     }
     const int lo_blk = lo_pos / 64;
@@ -548,270 +585,308 @@ __global__ __launch_bounds__(64 * CG * PG, SHARED ? 4 : 2) void k_attn_kv8(AttnK
     const int64_t head = (int64_t)j * a.c.Hkv + h;
     const int8_t *kb = a.c.k8 + head * a.c.cap * HD, *vb = a.c.v8 + head * a.c.cap * HD;
     const float *ks = a.c.ks + head * (a.c.cap / 64), *vs = a.c.vs + head * (a.c.cap / 64);
-    int u = u0 + pg;
-    // SHARED: this lane's bytes of the wave's loads
-    char *kt = smem + pg * 2 * TB, *vt = kt + TB;
-    // a load fills 64 slots: 8 rows of 128 bytes (the swizzle repeats every 16 rows) or 16 of 64
+    int u = u0 + wid;
+    // LDS: the wave's own slots of K and V and this lane's bytes of a load, which fills 64 pieces of 16 bytes: 8 rows
+    // of 128 bytes (the swizzle repeats every 16 rows) or 16 of 64
+    char *kt = smem + wid * 2 * TB, *vt = kt + TB;
     const uint32_t v_src = (lane >> 2) * 64 + 16 * ((lane & 3) ^ lds_swz<64>(lane >> 2));
     const uint32_t k_src[2] = {HD == 64 ? v_src : (lane >> 3) * 128 + 16 * ((lane & 7) ^ lds_swz<128>(lane >> 3)),
                                HD == 64 ? v_src : (lane >> 3) * 128 + 16 * ((lane & 7) ^ lds_swz<128>(8 + (lane >> 3)))};
-    static_assert(LD % 4 == 0 || HD == 64, "pairs of loads a wave");
     auto issue_k = [&](int b) {
 #pragma unroll
-        for (int i = 0; i < LD / 2; i++) {
-            const int at = 1024 * (cg * (LD / 2) + i);
-            lds_dma16_s(kb + (int64_t)b * TB + at, k_src[i & 1], kt + at);
-        }
+        for (int i = 0; i < NL; i++) lds_dma16_s(kb + (int64_t)b * TB + 1024 * i, k_src[i & 1], kt + 1024 * i);
     };
     auto issue_v = [&](int b) {
 #pragma unroll
-        for (int i = 0; i < LD / 2; i++) {
-            const int at = 1024 * (cg * (LD / 2) + i);
-            lds_dma16_s(vb + (int64_t)b * TB + at, v_src, vt + at);
-        }
+        for (int i = 0; i < NL; i++) lds_dma16_s(vb + (int64_t)b * TB + 1024 * i, v_src, vt + 1024 * i);
     };
     // otherwise the operands themselves, loaded again as soon as the products have read them
-    i32x4 kr[4][KS], vr[DT];
+    i32x4 kr[KT][KM], vr[VT][VM];
     auto load_k = [&](int b) {
         const int8_t *p = kb + (int64_t)b * TB + c * HD + 16 * g;
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+        for (int t = 0; t < KT; t++)
 #pragma unroll
-            for (int k = 0; k < KS; k++) kr[t][k] = *reinterpret_cast<const i32x4 *>(p + 16 * t * HD + 64 * k);
+            for (int m = 0; m < KM; m++) kr[t][m] = *reinterpret_cast<const i32x4 *>(p + R * t * HD + 16 * NG * m);
     };
     auto load_v = [&](int b) {
         const int8_t *p = vb + (int64_t)b * TB + c * 64 + 16 * g;
 #pragma unroll
-        for (int d = 0; d < DT; d++) vr[d] = *reinterpret_cast<const i32x4 *>(p + 16 * d * 64);
+        for (int t = 0; t < VT; t++)
+#pragma unroll
+            for (int m = 0; m < VM; m++) vr[t][m] = *reinterpret_cast<const i32x4 *>(p + R * t * 64 + 16 * NG * m);
     };
-    // the column's row, ahead of the first block: it is turned into digits while that is on its way
-    float x[KS][16];
-#pragma unroll
-    for (int s = 0; s < KS; s++)
-        kv8_load16<BF16>(a.q, (sq.r0 + qi) * a.ldq + (int64_t)(h * a.G + qg) * HD + 64 * s + 16 * g, a.vec_q, x[s]);
-    __builtin_amdgcn_sched_barrier(0);
-    if (u < u1) {
-        if constexpr (SHARED) {
-            issue_k(block_of(u));
-        } else {
-            load_k(block_of(u));
-            load_v(block_of(u));
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
+    float ksl = 0.0f, vsl = 0.0f;                              // lane i: the scales of this wave's block `it` + i
+    auto scales = [&]() {
+        const int ul = u + lane * PG;
+        ksl = ul < u1 ? ks[block_of(ul)] : 0.0f;
+        vsl = ul < u1 ? vs[block_of(ul)] : 0.0f;
+    };
+    auto row_at = [&](unsigned f) {
+        const unsigned i = f / (unsigned)a.G;
+        return (sq.r0 + i) * a.ldq + (int64_t)(h * a.G + (int)(f - i * (unsigned)a.G)) * HD;
+    };
 
-    // the column's row in signed digits: dims 64 s + 16 g + 0..15 of product s
-    i32x4 qd[KS][D];
-    float qf;                                                  // score = integer sum x qf x the block's scale
-    {
-        float m = 0.0f;
-        bool bad = false;
+    // The column's row, dims 16 (NG m + g) + 0..15 in x[m], the first blocks and their scales, at once.  LDS: the
+    // rows come through the V slots, once a block and by whole rows (a lane's own loads, 64 bytes apart, for all
+    // four waves: 1337 rows 44 -> 41 us), piece n of row r at n ^ (r & 15)
+    constexpr int ES = BF16 ? 2 : 4, QR = HD * ES, QP = QR / 16, NQ = R * QR / 1024 / PG;
+    float x[KM][16];
+    const bool by_lds = LDS && a.vec_q;
+    if (!by_lds) {
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
+        for (int m = 0; m < KM; m++) kv8_load16<BF16>(a.q, row_at(fr) + 16 * (NG * m + g), a.vec_q, x[m]);
+    }
+    if constexpr (LDS) {
+        static_assert(NQ >= 1 && R * QR <= PG * TB, "rows in the V slots");
+        auto chunk = [&](int n) { return smem + TB + n / NL * 2 * TB + n % NL * 1024; };
+        if (by_lds) {
 #pragma unroll
-            for (int e = 0; e < 16; e++) x[s][e] = a.scale < 0.0f ? -x[s][e] : x[s][e];   // the scores' factor is not negative
-#pragma unroll
-            for (int e = 0; e < 16; e++) { m = fmaxf(m, fabsf(x[s][e])); bad |= !kv8_finite(x[s][e]); }
-        }
-        m = xhalf_max(xrow16_max(m));
-        float nf = bad ? 1.0f : 0.0f;
-        nf = xhalf_max(xrow16_max(nf));
-        // a row below 1e-30 multiplies by the largest factor that stays finite with it
-        const float f = __fdiv_rn(N, fmaxf(m, 1e-30f));
-#pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                uint32_t n[4], d[D];
-#pragma unroll
-                for (int i = 0; i < 4; i++) n[i] = (uint32_t)(int)rintf(x[s][4 * e + i] * f) + 0x80808080u;
-                digits4<D, true>(n, d);
-#pragma unroll
-                for (int i = 0; i < D; i++) qd[s][i][e] = (int)d[i];
+            for (int i = 0; i < NQ; i++) {
+                const int n = wid * NQ + i, r = (64 * n + lane) / QP, piece = ((64 * n + lane) % QP) ^ (r & 15 & (QP - 1));
+                lds_dma16(reinterpret_cast<const char *>(a.q) + row_at(min(f0 + r, f1)) * ES + 16 * piece, chunk(n));
             }
-        qf = nf > 0.0f ? __builtin_nanf("") : fabsf(a.scale) * 1.4426950408889634f * __fdiv_rn(1.0f, f);
-    }
-
-    float m = -__builtin_inff(), l = 0.0f;                     // m: what O and l count from
-    f32x4 o[DT];
-#pragma unroll
-    for (int d = 0; d < DT; d++) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-    float ksl = 0.0f, vsl = 0.0f;                              // lane i: the scales of this group's block `it` + i
-    const int n_it = (u1 - u0 + PG - 1) / PG;
-    for (int it = 0; it < n_it; it++, u += PG) {
-        if ((it & 63) == 0) {
-            const int ul = u + lane * PG;
-            ksl = ul < u1 ? ks[block_of(ul)] : 0.0f;
-            vsl = ul < u1 ? vs[block_of(ul)] : 0.0f;
-            // waited for here: a wait at their use would drain the loads in flight in every turn
-            asm volatile("" : "+v"(ksl), "+v"(vsl));
         }
-        const bool live = u < u1;
-        const int b = block_of(u), bn = block_of(min(u + PG, u1 - 1));
-        if constexpr (SHARED) {
-            wait_vmcnt<0>();                                   // this wave's part of the block's K has landed
-            __syncthreads();                                   // ... and every wave's; V of the block before has been read
-            if (live) issue_v(b);
+        if (u < u1) {
+            issue_k(block_of(u));
+            scales();
         }
-        if (!live) {                                           // the other groups' last block
-            if (SHARED) __syncthreads();
-            continue;
-        }
-        const float ksb = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ksl), it & 63));
-        const float vsb = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vsl), it & 63));
-        // a product's sums are read behind the next product's issue
-        float s[16];
-        {
-            i32x4 acc[2][D];
+        if (by_lds) {
+            wait_vmcnt<0>();
+            __syncthreads();
 #pragma unroll
-            for (int t = 0; t <= 4; t++) {
-                if (t < 4) {
+            for (int m = 0; m < KM; m++)
 #pragma unroll
-                    for (int d = 0; d < D; d++) acc[t & 1][d] = i32x4{0, 0, 0, 0};
+                for (int e = 0; e < ES; e++) {
+                    const int at = c * QR + 16 * ((ES * (NG * m + g) + e) ^ (c & 15 & (QP - 1)));
+                    const char *p = chunk(at / 1024) + at % 1024;
+                    if constexpr (BF16) {
+                        const u16x8 v = *reinterpret_cast<const u16x8 *>(p);
 #pragma unroll
-                    for (int k = 0; k < KS; k++) {
-                        const int r = 16 * t + c;
-                        if (SHARED) kr[t][k] = *reinterpret_cast<const i32x4 *>(kt + r * HD + 16 * ((4 * k + g) ^ lds_swz<HD>(r)));
+                        for (int i = 0; i < 8; i++) x[m][8 * e + i] = bf16_to_f32(v[i]);
+                    } else {
+                        const f32x4 v = *reinterpret_cast<const f32x4 *>(p);
 #pragma unroll
-                        for (int d = 0; d < D; d++)
-                            acc[t & 1][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kr[t][k], qd[k][d], acc[t & 1][d], 0, 0, 0);
+                        for (int i = 0; i < 4; i++) x[m][4 * e + i] = v[i];
                     }
                 }
-                if (t > 0) {
+            wait_lds();
+            __syncthreads();                                   // every wave has its rows
+        }
+        if (u < u1) issue_v(block_of(u));
+    } else if (u < u1) {
+        load_k(block_of(u));
+        load_v(block_of(u));
+        scales();
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    // the row in bf16 terms
+    bf16x8 qd[KM][2][QT];
+    float qf;                                                  // score = sum x qf x the block's scale
+    {
+        float m = 0.0f, z = 0.0f;                              // z: NaN after a value that is not finite
 #pragma unroll
-                    for (int r = 0; r < 4; r++) s[4 * (t - 1) + r] = digit_sum<D>(acc[(t - 1) & 1], r);
-                }
+        for (int k = 0; k < KM; k++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) { m = fmaxf(m, fabsf(x[k][e])); z = fmaf(x[k][e], 0.0f, z); }
+        m = Mfma::max(m);
+        z = Mfma::sum(z);
+        // rows whose sums f32 might not hold, or whose terms bf16, a power of two nearer to 1
+        const int ex = (int)(__float_as_uint(m) >> 23) - 127, sh = z != 0.0f ? 0 : ex > 100 ? ex - 100 : ex < -60 ? ex + 60 : 0;
+        const float f = __uint_as_float((uint32_t)(127 - sh) << 23);
+        const float to = a.scale < 0.0f ? -f : f;              // the scores' factor is not negative
+        if (__any(to != 1.0f)) {
+#pragma unroll
+            for (int k = 0; k < KM; k++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[k][e] *= to;
+        }
+#pragma unroll
+        for (int k = 0; k < KM; k++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) kv8_terms<QT>(&x[k][8 * i], qd[k][i]);
+        // a row that is not finite: NaN, in its own column alone
+        qf = z != 0.0f ? __builtin_nanf("") : fabsf(a.scale) * 1.4426950408889634f * __uint_as_float((uint32_t)(127 + sh) << 23);
+    }
+    // waited for here and below: a wait at their use would drain the loads in flight in every turn
+    asm volatile("" : "+v"(ksl), "+v"(vsl));
+
+    float m = -__builtin_inff(), l = 0.0f;                     // m: what O and l count from
+    typename Mfma::Acc o[VT];
+#pragma unroll
+    for (int t = 0; t < VT; t++)
+#pragma unroll
+        for (int i = 0; i < NA; i++) o[t][i] = 0.0f;
+
+    for (int it = 0; u < u1; it++, u += PG) {
+        if ((it & 63) == 0 && it > 0) {
+            scales();
+            asm volatile("" : "+v"(ksl), "+v"(vsl));
+        }
+        // the block behind the last one is the last one again: the waits count the same
+        const int b = block_of(u), bn = block_of(min(u + PG, u1 - 1));
+        const float ksb = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(ksl), it & 63));
+        const float vsb = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vsl), it & 63));
+        if constexpr (LDS) wait_vmcnt<NL>();                   // K has landed; V's loads are behind it
+        __builtin_amdgcn_sched_barrier(0);
+        float s[KT * NA];
+#pragma unroll
+        for (int t = 0; t < KT; t++) {
+            typename Mfma::Acc acc;
+#pragma unroll
+            for (int i = 0; i < NA; i++) acc[i] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KM; k++) {
+                const int r = R * t + c;
+                if constexpr (LDS) kr[t][k] = *reinterpret_cast<const i32x4 *>(kt + r * HD + 16 * ((NG * k + g) ^ lds_swz<HD>(r)));
+                bf16x8 kv[2];
+                kv8_operand(kr[t][k], kv);
+#pragma unroll
+                for (int e = QT - 1; e >= 0; e--)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) acc = Mfma::mul(kv[i], qd[k][i][e], acc);
             }
+#pragma unroll
+            for (int i = 0; i < NA; i++) s[NA * t + i] = acc[i];
         }
-        if constexpr (!SHARED) {
-            __builtin_amdgcn_sched_barrier(0);
-            load_k(bn);                                        // a whole block ahead of their use
-            __builtin_amdgcn_sched_barrier(0);
+        // one product, then its share of the next operands' conversion: the two run side by side
+        constexpr int QN = KT * KM * 2 * QT;
+        __builtin_amdgcn_sched_group_barrier(0x100, KT * KM, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 24, 0);
+#pragma unroll
+        for (int i = 0; i < QN; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, KT * KM * 24 / QN, 0);
         }
-        // p from the integer sums; mb: the block's maximum
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (LDS) wait_lds();                         // K has been read
+        if constexpr (LDS) issue_k(bn);
+        else load_k(bn);                                       // a whole block ahead of their use
+        __builtin_amdgcn_sched_barrier(0);
+
+        // mb: the block's maximum of what the column sees
         const float kf = ksb * qf;
-        float mb, p[16];
-        if (ksb >= 0.0f && b * 64 + 63 <= sq.p0 + i_lo &&
-            (a.window == 0 || b * 64 > sq.p0 + i_hi - a.window || b * 64 + 63 < a.sinks)) {
-            // every row of the tile sees the whole block
+        float mb, kc = kf;
+        bool none = false;
+        if (ksb >= 0.0f && b * 64 + 63 <= sq.p0 + i_lo && (a.window == 0 || b * 64 > sq.p0 + i_hi - a.window || b * 64 + 63 < a.sinks)) {
+            // every row of the tile sees the whole block, and the largest sum is the largest score
             mb = s[0];
 #pragma unroll
-            for (int i = 1; i < 16; i++) mb = fmaxf(mb, s[i]);
-            mb = xhalf_max(xrow16_max(mb)) * kf;
-#pragma unroll
-            for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(s[i] * kf - mb);   // two roundings: at most 1, as the digits hold
+            for (int i = 1; i < KT * NA; i++) mb = fmaxf(mb, s[i]);
+            mb = Mfma::max(mb) * kf;
         } else {
             mb = -__builtin_inff();
+            kc = 1.0f;
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const int at = b * 64 + 16 * (i >> 2) + 4 * g + (i & 3);
+            for (int i = 0; i < KT * NA; i++) {
+                const int at = b * 64 + 4 * NG * (i >> 2) + 4 * g + (i & 3);
                 const bool seen = (at <= last) & ((at >= low) | (at < a.sinks));
                 s[i] = seen ? s[i] * kf : -__builtin_inff();
                 mb = fmaxf(mb, s[i]);
             }
-            mb = xhalf_max(xrow16_max(mb));
-            const float ref = mb == -__builtin_inff() ? 0.0f : mb;
-#pragma unroll
-            for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(s[i] - ref);
+            mb = Mfma::max(mb);
+            none = b * 64 > last || (min(b * 64 + 63, last) < low && b * 64 >= a.sinks);
         }
+        // a column that sees none of this block takes nothing of it, its scale neither; one whose largest score f32
+        // does not hold becomes NaN
+        const float vf = none ? 0.0f : vsb;
+        kc = none || kv8_finite(mb) ? kc : __builtin_nanf("");
+        asm("" : "+v"(kc));                                    // else a select on every weight
         const bool up = mb > m + 16.0f;
         if (__any(up)) {
             const float al = up ? __builtin_amdgcn_exp2f(m - mb) : 1.0f;
             m = up ? mb : m;
             l *= al;
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++)
+            for (int t = 0; t < VT; t++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) o[dt][r] *= al;
+                for (int i = 0; i < NA; i++) o[t][i] *= al;
         }
-        // a column that sees none of this block takes nothing of it, its scale neither
-        const float eb = mb == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(mb - m);
-        const float vf = mb == -__builtin_inff() ? 0.0f : vsb * eb * (1.0f / N);
-        i32x4 pd[D];
-        float sum = 0.0f;
+        const float ref = m == -__builtin_inff() ? 0.0f : m;
+        // the weights in the order of V's bytes: operand k's half i holds those of t = 2 i and 2 i + 1
+        bf16x8 pd[VM][2][PT];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            uint32_t n[4], d[D];
+        for (int k = 0; k < VM; k++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                sum += p[4 * t + r];
-                // 2^23 + the lower digits' offset: the sum's low bytes are round(N p) + that offset
-                n[r] = __float_as_uint(fmaf(p[4 * t + r], N, 8388608.0f + (D == 2 ? 128.0f : 32896.0f)));
+            for (int i = 0; i < 2; i++) {
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(fmaf(s[4 * (4 / NG * (2 * i + (e >> 2)) + k) + (e & 3)], kc, -ref));
+                l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                kv8_terms<PT>(p, pd[k][i]);
             }
-            digits4<D, false>(n, d);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (LDS) wait_vmcnt<NL>();                   // V has landed; the next K's loads are behind it
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int e = 0; e < D; e++) pd[e][t] = (int)d[e];
-        }
-        l = fmaf(sum, eb, l);
-        if constexpr (SHARED) {
-            wait_vmcnt<0>();                                   // V has landed, and every wave has read K
-            __syncthreads();
-            if (u + PG < u1) issue_k(bn);
-        }
-        {
-            i32x4 acc[2][D];
+        for (int t = 0; t < VT; t++) {
+            typename Mfma::Acc acc;
 #pragma unroll
-            for (int dt = 0; dt <= DT; dt++) {
-                if (dt < DT) {
-                    const int vrow = 16 * dt + c;
-                    if (SHARED) vr[dt] = *reinterpret_cast<const i32x4 *>(vt + vrow * 64 + 16 * (g ^ lds_swz<64>(vrow)));
+            for (int i = 0; i < NA; i++) acc[i] = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < D; e++) {
-                        const i32x4 z = {0, 0, 0, 0};
-                        acc[dt & 1][e] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vr[dt], pd[e], z, 0, 0, 0);
-                    }
-                }
-                if (dt > 0) {
+            for (int k = 0; k < VM; k++) {
+                const int r = R * t + c;
+                if constexpr (LDS) vr[t][k] = *reinterpret_cast<const i32x4 *>(vt + r * 64 + 16 * ((NG * k + g) ^ lds_swz<64>(r)));
+                bf16x8 vv[2];
+                kv8_operand(vr[t][k], vv);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) o[dt - 1][r] = fmaf(digit_sum<D>(acc[(dt - 1) & 1], r), vf, o[dt - 1][r]);
-                }
-                // one product, then its share of the last one's vector instructions: the two run side by side
-                if (dt > 0 && dt < DT) {
+                for (int e = PT - 1; e >= 0; e--)
 #pragma unroll
-                    for (int e = 0; e < D; e++) {
-                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                        __builtin_amdgcn_sched_group_barrier(0x002, D == 3 ? 7 : 6, 0);
-                    }
-                }
+                    for (int i = 0; i < 2; i++) acc = Mfma::mul(vv[i], pd[k][i][e], acc);
             }
+#pragma unroll
+            for (int i = 0; i < NA; i++) o[t][i] = fmaf(acc[i], vf, o[t][i]);
         }
-        if constexpr (!SHARED) {
-            __builtin_amdgcn_sched_barrier(0);
-            load_v(bn);
-            __builtin_amdgcn_sched_barrier(0);
+        constexpr int PN = VT * VM * 2 * PT;
+        __builtin_amdgcn_sched_group_barrier(0x100, VT * VM, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 24, 0);
+#pragma unroll
+        for (int i = 0; i < PN; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, (VT * VM * 24 + VT * NA) / PN, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (LDS) wait_lds();                         // V has been read
+        if constexpr (LDS) issue_v(bn);
+        else load_v(bn);
+        __builtin_amdgcn_sched_barrier(0);
     }
-    l = xhalf_sum(xrow16_sum(l));
+    if constexpr (LDS) wait_vmcnt<0>();                        // no load may land in LDS that the parts use
+    l = Mfma::sum(l);
 
-    const int cols = f0 < n_flat ? (int)min(16u, n_flat - f0) : 0;
-    float *part = a.part + ((((int64_t)j * a.c.Hkv + h) * a.tiles * CG + tile) * S + split) * kv8_part<HD>;
-    // the groups' parts of each tile, through the ring's LDS (every load into it has landed and been read)
-    float (*o_l)[16][HD + 4] = reinterpret_cast<float (*)[16][HD + 4]>(smem);
+    const int cols = (int)min((unsigned)R, n_flat - f0);
+    // the waves' parts of the tile, through the slots
+    float (*o_l)[R][HD + 4] = reinterpret_cast<float (*)[R][HD + 4]>(smem);
     __syncthreads();
     if (g == 0) { ml_l[wid][0][c] = m; ml_l[wid][1][c] = l; }
 #pragma unroll
-    for (int dt = 0; dt < DT; dt++) *reinterpret_cast<f32x4 *>(&o_l[wid][c][16 * dt + 4 * g]) = o[dt];
+    for (int t = 0; t < VT; t++)
+#pragma unroll
+        for (int i = 0; i < NA; i += 4)
+            *reinterpret_cast<f32x4 *>(&o_l[wid][c][R * t + NG * i + 4 * g]) = f32x4{o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]};
     __syncthreads();
-    for (int i = lane + 64 * pg; i < cols * (HD / 4); i += 64 * PG) {
+    for (int i = threadIdx.x; i < cols * (HD / 4); i += 64 * PG) {
         const int col = i / (HD / 4), d = 4 * (i % (HD / 4));
         float mm = -__builtin_inff();
 #pragma unroll
-        for (int w = 0; w < PG; w++) mm = fmaxf(mm, ml_l[w * CG + cg][0][col]);
+        for (int w = 0; w < PG; w++) mm = fmaxf(mm, ml_l[w][0][col]);
         const float ms = mm == -__builtin_inff() ? 0.0f : mm;
         float ll = 0.0f;
         f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int w = 0; w < PG; w++) {
-            const float e = __builtin_amdgcn_exp2f(ml_l[w * CG + cg][0][col] - ms);
-            ll = fmaf(ml_l[w * CG + cg][1][col], e, ll);
-            const f32x4 ow = *reinterpret_cast<const f32x4 *>(&o_l[w * CG + cg][col][d]);
+            const float e = __builtin_amdgcn_exp2f(ml_l[w][0][col] - ms);
+            ll = fmaf(ml_l[w][1][col], e, ll);
+            const f32x4 ow = *reinterpret_cast<const f32x4 *>(&o_l[w][col][d]);
 #pragma unroll
             for (int r = 0; r < 4; r++) v[r] = fmaf(ow[r], e, v[r]);
         }
         if (S > 1) {
-            if (d == 0) { part[col] = mm; part[16 + col] = ll; }
-            *reinterpret_cast<f32x4 *>(part + 32 + col * HD + d) = v;
+            const int at = tile * (R / 16) + (col >> 4), cc = col & 15;
+            float *part = a.part + ((((int64_t)j * a.c.Hkv + h) * a.tiles * (R / 16) + at) * S + split) * kv8_part<HD>;
+            if (d == 0) { part[cc] = mm; part[16 + cc] = ll; }
+            *reinterpret_cast<f32x4 *>(part + 32 + cc * HD + d) = v;
         } else {
             kv8_put<BF16, HD>(a, sq, h, f0 + col, d, v, ll);
         }
@@ -870,26 +945,30 @@ __global__ __launch_bounds__(256) void k_attn_kv8_merge(AttnKv8Args a) {
     }
 }
 
-template <bool BF16, int HD, int CG, int PG, bool SHARED>
+template <bool BF16, int HD, int R>
 static hipError_t go_attn_kv8(const AttnKv8Args &a, hipStream_t st) {
     const dim3 grid((unsigned)(a.tiles * a.splits * a.c.Hkv), (unsigned)a.c.n_seq);
-    hipLaunchKernelGGL((k_attn_kv8<BF16, HD, CG, PG, SHARED>), grid, dim3(64 * CG * PG), 0, st, a);
+    hipLaunchKernelGGL((k_attn_kv8<BF16, HD, R>), grid, dim3(64 * KV8_WAVES), 0, st, a);
     if (a.splits > 1)
-        hipLaunchKernelGGL((k_attn_kv8_merge<BF16, HD>), dim3((unsigned)a.tiles * CG, (unsigned)a.c.Hkv, (unsigned)a.c.n_seq), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((k_attn_kv8_merge<BF16, HD>), dim3((unsigned)a.tiles * (R / 16), (unsigned)a.c.Hkv, (unsigned)a.c.n_seq), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
-template <int CG, int PG, bool SHARED>
+template <int R>
 static hipError_t pick_attn_kv8(AttnKv8Args &a, bool bf16, int splits, hipStream_t st) {
-    const int64_t tiles = (a.c.max_rows * a.G + 16 * CG - 1) / (16 * CG), units = tiles * CG * a.c.Hkv * a.c.n_seq;
+    const int64_t tiles = (a.c.max_rows * a.G + R - 1) / R, units = tiles * (R / 16) * a.c.Hkv * a.c.n_seq;
     // the splits' parts fit the scratch area
     int64_t s = std::min<int64_t>(splits, (int64_t)QASR_KV8_PART_BYTES / (units * (32 + 16 * a.c.hd) * 4));
     s = std::max<int64_t>(1, std::min<int64_t>(s, 64));
-    if (tiles * s * a.c.Hkv * 64 * CG * PG > UINT32_MAX || tiles * CG * 256 > UINT32_MAX) return hipErrorInvalidValue;   // the grid's limit
+    if (tiles * s * a.c.Hkv * 64 * KV8_WAVES > UINT32_MAX || tiles * (R / 16) * 256 > UINT32_MAX) return hipErrorInvalidValue;   // the grid's limit
     a.tiles = (int)tiles;
     a.splits = (int)s;
-    if (bf16) return a.c.hd == 128 ? go_attn_kv8<true, 128, CG, PG, SHARED>(a, st) : go_attn_kv8<true, 64, CG, PG, SHARED>(a, st);
-    return a.c.hd == 128 ? go_attn_kv8<false, 128, CG, PG, SHARED>(a, st) : go_attn_kv8<false, 64, CG, PG, SHARED>(a, st);
+    // 512 blocks are on the card at a time.  Some more: so many of the shortest go first, and those of middle length
+    // follow them (1337 rows, 672 blocks: 37 us against 39 with the shortest last)
+    const int64_t per_tile = s * a.c.Hkv * a.c.n_seq, over = (tiles * per_tile - 512 + per_tile - 1) / per_tile;
+    a.first = over > 0 && 2 * over <= tiles ? (int)over : 0;
+    if (bf16) return a.c.hd == 128 ? go_attn_kv8<true, 128, R>(a, st) : go_attn_kv8<true, 64, R>(a, st);
+    return a.c.hd == 128 ? go_attn_kv8<false, 128, R>(a, st) : go_attn_kv8<false, 64, R>(a, st);
 }
 
 hipError_t launch_attention_kv8(const AttnKv8Args &a0, bool bf16, hipStream_t st) {
@@ -904,26 +983,26 @@ hipError_t launch_attention_kv8(const AttnKv8Args &a0, bool bf16, hipStream_t st
     if (rows <= 16) {
         // One tile a sequence and head (decoding): the operands straight into registers, as no
         // second tile shares them.  Positions are split over blocks of 4 waves up to 384 blocks,
-        // a wave left with one block of positions at least; below 25 of them the merge costs what
-        // the split saves.  us, 1 split against these, 8 KV heads x 2 heads of 128, bf16: one
-        // sequence at 4000 positions 25.2 -> 9.9, at 60000 323 -> 30, 4 at 16000 90 -> 24; at 1000
-        // positions 10.9 against 12.2; 32 at 4000 40.3 against 42.5 (2 splits), so one there.
+        // a wave left with one block of positions at least; below 9 of them, 25 from 128 tiles on,
+        // the merge costs what the split saves.  us, 1 split against these, 8 KV heads x 2 heads of
+        // 128, bf16: one sequence at 404 positions 8.9 / 10.1 (2 splits), at 1000 11.5 -> 10.1, at
+        // 4000 29 -> 10, at 60000 323 -> 33; 4 at 16000 98 -> 26; 8 at 1000 12.0 -> 11.1; 16 at 1500
+        // 15.0 / 16.7 (3 splits); 32 at 4000 41 / 42.5 (2 splits).
         const int64_t units = a.c.Hkv * (int64_t)a.c.n_seq;
-        const int splits = blocks <= 24 ? 1 : (int)std::min<int64_t>(384 / units, (blocks + 3) / 4);
-        return pick_attn_kv8<1, 4, false>(a, bf16, splits, st);
+        const int splits = blocks <= (units < 128 ? 8 : 24) ? 1 : (int)std::min<int64_t>(384 / units, (blocks + 3) / 4);
+        return pick_attn_kv8<16>(a, bf16, splits, st);
     }
-    // Two tiles a block.  2 groups of waves a block where 384 blocks are there, else 4 groups
-    // and splits up to 512 blocks, each wave left with 4 blocks of positions at least.  us, 2
-    // groups against 4: 1337 rows 29.4 / 32.4, with bf16 22.6 / 26.6; 404 rows 12.5 / 12.2; 2 x
-    // 300 rows behind 3000 positions 45 / 41; 4 x 67 rows, window 8192: 87 / 61, with 3 splits
-    // 43 + 5 / 38 + 5.
+    // Splits up to 512 blocks, which the card holds at a time; each wave left with two blocks of
+    // positions at least.  us with the merge, 1 split against these: 4 x 67 bf16 rows, window 8192,
+    // 70 -> 40; 3 x 100 f32 rows behind 8000 positions 97 -> 62; 67 f32 rows behind 20000 227 -> 52;
+    // 20 bf16 rows behind 4000 37 -> 20; 404 f32 rows alone 13.7 with 1 and 21 with 2.
     // Sequences shorter than max_rows leave their last tiles' blocks empty: counted are the tiles
     // that n_rows rows fill, and half a tile a sequence (up to 67 rows each, window 8192: 40.2 + 5.3
     // -> 30.7 + 6.5; 6 sequences of up to 100 f32 rows behind 6000 positions 85.7 -> 51 + 5.4).
     const int64_t tiles = std::min((rows + 31) / 32 * a.c.n_seq, (a.c.n_rows * a.G / 16 + a.c.n_seq) / 2 + 1);
     const int64_t units = tiles * a.c.Hkv;
-    if (units >= 384) return pick_attn_kv8<2, 2, true>(a, bf16, 1, st);
-    return pick_attn_kv8<2, 4, true>(a, bf16, (int)std::min<int64_t>(512 / units, blocks / 16), st);
+    if (units >= 384) return pick_attn_kv8<32>(a, bf16, 1, st);
+    return pick_attn_kv8<32>(a, bf16, (int)std::min<int64_t>(512 / units, blocks / 8), st);
 }
 
 }  // namespace qasr

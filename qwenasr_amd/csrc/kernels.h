@@ -401,7 +401,7 @@ struct AttnKv8Args {
     int window, sinks;        // window 0: every position up to the row's own
     int max_len;              // about the longest sequence: the split's measure
     float *part;              // the splits' parts (QASR_KV8_PART_BYTES)
-    int vec_q, vec_o, tiles, splits;   // set by the launcher
+    int vec_q, vec_o, tiles, splits, first;   // set by the launcher
 };
 #define QASR_KV8_PART_BYTES (32u << 20)
 hipError_t launch_attention_kv8(const AttnKv8Args &a, bool bf16, hipStream_t st);

@@ -1,5 +1,6 @@
 """The attention over the int8 cache where its numbers leave the ordinary range: very large scores, one position far
-above the rest.  Against float64."""
+above the rest, rows of q with one value far above the rest, more tiles than the card holds at a time.  Against
+float64."""
 import numpy as np
 import pytest
 
@@ -8,6 +9,8 @@ from conftest import rng
 from test_gpu_layer8 import BF16, F32, DevCache, held, prefix, up, values
 
 pytestmark = pytest.mark.gpu
+
+BLOCK = ref8.BLOCK
 
 
 def attend(dev, ref, q, counts, pos, scale, is_bf16, window=0, sinks=0, max_len=0):
@@ -20,6 +23,39 @@ def attend(dev, ref, q, counts, pos, scale, is_bf16, window=0, sinks=0, max_len=
                     heads, dim, cap, scale, row_start=dev.upload(prefix(counts)), max_len=max_len, window=window, sinks=sinks,
                     bf16=is_bf16)
     return values(out, is_bf16).reshape(q.shape)
+
+
+def weighted(ref, q, pos, scale, is_bf16, window=0, sinks=0):
+    """(result, bound) of one sequence's rows: the formula, and what arithmetic in 32 bits may lose of
+    sum_i weight_i |v_i|, the sum whose terms the result adds."""
+    u, (n, hq, dim) = F32, q.shape
+    k, v = ref.values("k")[0], ref.values("v")[0]
+    heads, cap, _ = k.shape
+    out, bound, p = np.zeros(q.shape), np.zeros(q.shape), np.arange(cap)
+    for i in range(n):
+        last = pos + i
+        seen = (p <= last) & ((p > last - window) | (p < sinks) if window else True)
+        if not seen.any():
+            continue
+        for h in range(hq):
+            kk, vv = k[h * heads // hq][seen], v[h * heads // hq][seen]
+            s = scale * (kk @ q[i, h])
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            out[i, h] = w @ vv
+            # a score's products are exact in up to 3 terms of q; sums of 3 dim of them in any order: 3 dim roundings of
+            # what they add up to.  Six more of the score itself (scale x log2 e, the block's scale, the row's factor, the
+            # product, the difference from the reference, the exponential's argument)
+            e = scale and (3 * dim * u * abs(scale) * (np.abs(kk) @ np.abs(q[i, h])) + 6 * u * np.abs(s - s.max()) + 6 * u * np.abs(s))
+            e = np.broadcast_to(e, s.shape)
+            # a weight: the exponential's two units; the terms that it goes into the product in (2^-17 of it in two, 2^-24
+            # in three); the product's sums, 64 positions in 3 terms in any order; the rescaling and the addition of each
+            # block, and the joining of at most 64 + 4 parts.  And the weights' sum, whose relative error is the largest one's
+            blocks = seen.sum() // BLOCK + 2
+            each = np.expm1(e) + (2.0 ** -17 if is_bf16 else u) + (2 + 192 + 2 * blocks + 72) * u
+            bound[i, h] = (w * each) @ np.abs(vv) + (w @ each) * np.abs(out[i, h])
+    t = BF16 if is_bf16 else F32
+    return out, bound + t * (np.abs(out) + bound)
 
 
 @pytest.mark.parametrize("is_bf16", [False, True])
@@ -44,3 +80,138 @@ def test_large_scores(dev, rows, sign, is_bf16):
     err = ((2.0 ** -16 if is_bf16 else 4 * F32) + (BF16 if is_bf16 else F32)) * np.abs(want)
     over = np.abs(got - want) > err
     assert not over.any(), (np.argwhere(over)[:3], got[over][:3], want[over][:3])
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("positions", [64, 384, 2048])
+@pytest.mark.parametrize("gap", [8, 10, 12, 20, 40])
+def test_dominant_position(dev, gap, positions, rows, is_bf16):
+    """One position `gap` above all others whose row of V is zero (a sink): the others alone make the result, and it is
+    as near as if their weights stood alone."""
+    r = rng(gap + positions + rows)
+    heads, group, dim, cap = 2, 2, 64, 2176
+    ref = ref8.Cache(1, heads, cap, dim)
+    # the others' scores are all 0, so that what their weights lose does not average out
+    ref.q["k"][:, :, 5, 0] = 127
+    ref.q["v"] = r.integers(20, 128, ref.shape)
+    ref.q["v"][:, :, 5] = 0
+    ref.s["k"][:] = 2.0 ** -5
+    ref.s["v"][:] = r.uniform(0.01, 0.04, ref.s["v"].shape).astype(np.float32)
+    q = np.zeros((rows, heads * group, dim))
+    q[:, :, 0] = held(np.array(gap * 32 / 127), is_bf16)
+    pos = positions - 1
+    got = attend(dev, ref, q, [rows], [pos], 1.0, is_bf16)
+    want, err = weighted(ref, q, pos, 1.0, is_bf16)
+    over = np.abs(got - want) > err
+    assert not over.any(), (np.abs(got / want - 1).max(), (err / np.abs(want)).max())
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows", [2, 40])
+@pytest.mark.parametrize("big", [1e3, 1e6, 1e12, 1e30])
+def test_row_with_one_large_value(dev, big, rows, is_bf16):
+    """A value of q far above its row's others where K has zeros: the others decide the scores as if they stood alone."""
+    r = rng(int(np.log10(big)) + rows)
+    heads, group, dim, cap, pos = 2, 2, 128, 256, 190
+    ref = ref8.Cache(1, heads, cap, dim).fill(r)
+    ref.q["k"][..., 77] = 0
+    q = held(r.normal(0, 1, (rows, heads * group, dim)), is_bf16)
+    scale = dim ** -0.5
+    want, err = weighted(ref, q, pos, float(np.float32(scale)), is_bf16)
+    q[..., 77] = held(np.array(big), is_bf16)
+    got = attend(dev, ref, q, [rows], [pos], scale, is_bf16)
+    over = np.abs(got - want) > err
+    assert not over.any(), (np.argwhere(over)[:3], np.abs(got - want).max(), err.max())
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows,spread", [(1, 1), (1, 4), (1, 12), (40, 1), (40, 4), (40, 12)])
+def test_peaked_rows(dev, rows, spread, is_bf16):
+    """Random rows whose scores spread over `spread`, K and V of outlying positions: what is lost, against the sum of weight x |v|."""
+    r = rng(rows + spread)
+    heads, group, dim, cap, pos = 2, 2, 128, 1024, 960
+    ref = ref8.Cache(1, heads, cap, dim).fill(r)
+    ref.q["v"][:, :, ::97] //= 32                            # some positions with next to nothing in V
+    q = held(r.normal(0, spread, (rows, heads * group, dim)), is_bf16)
+    scale = dim ** -0.5
+    got = attend(dev, ref, q, [rows], [pos], scale, is_bf16)
+    want, err = weighted(ref, q, pos, float(np.float32(scale)), is_bf16)
+    over = np.abs(got - want) > err
+    assert not over.any(), (np.argwhere(over)[:3], np.abs(got - want).max(), err.max())
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows", [2, 40])
+def test_rows_of_any_size(dev, rows, is_bf16):
+    """Rows of q from 1e-30 to 1e30 with a block scale that brings their scores back: no product of the two is out of range."""
+    r = rng(rows)
+    heads, group, dim, cap, pos = 2, 2, 64, 256, 150
+    for size in (1e-30, 1e-10, 1e10, 1e30):
+        ref = ref8.Cache(1, heads, cap, dim).fill(r)
+        ref.s["k"] = (ref.s["k"] / np.float32(size)).astype(np.float32)
+        q = held(r.normal(0, size, (rows, heads * group, dim)), is_bf16)
+        got = attend(dev, ref, q, [rows], [pos], 0.125, is_bf16)
+        want, err = weighted(ref, q, pos, 0.125, is_bf16)
+        over = np.abs(got - want) > err
+        assert not over.any(), (size, np.argwhere(over)[:3], np.abs(got - want).max(), err.max())
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows", [2, 40])
+def test_negative_block_scales(dev, rows, is_bf16):
+    """A value is int8 x scale, whatever the scale's sign."""
+    r = rng(rows)
+    heads, group, dim, cap, pos = 2, 2, 128, 512, 400
+    ref = ref8.Cache(1, heads, cap, dim).fill(r)
+    for n in "kv":
+        ref.s[n] *= r.choice([-1, 1], ref.s[n].shape).astype(np.float32)
+    q = held(r.normal(0, 8, (rows, heads * group, dim)), is_bf16)
+    got = attend(dev, ref, q, [rows], [pos], 0.125, is_bf16)
+    want, err = weighted(ref, q, pos, 0.125, is_bf16)
+    over = np.abs(got - want) > err
+    assert not over.any(), (np.argwhere(over)[:3], np.abs(got - want).max(), err.max())
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows", [2, 40])
+def test_scores_out_of_range(dev, rows, is_bf16):
+    """A block whose largest score f32 does not hold makes the rows that see it NaN, an infinite scale among them; a score
+    below f32's range beside others that it holds weighs nothing."""
+    r = rng(rows)
+    heads, group, dim, cap, pos = 1, 2, 64, 256, 40
+    ref = ref8.Cache(1, heads, cap, dim).fill(r)
+    ref.q["k"][..., 0] = -np.maximum(np.abs(ref.q["k"][..., 0]), 4)
+    q = np.zeros((rows, heads * group, dim))
+    q[:, 0, 0], q[:, 1, 0] = 1.0, -1.0
+    see = np.arange(rows) + pos >= 64
+    for scale in (np.inf, np.float32(3e38)):
+        ref.s["k"][0, 0, 1] = scale
+        got = attend(dev, ref, q, [rows], [pos], 0.5, is_bf16)
+        assert np.isfinite(got[~see]).all() and np.isnan(got[see]).all()
+    ref.s["k"][0, 0, 1] = 3e38
+    ref.q["k"][0, 0, 64, 0] = 0                              # the one score of that block that f32 holds, for head 0 its largest
+    got = attend(dev, ref, q, [rows], [pos], 0.5, is_bf16)
+    more = np.arange(rows) + pos > 64                        # a row that sees only that position of the block is finite in both heads
+    assert np.isnan(got[more][:, 1]).all() and np.isfinite(got[~more]).all() and np.isfinite(got[:, 0]).all()
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("counts,pos,heads", [([1100], [0], 8), ([2100], [0], 8), ([700, 1, 431], [5, 60, 0], 5)])
+def test_many_tiles(dev, counts, pos, heads, is_bf16):
+    """More blocks than the card holds at a time, in whatever order they come: every row is written, and is right."""
+    r = rng(sum(counts) + is_bf16)
+    group, dim, cap = 2, 64, 2176
+    ref = ref8.Cache(len(counts), heads, cap, dim).fill(r)
+    q = held(r.normal(0, 1, (sum(counts), heads * group, dim)), is_bf16)
+    got = attend(dev, ref, q, counts, pos, 0.125, is_bf16)
+    assert (np.abs(got - 3.0) > 0).any(2).all()              # the output held 3.0 before
+    start = prefix(counts)
+    for j, n in enumerate(counts):
+        one = ref8.Cache(1, heads, cap, dim)
+        for name in "kv":
+            one.q[name], one.s[name] = ref.q[name][j:j + 1], ref.s[name][j:j + 1]
+        for i in sorted({*range(0, n, 97), *range(n - 1, 0, -211)}):
+            want, err = weighted(one, q[start[j] + i:start[j] + i + 1], pos[j] + i, 0.125, is_bf16)
+            over = np.abs(got[start[j] + i] - want[0]) > err[0]
+            assert not over.any(), (j, i, np.abs(got[start[j] + i] - want[0]).max(), err.max())
