@@ -248,7 +248,8 @@ int qasr_hip_kv8_read(qasr_hip *h, void *k, void *v, int64_t ld, const int8_t *k
  * multiple of n_kv_heads; query head h reads KV head h / (n_heads / n_kv_heads))
  * over the cache: out [n_rows][n_heads * head_dim] of q's type = softmax(scale *
  * q . k) v.  Row i of sequence j sees the positions up to pos[j] + i; with window
- * > 0 only the last window of those and the first sinks.  A row that sees nothing
+ * > 0 only those behind pos[j] + i - window and the first sinks (a row past the
+ * capacity by a window or more: the sinks alone).  A row that sees nothing
  * gives zeros; rows behind the last sequence are left as they were.  Rows of q and
  * the cache's values enter exactly, sums are f32.  A weight is off by f32 rounding of
  * itself (bf16 rows: by 2^-17 of itself), however small it is beside its row's

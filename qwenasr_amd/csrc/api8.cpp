@@ -118,8 +118,7 @@ extern "C" int qasr_hip_attention_kv8(qasr_hip *h, void *out, const void *q, int
     CHECK_H(h);
     if (n_seq == 0 || n_rows == 0 || max_rows == 0) return QASR_OK;
     a.q = q; a.ldq = ldq; a.out = out; a.Hq = (int)n_heads; a.G = (int)(n_heads / n_kv_heads); a.scale = scale;
-    // a window of the capacity or more hides nothing; its sinks then do not matter
-    a.window = window > capacity ? 0 : (int)window;
+    a.window = std::min<int64_t>(window, (int64_t)1 << 33);       // past any position
     a.sinks = (int)std::min<int64_t>(sinks, capacity);
     a.max_len = (int)(max_len > 0 ? std::min<int64_t>(max_len, capacity) : capacity);
     a.part = reinterpret_cast<float *>(h->scratch);

@@ -567,16 +567,11 @@ __global__ __launch_bounds__(64 * KV8_WAVES, 2) void k_attn_kv8(AttnKv8Args a) {
     const unsigned f1 = n_flat - 1, fr = min(f0 + c, f1);      // a column past the last row repeats it
     const int i_lo = (int)(f0 / (unsigned)a.G), i_hi = (int)(min(f0 + R - 1, f1) / (unsigned)a.G);
     const int last = sq.p0 + (int)(fr / (unsigned)a.G);        // this column's own position, and its window's first
-    const int low = a.window > 0 ? last - a.window + 1 : INT32_MIN;
+    auto low_of = [&](int i) { return a.window > 0 ? (int)min(max((int64_t)a.c.pos[j] + i - a.window + 1, (int64_t)0), (int64_t)1 << 30) : 0; };
+    const int low = low_of((int)(fr / (unsigned)a.G)), low_hi = low_of(i_hi);
 
     // the blocks that some row of the tile sees: the sinks' and the window's; this split's run of them
-    const int hi_pos = min(sq.p0 + i_hi, a.c.cap - 1);
-    int lo_pos = 0, n_sink = 0;
-    if (a.window > 0) {
-        lo_pos = max(0, sq.p0 + i_lo - a.window + 1);
-        n_sink = min((a.sinks + 63) / 64, lo_pos / 64);
-    }
-    const int lo_blk = lo_pos / 64;
+    const int hi_pos = min(sq.p0 + i_hi, a.c.cap - 1), lo_blk = low_of(i_lo) / 64, n_sink = min((a.sinks + 63) / 64, lo_blk);
     const int n_blk = hi_pos < 0 ? 0 : n_sink + max(0, hi_pos / 64 - lo_blk + 1);
     const int per = n_blk / S, more = n_blk - per * S;         // the first `more` splits take one block more
     const int u0 = split * per + min(split, more), u1 = u0 + per + (split < more ? 1 : 0);
@@ -769,7 +764,7 @@ __global__ __launch_bounds__(64 * KV8_WAVES, 2) void k_attn_kv8(AttnKv8Args a) {
         const float kf = ksb * qf;
         float mb, kc = kf;
         bool none = false;
-        if (ksb >= 0.0f && b * 64 + 63 <= sq.p0 + i_lo && (a.window == 0 || b * 64 > sq.p0 + i_hi - a.window || b * 64 + 63 < a.sinks)) {
+        if (ksb >= 0.0f && b * 64 + 63 <= sq.p0 + i_lo && (b * 64 >= low_hi || b * 64 + 63 < a.sinks)) {
             // every row of the tile sees the whole block, and the largest sum is the largest score
             mb = s[0];
 #pragma unroll
@@ -978,7 +973,7 @@ hipError_t launch_attention_kv8(const AttnKv8Args &a0, bool bf16, hipStream_t st
     a.vec_o = (uintptr_t)a.out % 16 == 0;
     const int64_t rows = a.c.max_rows * a.G;
     // blocks of positions that the longest sequence's rows see
-    const int64_t seen = a.window > 0 ? std::min<int64_t>(a.max_len, (int64_t)a.window + a.sinks + a.c.max_rows) : a.max_len;
+    const int64_t seen = a.window > 0 ? std::min<int64_t>(a.max_len, a.window + a.sinks + a.c.max_rows) : a.max_len;
     const int64_t blocks = (seen + 63) / 64;
     if (rows <= 16) {
         // One tile a sequence and head (decoding): the operands straight into registers, as no

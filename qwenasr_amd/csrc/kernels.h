@@ -398,7 +398,8 @@ struct AttnKv8Args {
     void *out;                // [n_rows][Hq * hd] of q's type
     int Hq, G;
     float scale;
-    int window, sinks;        // window 0: every position up to the row's own
+    int64_t window;           // 0: every position up to the row's own; at most 2^33
+    int sinks;
     int max_len;              // about the longest sequence: the split's measure
     float *part;              // the splits' parts (QASR_KV8_PART_BYTES)
     int vec_q, vec_o, tiles, splits, first;   // set by the launcher

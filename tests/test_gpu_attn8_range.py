@@ -215,3 +215,26 @@ def test_many_tiles(dev, counts, pos, heads, is_bf16):
             want, err = weighted(one, q[start[j] + i:start[j] + i + 1], pos[j] + i, 0.125, is_bf16)
             over = np.abs(got[start[j] + i] - want[0]) > err[0]
             assert not over.any(), (j, i, np.abs(got[start[j] + i] - want[0]).max(), err.max())
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("sinks", [0, 3, 70])
+@pytest.mark.parametrize("pos,window", [(2000, 256), (2000, 257), (2000, 1000), (2000, 1900), (2000, 2000), (2000, 2010), (2000, 1 << 40), (250, 257),
+                                        (250, 1000), (3, 1 << 62), ((1 << 31) - 1, (1 << 31) - 1), ((1 << 31) - 1, (1 << 31) - 70), (1 << 30, (1 << 30) - 5)])
+def test_window_and_capacity(dev, pos, window, sinks, is_bf16):
+    """Rows past the capacity, windows around it and far larger: a row at p sees what is stored of (p - window, p] and the
+    first sinks.  One sequence of few rows, one of many."""
+    r = rng(sinks + window % 1000)
+    counts, heads, group, dim, cap = [3, 40], 2, 2, 64, 256
+    ref = ref8.Cache(2, heads, cap, dim).fill(r)
+    for rows in (counts, [2, 3]):
+        q = held(r.normal(0, 1, (sum(rows), heads * group, dim)), is_bf16)
+        got = attend(dev, ref, q, rows, [pos, pos], 0.125, is_bf16, window=window, sinks=sinks)
+        start = prefix(rows)
+        for j in range(2):
+            one = ref8.Cache(1, heads, cap, dim)
+            for name in "kv":
+                one.q[name], one.s[name] = ref.q[name][j:j + 1], ref.s[name][j:j + 1]
+            want, err = weighted(one, q[start[j]:start[j + 1]], pos, 0.125, is_bf16, window, sinks)
+            over = np.abs(got[start[j]:start[j + 1]] - want) > err
+            assert not over.any(), (rows, j, np.argwhere(over)[:3], np.abs(got[start[j]:start[j + 1]] - want).max())
