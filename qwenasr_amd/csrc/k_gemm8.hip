@@ -266,6 +266,7 @@ __global__ __launch_bounds__(64 * WM * WN * KP, KP == 1 ? 4 : 2) void k_gemm8(Ge
             if constexpr (MODE == G8_SWIGLU) *reinterpret_cast<f32x2 *>(tr + fr * OP + 8 * j + 2 * fg) = f32x2{v[0], v[1]};
             else *reinterpret_cast<f32x4 *>(tr + fr * OP + 16 * j + 4 * fg) = v;
         }
+        wave_lds_fence();                                    // the rows change lanes
         const int64_t m = m0 + wm * (BM / WM) + 16 * i;
         if (n0 + BN <= N) {
 #pragma unroll
@@ -303,6 +304,7 @@ __global__ __launch_bounds__(64 * WM * WN * KP, KP == 1 ? 4 : 2) void k_gemm8(Ge
                 }
             }
         }
+        wave_lds_fence();                                    // read, before the next 16 rows come
     }
 }
 
