@@ -121,7 +121,10 @@ __global__ __launch_bounds__(64 * WM * WN * KP, KP == 1 ? 4 : 2) void k_gemm8(Ge
     const int fr = lane & 15, fg = lane >> 4;
     const int64_t M = g.M, N = g.N, K = g.K;
     // blocks go to the 8 XCDs in turn: the row tiles of a strip of weights follow one
-    // another on one XCD, whose L2 then holds the strip once
+    // another on one XCD, whose L2 then holds the strip once.  (Row tiles that begin at
+    // different K-steps, for weights past the caches, gain 4% at 375 x 151936 x 1024 and 2000 x
+    // 60000 x 2048 and lose 9% at 404 x 20000 x 6144, 6% at 1337 x 24576 x 6144, 3% at 250 x
+    // 151936 x 2048: left out.)
     const unsigned rows = (unsigned)((M + BM - 1) / BM), xcd = blockIdx.x & 7, q = blockIdx.x >> 3;
     const unsigned strip = q / rows * 8 + xcd;
     const unsigned row = q - q / rows * rows;
@@ -129,12 +132,6 @@ __global__ __launch_bounds__(64 * WM * WN * KP, KP == 1 ? 4 : 2) void k_gemm8(Ge
     if (n0 >= N) return;
     char *ring = smem + grp * NS * STG;
     const int nk = (int)((K + BK - 1) / BK), nit = (nk + KP - 1) / KP;
-    // The K-step that this row tile begins with.  Weights that come from HBM (80 MB and more: the
-    // cache behind the L2s has let go of them) are fetched by a strip's row tiles at different
-    // places then, twice the bytes in flight with two tiles: 375 x 151936 x 1024 106 -> 100 us
-    // (though an L2 lets go of a part and 250 MB are fetched for 161), 2000 x 40000 x 2048 206 -> 192.  Weights that a cache holds are better met by all at once:
-    // 1337 x 12288 x 6144 118 us, 121.5 in turn; 32 x 12288 x 2048 7.6, 9.7.
-    const int turn = N * K >= 80000000 ? (int)((int64_t)row * nk / rows) : 0;
     // the epilogue's operands, ahead of the ring's loads
     f32x4 ws[NT], bias[NT];
     float as[MT];
@@ -162,7 +159,7 @@ __global__ __launch_bounds__(64 * WM * WN * KP, KP == 1 ? 4 : 2) void k_gemm8(Ge
     // the byte of K that this group's step begins with; past the end: K, nothing but zeros
     auto step = [&](int it) {
         const int kt = grp + KP * it;
-        return kt < nk ? (kt + turn < nk ? kt + turn : kt + turn - nk) * BK : (int)K;
+        return kt < nk ? kt * BK : (int)K;
     };
     auto issue = [&](int stage, int it) {
         char *st = ring + stage * STG;
