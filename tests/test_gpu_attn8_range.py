@@ -53,7 +53,9 @@ def weighted(ref, q, pos, scale, is_bf16, window=0, sinks=0):
             # block, and the joining of at most 64 + 4 parts.  And the weights' sum, whose relative error is the largest one's
             blocks = seen.sum() // BLOCK + 2
             each = np.expm1(e) + (2.0 ** -17 if is_bf16 else u) + (2 + 192 + 2 * blocks + 72) * u
-            bound[i, h] = (w * each) @ np.abs(vv) + (w @ each) * np.abs(out[i, h])
+            # and what f32 does not hold: a weight, the largest of which is 1 or more, and each of its three terms may lose
+            # what lies below 2^-126, and so may the result
+            bound[i, h] = (w * each) @ np.abs(vv) + (w @ each) * np.abs(out[i, h]) + 2.0 ** -126 * (4 * np.abs(vv).sum(0) + 1)
     t = BF16 if is_bf16 else F32
     return out, bound + t * (np.abs(out) + bound)
 
@@ -238,3 +240,34 @@ def test_window_and_capacity(dev, pos, window, sinks, is_bf16):
             want, err = weighted(one, q[start[j]:start[j + 1]], pos, 0.125, is_bf16, window, sinks)
             over = np.abs(got[start[j]:start[j + 1]] - want) > err
             assert not over.any(), (rows, j, np.argwhere(over)[:3], np.abs(got[start[j]:start[j + 1]] - want).max())
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows", [2, 40])
+@pytest.mark.parametrize("scale", [-0.1, 2.0])
+def test_very_peaked_rows(dev, scale, rows, is_bf16):
+    """Rows a thousand times an ordinary one's size: each result against the bound that its scores' size allows, and where
+    that leaves no doubt which position has all the weight, that position's row of V."""
+    r = rng(rows)
+    heads, group, dim, cap, pos = 2, 2, 128, 256, 120
+    ref = ref8.Cache(1, heads, cap, dim).fill(r)
+    q = held(r.normal(0, 1000, (rows, heads * group, dim)), is_bf16)
+    got = attend(dev, ref, q, [rows], [pos], scale, is_bf16)
+    want, err = weighted(ref, q, pos, float(np.float32(scale)), is_bf16)
+    over = np.abs(got - want) > err
+    assert not over.any(), (np.argwhere(over)[:3], np.abs(got - want).max(), err.max())
+    k, v = ref.values("k")[0], ref.values("v")[0]
+    sure = 0
+    for i in range(rows):
+        for h in range(heads * group):
+            s = float(np.float32(scale)) * (k[h // group, :pos + i + 1] @ q[i, h])
+            first, second = np.sort(s)[::-1][:2]
+            off = 3 * dim * F32 * abs(scale) * (np.abs(k[h // group, :pos + i + 1]) @ np.abs(q[i, h])).max()
+            if first - second > 2 * off + 40:
+                sure += 1
+                x = v[h // group, s.argmax()]
+                # the others together weigh less than a position's e^-40 each
+                rest = (pos + rows) * np.exp(-40) * np.abs(v).max()
+                err = ((2.0 ** -16 if is_bf16 else 8 * F32) + (BF16 if is_bf16 else F32)) * np.abs(x) + 1.01 * rest
+                assert (np.abs(got[i, h] - x) <= err).all(), (i, h)
+    assert sure >= rows                                      # most of them are
