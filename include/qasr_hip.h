@@ -184,9 +184,11 @@ int qasr_hip_bidirectional_attention(qasr_hip *h, float *out, const float *q, co
  * ordered on the handle's stream, allocate nothing and may be captured into a
  * graph from that stream.
  *
- * int8 rounding, here: to the nearest value, halves away from zero, decided
- * exactly (qasr_hip_quantize_act forms a product in f32 first and can differ by
- * one next to a half). */
+ * int8 rounding, here: to the nearest value, halves away from zero, decided in
+ * f64: exactly for the cache's values and for rows with neither residual nor
+ * norm_w, else from the sum and its products as f64 rounds them
+ * (qasr_hip_quantize_act forms a product in f32 first and can differ by one next
+ * to a half). */
 /* s = x + res; n = s / sqrt(mean(s^2) + eps) * norm_w; q = n rounded to int8
  * with one scale a row, max|n| / 127 (1 for a row of zeros).  x, res and sum hold
  * rows of hidden values, ld elements apart, f32 or (bf16 != 0) bf16; q is

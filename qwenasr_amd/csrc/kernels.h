@@ -343,8 +343,9 @@ hipError_t launch_head_norm_rope_strided(float *x, int64_t row_stride, const flo
 
 namespace qasr {
 // ---- an 8-bit layer over many rows (k_rows8.hip, k_gemm8.hip, k_kv8.hip) ------
-// |x| / s to the nearest whole number, halves up, at most 127: exact for f32
-// values in f64 (254 |x| and (2 k + 1) s have at most 32 bits); inv about 1 / s
+// ax / s to the nearest whole number, halves up, at most 127; inv about 1 / s.  Exact
+// where 2 ax and (2 k + 1) s are in f64: f32 values (25 and 32 bits) and 127 times
+// one; a product that f64 has rounded already is decided as it stands
 __device__ __forceinline__ int round_ratio(double ax, double s, double inv) {
     const int k = (int)fmin(floor(ax * inv), 127.0);
     return min(127, k + (2.0 * ax >= (double)(2 * k + 1) * s ? 1 : 0));
