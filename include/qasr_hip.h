@@ -253,7 +253,8 @@ int qasr_hip_kv8_read(qasr_hip *h, void *k, void *v, int64_t ld, const int8_t *k
  * > 0 only those behind pos[j] + i - window and the first sinks (a row past the
  * capacity by a window or more: the sinks alone).  A row that sees nothing
  * gives zeros; rows behind the last sequence are left as they were.  Rows of q and
- * the cache's values enter exactly, sums are f32.  A weight is off by f32 rounding of
+ * the cache's values enter exactly, sums are f32 (of values times up to 2^16: V of
+ * 1e28 and more may leave its range).  A weight is off by f32 rounding of
  * itself (bf16 rows: by 2^-17 of itself), however small it is beside its row's
  * largest.  Scores are f32: where the largest that a row sees among the positions of
  * a block is one that f32 does not hold, the row becomes NaN.  max_len (0:
