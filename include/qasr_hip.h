@@ -256,12 +256,12 @@ int qasr_hip_kv8_read(qasr_hip *h, void *k, void *v, int64_t ld, const int8_t *k
  * the cache's values enter exactly, sums are f32 (of values times up to 2^16: V of
  * 1e28 and more may leave its range).  A weight is off by f32 rounding of
  * itself (bf16 rows: by 2^-17 of itself), however small it is beside its row's
- * largest.  Scores are f32: where the largest that a row sees among the positions of
- * a block is one that f32 does not hold, the row becomes NaN.  max_len (0:
- * capacity): about the longest pos + rows, by which the work is split; results do
- * not depend on it beyond f32 rounding.  Uses the handle's scratch area, and so
- * does a graph that holds the call: launch it on the handle's stream, or in
- * order with that stream's work. */
+ * largest, down to 2^-100 of it.  Scores are f32: where the largest that a row sees
+ * among the positions of a block is one that f32 does not hold, the row becomes
+ * NaN.  max_len (0: capacity): about the longest pos + rows, by which the work is
+ * split; results do not depend on it beyond f32 rounding.  Uses the handle's scratch
+ * area, and so does a graph that holds the call: launch it on the handle's stream,
+ * or in order with that stream's work. */
 int qasr_hip_attention_kv8(qasr_hip *h, void *out, const void *q, int64_t ldq, const int8_t *k8, const int8_t *v8,
                            const float *k_scales, const float *v_scales, const int32_t *row_start, const int32_t *pos,
                            int64_t n_rows, int64_t n_seq, int64_t max_rows, int64_t max_len, int64_t n_heads,

@@ -91,7 +91,7 @@ def test_large_scores(dev, rows, sign, is_bf16):
 def test_dominant_position(dev, gap, positions, rows, is_bf16):
     """One position `gap` above all others whose row of V is zero (a sink): the others alone make the result, and it is
     as near as if their weights stood alone."""
-    r = rng(gap + positions + rows)
+    r = rng(int(gap) + positions + rows)
     heads, group, dim, cap = 2, 2, 64, 2176
     ref = ref8.Cache(1, heads, cap, dim)
     # the others' scores are all 0, so that what their weights lose does not average out
@@ -271,3 +271,10 @@ def test_very_peaked_rows(dev, scale, rows, is_bf16):
                 err = ((2.0 ** -16 if is_bf16 else 8 * F32) + (BF16 if is_bf16 else F32)) * np.abs(x) + 1.01 * rest
                 assert (np.abs(got[i, h] - x) <= err).all(), (i, h)
     assert sure >= rows                                      # most of them are
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_smallest_weights(dev, rows, is_bf16):
+    """Weights 2^-99 of the one in front of them, whose row of V is zero, keep their bits."""
+    test_dominant_position(dev, 99 * np.log(2), 384, rows, is_bf16)
