@@ -268,6 +268,108 @@ int qasr_hip_attention_kv8(qasr_hip *h, void *out, const void *q, int64_t ldq, c
                            int64_t n_kv_heads, int64_t head_dim, int64_t capacity, float scale, int64_t window,
                            int64_t sinks, int bf16);
 
+/* ---- several hypotheses of one prompt ------------------------------------
+ * No counterpart in the reference (which keeps one greedy hypothesis over one
+ * contiguous cache): a KV cache in pages that hypotheses and sessions share, the
+ * attention over it, and the log probabilities by which hypotheses are chosen.
+ * Calls take device pointers, are ordered on the handle's stream, allocate
+ * nothing and may be captured into a graph from that stream.  kvp_fork,
+ * kvp_compact, attention_kvp and token_logprobs use the handle's scratch area, and
+ * so does a graph that holds them: launch it on the handle's stream, or in order
+ * with that stream's work.
+ *
+ * A pool is n_pages pages of `page` positions (a power of two, 16 to 256):
+ *   [n_pages][n_kv_heads][page][head_dim]
+ * K and V of every layer are a pool each; page p is page p of all of them.
+ * table (int32 [n_seq][table_ld]): table[j][s] is the page that holds positions
+ * s * page .. of sequence j.  A sequence of len positions holds the pages that its
+ * first ceil(len / page) entries name; what stands behind those entries means
+ * nothing.  A page is free when no sequence holds it: a sequence is given up, or
+ * cut, by its length alone.  Entries outside [0, n_pages) name no page: the
+ * positions there do not exist, and no value in a table leads outside the pools.
+ * Lengths below 0 count as 0, those past table_ld * page as that. */
+#define QASR_KVP_MAX_PAGES (1 << 18)
+#define QASR_KVP_MAX_SEQ 4096
+/* New sequences from old ones: sequence j of n_out goes on from sequence parent[j]
+ * (null: j itself, n_out <= n_seq; outside [0, n_seq): it starts empty) with room
+ * for rows more positions, row_start[j + 1] - row_start[j] of them held to [0,
+ * max_rows] (row_start null: max_rows each).  pos_out[j] = the parent's length,
+ * where the new rows begin (kvp_write's and attention_kvp's pos), len_out[j] =
+ * pos_out[j] + rows (the next fork's len), table_out [n_out][table_ld].
+ * Forked sequences name the same pages.  A last page that is not full and that
+ * others hold too cannot take new rows for all of them: of the sequences with the
+ * most positions in it the first that gets new rows goes on in place, if any does,
+ * and every other one that gets rows gets a page of its own, into which the positions
+ * it has are copied in every pool.  These pages, then those for its further rows,
+ * go to the sequences in order, the lowest free page first; a page that no new
+ * sequence holds is free at once.  Entries behind a sequence's pages become -1.
+ * status (int32 [2]): {0, pages held now}; when the free pages do not suffice
+ * {pages missing, pages held without the new ones}, and when sequences grow past
+ * table_ld pages {minus their number, the same}: the new sequences are then all
+ * empty (table_out -1, pos_out and len_out 0), no page is written, and the old
+ * tables still hold.
+ * pools: n_pools pools, pool_stride bytes apart, whose pages are n_heads x page
+ * positions of row_bytes bytes (a multiple of 16; bf16: 2 head_dim); 16-byte
+ * aligned.  The outputs must not overlap the inputs. */
+int qasr_hip_kvp_fork(qasr_hip *h, int32_t *table_out, int32_t *pos_out, int32_t *len_out, int32_t *status,
+                      const int32_t *table, const int32_t *len, const int32_t *parent, const int32_t *row_start,
+                      int64_t max_rows, int64_t n_out, int64_t n_seq, int64_t table_ld, void *pools, int64_t n_pools,
+                      int64_t pool_stride, int64_t n_pages, int64_t n_heads, int64_t page, int64_t row_bytes);
+/* The n pages that sequences hold moved to pages 0 .. n - 1: those at n and behind
+ * go, in order, to the free ones before n, in every pool, and table_out (which may
+ * be table) names them there, -1 behind a sequence's pages.  status (int32 [2]):
+ * {pages moved, n}.  Pools as for the fork. */
+int qasr_hip_kvp_compact(qasr_hip *h, int32_t *table_out, int32_t *status, const int32_t *table, const int32_t *len,
+                         int64_t n_seq, int64_t table_ld, void *pools, int64_t n_pools, int64_t pool_stride,
+                         int64_t n_pages, int64_t n_heads, int64_t page, int64_t row_bytes);
+/* Rows k, v (f32 or bf16, head h of a row at h * head_dim, rows ld elements apart)
+ * into bf16 pages, rounded to nearest even.  Rows of all sequences follow one
+ * another: sequence j's are row_start[j] .. row_start[j + 1] (null: max_rows each), at most
+ * max_rows of them (those past max_rows are left out); its row i is at position
+ * pos[j] + i.  Rows whose position does not exist are left out.  A position that two
+ * sequences write to the same page holds one's values or the other's, in pieces.
+ * row_start is held to [0, n_rows].  head_dim 64 or 128; pools 16-byte aligned. */
+int qasr_hip_kvp_write(qasr_hip *h, uint16_t *k_pages, uint16_t *v_pages, int64_t n_pages, const void *k, const void *v,
+                       int64_t ld, const int32_t *table, int64_t table_ld, const int32_t *row_start, const int32_t *pos,
+                       int64_t n_rows, int64_t n_seq, int64_t max_rows, int64_t n_kv_heads, int64_t head_dim,
+                       int64_t page, int bf16);
+/* Attention of rows q (f32 or bf16, rows ldq elements apart, n_heads heads, a
+ * multiple of n_kv_heads; query head h reads KV head h / (n_heads / n_kv_heads))
+ * over bf16 pages: out [n_rows][n_heads * head_dim] of q's type = softmax(scale *
+ * q . k) v.  Rows as for the write; row i of sequence j sees the positions up to
+ * pos[j] + i.  A row that sees nothing gives zeros; rows behind the last sequence,
+ * and those past max_rows, are left as they were.
+ * shared (nullable; int32 [ceil(n_seq / group)]): the sequences come in groups of
+ * `group` that follow one another (the last may be smaller), and the first shared[g]
+ * positions of group g hold the same keys and values for all its members: they are
+ * read through its first sequence's table (which has to name them even if that
+ * sequence has no rows), once for the rows of all.  Groups of different size are
+ * filled up with sequences without rows.
+ * What a row does not see does not reach it, whatever its bits; in what it sees,
+ * infinities and NaN count as they do in the formula, in f32.  Products and sums
+ * are f32; rows of q enter exactly, and a weight is off by f32 rounding of itself
+ * (bf16 rows: by 2^-17 of itself).  Results are the same bits every time.
+ * max_len, max_own (0: unknown): about the longest pos + rows, and the most of it
+ * behind the shared positions, by which the work is split; results do not depend on
+ * them beyond f32 rounding. */
+int qasr_hip_attention_kvp(qasr_hip *h, void *out, const void *q, int64_t ldq, const uint16_t *k_pages,
+                           const uint16_t *v_pages, int64_t n_pages, const int32_t *table, int64_t table_ld,
+                           const int32_t *row_start, const int32_t *pos, int64_t n_rows, int64_t n_seq, int64_t max_rows,
+                           int64_t max_len, int64_t group, const int32_t *shared, int64_t max_own, int64_t n_heads,
+                           int64_t n_kv_heads, int64_t head_dim, int64_t page, float scale, int bf16);
+/* Of every row of logits (f32 or bf16 [rows][ld], the first cols used), with p its
+ * softmax: logp[r] = log p[targets[r]] (NaN for a target outside [0, cols)),
+ * entropy[r] = -sum p log p, and the k <= 32 likeliest tokens, top_ids and top_logp
+ * [rows][k], in falling order, equal logits by the lowest index; k <= cols.  Each of
+ * the three is left out when its pointers are null (top_ids and top_logp: either may
+ * be).  The sum of the others is kept beside a row's largest term, so a
+ * probability next to 1 keeps the bits of its logarithm.  A row that holds NaN or
+ * +infinity has NaN for values; in the order of top_ids NaN counts as -infinity.  A
+ * row of -infinity alone has logp and top_logp -infinity and entropy 0.  cols <=
+ * 2^20; targets int32. */
+int qasr_hip_token_logprobs(qasr_hip *h, float *logp, float *entropy, int32_t *top_ids, float *top_logp, int64_t k,
+                            const void *logits, int64_t ld, const int32_t *targets, int64_t rows, int64_t cols, int bf16);
+
 /* ---- checkpoints: safetensors (safetensors.rs) ---------------------------
  * A read-only mapping of one checkpoint file or of a directory's shards.
  * Tensor data stays in the mapping (no host copy); the *_load_st loaders

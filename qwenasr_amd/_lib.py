@@ -152,6 +152,12 @@ _SIGS = {
     "qasr_hip_kv8_read": (C.c_int, [P, P, P, I64, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, C.c_int]),
     "qasr_hip_attention_kv8": (C.c_int, [P, P, P, I64, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, F32,
                                          I64, I64, C.c_int]),
+    "qasr_hip_kvp_fork": (C.c_int, [P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, P, I64, I64, I64, I64, I64, I64]),
+    "qasr_hip_kvp_compact": (C.c_int, [P, P, P, P, P, I64, I64, P, I64, I64, I64, I64, I64, I64]),
+    "qasr_hip_kvp_write": (C.c_int, [P, P, P, I64, P, P, I64, P, I64, P, P, I64, I64, I64, I64, I64, I64, C.c_int]),
+    "qasr_hip_attention_kvp": (C.c_int, [P, P, P, I64, P, P, I64, P, I64, P, P, I64, I64, I64, I64, I64, P, I64, I64, I64,
+                                         I64, I64, F32, C.c_int]),
+    "qasr_hip_token_logprobs": (C.c_int, [P, P, P, P, P, I64, P, I64, P, I64, I64, C.c_int]),
     "qasr_hip_encoder_load": (C.c_int, [P, C.POINTER(EncConfig), C.POINTER(EncWeights), C.POINTER(P)]),
     "qasr_hip_encoder_load_st": (C.c_int, [P, P, C.POINTER(EncConfig), C.POINTER(P)]),
     "qasr_hip_encoder_free": (None, [P]),

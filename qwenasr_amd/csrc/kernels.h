@@ -407,4 +407,96 @@ struct AttnKv8Args {
 };
 #define QASR_KV8_PART_BYTES (32u << 20)
 hipError_t launch_attention_kv8(const AttnKv8Args &a, bool bf16, hipStream_t st);
+
+// ---- several hypotheses of one prompt (k_kvp.hip, k_attn_kvp.hip, k_logp.hip) ----
+// pages of every pool as the copies see them
+struct KvpPools {
+    char *base;
+    int64_t n_pools, pool_stride;   // bytes
+    int n_pages, heads, shift;      // 1 << shift positions a page
+    int units;                      // 16-byte pieces of one position of one head
+};
+struct KvpForkArgs {
+    KvpPools pools;
+    int32_t *table_out, *pos_out, *len_out, *status;
+    const int32_t *table, *len, *parent, *row_start;
+    int64_t max_rows;
+    int n_out, n_seq, table_ld;
+    int *work;                // scratch: KVP_WORK_INTS
+};
+struct KvpCompactArgs {
+    KvpPools pools;
+    int32_t *table_out, *status;
+    const int32_t *table, *len;
+    int n_seq, table_ld;
+    int *work;
+};
+hipError_t launch_kvp_fork(const KvpForkArgs &a, hipStream_t st);
+hipError_t launch_kvp_compact(const KvpCompactArgs &a, hipStream_t st);
+
+// rows of sequences whose positions lie in pages
+struct KvpSeqs {
+    const int32_t *table, *row_start, *pos;   // row_start null: max_rows each
+    int64_t n_rows, max_rows;
+    int n_seq, table_ld, n_pages, Hkv, hd, shift;
+};
+struct KvpRows {
+    int64_t r0;               // first row
+    int n;                    // rows
+    int p0;                   // position of the first row
+};
+// the rows and the place of sequence j, held to the buffers
+__device__ __forceinline__ KvpRows kvp_rows(const KvpSeqs &a, int j) {
+    KvpRows s;
+    int64_t r1;
+    if (a.row_start) {
+        s.r0 = min(max((int64_t)a.row_start[j], (int64_t)0), a.n_rows);
+        r1 = min(max((int64_t)a.row_start[j + 1], s.r0), a.n_rows);
+    } else {
+        s.r0 = min((int64_t)j * a.max_rows, a.n_rows);
+        r1 = min(s.r0 + a.max_rows, a.n_rows);
+    }
+    s.n = (int)min(r1 - s.r0, a.max_rows);
+    s.p0 = min(max(a.pos[j], -(1 << 30)), 1 << 30);
+    return s;
+}
+struct KvpWriteArgs {
+    KvpSeqs s;
+    uint16_t *kp, *vp;
+    const void *k, *v;
+    int64_t ld;
+    int vec;                  // rows 16-byte aligned (set by the launcher)
+};
+hipError_t launch_kvp_write(const KvpWriteArgs &a, bool bf16, hipStream_t st);
+
+struct AttnKvpArgs {
+    KvpSeqs s;
+    const uint16_t *kp, *vp;
+    const void *q;            // [n_rows][ldq] f32 or bf16
+    void *out;                // [n_rows][Hq * hd] of q's type
+    int64_t ldq;
+    const int32_t *shared;    // [ceil(n_seq / group)] or null
+    float scale;
+    int group, Hq, G;
+    int64_t max_len, max_own; // hints; > 0
+    float *part;              // the splits' parts (QASR_KVP_PART_BYTES)
+    // set by the launcher
+    int vec_q, vec_o, prefix, ptiles, otiles, sp, so, cp, co;
+};
+#define QASR_KVP_PART_BYTES (32u << 20)
+hipError_t launch_attention_kvp(const AttnKvpArgs &a, bool bf16, hipStream_t st);
+
+#define QASR_LOGP_MAX_K 32
+#define QASR_LOGP_MAX_COLS (1 << 20)
+struct LogpArgs {
+    float *logp, *entropy, *top_logp;   // each nullable
+    int32_t *top_ids;                   // nullable
+    const int32_t *targets;
+    const void *x;                      // [rows][ld]
+    int64_t ld, rows;
+    int cols, k, chunks;                // chunks of a row (set by the launcher)
+    char *part;                         // QASR_LOGP_PART_BYTES
+};
+#define QASR_LOGP_PART_BYTES (32u << 20)
+hipError_t launch_token_logprobs(const LogpArgs &a, bool bf16, hipStream_t st);
 }  // namespace qasr

@@ -186,3 +186,67 @@ def attention_kv8(out, q, k8, v8, k_scales, v_scales, pos, n_rows, n_seq, max_ro
     check(lib().qasr_hip_attention_kv8(_h(q), out.ptr, q.ptr, n_heads * head_dim if ldq is None else ldq, k8.ptr, v8.ptr,
                                        k_scales.ptr, v_scales.ptr, _p(row_start), pos.ptr, n_rows, n_seq, max_rows, max_len,
                                        n_heads, n_kv_heads, head_dim, capacity, scale, window, sinks, 1 if bf16 else 0))
+
+
+# ---------------------------------------------------------------------------
+# several hypotheses of one prompt (no counterpart in the reference):
+# include/qasr_hip.h holds the definitions and the pages' layout
+# ---------------------------------------------------------------------------
+
+def kvp_fork(table_out, pos_out, len_out, status, table, length, n_out, n_seq, table_ld, pools, n_pools, n_pages, n_heads,
+             page, row_bytes, parent=None, row_start=None, max_rows=0, pool_stride=None):
+    """Sequence j of n_out goes on from sequence parent[j] with room for its next rows.
+
+    table_out [n_out][table_ld], pos_out (where the new rows begin), len_out and
+    status ({0, pages held}, or what is missing) are int32 device arrays.  pools:
+    n_pools pools pool_stride bytes apart (default: one behind another) of pages
+    [n_heads][page][row_bytes].  parent None: every sequence goes on itself;
+    row_start None: max_rows new rows each."""
+    stride = n_pages * n_heads * page * row_bytes if pool_stride is None else pool_stride
+    check(lib().qasr_hip_kvp_fork(_h(table), table_out.ptr, pos_out.ptr, len_out.ptr, status.ptr, table.ptr, length.ptr,
+                                  _p(parent), _p(row_start), max_rows, n_out, n_seq, table_ld, pools.ptr, n_pools, stride,
+                                  n_pages, n_heads, page, row_bytes))
+
+
+def kvp_compact(table_out, status, table, length, n_seq, table_ld, pools, n_pools, n_pages, n_heads, page, row_bytes,
+                pool_stride=None):
+    """The pages in use moved to the front of every pool; table_out (may be table) names them there.
+
+    status: {pages moved, pages in use}; pools as for kvp_fork."""
+    stride = n_pages * n_heads * page * row_bytes if pool_stride is None else pool_stride
+    check(lib().qasr_hip_kvp_compact(_h(table), table_out.ptr, status.ptr, table.ptr, length.ptr, n_seq, table_ld, pools.ptr,
+                                     n_pools, stride, n_pages, n_heads, page, row_bytes))
+
+
+def kvp_write(k_pages, v_pages, n_pages, k, v, table, table_ld, pos, n_rows, n_seq, max_rows, n_kv_heads, head_dim, page,
+              row_start=None, ld=None, bf16=False):
+    """Rows k, v (f32, or bf16) into bf16 pages: row i of sequence j at position pos[j] + i of its table.
+
+    row_start (int32 [n_seq + 1]): the sequences' rows; None: max_rows each.
+    ld: elements between rows (default n_kv_heads * head_dim)."""
+    check(lib().qasr_hip_kvp_write(_h(k_pages), k_pages.ptr, v_pages.ptr, n_pages, k.ptr, v.ptr,
+                                   n_kv_heads * head_dim if ld is None else ld, table.ptr, table_ld, _p(row_start), pos.ptr,
+                                   n_rows, n_seq, max_rows, n_kv_heads, head_dim, page, 1 if bf16 else 0))
+
+
+def attention_kvp(out, q, k_pages, v_pages, n_pages, table, table_ld, pos, n_rows, n_seq, max_rows, n_heads, n_kv_heads,
+                  head_dim, page, scale, row_start=None, ldq=None, max_len=0, group=1, shared=None, max_own=0, bf16=False):
+    """softmax(scale q k) v over bf16 pages: row i of sequence j sees the positions up to pos[j] + i.
+
+    shared (int32, one a group of `group` sequences that follow one another): the
+    first positions that the members have in common, read once for all of them.
+    max_len, max_own: hints (the longest sequence, the most of it not shared)."""
+    check(lib().qasr_hip_attention_kvp(_h(q), out.ptr, q.ptr, n_heads * head_dim if ldq is None else ldq, k_pages.ptr,
+                                       v_pages.ptr, n_pages, table.ptr, table_ld, _p(row_start), pos.ptr, n_rows, n_seq,
+                                       max_rows, max_len, group, _p(shared), max_own, n_heads, n_kv_heads, head_dim, page,
+                                       scale, 1 if bf16 else 0))
+
+
+def token_logprobs(logits, rows, cols, ld=None, targets=None, logp=None, entropy=None, top_ids=None, top_logp=None, k=0,
+                   bf16=False):
+    """Log probabilities of given tokens, entropy and the k likeliest tokens of rows of logits (f32, or bf16).
+
+    logp [rows] with targets (int32 [rows]); entropy [rows]; top_ids (int32) and
+    top_logp [rows][k], likeliest first, equal logits by the lowest index."""
+    check(lib().qasr_hip_token_logprobs(_h(logits), _p(logp), _p(entropy), _p(top_ids), _p(top_logp), k, logits.ptr,
+                                        cols if ld is None else ld, _p(targets), rows, cols, 1 if bf16 else 0))
