@@ -289,7 +289,7 @@ int qasr_hip_attention_kv8(qasr_hip *h, void *out, const void *q, int64_t ldq, c
  * positions there do not exist, and no value in a table leads outside the pools.
  * Lengths below 0 count as 0, those past table_ld * page as that. */
 #define QASR_KVP_MAX_PAGES (1 << 18)
-#define QASR_KVP_MAX_SEQ 4096
+#define QASR_KVP_MAX_SEQ 2048
 /* New sequences from old ones: sequence j of n_out goes on from sequence parent[j]
  * (null: j itself, n_out <= n_seq; outside [0, n_seq): it starts empty) with room
  * for rows more positions, row_start[j + 1] - row_start[j] of them held to [0,

@@ -26,7 +26,7 @@ static int page_shift(int64_t page) {
 static int seq_args(int64_t n_seq, int64_t table_ld, int64_t n_pages, int64_t page) {
     if (page_shift(page) < 0) return bad("kvp: page must be 16, 32, 64, 128 or 256");
     if (n_pages <= 0 || n_pages > QASR_KVP_MAX_PAGES) return bad("kvp: n_pages must be in [1, 2^18]");
-    if (n_seq < 0 || n_seq > QASR_KVP_MAX_SEQ) return bad("kvp: at most 4096 sequences");
+    if (n_seq < 0 || n_seq > QASR_KVP_MAX_SEQ) return bad("kvp: at most 2048 sequences");
     if (table_ld <= 0 || table_ld * page > (1 << 30)) return bad("kvp: table_ld x page must be in [1, 2^30]");
     return QASR_OK;
 }
@@ -52,7 +52,7 @@ extern "C" int qasr_hip_kvp_fork(qasr_hip *h, int32_t *table_out, int32_t *pos_o
     KvpForkArgs a{};
     if (!table_out || !pos_out || !len_out || !status || !table || !len) return bad("kvp_fork: null pointer");
     if (int rc = seq_args(n_seq, table_ld, n_pages, page)) return rc;
-    if (n_out < 0 || n_out > QASR_KVP_MAX_SEQ) return bad("kvp_fork: at most 4096 sequences");
+    if (n_out < 0 || n_out > QASR_KVP_MAX_SEQ) return bad("kvp_fork: at most 2048 sequences");
     if (!parent && n_out > n_seq) return bad("kvp_fork: without parent n_out is at most n_seq");
     if (max_rows < 0 || max_rows > (1 << 24)) return bad("kvp_fork: max_rows must be in [0, 2^24]");
     if (int rc = pool_args(a.pools, pools, n_pools, pool_stride, n_pages, n_heads, page, row_bytes)) return rc;

@@ -11,76 +11,97 @@
 namespace qasr {
 
 #define KVP_THREADS 1024
+#define KVP_WAVES (KVP_THREADS / 64)
+#define KVP_SEQS QASR_KVP_MAX_SEQ
+#define KVP_PAGES QASR_KVP_MAX_PAGES
 #define KVP_PICK 2048            // page ids handed out through LDS; more go through scratch
 // scratch: [0] copies, from KVP_COPIES on {source, target, positions, -} each, then the
 // ids handed out, then where moved pages go
 #define KVP_COPIES 16
-#define KVP_PAGES QASR_KVP_MAX_PAGES
 #define KVP_PICKS (KVP_COPIES + 4 * (KVP_PAGES / 2))
 #define KVP_MAP (KVP_PICKS + KVP_PAGES)
 
-// exclusive sums over the block's threads; every thread has to come.  Returns the
-// sum before this thread, *total that of all.
-__device__ __forceinline__ int block_scan(int v, int *sums, int *total) {
+// sums over the wave's lanes up to and with each
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);                  // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, QASR_DPP_ROW_BCAST15, 0xA, 0xF, false);
+    return v + __builtin_amdgcn_update_dpp(0, v, QASR_DPP_ROW_BCAST31, 0xC, 0xF, false);
+}
+// exclusive sums of N values over the block's threads, and their totals; every thread
+// has to come, once for each `sums`
+template <int N>
+__device__ __forceinline__ void block_scan(int (&v)[N], int (&total)[N], int (*sums)[KVP_WAVES]) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    int x = v;
+    int x[N];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
+    for (int i = 0; i < N; i++) {
+        x[i] = wave_scan(v[i]);
+        if (lane == 63) sums[i][w] = x[i];
     }
-    __syncthreads();                             // sums may still be read from the last call
-    if (lane == 63) sums[w] = x;
     __syncthreads();
-    int before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < KVP_THREADS / 64; i++) {
-        const int s = sums[i];
-        before += i < w ? s : 0;
-        all += s;
+    for (int i = 0; i < N; i++) {
+        // lane w' of each row of 16 holds wave w's sum: one more scan gives all that come before
+        const int s = wave_scan(lane < KVP_WAVES ? sums[i][lane] : 0);
+        total[i] = __builtin_amdgcn_readlane(s, KVP_WAVES - 1);
+        v[i] = x[i] - v[i] + (w > 0 ? __shfl(s, w - 1, 64) : 0);
     }
-    *total = all;
-    return before + x - v;
 }
 
 __device__ __forceinline__ int kvp_held(int len, int shift) { return (len + (1 << shift) - 1) >> shift; }
 
-// Marks the pages of one sequence's entries [0, held); a last page that is not full
-// only in `used`.  put(slot, id) sees every entry but that one, last(id) that one.
-template <typename Put, typename Last>
-__device__ __forceinline__ void kvp_mark(const int32_t *row, int held, bool part, int n_pages, uint32_t *used, uint32_t *full, int first,
-                                         int id0, const Put &put, const Last &last) {
-    const int lane = threadIdx.x & 63;
-    for (int s = first + lane; s < held; s += 64) {
-        const int id = s == lane ? id0 : row[s];
-        const bool ok = (unsigned)id < (unsigned)n_pages, is_last = part && s == held - 1;
-        if (ok) {
-            atomicOr(&used[id >> 5], 1u << (id & 31));
-            if (!is_last && full) atomicOr(&full[id >> 5], 1u << (id & 31));
-        }
-        if (is_last) last(ok ? id : -1);
-        else put(s, id);
+// lanes that walk one sequence's entries together: a wave for few sequences, 16 lanes for many
+__device__ __forceinline__ int kvp_lanes(int n) { return n <= KVP_WAVES ? 64 : n <= 2 * KVP_WAVES ? 32 : 16; }
+
+// entries [0, held) of a sequence's row, four of a lane on their way at a time
+template <typename F>
+__device__ __forceinline__ void kvp_entries(const int32_t *row, int held, int lane, int lanes, const F &f) {
+    for (int s0 = lane; s0 < held; s0 += 4 * lanes) {
+        int id[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) id[u] = s0 + u * lanes < held ? row[s0 + u * lanes] : -1;
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (s0 + u * lanes < held) f(s0 + u * lanes, id[u]);
     }
+}
+
+// bits past n_pages count as used
+__device__ __forceinline__ uint32_t kvp_no_pages(int w, int n_pages) {
+    return w * 32 + 32 <= n_pages ? 0u : w * 32 >= n_pages ? ~0u : ~((1u << (n_pages & 31)) - 1);
 }
 
 // One block: the new tables, and what has to be copied.  Bound by its own latency: a
 // chain of loads (parent, length, entries) and a few passes over LDS.
-__global__ __launch_bounds__(KVP_THREADS) void k_kvp_fork(KvpForkArgs a) {
+//
+// Who keeps a common last page is decided in a hash table of such pages: each sequence
+// that holds one enters (positions in it, gets rows, -index), the largest stays.
+__global__ __launch_bounds__(KVP_THREADS) void k_kvp_fork(KvpForkArgs a, int slots) {
     extern __shared__ uint32_t lds[];
-    __shared__ int sums[KVP_THREADS / 64], over;
+    __shared__ int sums[3][KVP_WAVES], over;
     __shared__ unsigned long long all_need;
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int n_pages = a.pools.n_pages, nw = (n_pages + 31) / 32, shift = a.pools.shift, page = 1 << shift;
-    const int n = a.n_out, cap = a.table_ld << shift;
+    const int t = threadIdx.x, n = a.n_out;
+    const int n_pages = a.pools.n_pages, nw = (n_pages + 31) / 32, shift = a.pools.shift, page = 1 << shift, cap = a.table_ld << shift;
     uint32_t *used = lds, *full = used + nw;
-    int *len = reinterpret_cast<int *>(full + nw), *par = len + n, *tail = par + n, *info = tail + n, *base = info + n, *pick_l = base + n;
+    int *hash_id = reinterpret_cast<int *>(full + nw), *hash_key = hash_id + slots, *pick_l = hash_key + slots;
+    int *len = pick_l + KVP_PICK, *par = len + n, *tail = par + n, *info = tail + n, *base = info + n;
     int *picks = a.work + KVP_PICKS, *copies = a.work + KVP_COPIES;
     auto rows_of = [&](int j) -> int {
         if (!a.row_start) return (int)a.max_rows;
         return (int)min(max((int64_t)a.row_start[j + 1] - a.row_start[j], (int64_t)0), a.max_rows);
     };
-    for (int i = t; i < 2 * nw; i += KVP_THREADS) used[i] = 0;
     if (t == 0) over = 0, all_need = 0;
+    for (int i = t; i < nw; i += KVP_THREADS) {
+        used[i] = kvp_no_pages(i, n_pages);
+        full[i] = 0;
+    }
+    for (int i = t; i < slots; i += KVP_THREADS) {
+        hash_id[i] = -1;
+        hash_key[i] = 0;
+    }
     __syncthreads();
     for (int j = t; j < n; j += KVP_THREADS) {
         const int p = a.parent ? a.parent[j] : j;
@@ -95,112 +116,112 @@ __global__ __launch_bounds__(KVP_THREADS) void k_kvp_fork(KvpForkArgs a) {
         if (held + fresh > a.table_ld) atomicAdd(&over, 1);
     }
     __syncthreads();
-    // the entries that are taken over; the first 64 of four sequences are on their way at a time
-    for (int j0 = wave; j0 < n; j0 += 4 * (KVP_THREADS / 64)) {
-        int id[4];
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int j = j0 + u * (KVP_THREADS / 64);
-            id[u] = j < n && lane < kvp_held(len[j], shift) ? a.table[(int64_t)par[j] * a.table_ld + lane] : -1;
-        }
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int j = j0 + u * (KVP_THREADS / 64);
-            if (j >= n) break;
-            int32_t *out = a.table_out + (int64_t)j * a.table_ld;
-            kvp_mark(a.table + (int64_t)par[j] * a.table_ld, kvp_held(len[j], shift), (info[j] & 255) != 0, n_pages, used, full, 0, id[u],
-                     [&](int s, int v) { out[s] = v; }, [&](int v) { tail[j] = v; });
-        }
+    // the entries that are taken over
+    const int lanes = kvp_lanes(n), lane = t & (lanes - 1), g = t / lanes, groups = KVP_THREADS / lanes;
+    for (int j = g; j < n; j += groups) {
+        const int held = kvp_held(len[j], shift), last = (info[j] & 255) ? held - 1 : -1;
+        int32_t *out = a.table_out + (int64_t)j * a.table_ld;
+        kvp_entries(a.table + (int64_t)par[j] * a.table_ld, held, lane, lanes, [&](int s, int id) {
+            const bool ok = (unsigned)id < (unsigned)n_pages;
+            if (ok) {
+                atomicOr(&used[id >> 5], 1u << (id & 31));
+                if (s != last) atomicOr(&full[id >> 5], 1u << (id & 31));
+            }
+            if (s != last) out[s] = id;
+            else if (ok) tail[j] = id;
+        });
     }
     __syncthreads();
-    // who needs a copy of its last page: those that do not go on in place
-    for (int j = wave; j < n; j += KVP_THREADS / 64) {
-        const int inf = info[j], p = tail[j], fill = inf & 255;
-        if (p < 0 || !(inf & 256)) continue;
-        bool copy = (full[p >> 5] >> (p & 31)) & 1;
-        for (int i = lane; i < n && !copy; i += 64) {
-            const int other = info[i];
-            copy = tail[i] == p && ((other & 255) > fill || ((other & 255) == fill && (other & 256) && i < j));
+    // thread t has sequences 2 t and 2 t + 1 from here on
+    constexpr int PER = KVP_SEQS / KVP_THREADS;
+    int at_hash[PER], key[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int j = t * PER + i;
+        const int p = j < n ? tail[j] : -1;
+        at_hash[i] = -1;
+        if (p < 0) continue;
+        key[i] = (info[j] & 255) << 16 | (info[j] & 256) << 6 | (KVP_SEQS - j);
+        int h = (int)((uint32_t)p * 2654435761u >> 16) & (slots - 1);
+        while (true) {
+            const int was = atomicCAS(&hash_id[h], -1, p);
+            if (was == -1 || was == p) break;
+            h = (h + 1) & (slots - 1);                       // ends: there are twice as many places as sequences
         }
-        if (__any(copy) && lane == 0) info[j] = inf | 512;
+        atomicMax(&hash_key[h], key[i]);
+        at_hash[i] = h;
     }
     __syncthreads();
-    // places among the pages handed out: in order of the sequences
-    constexpr int PER = QASR_KVP_MAX_SEQ / KVP_THREADS;
-    const int j0 = t * PER;
+    int v[3] = {0, 0, 0}, total[3];
+    const int per_w = (nw + KVP_THREADS - 1) / KVP_THREADS, w0 = t * per_w;
     long long want = 0;
-    int cps = 0, total, n_copies, n_used;
+    int copy[PER];
 #pragma unroll
-    for (int i = 0; i < PER; i++)
-        if (j0 + i < n) {
-            const int c = (info[j0 + i] >> 9) & 1;
-            cps += c;
-            want += c + base[j0 + i];
-        }
+    for (int i = 0; i < PER; i++) {
+        const int j = t * PER + i;
+        copy[i] = 0;
+        if (j >= n) continue;
+        const int p = tail[j];
+        if (at_hash[i] >= 0 && (info[j] & 256)) copy[i] = ((full[p >> 5] >> (p & 31)) & 1) || hash_key[at_hash[i]] != key[i];
+        v[1] += copy[i];
+        want += copy[i] + base[j];
+    }
     if (want) atomicAdd(&all_need, (unsigned long long)want);
     // held to what is past any pool, so that the sums stay in 32 bits
-    int at = block_scan((int)min(want, 1LL << 20), sums, &total), cp = block_scan(cps, sums, &n_copies);
-    const int per_w = (nw + KVP_THREADS - 1) / KVP_THREADS, w0 = t * per_w;
-    int in_use = 0;
-    for (int i = 0; i < per_w; i++) in_use += w0 + i < nw ? __popc(used[w0 + i]) : 0;
-    block_scan(in_use, sums, &n_used);
-    const bool fail = over > 0 || total > n_pages - n_used;
+    v[0] = (int)min(want, 1LL << 20);
+    for (int i = 0; i < per_w; i++)
+        if (w0 + i < nw) v[2] += __popc(~used[w0 + i]);
+    block_scan(v, total, sums);
+    const int n_free = total[2], n_used = n_pages - n_free;
+    const bool fail = over > 0 || total[0] > n_free;
     if (t == 0) {
-        a.status[0] = over > 0 ? -over : fail ? (int)min((long long)all_need - (n_pages - n_used), 0x7fffffffLL) : 0;
-        a.status[1] = fail ? n_used : n_used + total;
-        a.work[0] = fail ? 0 : n_copies;
+        a.status[0] = over > 0 ? -over : fail ? (int)min((long long)all_need - n_free, 0x7fffffffLL) : 0;
+        a.status[1] = fail ? n_used : n_used + total[0];
+        a.work[0] = fail ? 0 : total[1];
     }
     if (fail) {
         for (int64_t i = t; i < (int64_t)n * a.table_ld; i += KVP_THREADS) a.table_out[i] = -1;
         for (int j = t; j < n; j += KVP_THREADS) a.pos_out[j] = a.len_out[j] = 0;
         return;
     }
+    // places among the pages handed out: in order of the sequences
+    int at = v[0], cp = v[1];
 #pragma unroll
-    for (int i = 0; i < PER; i++)
-        if (j0 + i < n) {
-            const int c = (info[j0 + i] >> 9) & 1, f = base[j0 + i];
-            base[j0 + i] = at;
-            if (c) {
-                copies[4 * cp] = tail[j0 + i];
-                copies[4 * cp + 2] = info[j0 + i] & 255;
-                info[j0 + i] |= cp << 10;
-            }
-            at += c + f;
-            cp += c;
-        }
+    for (int i = 0; i < PER; i++) {
+        const int j = t * PER + i;
+        if (j >= n) continue;
+        const int fresh = base[j];
+        base[j] = at;
+        at += copy[i] + fresh;
+        if (copy[i]) info[j] |= 512 | cp++ << 10;
+    }
     // the lowest free pages
-    const bool in_lds = total <= KVP_PICK;
-    int free_here = 0, all_free;
-    for (int i = 0; i < per_w; i++)
-        if (w0 + i < nw) free_here += __popc(~used[w0 + i]);
-    int rank = block_scan(free_here, sums, &all_free);           // bits past n_pages come last: never reached
-    for (int i = 0; i < per_w && rank < total; i++) {
+    const bool in_lds = total[0] <= KVP_PICK;
+    int rank = v[2];
+    for (int i = 0; i < per_w && rank < total[0]; i++) {
         if (w0 + i >= nw) break;
-        uint32_t f = ~used[w0 + i];
-        while (f && rank < total) {
+        for (uint32_t f = ~used[w0 + i]; f && rank < total[0]; f &= f - 1, rank++) {
             const int id = (w0 + i) * 32 + __builtin_ctz(f);
-            f &= f - 1;
             if (in_lds) pick_l[rank] = id;
             else picks[rank] = id;
-            rank++;
         }
     }
     __syncthreads();
     auto pick = [&](int r) { return in_lds ? pick_l[r] : picks[r]; };
-    for (int j = wave; j < n; j += KVP_THREADS / 64) {
-        const int l = len[j], held = kvp_held(l, shift), inf = info[j], c = (inf >> 9) & 1, rows = rows_of(j);
+    for (int j = g; j < n; j += groups) {
+        const int l = len[j], held = kvp_held(l, shift), inf = info[j], c = (inf >> 9) & 1, rows = rows_of(j), last = tail[j];
         const int end = kvp_held(l + rows, shift), first = (inf & 255) ? held - 1 : held, b = base[j];
         int32_t *out = a.table_out + (int64_t)j * a.table_ld;
-        for (int s = first + lane; s < a.table_ld; s += 64) {
-            int v = -1;
-            if (s < held) v = c ? pick(b) : tail[j] >= 0 ? tail[j] : a.table[(int64_t)par[j] * a.table_ld + s];
-            else if (s < end) v = pick(b + c + s - held);
-            out[s] = v;
+        for (int s = first + lane; s < a.table_ld; s += lanes) {
+            int id = -1;
+            if (s < held) id = c ? pick(b) : last >= 0 ? last : a.table[(int64_t)par[j] * a.table_ld + s];
+            else if (s < end) id = pick(b + c + s - held);
+            out[s] = id;
         }
         if (lane == 0) {
             a.pos_out[j] = l;
             a.len_out[j] = l + rows;
-            if (c) copies[4 * (inf >> 10) + 1] = pick(b);
+            if (c) *reinterpret_cast<int4 *>(copies + 4 * (inf >> 10)) = make_int4(last, pick(b), inf & 255, 0);
         }
     }
 }
@@ -208,33 +229,36 @@ __global__ __launch_bounds__(KVP_THREADS) void k_kvp_fork(KvpForkArgs a) {
 // One block: where pages go, and the tables with it.
 __global__ __launch_bounds__(KVP_THREADS) void k_kvp_compact(KvpCompactArgs a) {
     extern __shared__ uint32_t lds[];
-    __shared__ int sums[KVP_THREADS / 64];
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    __shared__ int sums[1][KVP_WAVES], sums2[2][KVP_WAVES];
+    const int t = threadIdx.x;
     const int n_pages = a.pools.n_pages, nw = (n_pages + 31) / 32, shift = a.pools.shift, n = a.n_seq, cap = a.table_ld << shift;
     uint32_t *used = lds;
+    int *held_l = reinterpret_cast<int *>(used + nw);
     int *copies = a.work + KVP_COPIES, *map = a.work + KVP_MAP;
     for (int i = t; i < nw; i += KVP_THREADS) used[i] = 0;
+    for (int j = t; j < n; j += KVP_THREADS) held_l[j] = kvp_held(min(max(a.len[j], 0), cap), shift);
     __syncthreads();
-    auto held_of = [&](int j) { return kvp_held(min(max(a.len[j], 0), cap), shift); };
-    for (int j = wave; j < n; j += KVP_THREADS / 64) {
-        const int32_t *row = a.table + (int64_t)j * a.table_ld;
-        const int held = held_of(j);
-        kvp_mark(row, held, false, n_pages, used, nullptr, 0, lane < held ? row[lane] : -1, [](int, int) {}, [](int) {});
-    }
+    const int lanes = kvp_lanes(n), lane = t & (lanes - 1), g = t / lanes, groups = KVP_THREADS / lanes;
+    for (int j = g; j < n; j += groups)
+        kvp_entries(a.table + (int64_t)j * a.table_ld, held_l[j], lane, lanes, [&](int, int id) {
+            if ((unsigned)id < (unsigned)n_pages) atomicOr(&used[id >> 5], 1u << (id & 31));
+        });
     __syncthreads();
     const int per_w = (nw + KVP_THREADS - 1) / KVP_THREADS, w0 = t * per_w;
-    int in_use = 0, n_used, n_moved, dummy;
-    for (int i = 0; i < per_w; i++) in_use += w0 + i < nw ? __popc(used[w0 + i]) : 0;
-    block_scan(in_use, sums, &n_used);
-    // bits of word w whose page comes before n_used
-    auto low = [&](int w) { return w * 32 + 32 <= n_used ? ~0u : w * 32 >= n_used ? 0u : (1u << (n_used & 31)) - 1; };
-    int from = 0, to = 0;
+    int v1[1] = {0}, t1[1], v[2] = {0, 0}, total[2];
+    for (int i = 0; i < per_w; i++) v1[0] += w0 + i < nw ? __popc(used[w0 + i]) : 0;
+    block_scan(v1, t1, sums);
+    const int n_used = t1[0];
+    // pages at n_used and behind that are held, and those before that are free: as many
+    auto low = [&](int w) { return ~kvp_no_pages(w, n_used); };
     for (int i = 0; i < per_w; i++)
         if (w0 + i < nw) {
-            from += __popc(used[w0 + i] & ~low(w0 + i));
-            to += __popc(~used[w0 + i] & low(w0 + i));
+            v[0] += __popc(used[w0 + i] & ~low(w0 + i));
+            v[1] += __popc(~used[w0 + i] & low(w0 + i));
         }
-    int src = block_scan(from, sums, &n_moved), dst = block_scan(to, sums, &dummy);
+    block_scan(v, total, sums2);
+    int src = v[0], dst = v[1];
+    const int n_moved = total[0];
     for (int i = 0; i < per_w; i++) {
         if (w0 + i >= nw) break;
         for (uint32_t f = used[w0 + i] & ~low(w0 + i); f; f &= f - 1) {
@@ -251,68 +275,66 @@ __global__ __launch_bounds__(KVP_THREADS) void k_kvp_compact(KvpCompactArgs a) {
     __syncthreads();
     for (int i = t; i < n_moved; i += KVP_THREADS) map[copies[4 * i]] = copies[4 * i + 1];
     __syncthreads();
-    for (int j = wave; j < n; j += KVP_THREADS / 64) {
-        const int held = held_of(j);
-        for (int s = lane; s < a.table_ld; s += 64) {
-            const int64_t at = (int64_t)j * a.table_ld + s;
-            int id = -1;
-            if (s < held) {
-                id = a.table[at];
-                if (id >= n_used && id < n_pages) id = map[id];
-            }
-            a.table_out[at] = id;
-        }
+    for (int j = g; j < n; j += groups) {
+        const int64_t row = (int64_t)j * a.table_ld;
+        const int held = held_l[j];
+        kvp_entries(a.table + row, held, lane, lanes, [&](int s, int id) { a.table_out[row + s] = id >= n_used && id < n_pages ? map[id] : id; });
+        for (int s = held + lane; s < a.table_ld; s += lanes) a.table_out[row + s] = -1;
     }
 }
 
-// The copies of every pool, in slices of a page; as many blocks as stay busy, each
-// taking what is left over in turn.  Only the positions that a page holds are moved.
-__global__ __launch_bounds__(256) void k_kvp_copy(KvpPools p, const int *work, int slices) {
-    const int64_t items = (int64_t)work[0] * p.n_pools * slices;
-    const int64_t page = ((int64_t)p.heads << p.shift) * p.units;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int slice = (int)(item % slices);
-        const int64_t rest = item / slices, pool = rest % p.n_pools;
-        const int *c = work + KVP_COPIES + 4 * (rest / p.n_pools);
-        const int per = c[2] * p.units, total = per * p.heads, gap = (p.units << p.shift) - per;
-        const uint4 *src = reinterpret_cast<const uint4 *>(p.base + pool * p.pool_stride) + c[0] * page;
-        uint4 *dst = reinterpret_cast<uint4 *>(p.base + pool * p.pool_stride) + c[1] * page;
-        const int lo = (int)((int64_t)total * slice / slices), hi = (int)((int64_t)total * (slice + 1) / slices);
-        for (int u = lo + threadIdx.x; u < hi; u += 4 * 256) {
+// The copies of every pool: a block takes some heads of a page, and a page for each
+// gridDim.z of them.  Only the positions that a page holds are moved; four 16-byte
+// pieces a thread are on their way at a time.
+__global__ __launch_bounds__(256) void k_kvp_copy(KvpPools p, const int *work, int per_block) {
+    const int count = work[0];
+    const int h0 = blockIdx.x * per_block, heads = min(per_block, p.heads - h0);
+    const int whole = p.units << p.shift;
+    for (int64_t i = blockIdx.z; i < count; i += gridDim.z) {
+        const int4 c = *reinterpret_cast<const int4 *>(work + KVP_COPIES + 4 * i);
+        const unsigned per = (unsigned)c.z * p.units, total = per * heads;
+        uint4 *pool = reinterpret_cast<uint4 *>(p.base + blockIdx.y * p.pool_stride);
+        const uint4 *src = pool + ((int64_t)c.x * p.heads + h0) * whole;
+        uint4 *dst = pool + ((int64_t)c.y * p.heads + h0) * whole;
+        for (unsigned u = threadIdx.x; u < total; u += 4 * 256) {
             uint4 v[4];
-            int at[4];
+            unsigned at[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int x = u + i * 256;
-                at[i] = x + x / per * gap;
-                if (x < hi) v[i] = src[at[i]];
+            for (int e = 0; e < 4; e++) {
+                const unsigned x = u + e * 256, h = heads == 1 ? 0 : x / per;
+                at[e] = x + h * (whole - per);
+                if (x < total) v[e] = src[at[e]];
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (u + i * 256 < hi) dst[at[i]] = v[i];
+            for (int e = 0; e < 4; e++)
+                if (u + e * 256 < total) dst[at[e]] = v[e];
         }
     }
 }
 
 static hipError_t launch_copies(const KvpPools &p, const int *work, int64_t most, hipStream_t st) {
-    const int64_t bytes = ((int64_t)p.heads << p.shift) * p.units * 16;
-    const int64_t slices = std::min<int64_t>(64, std::max<int64_t>(1, bytes / 16384));
-    const int64_t blocks = std::min<int64_t>(4096, most * p.n_pools * slices);
-    if (blocks > 0) hipLaunchKernelGGL(k_kvp_copy, dim3((unsigned)blocks), dim3(256), 0, st, p, work, (int)slices);
+    if (most <= 0) return hipSuccess;
+    const int per_block = (int)std::min<int64_t>(p.heads, std::max<int64_t>(1, 1024 / ((int64_t)p.units << p.shift)));
+    const unsigned x = (unsigned)((p.heads + per_block - 1) / per_block);
+    // blocks past the copies that there turn out to be end at once
+    const int64_t z = std::min<int64_t>({most, 65535, std::max<int64_t>(1, (1 << 20) / ((int64_t)x * p.n_pools))});
+    hipLaunchKernelGGL(k_kvp_copy, dim3(x, (unsigned)p.n_pools, (unsigned)z), dim3(256), 0, st, p, work, per_block);
     return hipGetLastError();
 }
 
 hipError_t launch_kvp_fork(const KvpForkArgs &a, hipStream_t st) {
-    if (a.pools.n_pages > KVP_PAGES || a.n_out > QASR_KVP_MAX_SEQ) return hipErrorInvalidValue;
-    const size_t lds = ((size_t)(a.pools.n_pages + 31) / 32 * 2 + 5 * (size_t)a.n_out + KVP_PICK) * 4;
-    hipLaunchKernelGGL(k_kvp_fork, dim3(1), dim3(KVP_THREADS), lds, st, a);
+    if (a.pools.n_pages > KVP_PAGES || a.n_out > KVP_SEQS) return hipErrorInvalidValue;
+    int slots = 64;
+    while (slots < 2 * a.n_out) slots *= 2;
+    const size_t lds = ((size_t)(a.pools.n_pages + 31) / 32 * 2 + 2 * (size_t)slots + 5 * (size_t)a.n_out + KVP_PICK) * 4;
+    hipLaunchKernelGGL(k_kvp_fork, dim3(1), dim3(KVP_THREADS), lds, st, a, slots);
     const hipError_t e = hipGetLastError();
     return e != hipSuccess ? e : launch_copies(a.pools, a.work, a.max_rows > 0 ? a.n_out : 0, st);
 }
 
 hipError_t launch_kvp_compact(const KvpCompactArgs &a, hipStream_t st) {
-    if (a.pools.n_pages > KVP_PAGES || a.n_seq > QASR_KVP_MAX_SEQ) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(k_kvp_compact, dim3(1), dim3(KVP_THREADS), (size_t)(a.pools.n_pages + 31) / 32 * 4, st, a);
+    if (a.pools.n_pages > KVP_PAGES || a.n_seq > KVP_SEQS) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(k_kvp_compact, dim3(1), dim3(KVP_THREADS), ((size_t)(a.pools.n_pages + 31) / 32 + a.n_seq) * 4, st, a);
     const hipError_t e = hipGetLastError();
     return e != hipSuccess ? e : launch_copies(a.pools, a.work, std::min<int64_t>(a.pools.n_pages / 2, (int64_t)a.n_seq * a.table_ld), st);
 }

@@ -171,14 +171,14 @@ def test_fork_that_does_not_fit(dev):
 def test_fork_of_many(dev):
     """The most sequences and pages there may be."""
     r = rng(13)
-    n, n_pages, width, page = 4096, 1 << 18, 70, 16
+    n, n_pages, width, page = 2048, 1 << 18, 130, 16
     pools = Pools(dev, r, 1, n_pages, 1, page, 16)
-    table = r.permutation(n_pages)[:n * 60].reshape(n, 60).astype(np.int32)
+    table = r.permutation(n_pages)[:n * 120].reshape(n, 120).astype(np.int32)
     table = np.hstack([table, np.full((n, 10), -1, np.int32)])
-    length = r.integers(1, 960, n)
-    table[1::2, :30] = table[0::2, :30]                              # pairs share what both have of their first half
+    length = r.integers(1, 1920, n)
+    table[1::2, :60] = table[0::2, :60]                              # pairs share what both have of their first half
     parent = r.integers(0, n, n)
-    print("fork 4096 of 4096", flush=True)
+    print("fork 2048 of 2048", flush=True)
     t, m, missing = run_fork(dev, pools, table, length, parent, [1] * n)
     assert not missing
     run_compact(dev, pools, t, m)

@@ -54,7 +54,7 @@ def logp(**kw):
     return call("qasr_hip_token_logprobs", *a.values())
 
 
-PAGED = [dict(page=0), dict(page=8), dict(page=48), dict(page=512), dict(n_pages=0), dict(n_pages=(1 << 18) + 1), dict(n_seq=-1), dict(n_seq=4097),
+PAGED = [dict(page=0), dict(page=8), dict(page=48), dict(page=512), dict(n_pages=0), dict(n_pages=(1 << 18) + 1), dict(n_seq=-1), dict(n_seq=2049),
          dict(table_ld=0), dict(table_ld=-1), dict(table_ld=1 << 27), dict(table=None)]
 POOL = [dict(pools=None), dict(pools=AT[8] + 8), dict(n_pools=0), dict(n_pools=65536), dict(pool_stride=8 * 2 * 16 * 256 - 16),
         dict(pool_stride=8 * 2 * 16 * 256 + 8), dict(n_heads=0), dict(n_heads=1025), dict(row_bytes=0), dict(row_bytes=24), dict(row_bytes=4112)]
@@ -63,7 +63,7 @@ CACHE = [dict(kp=None), dict(vp=None), dict(kp=P + 8), dict(vp=P + 2), dict(pos=
 BAD = ([(f, k) for f in (fork, compact, write, attn) for k in PAGED] + [(f, k) for f in (fork, compact) for k in POOL]
        + [(f, k) for f in (write, attn) for k in CACHE]
        + [(fork, k) for k in (dict(table_out=None), dict(pos_out=None), dict(len_out=None), dict(status=None), dict(len=None), dict(n_out=-1),
-                              dict(n_out=4097), dict(parent=None), dict(max_rows=-1), dict(max_rows=1 << 25), dict(table_out=AT[4]),
+                              dict(n_out=2049), dict(parent=None), dict(max_rows=-1), dict(max_rows=1 << 25), dict(table_out=AT[4]),
                               dict(table_out=AT[4] + 28), dict(pos_out=AT[5]), dict(len_out=AT[6] + 8), dict(status=AT[7] + 12),
                               dict(pos_out=AT[2]), dict(status=AT[0] + 44))]
        + [(compact, k) for k in (dict(table_out=None), dict(status=None), dict(len=None), dict(table_out=AT[4] + 16), dict(status=AT[4]),
