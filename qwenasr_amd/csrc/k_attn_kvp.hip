@@ -147,6 +147,12 @@ __device__ __forceinline__ int64_t kvp_at(const AttnKvpArgs &a, int id, int h, i
     return ((((int64_t)max(id, 0) * a.s.Hkv + h) << a.s.shift) + (pos & ((1 << a.s.shift) - 1))) * HD;
 }
 
+// a value that all lanes hold alike, in a scalar register
+__device__ __forceinline__ int kvp_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t kvp_uniform(int64_t v) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
 template <int HD>
 struct KvpK { bf16x8 k[2][HD / 32]; };
 template <int HD>
@@ -185,34 +191,37 @@ __device__ __forceinline__ void kvp_load_v(const AttnKvpArgs &a, KvpIds ids, int
 __device__ __forceinline__ float kvp_max_groups(float v) { return xhalf_max(xrow16_max(v)); }
 __device__ __forceinline__ float kvp_sum_groups(float v) { return xhalf_sum(xrow16_sum(v)); }
 
-// The rows of one 16-query tile over the wave's positions again, one at a time: a lane
-// group holds a quarter of the dims of its column's query, the same as in o.
-template <bool BF16, int HD>
-__device__ __noinline__ void attn_kvp_again(const AttnKvpArgs &a, const KvpSegment &sg, int h, int64_t q_at, bool live, int lim, int first,
+// The rows of one tile of queries over the wave's positions again, one at a time: a
+// lane holds the dims of its column's query that it holds in o, a quarter (16 columns) or
+// a half (32) of them, RUN consecutive ones at a time.
+template <bool BF16, int HD, int COLS>
+__device__ __forceinline__ void attn_kvp_again(const AttnKvpArgs &a, const KvpSegment &sg, int h, int64_t q_at, bool live, int lim, int first,
                                             int end, int step, float kc, float *om) {
-    constexpr int D = HD / 4;
-    const int lane = threadIdx.x & 63, g = lane >> 4;
+    constexpr int D = HD * COLS / 64, RUN = COLS == 16 ? D : HD / 8, STRIDE = 64 / COLS * RUN;
+    const int lane = threadIdx.x & 63, g = lane / COLS * RUN;
     float q[D], o[D], m = KVP_NEG_INF, l = 0.0f;
 #pragma unroll
     for (int d = 0; d < D; d++) q[d] = o[d] = 0.0f;
-    if (live) kvp_load_q<BF16, D>(a.q, q_at + g * D, false, q);
+    if (live)
+#pragma unroll
+        for (int d = 0; d < D; d += RUN) kvp_load_q<BF16, RUN>(a.q, q_at + g + d / RUN * STRIDE, false, q + d);
     for (int base = first; base < end; base += step) {
         const KvpIds ids = kvp_ids(a, sg.table, base);
         for (int p = base; p < min(base + 32, end); p++) {
             const int id = p - base < 16 ? ids.id[0] : ids.id[1];
             if (id < 0 || p < sg.lo) continue;
-            const int64_t at = kvp_at<HD>(a, id, h, p) + g * D;
+            const int64_t at = kvp_at<HD>(a, id, h, p) + g;
             float s = 0.0f;
 #pragma unroll
-            for (int d = 0; d < D; d++) s = fmaf(q[d], bf16_to_f32(a.kp[at + d]), s);
-            s = kvp_sum_groups(s) * kc;
+            for (int d = 0; d < D; d++) s = fmaf(q[d], bf16_to_f32(a.kp[at + d / RUN * STRIDE + d % RUN]), s);
+            s = (COLS == 16 ? kvp_sum_groups(s) : xhalf_sum(s)) * kc;
             if (!live || p > lim) continue;
             const float mn = fmaxf(m, s), ref = mn == KVP_NEG_INF ? 0.0f : mn;
             const float al = __builtin_amdgcn_exp2f(m - ref), w = __builtin_amdgcn_exp2f(s - ref);
             m = mn;
             l = l * al + w;
 #pragma unroll
-            for (int d = 0; d < D; d++) o[d] = fmaf(w, bf16_to_f32(a.vp[at + d]), o[d] * al);
+            for (int d = 0; d < D; d++) o[d] = fmaf(w, bf16_to_f32(a.vp[at + d / RUN * STRIDE + d % RUN]), o[d] * al);
         }
     }
     if (m == __builtin_inff()) {                 // an infinite score: NaN, in every part
@@ -428,7 +437,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp(AttnKvpArgs a) {
             l[n] = kvp_sum_groups(l[n]);
             if (__any(live[n] && z != 0.0f)) {
                 float om[HD / 4 + 2];
-                attn_kvp_again<BF16, HD>(a, sg, h, q_at[n], live[n], lim[n], first, end, STEP, a.scale * 1.4426950408889634f, om);
+                attn_kvp_again<BF16, HD, 16>(a, sg, h, q_at[n], live[n], lim[n], first, end, STEP, a.scale * 1.4426950408889634f, om);
 #pragma unroll
                 for (int t = 0; t < VT; t++)
 #pragma unroll
@@ -503,6 +512,220 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp(AttnKvpArgs a) {
     }
 }
 
+// Many rows of a sequence: a block of four waves, 32 query columns each, goes through the
+// positions together; K and V come 32 positions at a time through a ring of three LDS
+// stages, so a block reads them once.  v_mfma 32x32x16: S^T leaves lane half hf of a
+// column positions 8 (r / 4) + 4 hf + r % 4, and the second product's k is numbered like
+// that, as above.  16-byte piece n of position r stands at n ^ (r & 15) (128 dims) or
+// n ^ ((r / 2) & 7) (64), which spreads the 16 lanes that LDS serves at a time over all banks.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+template <bool BF16, int HD>
+__global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
+    constexpr int KC = HD / 16, DV = HD / 32, QT = BF16 ? 1 : 3, PT = BF16 ? 2 : 3, R = 128;
+    constexpr int ROW = HD * 2, TB = 32 * ROW, NS = 3, NL = TB / 4096, PR = ROW / 16, RPL = 64 / PR;
+    __shared__ __attribute__((aligned(1024))) char ring[NS * 2 * TB];
+    const int lane = threadIdx.x & 63, c = lane & 31, hf = lane >> 5;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    // ---- which rows, which positions; the tiles with the most positions first
+    unsigned b = blockIdx.x;
+    const int h = b % a.s.Hkv;
+    b /= a.s.Hkv;
+    const int tile = a.otiles - 1 - (int)(b % (unsigned)a.otiles), split = b / a.otiles % (unsigned)a.so, j = b / a.otiles / a.so;
+    const int cap = a.s.table_ld << a.s.shift;
+    const KvpRows sq = kvp_rows(a.s, j);
+    const unsigned n_flat = (unsigned)sq.n * (unsigned)a.G, f0 = (unsigned)tile * R, fw = f0 + 32 * wid;
+    if (f0 >= n_flat) return;
+    KvpSegment sg;
+    sg.table = a.s.table + (int64_t)j * a.s.table_ld;
+    sg.lo = 0;
+    sg.hi = (int)min((int64_t)cap, max((int64_t)sq.p0 + sq.n, (int64_t)0));
+    const int from = split * a.co;
+    if (split > 0 && from >= sg.hi) return;
+    const int upto = split + 1 < a.so ? min(from + a.co, sg.hi) : sg.hi;
+    auto last_seen = [&](unsigned f) { return min(sq.p0 + (int)((min(f, n_flat) - 1) / (unsigned)a.G), cap - 1); };
+    const int block_end = min(upto, last_seen(f0 + R) + 1), n_it = kvp_uniform(block_end > from ? (block_end - from + 31) / 32 : 0);
+    const int end = kvp_uniform(fw < n_flat ? min(upto, last_seen(fw + 32) + 1) : from);      // this wave's
+    const int all_see = kvp_uniform(fw < n_flat ? sq.p0 + (int)(fw / (unsigned)a.G) : -1);    // what its first row sees
+
+    // ---- a stage: each wave loads 8 positions of K and of V
+    uint32_t src[NL];
+#pragma unroll
+    for (int i = 0; i < NL; i++) {
+        const int r = 8 * wid + RPL * i + lane / PR, n = (lane % PR) ^ (HD == 128 ? r & 15 : (r >> 1) & 7);
+        src[i] = (uint32_t)((r & 15) * ROW + 16 * n);
+    }
+    auto id_of = [&](int base) -> int {                          // the page of this wave's 8 positions
+        const int s = (base + 16 * (wid >> 1)) >> a.s.shift;
+        return s < a.s.table_ld ? __builtin_amdgcn_readfirstlane(sg.table[s]) : -1;
+    };
+    auto base_of = [&](int it) { return from + 32 * min(it, n_it - 1); };
+    auto issue = [&](int slot, int base, int id) {
+        const int64_t at = kvp_uniform(kvp_at<HD>(a, (unsigned)id < (unsigned)a.s.n_pages ? id : 0, h, base + 16 * (wid >> 1)));
+        char *to = ring + slot * 2 * TB + 1024 * NL * wid;
+#pragma unroll
+        for (int i = 0; i < NL; i++) lds_dma16_s(a.kp + at, src[i], to + 1024 * i);
+#pragma unroll
+        for (int i = 0; i < NL; i++) lds_dma16_s(a.vp + at, src[i], to + TB + 1024 * i);
+    };
+    int id_next = 0;
+    if (n_it > 0) {
+        issue(0, base_of(0), id_of(base_of(0)));
+        issue(1, base_of(1), id_of(base_of(1)));
+        id_next = id_of(base_of(2));
+    }
+
+    // ---- the queries
+    const float kc = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.4426950408889634f;
+    const unsigned f = fw + c;
+    const bool live = f < n_flat;
+    const unsigned i_row = live ? f / (unsigned)a.G : 0, head = h * a.G + (live ? f % (unsigned)a.G : 0);
+    const int64_t q_at = (sq.r0 + i_row) * a.ldq + (int64_t)head * HD, qi = (sq.r0 + i_row) * a.Hq + head;
+    const int lim = live ? min(sq.p0 + (int)i_row, cap - 1) : 0x7fffffff;
+    bf16x8 q[QT][KC];
+#pragma unroll
+    for (int i = 0; i < KC; i++) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = 0.0f;
+        if (live) kvp_load_q<BF16, 8>(a.q, q_at + 16 * i + 8 * hf, a.vec_q, x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = a.scale == 0.0f ? 0.0f : a.scale < 0.0f ? -x[e] : x[e];
+        bf16x8 tr[QT];
+        kvp_terms<QT>(x, tr);
+#pragma unroll
+        for (int t = 0; t < QT; t++) q[t][i] = tr[t];
+    }
+
+    f32x16 o[DV];
+    float m = KVP_NEG_INF, l = 0.0f;
+#pragma unroll
+    for (int t = 0; t < DV; t++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[t][r] = 0.0f;
+    KvpIds ids = kvp_ids(a, sg.table, n_it > 0 ? base_of(0) : 0);
+    for (int it = 0; it < n_it; it++) {
+        wait_vmcnt<2 * NL>();                                    // this wave's loads of the stage have landed
+        __syncthreads();                                         // ... and every wave's; the stage before is free
+        issue((it + 2) % NS, base_of(it + 2), id_next);
+        id_next = id_of(base_of(it + 3));
+        const KvpIds now = ids;
+        ids = kvp_ids(a, sg.table, base_of(it + 1));
+        const int base = from + 32 * it;
+        if (base >= end) continue;
+        const char *ks = ring + it % NS * 2 * TB, *vs = ks + TB;
+        f32x16 s;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < KC; i++) {
+            const int n = (2 * i + hf) ^ (HD == 128 ? c & 15 : (c >> 1) & 7);
+            const bf16x8 k = *reinterpret_cast<const bf16x8 *>(ks + c * ROW + 16 * n);
+#pragma unroll
+            for (int t = QT - 1; t >= 0; t--) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[t][i], s, 0, 0, 0);
+        }
+        const bool edge = base + 31 > all_see || base + 32 > end || (now.id[0] | now.id[1]) < 0;
+        if (edge) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int pos = base + 8 * (r >> 2) + 4 * hf + (r & 3);
+                s[r] = pos <= min(lim, end - 1) && now.id[r >> 3] >= 0 ? s[r] : KVP_NEG_INF;
+            }
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; r++) mx = fmaxf(mx, s[r]);
+        mx = xhalf_max(mx) * kc;
+        if (__any(mx > m + KVP_SLACK)) {
+            const float mn = fmaxf(m, mx), ref = mn == KVP_NEG_INF ? 0.0f : mn;
+            const float al = __builtin_amdgcn_exp2f(m - ref);
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int t = 0; t < DV; t++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[t][r] *= al;
+        }
+        const float ref = m == KVP_NEG_INF ? 0.0f : m;
+        float w[16];
+#pragma unroll
+        for (int r = 0; r < 16; r++) w[r] = __builtin_amdgcn_exp2f(fmaf(s[r], kc, -ref));
+        l += (((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]))) + (((w[8] + w[9]) + (w[10] + w[11])) + ((w[12] + w[13]) + (w[14] + w[15])));
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            bf16x8 p[PT];
+            kvp_terms<PT>(w + 8 * x, p);
+            uint32_t v[8][DV / 2];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int r = 16 * x + 8 * (e >> 2) + 4 * hf + (e & 3), swz = HD == 128 ? r & 15 : (r >> 1) & 7;
+                const char *row = vs + r * ROW;
+                if (HD == 128) {
+                    const uint2 u = *reinterpret_cast<const uint2 *>(row + 16 * ((c >> 1) ^ swz) + 8 * (c & 1));
+                    v[e][0] = u.x;
+                    v[e][DV / 2 - 1] = u.y;
+                } else {
+                    v[e][0] = *reinterpret_cast<const uint32_t *>(row + 16 * ((c >> 2) ^ swz) + 4 * (c & 3));
+                }
+                if (edge) {
+                    // V of positions that no row here sees may hold anything
+#pragma unroll
+                    for (int d = 0; d < DV / 2; d++) v[e][d] = base + r < end && now.id[x] >= 0 ? v[e][d] : 0u;
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < DV; t++) {
+                uint32_t d[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) d[e] = __builtin_amdgcn_perm(v[2 * e + 1][t >> 1], v[2 * e][t >> 1], (t & 1) ? 0x07060302 : 0x05040100);
+                const bf16x8 vt = __builtin_bit_cast(bf16x8, make_uint4(d[0], d[1], d[2], d[3]));
+#pragma unroll
+                for (int y = PT - 1; y >= 0; y--) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, p[y], o[t], 0, 0, 0);
+            }
+        }
+    }
+    wait_vmcnt<0>();                                             // no load may land in LDS after the block ends
+    // sums that are not finite: again, row by row
+    float z = l * 0.0f;
+#pragma unroll
+    for (int t = 0; t < DV; t++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) z = fmaf(o[t][r], 0.0f, z);
+    l = xhalf_sum(l);
+    if (__any(live && z != 0.0f)) {
+        float om[HD / 2 + 2];
+        attn_kvp_again<BF16, HD, 32>(a, sg, h, q_at, live, lim, from, end, 32, a.scale * 1.4426950408889634f, om);
+#pragma unroll
+        for (int t = 0; t < DV; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[t][r] = om[4 * DV * (r >> 2) + DV * (r & 3) + t];
+        m = om[HD / 2];
+        l = om[HD / 2 + 1];
+    }
+    if (!live) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float *part = a.part + (qi * a.so + split) * kvp_part<HD>;
+#pragma unroll
+    for (int x = 0; x < 4; x++) {
+        float v[4 * DV];
+        const int d = 4 * DV * (2 * x + hf);
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int t = 0; t < DV; t++) v[DV * r + t] = o[t][4 * x + r];
+        if (a.so == 1) {
+#pragma unroll
+            for (int e = 0; e < 4 * DV; e++) v[e] *= inv;
+#pragma unroll
+            for (int e = 0; e < 4 * DV; e += 8) kvp_store<BF16, 8>(a.out, qi * HD + d + e, a.vec_o, v + e);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4 * DV; e += 2) *reinterpret_cast<float2 *>(part + d + e) = make_float2(v[e], v[e + 1]);
+        }
+    }
+    if (a.so > 1 && hf == 0) *reinterpret_cast<float2 *>(part + HD) = make_float2(m, l);
+}
+
 // The parts of each row and head, in order; a wave a head.  Each lane weighs one part,
 // then the sums' loads do not wait for one another.
 template <bool BF16, int HD>
@@ -546,25 +769,54 @@ __global__ __launch_bounds__(256) void k_attn_kvp_merge(AttnKvpArgs a) {
     }
 }
 
-template <bool BF16, int HD, int NT, int WQ>
-static hipError_t go_attn_kvp(AttnKvpArgs &a, hipStream_t st) {
-    constexpr int R = 16 * NT * WQ;
-    const int64_t n_groups = a.prefix ? (a.s.n_seq + a.group - 1) / a.group : 0;
-    const int64_t otiles = (a.s.max_rows * a.G + R - 1) / R;
-    const int64_t ptiles = a.prefix ? ((int64_t)a.group * a.s.max_rows * a.G + R - 1) / R : 0;
-    a.otiles = (int)otiles;
-    a.ptiles = (int)ptiles;
-    const int64_t blocks = (n_groups * a.sp * ptiles + (int64_t)a.s.n_seq * a.so * otiles) * a.s.Hkv;
-    if (blocks * 256 > UINT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_attn_kvp<BF16, HD, NT, WQ>), dim3((unsigned)blocks), dim3(256), 0, st, a);
-    if (a.prefix || a.so > 1)
-        hipLaunchKernelGGL((k_attn_kvp_merge<BF16, HD>), dim3((unsigned)a.s.max_rows, (unsigned)a.s.n_seq, (unsigned)(a.Hq + 3) / 4), dim3(256), 0, st, a);
+template <bool BF16, int HD>
+static hipError_t go_merge(const AttnKvpArgs &a, hipStream_t st) {
+    hipLaunchKernelGGL((k_attn_kvp_merge<BF16, HD>), dim3((unsigned)a.s.max_rows, (unsigned)a.s.n_seq, (unsigned)(a.Hq + 3) / 4), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
-template <bool BF16, int NT, int WQ>
-static hipError_t pick_attn_kvp(AttnKvpArgs &a, hipStream_t st) {
-    return a.s.hd == 128 ? go_attn_kvp<BF16, 128, NT, WQ>(a, st) : go_attn_kvp<BF16, 64, NT, WQ>(a, st);
+// splits of `len` positions over blocks that take `step` of them a turn: up to 512 blocks
+// (two a CU) at `units` tiles, each with `turns` turns at least
+static void kvp_split(int64_t units, int64_t len, int64_t most, int step, int turns, int &s, int &chunk) {
+    const int64_t tiles = (len + 31) / 32 + 1;
+    const int64_t n = std::max<int64_t>(1, std::min({most, 512 / std::max<int64_t>(1, units), tiles * 32 / (step * turns)}));
+    chunk = (int)((tiles + n - 1) / n * 32);
+    s = (int)((tiles * 32 + chunk - 1) / chunk);
+}
+
+template <bool BF16, int HD>
+static hipError_t go_rows(AttnKvpArgs &a, int64_t room, hipStream_t st) {
+    const int64_t tiles = (a.s.max_rows * a.G + 127) / 128;
+    // sequences shorter than max_rows leave tiles empty: counted are those that n_rows rows fill, half a one a sequence
+    const int64_t units = std::min(tiles * a.s.n_seq, (a.s.n_rows * a.G / 64 + a.s.n_seq) / 2 + 1) * a.s.Hkv;
+    kvp_split(units, a.max_len, std::max<int64_t>(1, room), 32, 4, a.so, a.co);
+    a.otiles = (int)tiles;
+    const int64_t blocks = (int64_t)a.s.n_seq * a.so * tiles * a.s.Hkv;
+    if (blocks * 256 > UINT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_attn_kvp_rows<BF16, HD>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    return a.so > 1 ? go_merge<BF16, HD>(a, st) : hipGetLastError();
+}
+
+template <bool BF16, int HD>
+static hipError_t go_few(AttnKvpArgs &a, int64_t room, hipStream_t st) {
+    constexpr int R = 16;
+    const int64_t n_groups = a.prefix ? (a.s.n_seq + a.group - 1) / a.group : 0;
+    const int64_t otiles = (a.s.max_rows * a.G + R - 1) / R, ptiles = a.prefix ? ((int64_t)a.group * a.s.max_rows * a.G + R - 1) / R : 0;
+    a.otiles = (int)otiles;
+    a.ptiles = (int)ptiles;
+    a.sp = 1;
+    a.cp = 1 << 30;
+    if (a.prefix) kvp_split(n_groups * ptiles * a.s.Hkv, a.max_len, room / 2, 128, 1, a.sp, a.cp);
+    kvp_split((int64_t)a.s.n_seq * a.s.Hkv * otiles, a.prefix ? a.max_own : a.max_len, a.prefix ? room - a.sp : std::max<int64_t>(1, room), 128, 1, a.so, a.co);
+    const int64_t blocks = (n_groups * a.sp * ptiles + (int64_t)a.s.n_seq * a.so * otiles) * a.s.Hkv;
+    if (blocks * 256 > UINT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_attn_kvp<BF16, HD, 1, 1>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    return a.prefix || a.so > 1 ? go_merge<BF16, HD>(a, st) : hipGetLastError();
+}
+
+template <bool BF16, int HD>
+static hipError_t go_attn_kvp(AttnKvpArgs &a, int64_t room, hipStream_t st) {
+    return a.s.max_rows * a.G > 32 ? go_rows<BF16, HD>(a, room, st) : go_few<BF16, HD>(a, room, st);
 }
 
 hipError_t launch_attention_kvp(const AttnKvpArgs &a0, bool bf16, hipStream_t st) {
@@ -572,32 +824,11 @@ hipError_t launch_attention_kvp(const AttnKvpArgs &a0, bool bf16, hipStream_t st
     if ((a.s.hd != 64 && a.s.hd != 128) || a.s.n_seq > 65535 || a.s.Hkv > 65535) return hipErrorInvalidValue;
     a.vec_q = (uintptr_t)a.q % 16 == 0 && (a.ldq * (bf16 ? 2 : 4)) % 16 == 0;
     a.vec_o = (uintptr_t)a.out % 16 == 0;
-    const int64_t rows = a.s.max_rows * a.G;
     // parts that fit the scratch area, for every row and head
     const int64_t room = std::min<int64_t>(64, (int64_t)QASR_KVP_PART_BYTES / (a.s.n_rows * a.Hq * (a.s.hd + 2) * 4));
-    a.prefix = a.shared && rows <= 32 && room >= 2;
-    const int64_t n_groups = a.prefix ? (a.s.n_seq + a.group - 1) / a.group : 0;
-    if (rows > 32) {
-        a.sp = a.so = a.cp = a.co = 1;
-        a.co = 1 << 30;
-        return bf16 ? pick_attn_kvp<true, 2, 4>(a, st) : pick_attn_kvp<false, 1, 4>(a, st);
-    }
-    // few rows: four waves a block, each with every fourth tile of positions; splits up to two blocks a CU
-    auto split = [](int64_t units, int64_t len, int64_t most, int &s, int &chunk) {
-        const int64_t tiles = (len + 31) / 32 + 1;
-        const int64_t n = std::max<int64_t>(1, std::min({most, 512 / std::max<int64_t>(1, units), (tiles + 3) / 4}));
-        chunk = (int)((tiles + n - 1) / n * 32);
-        s = (int)((tiles * 32 + chunk - 1) / chunk);
-    };
-    const int R = 16;
-    a.sp = 1;
-    a.cp = 1 << 30;
-    if (a.prefix) {
-        const int64_t ptiles = ((int64_t)a.group * a.s.max_rows * a.G + R - 1) / R;
-        split(n_groups * ptiles * a.s.Hkv, a.max_len, room / 2, a.sp, a.cp);
-    }
-    split((int64_t)a.s.n_seq * a.s.Hkv * ((rows + R - 1) / R), a.prefix ? a.max_own : a.max_len, a.prefix ? room - a.sp : std::max<int64_t>(1, room), a.so, a.co);
-    return bf16 ? pick_attn_kvp<true, 1, 1>(a, st) : pick_attn_kvp<false, 1, 1>(a, st);
+    a.prefix = a.shared && a.s.max_rows * a.G <= 32 && room >= 2;
+    if (bf16) return a.s.hd == 128 ? go_attn_kvp<true, 128>(a, room, st) : go_attn_kvp<true, 64>(a, room, st);
+    return a.s.hd == 128 ? go_attn_kvp<false, 128>(a, room, st) : go_attn_kvp<false, 64>(a, room, st);
 }
 
 }  // namespace qasr
