@@ -129,18 +129,30 @@ __device__ __forceinline__ void kvp_store(void *out, int64_t at, bool vec, const
     }
 }
 
-// the pages of a tile's two halves; -1: no page
+// The pages of a tile's two halves; -1: no page.  A wave keeps 64 entries of the table,
+// one a lane, and takes them out by lane: a load for each tile would be a wait for
+// everything that is on its way.  For tiles in rising order.
 struct KvpIds { int id[2]; };
-__device__ __forceinline__ KvpIds kvp_ids(const AttnKvpArgs &a, const int32_t *table, int base) {
-    KvpIds r;
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        const int s = (base + 16 * h) >> a.s.shift;
-        r.id[h] = s < a.s.table_ld ? __builtin_amdgcn_readfirstlane(table[s]) : -1;
-        if ((unsigned)r.id[h] >= (unsigned)a.s.n_pages) r.id[h] = -1;
+struct KvpTable {
+    const int32_t *table;
+    int first, entry;
+    __device__ __forceinline__ void load(const AttnKvpArgs &a, int s) {
+        first = s;
+        entry = table[min(s + (int)(threadIdx.x & 63), a.s.table_ld - 1)];
     }
-    return r;
-}
+    __device__ __forceinline__ KvpTable(const AttnKvpArgs &a, const int32_t *t, int base) : table(t) { load(a, base >> a.s.shift); }
+    __device__ __forceinline__ KvpIds at(const AttnKvpArgs &a, int base) {
+        const int s0 = base >> a.s.shift, s1 = (base + 16) >> a.s.shift;
+        if (s1 - first > 63) load(a, s0);
+        KvpIds r;
+        r.id[0] = __builtin_amdgcn_readlane(entry, s0 - first);
+        r.id[1] = s1 < a.s.table_ld ? __builtin_amdgcn_readlane(entry, s1 - first) : -1;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+            if ((unsigned)r.id[h] >= (unsigned)a.s.n_pages) r.id[h] = -1;
+        return r;
+    }
+};
 // first value of a half's 16 positions of head h
 template <int HD>
 __device__ __forceinline__ int64_t kvp_at(const AttnKvpArgs &a, int id, int h, int pos) {
@@ -153,22 +165,29 @@ __device__ __forceinline__ int64_t kvp_uniform(int64_t v) {
     return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
 }
 
+// 16 or 8 bytes; ONCE: not to be kept in the caches, as nobody else reads them
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <bool ONCE, typename T>
+__device__ __forceinline__ T kvp_load(const uint16_t *p) {
+    return ONCE ? __builtin_nontemporal_load(reinterpret_cast<const T *>(p)) : *reinterpret_cast<const T *>(p);
+}
 template <int HD>
 struct KvpK { bf16x8 k[2][HD / 32]; };
-template <int HD>
+template <int HD, bool ONCE>
 __device__ __forceinline__ void kvp_load_k(const AttnKvpArgs &a, KvpIds ids, int h, int base, KvpK<HD> &o) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int x = 0; x < 2; x++) {
         const uint16_t *p = a.kp + kvp_at<HD>(a, ids.id[x], h, base + 16 * x) + c * HD + 8 * g;
 #pragma unroll
-        for (int i = 0; i < HD / 32; i++) o.k[x][i] = *reinterpret_cast<const bf16x8 *>(p + 32 * i);
+        for (int i = 0; i < HD / 32; i++) o.k[x][i] = kvp_load<ONCE, bf16x8>(p + 32 * i);
     }
 }
 // row e of a lane: position 4 g + (e & 3) of half e / 4, dims HD / 16 * c ..
 template <int HD>
 struct KvpV { uint32_t v[8][HD / 32]; };
-template <int HD>
+template <int HD, bool ONCE>
 __device__ __forceinline__ void kvp_load_v(const AttnKvpArgs &a, KvpIds ids, int h, int base, KvpV<HD> &o) {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
 #pragma unroll
@@ -177,12 +196,12 @@ __device__ __forceinline__ void kvp_load_v(const AttnKvpArgs &a, KvpIds ids, int
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             if (HD == 128) {
-                const uint4 u = *reinterpret_cast<const uint4 *>(p + e * HD);
-                o.v[4 * x + e][0] = u.x; o.v[4 * x + e][1] = u.y;
-                o.v[4 * x + e][HD / 32 - 2] = u.z; o.v[4 * x + e][HD / 32 - 1] = u.w;
+                const u32x4 u = kvp_load<ONCE, u32x4>(p + e * HD);
+                o.v[4 * x + e][0] = u[0]; o.v[4 * x + e][1] = u[1];
+                o.v[4 * x + e][HD / 32 - 2] = u[2]; o.v[4 * x + e][HD / 32 - 1] = u[3];
             } else {
-                const uint2 u = *reinterpret_cast<const uint2 *>(p + e * HD);
-                o.v[4 * x + e][0] = u.x; o.v[4 * x + e][1] = u.y;
+                const u32x2 u = kvp_load<ONCE, u32x2>(p + e * HD);
+                o.v[4 * x + e][0] = u[0]; o.v[4 * x + e][1] = u[1];
             }
         }
     }
@@ -205,8 +224,10 @@ __device__ __forceinline__ void attn_kvp_again(const AttnKvpArgs &a, const KvpSe
     if (live)
 #pragma unroll
         for (int d = 0; d < D; d += RUN) kvp_load_q<BF16, RUN>(a.q, q_at + g + d / RUN * STRIDE, false, q + d);
+    if (first >= end) return;
+    KvpTable table(a, sg.table, first);
     for (int base = first; base < end; base += step) {
-        const KvpIds ids = kvp_ids(a, sg.table, base);
+        const KvpIds ids = table.at(a, base);
         for (int p = base; p < min(base + 32, end); p++) {
             const int id = p - base < 16 ? ids.id[0] : ids.id[1];
             if (id < 0 || p < sg.lo) continue;
@@ -239,16 +260,21 @@ __device__ __forceinline__ void attn_kvp_again(const AttnKvpArgs &a, const KvpSe
 template <int HD>
 constexpr int kvp_part = HD + 2;                 // floats of a query's part: O, maximum, sum
 
-// blocks: h fastest, then the tile of rows, the split, the group or sequence; the
-// prefixes' first
-template <bool BF16, int HD, int NT, int WQ>
-__global__ __launch_bounds__(256, 2) void k_attn_kvp(AttnKvpArgs a) {
-    constexpr int KC = HD / 32, VT = HD / 16, QT = BF16 ? 1 : 3, PT = BF16 ? 2 : 3, WK = 4 / WQ, R = 16 * NT * WQ;
-    __shared__ float o_l[WK == 1 ? 1 : WK][WK == 1 ? 1 : 16 * NT][HD + 4];
-    __shared__ float ml_l[WK == 1 ? 1 : WK][2][16 * NT];
-    __shared__ int64_t qi_l[WK == 1 ? 1 : 16 * NT];
+// Few rows of a sequence, and prefixes: a block of W waves takes 16 query columns, each
+// wave every W-th 32 positions straight into registers, as no second tile shares them.
+// Blocks: h fastest, then the tile of rows, the split, the group or sequence; the
+// prefixes' first.  What bounds short ones is the chain rows -> table -> K -> products ->
+// merge, so each load goes out as soon as its address is known.
+template <bool BF16, int HD, int W, bool ONCE, bool AHEAD>
+__global__ __launch_bounds__(64 * W, 2) void k_attn_kvp(AttnKvpArgs a) {
+    constexpr int KC = HD / 32, VT = HD / 16, QT = BF16 ? 1 : 3, PT = BF16 ? 2 : 3, R = 16, STEP = 32 * W;
+    __shared__ float o_l[W][R][HD + 4];
+    __shared__ float ml_l[W][2][R];
+    __shared__ bf16x8 q_l[QT][KC][64];
+    static_assert(KC <= W, "a chunk of q a wave");
+    __shared__ int64_t qi_l[R];
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wq = wid / WK, wk = wid % WK;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
     // ---- which rows, which positions
     unsigned b = blockIdx.x;
@@ -261,147 +287,125 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp(AttnKvpArgs a) {
     const int tiles = is_prefix ? a.ptiles : a.otiles, splits = is_prefix ? a.sp : a.so, chunk = is_prefix ? a.cp : a.co;
     const int tile = b % tiles, split = b / tiles % splits, unit = b / tiles / splits;
     const int cap = a.s.table_ld << a.s.shift;
-    // a prefix takes max_rows rows of each member, those that a member does not have among them
-    KvpSegment sg;
     const int j0 = is_prefix ? unit * a.group : unit;
-    KvpRows sq{};
-    unsigned n_flat;
-    if (is_prefix) {
-        sg.lo = 0;
-        sg.hi = min(max(a.shared[unit], 0), cap);
-        n_flat = (unsigned)min(a.group, a.s.n_seq - j0) * (unsigned)a.s.max_rows * (unsigned)a.G;
-    } else {
-        sq = kvp_rows(a.s, j0);
-        sg.lo = a.prefix ? min(max(a.shared[j0 / a.group], 0), cap) : 0;
-        sg.hi = (int)min((int64_t)cap, max((int64_t)sq.p0 + sq.n, (int64_t)0));
-        n_flat = (unsigned)sq.n * (unsigned)a.G;
-    }
+    // the lane's row: of a prefix one of max_rows of each member, which a member may not have
+    const unsigned f = (unsigned)tile * R + c, slot = f / (unsigned)a.G, head = h * a.G + f % (unsigned)a.G;
+    const int members = is_prefix ? min(a.group, a.s.n_seq - j0) : 1;
+    const int k_row = is_prefix ? (int)(slot / (unsigned)a.s.max_rows) : 0, i_row = is_prefix ? (int)(slot % (unsigned)a.s.max_rows) : (int)slot;
+    const KvpRows sq = kvp_rows(a.s, j0 + min(k_row, members - 1));
+    const int sh = a.prefix ? min(max(a.shared[is_prefix ? unit : j0 / a.group], 0), cap) : 0;
+    KvpSegment sg;
     sg.table = a.s.table + (int64_t)j0 * a.s.table_ld;
-    const unsigned f0 = (unsigned)tile * R;
-    if (f0 >= n_flat) return;
+    sg.lo = is_prefix ? 0 : kvp_uniform(sh);
+    sg.hi = kvp_uniform(is_prefix ? sh : (int)min((int64_t)cap, max((int64_t)sq.p0 + sq.n, (int64_t)0)));
+    const bool live = k_row < members && i_row < sq.n;
     const int from = (sg.lo & ~31) + split * chunk;
-    // an own part exists even if it is empty (it may be all that a row has); a prefix's only where there are positions
-    if (split > 0 ? from >= sg.hi : is_prefix && sg.hi <= 0) return;
-    const int upto = split + 1 < splits ? min(from + chunk, sg.hi) : sg.hi;
-
-    // ---- the queries
-    const unsigned fw = f0 + wq * 16 * NT;
-    const float kc = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.4426950408889634f;
-    bf16x8 q[NT][QT][KC];
-    int64_t q_at[NT], qi[NT];
-    int lim[NT], wave_max = -1, wave_min = 0x7fffffff;
-    bool live[NT];
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const unsigned f = fw + 16 * n + c, slot = f / (unsigned)a.G, head = h * a.G + f % (unsigned)a.G;
-        KvpRows of = sq;
-        int i = (int)slot;
-        live[n] = f < n_flat;
-        if (is_prefix && live[n]) {
-            i = (int)(slot % (unsigned)a.s.max_rows);
-            of = kvp_rows(a.s, j0 + (int)(slot / (unsigned)a.s.max_rows));
-            live[n] = i < of.n;
-        }
-        q_at[n] = (of.r0 + i) * a.ldq + (int64_t)head * HD;
-        qi[n] = (of.r0 + i) * a.Hq + head;
-        const int at = is_prefix ? min(sg.hi - 1, of.p0 + i) : of.p0 + i;
-        // rows past the end see everything, so that they ask for no mask: they are written nowhere
-        lim[n] = live[n] ? min(at, cap - 1) : 0x7fffffff;
-        wave_max = max(wave_max, live[n] ? lim[n] : -1);
-        wave_min = min(wave_min, lim[n]);
-        float x[KC][8];
-#pragma unroll
-        for (int i = 0; i < KC; i++) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[i][e] = 0.0f;
-            if (live[n]) kvp_load_q<BF16, 8>(a.q, q_at[n] + 32 * i + 8 * g, a.vec_q, x[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < KC; i++) {
-            // a negative scale is the queries', a zero one makes them zero
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[i][e] = a.scale == 0.0f ? 0.0f : a.scale < 0.0f ? -x[i][e] : x[i][e];
-            bf16x8 tr[QT];
-            kvp_terms<QT>(x[i], tr);
-#pragma unroll
-            for (int t = 0; t < QT; t++) q[n][t][i] = tr[t];
-        }
+    const int64_t qi = (sq.r0 + i_row) * a.Hq + head;
+    const bool whole = !a.prefix && a.so == 1;
+    const int P = (a.prefix ? a.sp : 0) + a.so, part_i = is_prefix ? split : (a.prefix ? a.sp : 0) + split;
+    if (!__any(live)) return;
+    if (!whole && from >= sg.hi) {                               // a part without positions
+        if (live && threadIdx.x < 16) *reinterpret_cast<float2 *>(a.part + (qi * P + part_i) * kvp_part<HD> + HD) = make_float2(KVP_NEG_INF, 0.0f);
+        return;
     }
+    const int upto = split + 1 < splits ? min(from + chunk, sg.hi) : sg.hi;
+    const int first = from + 32 * wid;
+    KvpTable table(a, sg.table, min(first, cap - 1));
+
+    // rows past the end see everything, so that they ask for no mask: they are written nowhere
+    const int lim = live ? min(is_prefix ? min(sg.hi - 1, sq.p0 + i_row) : sq.p0 + i_row, cap - 1) : 0x7fffffff;
+    int wave_max = live ? lim : -1, wave_min = lim;
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) {
         wave_max = max(wave_max, __shfl_xor(wave_max, o, 64));
         wave_min = min(wave_min, __shfl_xor(wave_min, o, 64));
     }
-    wave_max = __builtin_amdgcn_readfirstlane(wave_max);
-    wave_min = __builtin_amdgcn_readfirstlane(wave_min);
+    wave_max = kvp_uniform(wave_max);
+    wave_min = kvp_uniform(wave_min);
+    const int end = min(upto, wave_max + 1);
+
+    // ---- the first tiles, and the queries: each wave brings a chunk of their dims into terms, for all of them
+    KvpK<HD> k0, k1;
+    KvpV<HD> v0, v1;
+    KvpIds id0, id1;
+    if (first < end) {
+        id0 = table.at(a, first);
+        kvp_load_k<HD, ONCE>(a, id0, h, first, k0);
+        kvp_load_v<HD, ONCE>(a, id0, h, first, v0);
+    }
+    const int64_t q_at = (sq.r0 + i_row) * a.ldq + (int64_t)head * HD;
+    // a negative scale is the queries', a zero one makes them zero
+    const float kc = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.4426950408889634f, sign = a.scale == 0.0f ? 0.0f : a.scale < 0.0f ? -1.0f : 1.0f;
+    if (wid < KC) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = 0.0f;
+        if (live) kvp_load_q<BF16, 8>(a.q, q_at + 32 * wid + 8 * g, a.vec_q, x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] *= sign;
+        bf16x8 tr[QT];
+        kvp_terms<QT>(x, tr);
+#pragma unroll
+        for (int t = 0; t < QT; t++) q_l[t][wid][lane] = tr[t];
+    }
+    __syncthreads();
 
     // ---- the positions
-    f32x4 o[NT][VT];
-    float m[NT], l[NT];
+    f32x4 o[VT];
+    float m = KVP_NEG_INF, l = 0.0f;
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        m[n] = KVP_NEG_INF;
-        l[n] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < VT; t++) o[n][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-    constexpr int STEP = 32 * WK;
-    const int first = from + 32 * wk, end = min(upto, wave_max + 1);
+    for (int t = 0; t < VT; t++) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     if (first < end) {
-        KvpK<HD> k;
-        KvpIds ids = kvp_ids(a, sg.table, first), next_ids = kvp_ids(a, sg.table, min(first + STEP, end - 1) & ~31);
-        kvp_load_k<HD>(a, ids, h, first, k);
-        for (int base = first; base < end; base += STEP) {
-            KvpV<HD> v;
-            kvp_load_v<HD>(a, ids, h, base, v);
-            KvpK<HD> kn;
-            const int nb = base + STEP < end ? base + STEP : base;
-            const KvpIds now = ids;
-            ids = base + STEP < end ? next_ids : ids;
-            kvp_load_k<HD>(a, ids, h, nb, kn);
-            next_ids = kvp_ids(a, sg.table, min(nb + STEP, end - 1) & ~31);
-
-            const bool edge = base < sg.lo || base + 31 > wave_min || base + 32 > end || (now.id[0] | now.id[1]) < 0;
-            bf16x8 p[NT][PT];
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-                f32x4 s[2];
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    s[x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int i = 0; i < KC; i++)
-#pragma unroll
-                        for (int t = QT - 1; t >= 0; t--) s[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k.k[x][i], q[n][t][i], s[x], 0, 0, 0);
-                }
-                if (edge) {
-#pragma unroll
-                    for (int x = 0; x < 2; x++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const int pos = base + 16 * x + 4 * g + r;
-                            s[x][r] = pos >= sg.lo && pos <= min(lim[n], end - 1) && now.id[x] >= 0 ? s[x][r] : KVP_NEG_INF;
-                        }
-                }
-                float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-                mx = kvp_max_groups(mx) * kc;
-                if (__any(mx > m[n] + KVP_SLACK)) {
-                    const float mn = fmaxf(m[n], mx), ref = mn == KVP_NEG_INF ? 0.0f : mn;
-                    const float al = __builtin_amdgcn_exp2f(m[n] - ref);
-                    m[n] = mn;
-                    l[n] *= al;
-#pragma unroll
-                    for (int t = 0; t < VT; t++)
-#pragma unroll
-                        for (int r = 0; r < 4; r++) o[n][t][r] *= al;
-                }
-                const float ref = m[n] == KVP_NEG_INF ? 0.0f : m[n];
-                float w[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) w[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], kc, -ref));
-                l[n] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-                kvp_terms<PT>(w, p[n]);
+        // One tile.  AHEAD: the next one's K and V go out at once, into registers of their own; else into the same
+        // ones as soon as the products have read them, and other waves are there to wait with
+        auto turn = [&](int base, KvpK<HD> &k, KvpV<HD> &v, KvpIds now, KvpK<HD> &kn, KvpV<HD> &vn, KvpIds &next) {
+            const bool more = base + STEP < end;
+            if (more) next = table.at(a, base + STEP);
+            if (AHEAD && more) {
+                kvp_load_k<HD, ONCE>(a, next, h, base + STEP, kn);
+                kvp_load_v<HD, ONCE>(a, next, h, base + STEP, vn);
             }
+            const bool edge = base < sg.lo || base + 31 > wave_min || base + 32 > end || (now.id[0] | now.id[1]) < 0;
+            f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+            int at = lane;
+            asm volatile("" : "+v"(at));                 // q stays in LDS: kept over the turns it takes 48 registers
+#pragma unroll
+            for (int i = 0; i < KC; i++)
+#pragma unroll
+                for (int t = QT - 1; t >= 0; t--) {
+                    const bf16x8 q = q_l[t][i][at];
+#pragma unroll
+                    for (int y = 0; y < 2; y++) s[y] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k.k[y][i], q, s[y], 0, 0, 0);
+                }
+            if (!AHEAD && more) kvp_load_k<HD, ONCE>(a, next, h, base + STEP, kn);
+            if (edge) {
+#pragma unroll
+                for (int y = 0; y < 2; y++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int pos = base + 16 * y + 4 * g + r;
+                        s[y][r] = pos >= sg.lo && pos <= min(lim, end - 1) && now.id[y] >= 0 ? s[y][r] : KVP_NEG_INF;
+                    }
+            }
+            float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+            mx = kvp_max_groups(mx) * kc;
+            if (__any(mx > m + KVP_SLACK)) {
+                const float mn = fmaxf(m, mx), ref = mn == KVP_NEG_INF ? 0.0f : mn;
+                const float al = __builtin_amdgcn_exp2f(m - ref);
+                m = mn;
+                l *= al;
+#pragma unroll
+                for (int t = 0; t < VT; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) o[t][r] *= al;
+            }
+            const float ref = m == KVP_NEG_INF ? 0.0f : m;
+            float w[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][e & 3], kc, -ref));
+            l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+            bf16x8 p[PT];
+            kvp_terms<PT>(w, p);
             if (edge) {
                 // V of positions that no row here sees may hold anything
 #pragma unroll
@@ -420,95 +424,82 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp(AttnKvpArgs a) {
                 for (int e = 0; e < 4; e++) d[e] = __builtin_amdgcn_perm(v.v[2 * e + 1][t >> 1], v.v[2 * e][t >> 1], (t & 1) ? 0x07060302 : 0x05040100);
                 const bf16x8 vt = __builtin_bit_cast(bf16x8, make_uint4(d[0], d[1], d[2], d[3]));
 #pragma unroll
-                for (int n = 0; n < NT; n++)
-#pragma unroll
-                    for (int x = PT - 1; x >= 0; x--) o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, p[n][x], o[n][t], 0, 0, 0);
+                for (int y = PT - 1; y >= 0; y--) o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, p[y], o[t], 0, 0, 0);
             }
-            k = kn;
+            if (!AHEAD && more) kvp_load_v<HD, ONCE>(a, next, h, base + STEP, vn);
+        };
+        if (AHEAD) {
+            for (int base = first; base < end; base += 2 * STEP) {
+                turn(base, k0, v0, id0, k1, v1, id1);
+                if (base + STEP < end) turn(base + STEP, k1, v1, id1, k0, v0, id0);
+            }
+        } else {
+            for (int base = first; base < end; base += STEP) {
+                turn(base, k0, v0, id0, k0, v0, id1);
+                id0 = id1;
+            }
         }
         // sums that are not finite: again, row by row
+        float z4[4] = {l * 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            float z = l[n] * 0.0f;
+        for (int t = 0; t < VT; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) z4[r] = fmaf(o[t][r], 0.0f, z4[r]);
+        const float z = (z4[0] + z4[1]) + (z4[2] + z4[3]);
+        l = kvp_sum_groups(l);
+        if (__any(live && z != 0.0f)) {
+            float om[HD / 4 + 2];
+            attn_kvp_again<BF16, HD, 16>(a, sg, h, q_at, live, lim, first, end, STEP, a.scale * 1.4426950408889634f, om);
 #pragma unroll
             for (int t = 0; t < VT; t++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) z = fmaf(o[n][t][r], 0.0f, z);
-            l[n] = kvp_sum_groups(l[n]);
-            if (__any(live[n] && z != 0.0f)) {
-                float om[HD / 4 + 2];
-                attn_kvp_again<BF16, HD, 16>(a, sg, h, q_at[n], live[n], lim[n], first, end, STEP, a.scale * 1.4426950408889634f, om);
-#pragma unroll
-                for (int t = 0; t < VT; t++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) o[n][t][r] = om[VT * r + t];
-                m[n] = om[HD / 4];
-                l[n] = om[HD / 4 + 1];
-            }
+                for (int r = 0; r < 4; r++) o[t][r] = om[VT * r + t];
+            m = om[HD / 4];
+            l = om[HD / 4 + 1];
         }
     }
 
-    // ---- out: the rows themselves, or their part
-    const bool whole = !a.prefix && a.so == 1;
-    const int P = (a.prefix ? a.sp : 0) + a.so, part_i = is_prefix ? split : (a.prefix ? a.sp : 0) + split;
-    auto put = [&](int64_t qi, int d, float *v, auto count, float ll, float mm) {
-        if (whole) {
-            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-#pragma unroll
-            for (int e = 0; e < decltype(count)::value; e++) v[e] *= inv;
-            kvp_store<BF16, decltype(count)::value>(a.out, qi * HD + d, a.vec_o, v);
-        } else {
-            float *part = a.part + (qi * P + part_i) * kvp_part<HD>;
-#pragma unroll
-            for (int e = 0; e < decltype(count)::value; e += 2) *reinterpret_cast<float2 *>(part + d + e) = make_float2(v[e], v[e + 1]);
-            if (d == 0) *reinterpret_cast<float2 *>(part + HD) = make_float2(mm, ll);
-        }
-    };
-    if (WK == 1) {
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-            if (!live[n]) continue;
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                float v[VT];
-#pragma unroll
-                for (int t = 0; t < VT; t++) v[t] = o[n][t][r];
-                put(qi[n], VT * (4 * g + r), v, std::integral_constant<int, VT>{}, l[n], m[n]);
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
+    // ---- the waves' parts together; out: the rows themselves, or their part
+    if (live) {
         if (g == 0) {
-            ml_l[wk][0][16 * n + c] = m[n];
-            ml_l[wk][1][16 * n + c] = l[n];
-            if (wk == 0) qi_l[16 * n + c] = live[n] ? qi[n] : -1;
+            ml_l[wid][0][c] = m;
+            ml_l[wid][1][c] = l;
         }
 #pragma unroll
         for (int r = 0; r < 4; r++)
 #pragma unroll
             for (int t = 0; t < VT; t += 4)
-                *reinterpret_cast<f32x4 *>(&o_l[wk][16 * n + c][VT * (4 * g + r) + t]) = f32x4{o[n][t][r], o[n][t + 1][r], o[n][t + 2][r], o[n][t + 3][r]};
+                *reinterpret_cast<f32x4 *>(&o_l[wid][c][VT * (4 * g + r) + t]) = f32x4{o[t][r], o[t + 1][r], o[t + 2][r], o[t + 3][r]};
     }
+    if (wid == 0 && g == 0) qi_l[c] = live ? qi : -1;
     __syncthreads();
-    const int cols = (int)min((unsigned)R, n_flat - f0);
-    for (int i = threadIdx.x; i < cols * (HD / 4); i += 256) {
+    for (int i = threadIdx.x; i < R * (HD / 4); i += 64 * W) {
         const int col = i / (HD / 4), d = 4 * (i % (HD / 4));
-        if (qi_l[col] < 0) continue;
-        float mm = KVP_NEG_INF, ll = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const int64_t to = qi_l[col];
+        if (to < 0) continue;
+        float mm = KVP_NEG_INF, ll = 0.0f, r4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < WK; w++) mm = fmaxf(mm, ml_l[w][0][col]);
+        for (int w = 0; w < W; w++) mm = fmaxf(mm, ml_l[w][0][col]);
         const float ref = mm == KVP_NEG_INF ? 0.0f : mm;
 #pragma unroll
-        for (int w = 0; w < WK; w++) {
+        for (int w = 0; w < W; w++) {
             const float e = __builtin_amdgcn_exp2f(ml_l[w][0][col] - ref);
             ll = fmaf(ml_l[w][1][col], e, ll);
             const f32x4 ow = *reinterpret_cast<const f32x4 *>(&o_l[w][col][d]);
 #pragma unroll
-            for (int r = 0; r < 4; r++) v[r] = fmaf(ow[r], e, v[r]);
+            for (int r = 0; r < 4; r++) r4[r] = fmaf(ow[r], e, r4[r]);
         }
-        put(qi_l[col], d, v, std::integral_constant<int, 4>{}, ll, mm);
+        if (whole) {
+            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+#pragma unroll
+            for (int r = 0; r < 4; r++) r4[r] *= inv;
+            kvp_store<BF16, 4>(a.out, to * HD + d, a.vec_o, r4);
+        } else {
+            float *part = a.part + (to * P + part_i) * kvp_part<HD>;
+            *reinterpret_cast<float2 *>(part + d) = make_float2(r4[0], r4[1]);
+            *reinterpret_cast<float2 *>(part + d + 2) = make_float2(r4[2], r4[3]);
+            if (d == 0) *reinterpret_cast<float2 *>(part + HD) = make_float2(mm, ll);
+        }
     }
 }
 
@@ -531,7 +522,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
     unsigned b = blockIdx.x;
     const int h = b % a.s.Hkv;
     b /= a.s.Hkv;
-    const int tile = a.otiles - 1 - (int)(b % (unsigned)a.otiles), split = b / a.otiles % (unsigned)a.so, j = b / a.otiles / a.so;
+    const int j = b % (unsigned)a.s.n_seq, split = b / a.s.n_seq % (unsigned)a.so, tile = a.otiles - 1 - (int)(b / a.s.n_seq / a.so);
     const int cap = a.s.table_ld << a.s.shift;
     const KvpRows sq = kvp_rows(a.s, j);
     const unsigned n_flat = (unsigned)sq.n * (unsigned)a.G, f0 = (unsigned)tile * R, fw = f0 + 32 * wid;
@@ -541,7 +532,13 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
     sg.lo = 0;
     sg.hi = (int)min((int64_t)cap, max((int64_t)sq.p0 + sq.n, (int64_t)0));
     const int from = split * a.co;
-    if (split > 0 && from >= sg.hi) return;
+    if (split > 0 && from >= sg.hi) {                            // a part without positions
+        const unsigned f = f0 + threadIdx.x;
+        if (threadIdx.x < R && f < n_flat)
+            *reinterpret_cast<float2 *>(a.part + (((sq.r0 + f / (unsigned)a.G) * a.Hq + h * a.G + f % (unsigned)a.G) * a.so + split) * kvp_part<HD> + HD) =
+                make_float2(KVP_NEG_INF, 0.0f);
+        return;
+    }
     const int upto = split + 1 < a.so ? min(from + a.co, sg.hi) : sg.hi;
     auto last_seen = [&](unsigned f) { return min(sq.p0 + (int)((min(f, n_flat) - 1) / (unsigned)a.G), cap - 1); };
     const int block_end = min(upto, last_seen(f0 + R) + 1), n_it = kvp_uniform(block_end > from ? (block_end - from + 31) / 32 : 0);
@@ -555,28 +552,27 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
         const int r = 8 * wid + RPL * i + lane / PR, n = (lane % PR) ^ (HD == 128 ? r & 15 : (r >> 1) & 7);
         src[i] = (uint32_t)((r & 15) * ROW + 16 * n);
     }
-    auto id_of = [&](int base) -> int {                          // the page of this wave's 8 positions
-        const int s = (base + 16 * (wid >> 1)) >> a.s.shift;
-        return s < a.s.table_ld ? __builtin_amdgcn_readfirstlane(sg.table[s]) : -1;
-    };
     auto base_of = [&](int it) { return from + 32 * min(it, n_it - 1); };
-    auto issue = [&](int slot, int base, int id) {
-        const int64_t at = kvp_uniform(kvp_at<HD>(a, (unsigned)id < (unsigned)a.s.n_pages ? id : 0, h, base + 16 * (wid >> 1)));
-        char *to = ring + slot * 2 * TB + 1024 * NL * wid;
+    auto issue = [&](int slot, int base, KvpIds ids) {
+        const int64_t at = kvp_uniform(kvp_at<HD>(a, wid < 2 ? ids.id[0] : ids.id[1], h, base + 16 * (wid >> 1)));
+        char *to = ring + slot + 1024 * NL * wid;
 #pragma unroll
         for (int i = 0; i < NL; i++) lds_dma16_s(a.kp + at, src[i], to + 1024 * i);
 #pragma unroll
         for (int i = 0; i < NL; i++) lds_dma16_s(a.vp + at, src[i], to + TB + 1024 * i);
     };
-    int id_next = 0;
+    KvpTable table(a, sg.table, n_it > 0 ? from : 0);
+    KvpIds ids0, ids1;                                           // of this turn's tile and the next one's
     if (n_it > 0) {
-        issue(0, base_of(0), id_of(base_of(0)));
-        issue(1, base_of(1), id_of(base_of(1)));
-        id_next = id_of(base_of(2));
+        ids0 = table.at(a, base_of(0));
+        issue(0, base_of(0), ids0);
+        ids1 = table.at(a, base_of(1));
+        issue(2 * TB, base_of(1), ids1);
     }
 
     // ---- the queries
-    const float kc = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.4426950408889634f;
+    // a negative scale is the queries', a zero one makes them zero
+    const float kc = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.4426950408889634f, sign = a.scale == 0.0f ? 0.0f : a.scale < 0.0f ? -1.0f : 1.0f;
     const unsigned f = fw + c;
     const bool live = f < n_flat;
     const unsigned i_row = live ? f / (unsigned)a.G : 0, head = h * a.G + (live ? f % (unsigned)a.G : 0);
@@ -590,7 +586,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
         for (int e = 0; e < 8; e++) x[e] = 0.0f;
         if (live) kvp_load_q<BF16, 8>(a.q, q_at + 16 * i + 8 * hf, a.vec_q, x);
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = a.scale == 0.0f ? 0.0f : a.scale < 0.0f ? -x[e] : x[e];
+        for (int e = 0; e < 8; e++) x[e] *= sign;
         bf16x8 tr[QT];
         kvp_terms<QT>(x, tr);
 #pragma unroll
@@ -603,24 +599,28 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
     for (int t = 0; t < DV; t++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[t][r] = 0.0f;
-    KvpIds ids = kvp_ids(a, sg.table, n_it > 0 ? base_of(0) : 0);
+    // where this lane reads in a stage: K's first piece, V's first position
+    const int k_at = c * ROW + 16 * (hf ^ (HD == 128 ? c & 15 : (c >> 1) & 7));
+    const int v_at = TB + 4 * hf * ROW + (HD == 128 ? 16 * ((c >> 1) ^ (4 * hf)) + 8 * (c & 1) : 16 * ((c >> 2) ^ (2 * hf)) + 4 * (c & 3));
+    int stage = 0, ahead = 4 * TB;
     for (int it = 0; it < n_it; it++) {
         wait_vmcnt<2 * NL>();                                    // this wave's loads of the stage have landed
         __syncthreads();                                         // ... and every wave's; the stage before is free
-        issue((it + 2) % NS, base_of(it + 2), id_next);
-        id_next = id_of(base_of(it + 3));
-        const KvpIds now = ids;
-        ids = kvp_ids(a, sg.table, base_of(it + 1));
+        const KvpIds now = ids0;
+        ids0 = ids1;
+        ids1 = table.at(a, base_of(it + 2));
+        issue(ahead, base_of(it + 2), ids1);
+        const int ks = k_at + stage, vs = v_at + stage;
+        ahead = stage;
+        stage = stage == 2 * (NS - 1) * TB ? 0 : stage + 2 * TB;
         const int base = from + 32 * it;
         if (base >= end) continue;
-        const char *ks = ring + it % NS * 2 * TB, *vs = ks + TB;
         f32x16 s;
 #pragma unroll
         for (int r = 0; r < 16; r++) s[r] = 0.0f;
 #pragma unroll
         for (int i = 0; i < KC; i++) {
-            const int n = (2 * i + hf) ^ (HD == 128 ? c & 15 : (c >> 1) & 7);
-            const bf16x8 k = *reinterpret_cast<const bf16x8 *>(ks + c * ROW + 16 * n);
+            const bf16x8 k = *reinterpret_cast<const bf16x8 *>(ring + (ks ^ (32 * i)));
 #pragma unroll
             for (int t = QT - 1; t >= 0; t--) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[t][i], s, 0, 0, 0);
         }
@@ -658,14 +658,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
             uint32_t v[8][DV / 2];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const int r = 16 * x + 8 * (e >> 2) + 4 * hf + (e & 3), swz = HD == 128 ? r & 15 : (r >> 1) & 7;
-                const char *row = vs + r * ROW;
+                const int n = 8 * (e >> 2) + (e & 3), r = 16 * x + n + 4 * hf;
+                const char *row = ring + (vs ^ (16 * (HD == 128 ? n : n >> 1))) + (16 * x + n) * ROW;
                 if (HD == 128) {
-                    const uint2 u = *reinterpret_cast<const uint2 *>(row + 16 * ((c >> 1) ^ swz) + 8 * (c & 1));
+                    const uint2 u = *reinterpret_cast<const uint2 *>(row);
                     v[e][0] = u.x;
                     v[e][DV / 2 - 1] = u.y;
                 } else {
-                    v[e][0] = *reinterpret_cast<const uint32_t *>(row + 16 * ((c >> 2) ^ swz) + 4 * (c & 3));
+                    v[e][0] = *reinterpret_cast<const uint32_t *>(row);
                 }
                 if (edge) {
                     // V of positions that no row here sees may hold anything
@@ -726,39 +726,46 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
     if (a.so > 1 && hf == 0) *reinterpret_cast<float2 *>(part + HD) = make_float2(m, l);
 }
 
-// The parts of each row and head, in order; a wave a head.  Each lane weighs one part,
-// then the sums' loads do not wait for one another.
+// The parts of each row and head, in order; a wave a head.  Bound by its chain of loads: a
+// part that has no positions says so by its sum, so that nothing but the rows' places has
+// to be known, and the first eight parts are on their way with the weights.
 template <bool BF16, int HD>
 __global__ __launch_bounds__(256) void k_attn_kvp_merge(AttnKvpArgs a) {
+    constexpr int E = HD / 64;
     const int lane = threadIdx.x & 63;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int j = blockIdx.y, i = blockIdx.x, head = blockIdx.z * 4 + wid;
     const KvpRows sq = kvp_rows(a.s, j);
     if (i >= sq.n || head >= a.Hq) return;
-    const int cap = a.s.table_ld << a.s.shift, sp = a.prefix ? a.sp : 0, P = sp + a.so;
-    const int sh = a.prefix ? min(max(a.shared[j / a.group], 0), cap) : 0;
-    const int hi = (int)min((int64_t)cap, max((int64_t)sq.p0 + sq.n, (int64_t)0)), lo = sh & ~31;
-    // the parts that the blocks wrote
-    const int np = a.prefix ? min(sp, (sh + a.cp - 1) / a.cp) : 0, no = hi > lo ? min(a.so, (hi - lo + a.co - 1) / a.co) : 1;
+    const int P = (a.prefix ? a.sp : 0) + a.so;
     const int64_t qi = (sq.r0 + i) * a.Hq + head;
     const float *part = a.part + qi * P * kvp_part<HD>;
-    const bool have = lane < sp ? lane < np : lane < sp + no;
-    float2 ml = make_float2(KVP_NEG_INF, 0.0f);
-    if (have) ml = *reinterpret_cast<const float2 *>(part + lane * kvp_part<HD> + HD);
-    float mm = ml.x;
+    const float2 ml = *reinterpret_cast<const float2 *>(part + min(lane, P - 1) * kvp_part<HD> + HD);
+    float p[8][E];
+    auto load = [&](int x0) {
 #pragma unroll
-    for (int s = 32; s > 0; s >>= 1) mm = fmaxf(mm, __shfl_xor(mm, s, 64));
-    const float w = have ? __builtin_amdgcn_exp2f(ml.x - (mm == KVP_NEG_INF ? 0.0f : mm)) : 0.0f;
-    const float ll = wave_sum_f32(ml.y * w);
-    constexpr int E = HD / 64;
+        for (int u = 0; u < 8; u++)
+#pragma unroll
+            for (int e = 0; e < E; e++) p[u][e] = part[min(x0 + u, P - 1) * kvp_part<HD> + E * lane + e];
+    };
+    load(0);
+    const float mx = lane < P ? ml.x : KVP_NEG_INF;
+    const float mm = wave_max_f32(mx);
+    const float w = mx == KVP_NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(mx - mm);
+    const float ll = wave_sum_f32(mx == KVP_NEG_INF ? 0.0f : ml.y * w);
     float v[E];
 #pragma unroll
     for (int e = 0; e < E; e++) v[e] = 0.0f;
-    for (int x = 0; x < P; x++) {
-        if (x < sp ? x >= np : x >= sp + no) continue;
-        const float wx = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), x));
+    for (int x0 = 0; x0 < P; x0 += 8) {
+        if (x0 > 0) load(x0);
 #pragma unroll
-        for (int e = 0; e < E; e++) v[e] = fmaf(part[x * kvp_part<HD> + E * lane + e], wx, v[e]);
+        for (int u = 0; u < 8; u++) {
+            const int x = min(x0 + u, 63);
+            const float wx = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), x));
+            const bool is = x0 + u < P && __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mx), x)) != KVP_NEG_INF;
+#pragma unroll
+            for (int e = 0; e < E; e++) v[e] = is ? fmaf(p[u][e], wx, v[e]) : v[e];
+        }
     }
     const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
@@ -775,11 +782,11 @@ static hipError_t go_merge(const AttnKvpArgs &a, hipStream_t st) {
     return hipGetLastError();
 }
 
-// splits of `len` positions over blocks that take `step` of them a turn: up to 512 blocks
-// (two a CU) at `units` tiles, each with `turns` turns at least
-static void kvp_split(int64_t units, int64_t len, int64_t most, int step, int turns, int &s, int &chunk) {
+// splits of `len` positions over blocks that take `step` of them a turn: up to `blocks` of
+// them at `units` tiles, each with `turns` turns at least
+static void kvp_split(int64_t units, int64_t len, int64_t most, int blocks, int step, int turns, int &s, int &chunk) {
     const int64_t tiles = (len + 31) / 32 + 1;
-    const int64_t n = std::max<int64_t>(1, std::min({most, 512 / std::max<int64_t>(1, units), tiles * 32 / (step * turns)}));
+    const int64_t n = std::max<int64_t>(1, std::min({most, blocks / std::max<int64_t>(1, units), tiles * 32 / (step * turns)}));
     chunk = (int)((tiles + n - 1) / n * 32);
     s = (int)((tiles * 32 + chunk - 1) / chunk);
 }
@@ -789,7 +796,7 @@ static hipError_t go_rows(AttnKvpArgs &a, int64_t room, hipStream_t st) {
     const int64_t tiles = (a.s.max_rows * a.G + 127) / 128;
     // sequences shorter than max_rows leave tiles empty: counted are those that n_rows rows fill, half a one a sequence
     const int64_t units = std::min(tiles * a.s.n_seq, (a.s.n_rows * a.G / 64 + a.s.n_seq) / 2 + 1) * a.s.Hkv;
-    kvp_split(units, a.max_len, std::max<int64_t>(1, room), 32, 4, a.so, a.co);
+    kvp_split(units, a.max_len, std::max<int64_t>(1, room), 512, 32, 4, a.so, a.co);
     a.otiles = (int)tiles;
     const int64_t blocks = (int64_t)a.s.n_seq * a.so * tiles * a.s.Hkv;
     if (blocks * 256 > UINT32_MAX) return hipErrorInvalidValue;
@@ -797,21 +804,32 @@ static hipError_t go_rows(AttnKvpArgs &a, int64_t room, hipStream_t st) {
     return a.so > 1 ? go_merge<BF16, HD>(a, st) : hipGetLastError();
 }
 
+template <bool BF16, int HD, int W, bool ONCE, bool AHEAD>
+static hipError_t run_few(const AttnKvpArgs &a, int64_t blocks, hipStream_t st) {
+    if (blocks * 64 * W > UINT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_attn_kvp<BF16, HD, W, ONCE, AHEAD>), dim3((unsigned)blocks), dim3(64 * W), 0, st, a);
+    return a.prefix || a.so > 1 ? go_merge<BF16, HD>(a, st) : hipGetLastError();
+}
+
 template <bool BF16, int HD>
 static hipError_t go_few(AttnKvpArgs &a, int64_t room, hipStream_t st) {
     constexpr int R = 16;
-    const int64_t n_groups = a.prefix ? (a.s.n_seq + a.group - 1) / a.group : 0;
-    const int64_t otiles = (a.s.max_rows * a.G + R - 1) / R, ptiles = a.prefix ? ((int64_t)a.group * a.s.max_rows * a.G + R - 1) / R : 0;
+    const int64_t otiles = (a.s.max_rows * a.G + R - 1) / R, own = (int64_t)a.s.n_seq * a.s.Hkv * otiles;
+    a.prefix = a.prefix && (own > 256 || a.max_len > 640);
+    const int64_t n_groups = a.prefix ? (a.s.n_seq + a.group - 1) / a.group : 0, ptiles = a.prefix ? ((int64_t)a.group * a.s.max_rows * a.G + R - 1) / R : 0;
     a.otiles = (int)otiles;
     a.ptiles = (int)ptiles;
-    a.sp = 1;
-    a.cp = 1 << 30;
-    if (a.prefix) kvp_split(n_groups * ptiles * a.s.Hkv, a.max_len, room / 2, 128, 1, a.sp, a.cp);
-    kvp_split((int64_t)a.s.n_seq * a.s.Hkv * otiles, a.prefix ? a.max_own : a.max_len, a.prefix ? room - a.sp : std::max<int64_t>(1, room), 128, 1, a.so, a.co);
-    const int64_t blocks = (n_groups * a.sp * ptiles + (int64_t)a.s.n_seq * a.so * otiles) * a.s.Hkv;
-    if (blocks * 256 > UINT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_attn_kvp<BF16, HD, 1, 1>), dim3((unsigned)blocks), dim3(256), 0, st, a);
-    return a.prefix || a.so > 1 ? go_merge<BF16, HD>(a, st) : hipGetLastError();
+    a.sp = a.so = 1;
+    a.cp = a.co = 1 << 30;
+    const int64_t blocks_own = own, blocks_pre = n_groups * ptiles * a.s.Hkv;
+    if (!a.prefix) {
+        if (a.max_len > 512) kvp_split(own, a.max_len, room, 256, 256, 1, a.so, a.co);
+        const bool once = otiles == 1 && (int64_t)a.s.n_seq * a.max_len * a.s.Hkv * HD * 4 >= (int64_t)256 << 20;
+        return once ? run_few<BF16, HD, 8, true, false>(a, own * a.so, st) : run_few<BF16, HD, 8, false, true>(a, own * a.so, st);
+    }
+    kvp_split(own, a.max_own, room / 2, 768, 128, 1, a.so, a.co);
+    kvp_split(blocks_pre, a.max_len, room - a.so, (int)std::max<int64_t>(768 - own * a.so, 256), 128, 1, a.sp, a.cp);
+    return run_few<BF16, HD, 4, false, false>(a, blocks_pre * a.sp + own * a.so, st);
 }
 
 template <bool BF16, int HD>

@@ -378,7 +378,9 @@ ATTN = [
 def test_attention(dev, counts, pos, group, shared, heads, g, dim, page, is_bf16):
     print(f"attention {counts[:8]} at {pos[:8]} group={group} shared={shared} heads={heads} x {g} dim={dim} page={page} bf16={is_bf16}", flush=True)
     r = rng(sum(counts) + heads + page)
-    c = Cache(dev, r, [a + b for a, b in zip(counts, pos)], page, heads, dim, group, shared)
+    # tables of 700 positions and more: without hints prefixes are read once (shorter ones are not worth a merge)
+    c = Cache(dev, r, [a + b for a, b in zip(counts, pos)], page, heads, dim, group, shared,
+              width=pages_of(max(700, *(a + b for a, b in zip(counts, pos))), page) + 1)
     q = r.normal(0, 1, (sum(counts), heads * g, dim))
     pad, off = ((0, 0), (8, 0), (3, 1))[(sum(counts) + page // 16) % 3]
     got = attention(dev, c, q, counts, pos, g, group, shared, is_bf16, pad, off)
@@ -466,7 +468,7 @@ def test_attention_not_finite_behind_a_shared_prefix(dev, is_bf16):
     """NaN in what one member holds behind the prefix, and in the prefix past what a short member sees."""
     r = rng(20)
     counts, pos = [1] * 6, [100, 101, 102, 103, 60, 105]
-    c = Cache(dev, r, [p + 1 for p in pos], 16, 2, 128, 6, [96])
+    c = Cache(dev, r, [p + 1 for p in pos], 16, 2, 128, 6, [96], width=50)
     q = r.normal(0, 1, (6, 4, 128))
     clean = attention(dev, c, q, counts, pos, 2, 6, [96], is_bf16)
     for x in "kv":
@@ -483,7 +485,7 @@ def test_attention_rows_past_max_rows(dev):
     from qwenasr_amd import kernels as K
     r = rng(21)
     counts, pos, most = [5, 2, 7, 1], [60, 61, 62, 63], 3
-    c = Cache(dev, r, [a + b for a, b in zip(counts, pos)], 32, 2, 64, 4, [60])
+    c = Cache(dev, r, [a + b for a, b in zip(counts, pos)], 32, 2, 64, 4, [60], width=25)
     q = r.normal(0, 1, (15, 4, 64))
     for group, shared in ((1, None), (4, [60]), (2, [60, 32])):
         got = attention(dev, c, q, counts, pos, 2, group, shared, max_rows=most)
@@ -697,7 +699,7 @@ def test_nothing_to_do(dev):
 class Step:
     """One step of n-best decoding over a toy model: fork, per layer write and attention, the head, log probabilities.  The
     model: a token's rows of q, k, v per layer, and a head over the sum of the layers' attention."""
-    PAGE, HEADS, G, DIM, LAYERS, VOCAB, PAGES, WIDTH = 16, 2, 2, 64, 2, 300, 120, 8
+    PAGE, HEADS, G, DIM, LAYERS, VOCAB, PAGES, WIDTH = 16, 2, 2, 64, 2, 300, 120, 48
 
     def __init__(self, dev, r, n, group):
         self.dev, self.n, self.group = dev, n, group
