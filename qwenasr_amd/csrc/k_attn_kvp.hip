@@ -31,6 +31,10 @@ namespace qasr {
 #define KVP_NEG_INF (-__builtin_inff())
 // a running maximum is moved only when it is passed by 2^8: weights stay below 2^8
 #define KVP_SLACK 8.0f
+#ifndef KVP_RW
+#define KVP_RW 2
+#define KVP_PG 2
+#endif
 
 template <int HD>
 struct KvpDims {
@@ -503,26 +507,71 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_kvp(AttnKvpArgs a) {
     }
 }
 
-// Many rows of a sequence: a block of four waves, 32 query columns each, goes through the
-// positions together; K and V come 32 positions at a time through a ring of three LDS
-// stages, so a block reads them once.  v_mfma 32x32x16: S^T leaves lane half hf of a
+// The i-th of the tiles of R rows x heads that there are, those furthest back in their
+// sequences first: those of the last index that a sequence has, in order of the sequences, and so
+// on.  Blocks that have none (there are as many as the host can tell) come last: between
+// the others they leave the CUs' registers in pieces (six prompts of up to 1337 rows: 400 of
+// 512 blocks at a time).
+struct KvpTile { int j, tile; };
+template <int R>
+__device__ __forceinline__ KvpTile kvp_tile(const AttnKvpArgs &a, int i) {
+    const int lane = threadIdx.x & 63;
+    auto tiles_of = [&](int j) { return j < a.s.n_seq ? (int)(((unsigned)kvp_rows(a.s, j).n * (unsigned)a.G + R - 1) / R) : 0; };
+    if (a.s.n_seq == 1) return {0, tiles_of(0) - 1 - i};
+    const int mine = tiles_of(lane);
+    // tiles of index t and more
+    auto from = [&](int t) {
+        int n = max(0, mine - t);
+        for (int j = 64 + lane; j < a.s.n_seq; j += 64) n += max(0, tiles_of(j) - t);
+        return wave_sum_i32(n);
+    };
+    if (i >= from(0)) return {0, -1};
+    int t = 0, end = a.otiles;                   // from(t) > i >= from(end)
+    while (end - t > 1) {
+        const int mid = (t + end) / 2;
+        if (from(mid) > i) t = mid;
+        else end = mid;
+    }
+    int r = i - from(t + 1);                     // of the sequences that have it
+    for (int j0 = 0; j0 < a.s.n_seq; j0 += 64) {
+        const unsigned long long has = __ballot((j0 == 0 ? mine : tiles_of(j0 + lane)) > t);
+        const int n = __popcll(has);
+        if (r < n) {
+            const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(has >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)has, 0));
+            return {j0 + __ffsll((unsigned long long)__ballot(((has >> lane) & 1) && before == r)) - 1, t};
+        }
+        r -= n;
+    }
+    return {0, -1};
+}
+
+// Many rows of a sequence: a block of eight waves, RW of them side by side with 32 query
+// columns each, PG = 8 / RW groups of them over every PG-th 32 positions.  A group's K and V
+// come through a ring of LDS stages, once for its RW waves; the groups' sums are joined at the
+// end.  v_mfma 32x32x16: S^T leaves lane half hf of a
 // column positions 8 (r / 4) + 4 hf + r % 4, and the second product's k is numbered like
 // that, as above.  16-byte piece n of position r stands at n ^ (r & 15) (128 dims) or
 // n ^ ((r / 2) & 7) (64), which spreads the 16 lanes that LDS serves at a time over all banks.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-template <bool BF16, int HD>
-__global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
-    constexpr int KC = HD / 16, DV = HD / 32, QT = BF16 ? 1 : 3, PT = BF16 ? 2 : 3, R = 128;
-    constexpr int ROW = HD * 2, TB = 32 * ROW, NS = 3, NL = TB / 4096, PR = ROW / 16, RPL = 64 / PR;
-    __shared__ __attribute__((aligned(1024))) char ring[NS * 2 * TB];
+template <bool BF16, int HD, int RW, int PG>
+__global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
+    constexpr int KC = HD / 16, DV = HD / 32, QT = BF16 ? 1 : 3, PT = BF16 ? 2 : 3, R = 32 * RW;
+    // bytes of a position and of a tile; loads of a wave for K of a tile; 16-byte pieces of a position, positions of a load
+    constexpr int ROW = HD * 2, TB = 32 * ROW, NS = PG * RW == 8 && RW == 2 ? 2 : PG == 1 || RW == 4 ? 3 : 2, NL = TB / 1024 / RW, PR = ROW / 16, RPL = 64 / PR;
+    constexpr int RING = NS * 2 * TB, JOIN = (PG - 1) * RW * (16 * DV + 2) * 256;
+    __shared__ __attribute__((aligned(1024))) char smem[PG * RING > JOIN ? PG * RING : JOIN];
     const int lane = threadIdx.x & 63, c = lane & 31, hf = lane >> 5;
-    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wid = wave % RW, grp = wave / RW;
+    char *const ring = smem + grp * RING;
 
-    // ---- which rows, which positions; the tiles with the most positions first
+    // ---- which rows, which positions
     unsigned b = blockIdx.x;
     const int h = b % a.s.Hkv;
     b /= a.s.Hkv;
-    const int j = b % (unsigned)a.s.n_seq, split = b / a.s.n_seq % (unsigned)a.so, tile = a.otiles - 1 - (int)(b / a.s.n_seq / a.so);
+    const int split = b % (unsigned)a.so;
+    const KvpTile at_tile = kvp_tile<R>(a, (int)(b / (unsigned)a.so));
+    const int tile = at_tile.tile, j = at_tile.j;
+    if (tile < 0) return;
     const int cap = a.s.table_ld << a.s.shift;
     const KvpRows sq = kvp_rows(a.s, j);
     const unsigned n_flat = (unsigned)sq.n * (unsigned)a.G, f0 = (unsigned)tile * R, fw = f0 + 32 * wid;
@@ -541,20 +590,22 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
     }
     const int upto = split + 1 < a.so ? min(from + a.co, sg.hi) : sg.hi;
     auto last_seen = [&](unsigned f) { return min(sq.p0 + (int)((min(f, n_flat) - 1) / (unsigned)a.G), cap - 1); };
-    const int block_end = min(upto, last_seen(f0 + R) + 1), n_it = kvp_uniform(block_end > from ? (block_end - from + 31) / 32 : 0);
+    const int block_end = min(upto, last_seen(f0 + R) + 1), n_it = kvp_uniform(block_end > from ? (block_end - from + 32 * PG - 1) / (32 * PG) : 0);
     const int end = kvp_uniform(fw < n_flat ? min(upto, last_seen(fw + 32) + 1) : from);      // this wave's
     const int all_see = kvp_uniform(fw < n_flat ? sq.p0 + (int)(fw / (unsigned)a.G) : -1);    // what its first row sees
 
-    // ---- a stage: each wave loads 8 positions of K and of V
+    // ---- a stage: each wave of the group loads 32 / RW positions of K and of V
     uint32_t src[NL];
 #pragma unroll
     for (int i = 0; i < NL; i++) {
-        const int r = 8 * wid + RPL * i + lane / PR, n = (lane % PR) ^ (HD == 128 ? r & 15 : (r >> 1) & 7);
-        src[i] = (uint32_t)((r & 15) * ROW + 16 * n);
+        const int r = 32 / RW * wid + RPL * i + lane / PR, n = (lane % PR) ^ (HD == 128 ? r & 15 : (r >> 1) & 7);
+        src[i] = (uint32_t)((r & 15) * ROW + 16 * n);                // within a half of the tile
     }
-    auto base_of = [&](int it) { return from + 32 * min(it, n_it - 1); };
+    // the group's tiles; past its last one, that again: nothing sees it
+    auto base_of = [&](int it) { return min(from + 32 * (PG * min(it, n_it - 1) + grp), (block_end - 1) & ~31); };
     auto issue = [&](int slot, int base, KvpIds ids) {
-        const int64_t at = kvp_uniform(kvp_at<HD>(a, wid < 2 ? ids.id[0] : ids.id[1], h, base + 16 * (wid >> 1)));
+        const int half = wid / (RW / 2);
+        const int64_t at = kvp_uniform(kvp_at<HD>(a, half ? ids.id[1] : ids.id[0], h, base + 16 * half));
         char *to = ring + slot + 1024 * NL * wid;
 #pragma unroll
         for (int i = 0; i < NL; i++) lds_dma16_s(a.kp + at, src[i], to + 1024 * i);
@@ -566,8 +617,10 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
     if (n_it > 0) {
         ids0 = table.at(a, base_of(0));
         issue(0, base_of(0), ids0);
-        ids1 = table.at(a, base_of(1));
-        issue(2 * TB, base_of(1), ids1);
+        if (NS == 3) {
+            ids1 = table.at(a, base_of(1));
+            issue(2 * TB, base_of(1), ids1);
+        }
     }
 
     // ---- the queries
@@ -602,18 +655,19 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
     // where this lane reads in a stage: K's first piece, V's first position
     const int k_at = c * ROW + 16 * (hf ^ (HD == 128 ? c & 15 : (c >> 1) & 7));
     const int v_at = TB + 4 * hf * ROW + (HD == 128 ? 16 * ((c >> 1) ^ (4 * hf)) + 8 * (c & 1) : 16 * ((c >> 2) ^ (2 * hf)) + 4 * (c & 3));
-    int stage = 0, ahead = 4 * TB;
+    int stage = 0, ahead = 2 * (NS - 1) * TB;
     for (int it = 0; it < n_it; it++) {
-        wait_vmcnt<2 * NL>();                                    // this wave's loads of the stage have landed
+        wait_vmcnt<2 * NL * (NS - 2)>();                         // this wave's loads of the stage have landed
         __syncthreads();                                         // ... and every wave's; the stage before is free
         const KvpIds now = ids0;
-        ids0 = ids1;
-        ids1 = table.at(a, base_of(it + 2));
-        issue(ahead, base_of(it + 2), ids1);
+        if (NS == 3) ids0 = ids1;
+        KvpIds &ids = NS == 3 ? ids1 : ids0;
+        ids = table.at(a, base_of(it + NS - 1));
+        issue(ahead, base_of(it + NS - 1), ids);
         const int ks = k_at + stage, vs = v_at + stage;
         ahead = stage;
         stage = stage == 2 * (NS - 1) * TB ? 0 : stage + 2 * TB;
-        const int base = from + 32 * it;
+        const int base = from + 32 * (PG * it + grp);
         if (base >= end) continue;
         f32x16 s;
 #pragma unroll
@@ -658,7 +712,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
             uint32_t v[8][DV / 2];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const int n = 8 * (e >> 2) + (e & 3), r = 16 * x + n + 4 * hf;
+                const int n = 8 * (e >> 2) + (e & 3);
                 const char *row = ring + (vs ^ (16 * (HD == 128 ? n : n >> 1))) + (16 * x + n) * ROW;
                 if (HD == 128) {
                     const uint2 u = *reinterpret_cast<const uint2 *>(row);
@@ -667,11 +721,13 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
                 } else {
                     v[e][0] = *reinterpret_cast<const uint32_t *>(row);
                 }
-                if (edge) {
-                    // V of positions that no row here sees may hold anything
+            }
+            if (edge) {
+                // V of positions that no row here sees may hold anything
 #pragma unroll
-                    for (int d = 0; d < DV / 2; d++) v[e][d] = base + r < end && now.id[x] >= 0 ? v[e][d] : 0u;
-                }
+                for (int e = 0; e < 8; e++)
+#pragma unroll
+                    for (int d = 0; d < DV / 2; d++) v[e][d] = base + 16 * x + 8 * (e >> 2) + (e & 3) + 4 * hf < end && now.id[x] >= 0 ? v[e][d] : 0u;
             }
 #pragma unroll
             for (int t = 0; t < DV; t++) {
@@ -694,7 +750,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
     l = xhalf_sum(l);
     if (__any(live && z != 0.0f)) {
         float om[HD / 2 + 2];
-        attn_kvp_again<BF16, HD, 32>(a, sg, h, q_at, live, lim, from, end, 32, a.scale * 1.4426950408889634f, om);
+        attn_kvp_again<BF16, HD, 32>(a, sg, h, q_at, live, lim, from + 32 * grp, end, 32 * PG, a.scale * 1.4426950408889634f, om);
 #pragma unroll
         for (int t = 0; t < DV; t++)
 #pragma unroll
@@ -702,7 +758,41 @@ __global__ __launch_bounds__(256, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
         m = om[HD / 2];
         l = om[HD / 2 + 1];
     }
-    if (!live) return;
+    // the groups' sums, in order, into the first's: every lane's from the same lane of the others
+    if (PG > 1) __syncthreads();
+    float *const join = reinterpret_cast<float *>(smem) + lane;
+    auto join_at = [&](int g, int r) -> float & { return join[((g - 1) * RW + wid) * (16 * DV + 2) * 64 + r * 64]; };
+    if (grp > 0) {
+        join_at(grp, 0) = m;
+        join_at(grp, 1) = l;
+#pragma unroll
+        for (int t = 0; t < DV; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) join_at(grp, 2 + 16 * t + r) = o[t][r];
+    }
+    if (PG > 1) __syncthreads();
+    if (grp > 0 || !live) return;
+    if (PG > 1) {
+        float mm = m;
+#pragma unroll
+        for (int g = 1; g < PG; g++) mm = fmaxf(mm, join_at(g, 0));
+        const float ref = mm == KVP_NEG_INF ? 0.0f : mm, own = __builtin_amdgcn_exp2f(m - ref);
+        l *= own;
+#pragma unroll
+        for (int t = 0; t < DV; t++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[t][r] *= own;
+#pragma unroll
+        for (int g = 1; g < PG; g++) {
+            const float w = __builtin_amdgcn_exp2f(join_at(g, 0) - ref);
+            l = fmaf(join_at(g, 1), w, l);
+#pragma unroll
+            for (int t = 0; t < DV; t++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[t][r] = fmaf(join_at(g, 2 + 16 * t + r), w, o[t][r]);
+        }
+        m = mm;
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     float *part = a.part + (qi * a.so + split) * kvp_part<HD>;
 #pragma unroll
@@ -791,16 +881,17 @@ static void kvp_split(int64_t units, int64_t len, int64_t most, int blocks, int 
     s = (int)((tiles * 32 + chunk - 1) / chunk);
 }
 
-template <bool BF16, int HD>
+template <bool BF16, int HD, int RW, int PG>
 static hipError_t go_rows(AttnKvpArgs &a, int64_t room, hipStream_t st) {
-    const int64_t tiles = (a.s.max_rows * a.G + 127) / 128;
+    constexpr int R = 32 * RW;
+    const int64_t tiles = (a.s.max_rows * a.G + R - 1) / R;
     // sequences shorter than max_rows leave tiles empty: counted are those that n_rows rows fill, half a one a sequence
-    const int64_t units = std::min(tiles * a.s.n_seq, (a.s.n_rows * a.G / 64 + a.s.n_seq) / 2 + 1) * a.s.Hkv;
-    kvp_split(units, a.max_len, std::max<int64_t>(1, room), 512, 32, 4, a.so, a.co);
+    const int64_t units = std::min(tiles * a.s.n_seq, (a.s.n_rows * a.G * 2 / R + a.s.n_seq) / 2 + 1) * a.s.Hkv;
+    kvp_split(units, a.max_len, std::max<int64_t>(1, room), 2048 / (RW * PG), 32 * PG, 4, a.so, a.co);
     a.otiles = (int)tiles;
-    const int64_t blocks = (int64_t)a.s.n_seq * a.so * tiles * a.s.Hkv;
-    if (blocks * 256 > UINT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_attn_kvp_rows<BF16, HD>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    const int64_t blocks = std::min(tiles * a.s.n_seq, a.s.n_rows * a.G / R + a.s.n_seq) * a.so * a.s.Hkv;
+    if (blocks * 64 * RW * PG > UINT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_attn_kvp_rows<BF16, HD, RW, PG>), dim3((unsigned)blocks), dim3(64 * RW * PG), 0, st, a);
     return a.so > 1 ? go_merge<BF16, HD>(a, st) : hipGetLastError();
 }
 
@@ -834,7 +925,7 @@ static hipError_t go_few(AttnKvpArgs &a, int64_t room, hipStream_t st) {
 
 template <bool BF16, int HD>
 static hipError_t go_attn_kvp(AttnKvpArgs &a, int64_t room, hipStream_t st) {
-    return a.s.max_rows * a.G > 32 ? go_rows<BF16, HD>(a, room, st) : go_few<BF16, HD>(a, room, st);
+    return a.s.max_rows * a.G > 32 ? go_rows<BF16, HD, KVP_RW, KVP_PG>(a, room, st) : go_few<BF16, HD>(a, room, st);
 }
 
 hipError_t launch_attention_kvp(const AttnKvpArgs &a0, bool bf16, hipStream_t st) {
