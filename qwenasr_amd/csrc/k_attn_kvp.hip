@@ -31,10 +31,6 @@ namespace qasr {
 #define KVP_NEG_INF (-__builtin_inff())
 // a running maximum is moved only when it is passed by 2^8: weights stay below 2^8
 #define KVP_SLACK 8.0f
-#ifndef KVP_RW
-#define KVP_RW 2
-#define KVP_PG 2
-#endif
 
 template <int HD>
 struct KvpDims {
@@ -545,8 +541,8 @@ __device__ __forceinline__ KvpTile kvp_tile(const AttnKvpArgs &a, int i) {
     return {0, -1};
 }
 
-// Many rows of a sequence: a block of eight waves, RW of them side by side with 32 query
-// columns each, PG = 8 / RW groups of them over every PG-th 32 positions.  A group's K and V
+// Many rows of a sequence: a block of RW x PG waves, RW of them side by side with 32 query
+// columns each, PG groups of them over every PG-th 32 positions.  A group's K and V
 // come through a ring of LDS stages, once for its RW waves; the groups' sums are joined at the
 // end.  v_mfma 32x32x16: S^T leaves lane half hf of a
 // column positions 8 (r / 4) + 4 hf + r % 4, and the second product's k is numbered like
@@ -556,8 +552,8 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <bool BF16, int HD, int RW, int PG>
 __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
     constexpr int KC = HD / 16, DV = HD / 32, QT = BF16 ? 1 : 3, PT = BF16 ? 2 : 3, R = 32 * RW;
-    // bytes of a position and of a tile; loads of a wave for K of a tile; 16-byte pieces of a position, positions of a load
-    constexpr int ROW = HD * 2, TB = 32 * ROW, NS = PG * RW == 8 && RW == 2 ? 2 : PG == 1 || RW == 4 ? 3 : 2, NL = TB / 1024 / RW, PR = ROW / 16, RPL = 64 / PR;
+    // bytes of a position and of a tile (a ring of two: three held a CU to one block); loads of a wave for K of a tile; 16-byte pieces of a position, positions of a load
+    constexpr int ROW = HD * 2, TB = 32 * ROW, NS = 2, NL = TB / 1024 / RW, PR = ROW / 16, RPL = 64 / PR;
     constexpr int RING = NS * 2 * TB, JOIN = (PG - 1) * RW * (16 * DV + 2) * 256;
     __shared__ __attribute__((aligned(1024))) char smem[PG * RING > JOIN ? PG * RING : JOIN];
     const int lane = threadIdx.x & 63, c = lane & 31, hf = lane >> 5;
@@ -613,14 +609,10 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
         for (int i = 0; i < NL; i++) lds_dma16_s(a.vp + at, src[i], to + TB + 1024 * i);
     };
     KvpTable table(a, sg.table, n_it > 0 ? from : 0);
-    KvpIds ids0, ids1;                                           // of this turn's tile and the next one's
+    KvpIds ids;
     if (n_it > 0) {
-        ids0 = table.at(a, base_of(0));
-        issue(0, base_of(0), ids0);
-        if (NS == 3) {
-            ids1 = table.at(a, base_of(1));
-            issue(2 * TB, base_of(1), ids1);
-        }
+        ids = table.at(a, base_of(0));
+        issue(0, base_of(0), ids);
     }
 
     // ---- the queries
@@ -655,36 +647,50 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
     // where this lane reads in a stage: K's first piece, V's first position
     const int k_at = c * ROW + 16 * (hf ^ (HD == 128 ? c & 15 : (c >> 1) & 7));
     const int v_at = TB + 4 * hf * ROW + (HD == 128 ? 16 * ((c >> 1) ^ (4 * hf)) + 8 * (c & 1) : 16 * ((c >> 2) ^ (2 * hf)) + 4 * (c & 3));
-    int stage = 0, ahead = 2 * (NS - 1) * TB;
+    int stage = 0;
     for (int it = 0; it < n_it; it++) {
-        wait_vmcnt<2 * NL * (NS - 2)>();                         // this wave's loads of the stage have landed
-        __syncthreads();                                         // ... and every wave's; the stage before is free
-        const KvpIds now = ids0;
-        if (NS == 3) ids0 = ids1;
-        KvpIds &ids = NS == 3 ? ids1 : ids0;
-        ids = table.at(a, base_of(it + NS - 1));
-        issue(ahead, base_of(it + NS - 1), ids);
+        wait_vmcnt<0>();                                         // this wave's loads of the stage have landed
+        __syncthreads();                                         // ... and every wave's; the other stage is free
+        const KvpIds now = ids;
+        ids = table.at(a, base_of(it + 1));
         const int ks = k_at + stage, vs = v_at + stage;
-        ahead = stage;
-        stage = stage == 2 * (NS - 1) * TB ? 0 : stage + 2 * TB;
+        stage ^= 2 * TB;
+        issue(stage, base_of(it + 1), ids);
         const int base = from + 32 * (PG * it + grp);
         if (base >= end) continue;
+        // the tile's K first, all of it, and V as early as registers are free: LDS answers late
+        bf16x8 k[KC];
+#pragma unroll
+        for (int i = 0; i < KC; i++) k[i] = *reinterpret_cast<const bf16x8 *>(ring + (ks ^ (32 * i)));
+        uint32_t v[2][8][DV / 2];
+        auto load_v = [&](int x) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int n = 8 * (e >> 2) + (e & 3);
+                const char *row = ring + (vs ^ (16 * (HD == 128 ? n : n >> 1))) + (16 * x + n) * ROW;
+                if (HD == 128) {
+                    const uint2 u = *reinterpret_cast<const uint2 *>(row);
+                    v[x][e][0] = u.x;
+                    v[x][e][DV / 2 - 1] = u.y;
+                } else {
+                    v[x][e][0] = *reinterpret_cast<const uint32_t *>(row);
+                }
+            }
+        };
+        asm volatile("" ::: "memory");
         f32x16 s;
 #pragma unroll
         for (int r = 0; r < 16; r++) s[r] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < KC; i++) {
-            const bf16x8 k = *reinterpret_cast<const bf16x8 *>(ring + (ks ^ (32 * i)));
+        for (int i = 0; i < KC; i++)
 #pragma unroll
-            for (int t = QT - 1; t >= 0; t--) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[t][i], s, 0, 0, 0);
-        }
+            for (int t = QT - 1; t >= 0; t--) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k[i], q[t][i], s, 0, 0, 0);
+        load_v(0);
         const bool edge = base + 31 > all_see || base + 32 > end || (now.id[0] | now.id[1]) < 0;
         if (edge) {
+            const int upto_r = min(lim, end - 1) - base - 4 * hf;
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int pos = base + 8 * (r >> 2) + 4 * hf + (r & 3);
-                s[r] = pos <= min(lim, end - 1) && now.id[r >> 3] >= 0 ? s[r] : KVP_NEG_INF;
-            }
+            for (int r = 0; r < 16; r++) s[r] = 8 * (r >> 2) + (r & 3) <= upto_r && now.id[r >> 3] >= 0 ? s[r] : KVP_NEG_INF;
         }
         float mx = s[0];
 #pragma unroll
@@ -709,31 +715,19 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
         for (int x = 0; x < 2; x++) {
             bf16x8 p[PT];
             kvp_terms<PT>(w + 8 * x, p);
-            uint32_t v[8][DV / 2];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int n = 8 * (e >> 2) + (e & 3);
-                const char *row = ring + (vs ^ (16 * (HD == 128 ? n : n >> 1))) + (16 * x + n) * ROW;
-                if (HD == 128) {
-                    const uint2 u = *reinterpret_cast<const uint2 *>(row);
-                    v[e][0] = u.x;
-                    v[e][DV / 2 - 1] = u.y;
-                } else {
-                    v[e][0] = *reinterpret_cast<const uint32_t *>(row);
-                }
-            }
+            if (x == 0) load_v(1);
             if (edge) {
                 // V of positions that no row here sees may hold anything
 #pragma unroll
                 for (int e = 0; e < 8; e++)
 #pragma unroll
-                    for (int d = 0; d < DV / 2; d++) v[e][d] = base + 16 * x + 8 * (e >> 2) + (e & 3) + 4 * hf < end && now.id[x] >= 0 ? v[e][d] : 0u;
+                    for (int d = 0; d < DV / 2; d++) v[x][e][d] = base + 16 * x + 8 * (e >> 2) + (e & 3) + 4 * hf < end && now.id[x] >= 0 ? v[x][e][d] : 0u;
             }
 #pragma unroll
             for (int t = 0; t < DV; t++) {
                 uint32_t d[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) d[e] = __builtin_amdgcn_perm(v[2 * e + 1][t >> 1], v[2 * e][t >> 1], (t & 1) ? 0x07060302 : 0x05040100);
+                for (int e = 0; e < 4; e++) d[e] = __builtin_amdgcn_perm(v[x][2 * e + 1][t >> 1], v[x][2 * e][t >> 1], (t & 1) ? 0x07060302 : 0x05040100);
                 const bf16x8 vt = __builtin_bit_cast(bf16x8, make_uint4(d[0], d[1], d[2], d[3]));
 #pragma unroll
                 for (int y = PT - 1; y >= 0; y--) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, p[y], o[t], 0, 0, 0);
@@ -925,7 +919,14 @@ static hipError_t go_few(AttnKvpArgs &a, int64_t room, hipStream_t st) {
 
 template <bool BF16, int HD>
 static hipError_t go_attn_kvp(AttnKvpArgs &a, int64_t room, hipStream_t st) {
-    return a.s.max_rows * a.G > 32 ? go_rows<BF16, HD, KVP_RW, KVP_PG>(a, room, st) : go_few<BF16, HD>(a, room, st);
+    const int64_t rows = a.s.max_rows * a.G;
+    if (rows <= 32) return go_few<BF16, HD>(a, room, st);
+    // Four groups over the positions where the tiles are one a CU at most, and enough to need no split; else two, and two
+    // blocks a CU.  us, two / four, 8 KV heads x 2 heads of 128, f32: 32 x 20 rows behind 1000 positions 43.2 / 37.9, 2 x
+    // 512 behind 4000 110 / 104, 404 alone 17.4 / 17.9; 6 x 404 20.7 / 29.0, 8 x 512 behind 4000 330 / 372.  (Four side by
+    // side, two groups: 8 x 512 336, but six ragged prompts of 1337 134 against 113.)
+    const int64_t units = std::min((rows + 63) / 64 * a.s.n_seq, (a.s.n_rows * a.G / 32 + a.s.n_seq) / 2 + 1) * a.s.Hkv;
+    return units >= 128 && units <= 256 ? go_rows<BF16, HD, 2, 4>(a, room, st) : go_rows<BF16, HD, 2, 2>(a, room, st);
 }
 
 hipError_t launch_attention_kvp(const AttnKvpArgs &a0, bool bf16, hipStream_t st) {

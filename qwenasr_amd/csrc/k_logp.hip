@@ -8,11 +8,11 @@
 // The largest term of a row, 1, is not part of the sum (s): log p = x - M - log1p(s), so a
 // probability next to 1 keeps the bits of its logarithm, where log(1 + s) would lose them.
 //
-// The k largest: 64 lanes' maxima (each over the chunk's values in that lane's places)
-// as keys (value, then lowest index).  At least k values are not below the k-th
-// largest of these keys T, and no value outside the k lanes whose key reaches it
-// can be above T: what is not below T is at most k lanes' values, whatever the row holds,
-// a few more than k as a rule, and is ranked by counting.
+// The k largest: 64 lanes' maxima (each over the chunk's values in that lane's places).  At
+// least k values are not below the k-th largest of these maxima, T, and what is not below
+// T stands in the k lanes that reach it, a few more than k values as a rule: they are ranked
+// by counting.  Where T is a value that many share (masked vocabularies, rows of one value)
+// they may not fit; then the largest are taken out one after another.
 #include "kernels.h"
 #include "gemm_common.h"
 
@@ -22,6 +22,7 @@ typedef unsigned long long u64;
 #define LOGP_E 32                       // values a thread
 // a row's chunks: those of 256 threads, and one more for what its first begins late by
 #define LOGP_CHUNKS (QASR_LOGP_MAX_COLS / (256 * LOGP_E) + 1)
+#define LOGP_CAND 1024                  // values a chunk ranks by counting
 #define LOGP_LOG2E 1.4426950408889634f
 #define LOGP_LN2 0.6931471805599453f
 
@@ -38,10 +39,6 @@ __device__ __forceinline__ int logp_id(u64 key) { return (int)~(uint32_t)key; }
 __device__ __forceinline__ float logp_value(u64 key) {
     const uint32_t u = (uint32_t)(key >> 32);
     return __uint_as_float((u >> 31) ? u & 0x7fffffffu : ~u);
-}
-
-__device__ __forceinline__ u64 shfl64(u64 v, int lane) {
-    return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
 }
 
 // the row's results, by one block
@@ -64,10 +61,9 @@ __device__ __forceinline__ float logp_at(const LogpArgs &a, int64_t row, int i) 
 template <bool BF16, int W>
 __global__ __launch_bounds__(64 * W) void k_logp(LogpArgs a, int64_t row0) {
     constexpr int V = BF16 ? 8 : 4, T = 64 * W, NV = LOGP_E / V, CH = T * LOGP_E;
-    __shared__ float red[3][W];
-    __shared__ u64 lane_key[W][64], limit;
-    __shared__ u64 cand[QASR_LOGP_MAX_K * W * LOGP_E];
-    __shared__ int n_cand;
+    __shared__ float red[3][W], lane_max[W][64], limit;
+    __shared__ int red_n[W], n_cand;
+    __shared__ u64 cand[LOGP_CAND], best_l[W];
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
     const int64_t row = row0 + blockIdx.y;
     // chunks begin at 16-byte places: `off` values before the row's first are none of its
@@ -78,29 +74,55 @@ __global__ __launch_bounds__(64 * W) void k_logp(LogpArgs a, int64_t row0) {
     const int i0 = (int)blockIdx.x * CH - off;
     float x[LOGP_E];
     const float none = -__builtin_inff();
+    if (i0 >= 0 && i0 + CH <= a.cols) {
 #pragma unroll
-    for (int n = 0; n < NV; n++) {
-        const int i = i0 + (n * T + t) * V;
-        if (i >= 0 && i + V <= a.cols) {
-            const uint4 u = *reinterpret_cast<const uint4 *>(row_p + (int64_t)i * ES);
+        for (int n = 0; n < NV; n++) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(row_p + (int64_t)(i0 + (n * T + t) * V) * ES);
             const uint32_t d[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
             for (int e = 0; e < V; e++)
                 x[n * V + e] = BF16 ? __uint_as_float((e & 1) ? d[e / 2] & 0xffff0000u : d[e / 2] << 16) : __uint_as_float(d[e]);
-        } else {
+        }
+    } else {
 #pragma unroll
-            for (int e = 0; e < V; e++) x[n * V + e] = i + e >= 0 && i + e < a.cols ? logp_at<BF16>(a, row, i + e) : none;
+        for (int n = 0; n < NV; n++) {
+            const int i = i0 + (n * T + t) * V;
+            if (i >= 0 && i + V <= a.cols) {
+                const uint4 u = *reinterpret_cast<const uint4 *>(row_p + (int64_t)i * ES);
+                const uint32_t d[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int e = 0; e < V; e++)
+                    x[n * V + e] = BF16 ? __uint_as_float((e & 1) ? d[e / 2] & 0xffff0000u : d[e / 2] << 16) : __uint_as_float(d[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; e++) x[n * V + e] = i + e >= 0 && i + e < a.cols ? logp_at<BF16>(a, row, i + e) : none;
+            }
         }
     }
     float tm = none;
 #pragma unroll
     for (int e = 0; e < LOGP_E; e++) tm = fmaxf(tm, x[e]);
     float M = wave_max_f32(tm);
+    if (t == 0) n_cand = 0;
     if (W > 1) {
         if (lane == 0) red[0][w] = M;
+        lane_max[w][lane] = tm;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < W; i++) M = fmaxf(M, red[0][i]);
+    }
+    // the k-th largest of the lanes' maxima, by the first wave, while the others go on
+    if (a.k > 0 && w == 0) {
+        float g = tm;
+#pragma unroll
+        for (int i = 1; i < W; i++) g = fmaxf(g, lane_max[i][lane]);
+        int above = 0;
+        if (a.k > 1)
+#pragma unroll 16
+            for (int i = 0; i < 64; i++) above += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), i)) > g;
+        // the least of the maxima that fewer than k pass
+        const float lim = -wave_max_f32(a.k > 1 ? above < a.k ? -g : none : -M);
+        if (lane == 0) limit = lim;
     }
     // the sums; the terms of the maximum, exactly 1 each, are counted, all but one
     float s = 0.0f, h = 0.0f;
@@ -133,22 +155,19 @@ __global__ __launch_bounds__(64 * W) void k_logp(LogpArgs a, int64_t row0) {
     s = wave_sum_f32(s);
     h = wave_sum_f32(h);
     ones = wave_sum_i32(ones);
-    if (W > 1) {
-        if (lane == 0) {
-            red[1][w] = s;
-            red[2][w] = h;
-            lane_key[w][0] = (u64)ones;
-        }
-        __syncthreads();
-        s = h = 0.0f;
-        ones = 0;
+    if (lane == 0) {
+        red[1][w] = s;
+        red[2][w] = h;
+        red_n[w] = ones;
+    }
+    __syncthreads();
+    s = h = 0.0f;
+    ones = 0;
 #pragma unroll
-        for (int i = 0; i < W; i++) {
-            s += red[1][i];
-            h += red[2][i];
-            ones += (int)lane_key[i][0];
-        }
-        __syncthreads();
+    for (int i = 0; i < W; i++) {
+        s += red[1][i];
+        h += red[2][i];
+        ones += red_n[i];
     }
     const LogpPart part{M, s + (float)max(ones - 1, 0), h * LOGP_LN2};
     const bool only = a.chunks == 1;
@@ -165,96 +184,111 @@ __global__ __launch_bounds__(64 * W) void k_logp(LogpArgs a, int64_t row0) {
     if (a.k == 0) return;
 
     // ---- the k largest
-    u64 key = 0;                                  // 0: below the key of any value
-    {
-        int best = -1;
-#pragma unroll
-        for (int n = NV - 1; n >= 0; n--)
-#pragma unroll
-            for (int e = V - 1; e >= 0; e--) {
-                const int i = i0 + (n * T + t) * V + e;
-                if (fmaxf(x[n * V + e], none) == tm && i >= 0 && i < a.cols) best = i;
-            }
-        if (best >= 0) key = logp_key(tm, best);
-    }
-    lane_key[w][lane] = key;
-    if (t == 0) n_cand = 0;
-    __syncthreads();
-    if (w == 0) {
-        u64 g = 0;
-#pragma unroll
-        for (int i = 0; i < W; i++) g = max(g, lane_key[i][lane]);
-        int above = 0;
-        for (int i = 0; i < 64; i++) {
-            const u64 o = shfl64(g, i);
-            above += o > g || (o == g && i < lane);
-        }
-        if (above == a.k - 1) limit = g;
-    }
-    __syncthreads();
-    const u64 lim = limit;
-    if (key >= lim && key != 0) {
+    const float lim = limit;
+    if (__any(tm >= lim)) {
 #pragma unroll
         for (int n = 0; n < NV; n++)
 #pragma unroll
-            for (int e = 0; e < V; e++) {
-                const int i = i0 + (n * T + t) * V + e;
-                const u64 y = logp_key(x[n * V + e], i);
-                if (y >= lim && i >= 0 && i < a.cols) cand[atomicAdd(&n_cand, 1)] = y;
+            for (int q = 0; q < V; q += 4) {
+                const float *y = x + n * V + q;
+                if (!__any(!(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) < lim))) continue;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int i = i0 + (n * T + t) * V + q + e;
+                    if (!(fmaxf(y[e], none) < lim) && i >= 0 && i < a.cols) {
+                        const int c = atomicAdd(&n_cand, 1);
+                        if (c < LOGP_CAND) cand[c] = logp_key(y[e], i);
+                    }
+                }
             }
     }
     __syncthreads();
     const int n = n_cand;
     u64 *top = reinterpret_cast<u64 *>(base + 16);
-    for (int i = t; i < n; i += T) {
-        const u64 y = cand[i];
-        int rank = 0;
-        for (int j = 0; j < n; j++) rank += cand[j] > y;
-        if (rank < a.k) {
-            if (only) logp_top(a, row, rank, y, part);
-            else top[rank] = y;
+    if (n <= LOGP_CAND) {
+        for (int i = t; i < n; i += T) {
+            const u64 y = cand[i];
+            int rank = 0;
+            for (int j = 0; j < n; j++) rank += cand[j] > y;
+            if (rank < a.k) {
+                if (only) logp_top(a, row, rank, y, part);
+                else top[rank] = y;
+            }
+        }
+        if (!only)
+            for (int i = n + t; i < a.k; i += T) top[i] = 0;
+        return;
+    }
+    // more than there is room for, so more than k: the largest key below the last one, k times
+    u64 last = ~0ull;
+    for (int r = 0; r < a.k; r++) {
+        u64 best = 0;
+#pragma unroll
+        for (int e = 0; e < LOGP_E; e++) {
+            const int i = i0 + (e / V * T + t) * V + e % V;
+            const u64 y = logp_key(x[e], i);
+            if (i >= 0 && i < a.cols && y < last && y > best) best = y;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) best = max(best, (u64)__shfl_xor((unsigned long long)best, o, 64));
+        if (lane == 0) best_l[w] = best;
+        __syncthreads();
+        last = 0;
+#pragma unroll
+        for (int i = 0; i < W; i++) last = max(last, best_l[i]);
+        __syncthreads();
+        if (t == 0) {
+            if (only) logp_top(a, row, r, last, part);
+            else top[r] = last;
         }
     }
-    if (!only)
-        for (int i = n + t; i < a.k; i += T) top[i] = 0;
 }
 
-// A row's chunks joined: one block a row.  A key can be among the k largest only if
-// its place in its own list and the lists whose first key is larger are fewer than k.
+// A row's chunks joined: one block a row, a lane of every wave a chunk or two.  A key can
+// be among the k largest only if its place in its own list and the lists whose first key
+// is larger are fewer than k.
 template <bool BF16>
 __global__ __launch_bounds__(256) void k_logp_join(LogpArgs a, int64_t row0) {
+    constexpr int U = (LOGP_CHUNKS + 63) / 64;
     __shared__ u64 cand[QASR_LOGP_MAX_K * QASR_LOGP_MAX_K], head[LOGP_CHUNKS];
-    __shared__ float m_l[LOGP_CHUNKS], s_l[LOGP_CHUNKS], h_l[LOGP_CHUNKS];
     __shared__ int n_cand;
-    const int t = threadIdx.x, n = a.chunks;
+    const int t = threadIdx.x, lane = t & 63, n = a.chunks;
     const int64_t row = row0 + blockIdx.x, step = logp_part(a.k);
     const char *base = a.part + (int64_t)blockIdx.x * n * step;
-    for (int i = t; i < n; i += 256) {
-        const float4 p = *reinterpret_cast<const float4 *>(base + i * step);
-        m_l[i] = p.x;
-        s_l[i] = p.y;
-        h_l[i] = p.z;
-        head[i] = a.k > 0 ? *reinterpret_cast<const u64 *>(base + i * step + 16) : 0;
+    const int target = a.logp ? a.targets[row] : -1;
+    float4 p[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int i = lane + 64 * u;
+        p[u] = i < n ? *reinterpret_cast<const float4 *>(base + i * step) : make_float4(-__builtin_inff(), 0.0f, 0.0f, 0.0f);
     }
+    if (a.k > 0)
+        for (int i = t; i < n; i += 256) head[i] = *reinterpret_cast<const u64 *>(base + i * step + 16);
     if (t == 0) n_cand = 0;
+    const bool has = (unsigned)target < (unsigned)a.cols;
+    const float x_target = has ? logp_at<BF16>(a, row, target) : 0.0f;
     __syncthreads();
-    // in chunk order, by every thread alike
     LogpPart r{-__builtin_inff(), 0.0f, 0.0f};
-    for (int i = 0; i < n; i++) r.m = fmaxf(r.m, m_l[i]);
-    bool first = true;
+#pragma unroll
+    for (int u = 0; u < U; u++) r.m = fmaxf(r.m, p[u].x);
+    r.m = wave_max_f32(r.m);
+    // the chunk whose largest term is the row's: the first of them
+    int mine = 0x7fffffff;
+#pragma unroll
+    for (int u = U - 1; u >= 0; u--) mine = p[u].x == r.m && r.m != -__builtin_inff() ? lane + 64 * u : mine;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mine = min(mine, __shfl_xor(mine, o, 64));
     const float ref = r.m == -__builtin_inff() ? 0.0f : r.m;
-    for (int i = 0; i < n; i++) {
-        const float d = m_l[i] - ref, w = expf(d);       // a chunk of -infinity alone: 0
-        const bool one = first && m_l[i] == r.m && r.m != -__builtin_inff();
-        first = first && !one;
-        r.s += one ? s_l[i] : w * s_l[i] + (m_l[i] == -__builtin_inff() ? 0.0f : w);
-        r.h += w * (h_l[i] + (m_l[i] == -__builtin_inff() ? 0.0f : (1.0f + s_l[i]) * fmaxf(d, -200.0f)));
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const float d = p[u].x - ref, w = expf(d);       // a chunk of -infinity alone: 0
+        const bool empty = p[u].x == -__builtin_inff();
+        r.s += lane + 64 * u == mine ? p[u].y : w * p[u].y + (empty ? 0.0f : w);
+        r.h += w * (p[u].z + (empty ? 0.0f : (1.0f + p[u].y) * fmaxf(d, -200.0f)));
     }
-    if (t == 0) {
-        const int g = a.logp ? a.targets[row] : -1;
-        const bool has = (unsigned)g < (unsigned)a.cols;
-        logp_row(a, row, r, has ? logp_at<BF16>(a, row, g) : 0.0f, has);
-    }
+    r.s = wave_sum_f32(r.s);
+    r.h = wave_sum_f32(r.h);
+    if (t == 0) logp_row(a, row, r, x_target, has);
     if (a.k == 0) return;
     for (int i = t; i < n * a.k; i += 256) {
         const int c = i / a.k, place = i % a.k;

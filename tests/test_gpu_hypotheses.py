@@ -370,6 +370,8 @@ ATTN = [
     ([300, 1, 131], [10, 600, 0], 3, [0], 2, 3, 128, 64),
     ([45], [2500], 1, None, 1, 1, 64, 32),                                                # splits of one tile
     ([129, 128], [-20, 333], 1, None, 1, 1, 128, 128),
+    ([30, 17] * 10, [3 * j for j in range(20)], 1, None, 8, 2, 64, 16),                   # a tile for each of 160 CUs
+    ([33, 50, 20, 41] * 4, [9 * j for j in range(16)], 4, [0] * 4, 8, 1, 128, 32),
 ]
 
 
