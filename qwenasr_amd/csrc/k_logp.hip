@@ -12,7 +12,7 @@
 // least k values are not below the k-th largest of these maxima, T, and what is not below
 // T stands in the k lanes that reach it, a few more than k values as a rule: they are ranked
 // by counting.  Where T is a value that many share (masked vocabularies, rows of one value)
-// they may not fit; then the largest are taken out one after another.
+// those above it are taken, and the first of those that have it.
 #include "kernels.h"
 #include "gemm_common.h"
 
@@ -58,8 +58,9 @@ __device__ __forceinline__ float logp_at(const LogpArgs &a, int64_t row, int i) 
     return BF16 ? bf16_to_f32(reinterpret_cast<const uint16_t *>(a.x)[at]) : reinterpret_cast<const float *>(a.x)[at];
 }
 
+// five waves a SIMD: with four, f32 375 x 151936 47 -> 52 us
 template <bool BF16, int W>
-__global__ __launch_bounds__(64 * W) void k_logp(LogpArgs a, int64_t row0) {
+__global__ __launch_bounds__(64 * W, 5) void k_logp(LogpArgs a, int64_t row0) {
     constexpr int V = BF16 ? 8 : 4, T = 64 * W, NV = LOGP_E / V, CH = T * LOGP_E;
     __shared__ float red[3][W], lane_max[W][64], limit;
     __shared__ int red_n[W], n_cand;
@@ -203,8 +204,53 @@ __global__ __launch_bounds__(64 * W) void k_logp(LogpArgs a, int64_t row0) {
             }
     }
     __syncthreads();
-    const int n = n_cand;
+    int n = n_cand;
     u64 *top = reinterpret_cast<u64 *>(base + 16);
+    if (n > LOGP_CAND) {
+        // a value that many share: those above it, then as many of it as are wanted, in order
+        __syncthreads();
+        if (t == 0) n_cand = 0;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < LOGP_E; e++) {
+            const int i = i0 + (e / V * T + t) * V + e % V;
+            if (x[e] > lim && i >= 0 && i < a.cols) {
+                const int c = atomicAdd(&n_cand, 1);
+                if (c < LOGP_CAND) cand[c] = logp_key(x[e], i);
+            }
+        }
+        __syncthreads();
+        n = n_cand;
+        if (n < a.k) {
+#pragma unroll
+            for (int v = 0; v < NV; v++) {
+                if (n >= a.k) break;
+                const int i = i0 + (v * T + t) * V;
+                unsigned ties = 0;
+#pragma unroll
+                for (int e = 0; e < V; e++) ties |= (fmaxf(x[v * V + e], none) == lim && i + e >= 0 && i + e < a.cols ? 1u : 0u) << e;
+                const int mine = __popc(ties);
+                int before = mine;
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) {
+                    const int y = __shfl_up(before, o, 64);
+                    before += lane >= o ? y : 0;
+                }
+                __syncthreads();
+                if (lane == 63) red_n[w] = before;
+                __syncthreads();
+                before += n - mine;
+#pragma unroll
+                for (int u = 0; u < W; u++) {
+                    before += u < w ? red_n[u] : 0;
+                    n += red_n[u];
+                }
+                for (; ties && before < a.k; ties &= ties - 1, before++) cand[before] = logp_key(lim, i + __builtin_ctz(ties));
+            }
+            n = min(n, a.k);
+            __syncthreads();
+        }
+    }
     if (n <= LOGP_CAND) {
         for (int i = t; i < n; i += T) {
             const u64 y = cand[i];
@@ -219,7 +265,7 @@ __global__ __launch_bounds__(64 * W) void k_logp(LogpArgs a, int64_t row0) {
             for (int i = n + t; i < a.k; i += T) top[i] = 0;
         return;
     }
-    // more than there is room for, so more than k: the largest key below the last one, k times
+    // still more than there is room for, so more than k: the largest key below the last one, k times
     u64 last = ~0ull;
     for (int r = 0; r < a.k; r++) {
         u64 best = 0;
@@ -249,9 +295,10 @@ __global__ __launch_bounds__(64 * W) void k_logp(LogpArgs a, int64_t row0) {
 // is larger are fewer than k.
 template <bool BF16>
 __global__ __launch_bounds__(256) void k_logp_join(LogpArgs a, int64_t row0) {
-    constexpr int U = (LOGP_CHUNKS + 63) / 64;
-    __shared__ u64 cand[QASR_LOGP_MAX_K * QASR_LOGP_MAX_K], head[LOGP_CHUNKS];
-    __shared__ int n_cand;
+    constexpr int U = (LOGP_CHUNKS + 63) / 64, MAX_K = QASR_LOGP_MAX_K;
+    extern __shared__ u64 keys[];                                // [chunks][k]
+    __shared__ u64 cand[MAX_K * (MAX_K + 1) / 2];
+    __shared__ int n_cand, list[MAX_K];
     const int t = threadIdx.x, lane = t & 63, n = a.chunks;
     const int64_t row = row0 + blockIdx.x, step = logp_part(a.k);
     const char *base = a.part + (int64_t)blockIdx.x * n * step;
@@ -262,8 +309,10 @@ __global__ __launch_bounds__(256) void k_logp_join(LogpArgs a, int64_t row0) {
         const int i = lane + 64 * u;
         p[u] = i < n ? *reinterpret_cast<const float4 *>(base + i * step) : make_float4(-__builtin_inff(), 0.0f, 0.0f, 0.0f);
     }
-    if (a.k > 0)
-        for (int i = t; i < n; i += 256) head[i] = *reinterpret_cast<const u64 *>(base + i * step + 16);
+    const int at_once = a.k > 0 ? 256 / a.k : 1;                 // lists
+    if (a.k > 0 && t < at_once * a.k)
+        for (int c = t / a.k; c < n; c += at_once) keys[c * a.k + t % a.k] = *reinterpret_cast<const u64 *>(base + c * step + 16 + 8 * (t % a.k));
+    if (t < MAX_K) list[t] = -1;
     if (t == 0) n_cand = 0;
     const bool has = (unsigned)target < (unsigned)a.cols;
     const float x_target = has ? logp_at<BF16>(a, row, target) : 0.0f;
@@ -290,13 +339,19 @@ __global__ __launch_bounds__(256) void k_logp_join(LogpArgs a, int64_t row0) {
     r.h = wave_sum_f32(r.h);
     if (t == 0) logp_row(a, row, r, x_target, has);
     if (a.k == 0) return;
-    for (int i = t; i < n * a.k; i += 256) {
-        const int c = i / a.k, place = i % a.k;
-        const u64 y = *reinterpret_cast<const u64 *>(base + c * step + 16 + 8 * place);
-        if (y == 0) continue;
-        int above = place;
-        for (int j = 0; j < n; j++) above += j != c && head[j] > y;
-        if (above < a.k) cand[atomicAdd(&n_cand, 1)] = y;
+    // the lists by their first keys, then of the r-th list the k - r first
+    for (int i = t; i < n; i += 256) {
+        const u64 y = keys[i * a.k];
+        int rank = 0;
+        for (int j = 0; j < n; j++) rank += keys[j * a.k] > y;
+        if (y != 0 && rank < a.k) list[rank] = i;
+    }
+    __syncthreads();
+    for (int i = t; i < a.k * a.k; i += 256) {
+        const int r = i / a.k, place = i % a.k;
+        if (r + place >= a.k || list[r] < 0) continue;
+        const u64 y = keys[list[r] * a.k + place];
+        if (y != 0) cand[atomicAdd(&n_cand, 1)] = y;
     }
     __syncthreads();
     const int found = n_cand;
@@ -318,14 +373,15 @@ static hipError_t go_logp(LogpArgs a, hipStream_t st) {
     for (int64_t r = 0; r < a.rows; r += rows) {
         const unsigned n = (unsigned)std::min(rows, a.rows - r);
         hipLaunchKernelGGL((k_logp<BF16, W>), dim3((unsigned)a.chunks, n), dim3(64 * W), 0, st, a, r);
-        if (a.chunks > 1) hipLaunchKernelGGL((k_logp_join<BF16>), dim3(n), dim3(256), 0, st, a, r);
+        if (a.chunks > 1) hipLaunchKernelGGL((k_logp_join<BF16>), dim3(n), dim3(256), (size_t)a.chunks * a.k * 8, st, a, r);
     }
     return hipGetLastError();
 }
 
 hipError_t launch_token_logprobs(const LogpArgs &a, bool bf16, hipStream_t st) {
     if (a.k > QASR_LOGP_MAX_K || a.cols > QASR_LOGP_MAX_COLS) return hipErrorInvalidValue;
-    // a wave a row where that holds it
+    // a wave a row where that holds it (as the form for few long rows, more and smaller chunks, it is slower:
+    // 8 x 151936 14.1 -> 16.9 us)
     if (a.cols + 7 <= 64 * LOGP_E) return bf16 ? go_logp<true, 1>(a, st) : go_logp<false, 1>(a, st);
     return bf16 ? go_logp<true, 4>(a, st) : go_logp<false, 4>(a, st);
 }

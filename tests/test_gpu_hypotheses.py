@@ -617,6 +617,29 @@ def test_logprobs_ties_go_to_the_lowest_index(dev, cols, is_bf16):
     check_logp(x, targets, 32, logprobs(dev, x, targets, 32, is_bf16))
 
 
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows,cols", [(12, 3000), (12, 9000), (60, 30000), (5, 151936)])
+def test_logprobs_masked_vocabularies(dev, rows, cols, is_bf16):
+    """Few values left, the others -infinity or the type's lowest; and places of a few lanes that hold all the large ones."""
+    r = rng(rows + cols)
+    x = r.normal(0, 2, (rows, cols))
+    low = -3.3895314e38
+    for i in range(rows):
+        left = r.permutation(cols)[:(1, 3, 31, 32, 33, 200)[i % 6]]
+        masked = np.full(cols, (-np.inf, low, -1e4)[i // 6 % 3])
+        masked[left] = x[i, left]
+        if i % 7 != 6:
+            x[i] = masked
+        else:
+            at = np.arange(cols)
+            x[i, at % (512 if is_bf16 else 256) // (8 if is_bf16 else 4) < 8] += 60
+    x[1] = low
+    x[1, cols // 2:] = -np.inf
+    x = held(x, is_bf16).astype(np.float32)
+    targets = x.argmax(1)
+    check_logp(x, targets, 32, logprobs(dev, x, targets, 32, is_bf16))
+
+
 @pytest.mark.parametrize("cols", [50, 9000])
 def test_logprobs_next_to_one(dev, cols):
     """A probability of 1 - 1e-9 has a logarithm of -1e-9, not 0; its entropy likewise."""
