@@ -58,13 +58,14 @@ __device__ __forceinline__ float logp_at(const LogpArgs &a, int64_t row, int i) 
     return BF16 ? bf16_to_f32(reinterpret_cast<const uint16_t *>(a.x)[at]) : reinterpret_cast<const float *>(a.x)[at];
 }
 
-// five waves a SIMD: with four, f32 375 x 151936 47 -> 52 us
-template <bool BF16, int W>
-__global__ __launch_bounds__(64 * W, 5) void k_logp(LogpArgs a, int64_t row0) {
-    constexpr int V = BF16 ? 8 : 4, T = 64 * W, NV = LOGP_E / V, CH = T * LOGP_E;
+// W waves with E values a thread; five waves a SIMD (with four, f32 375 x 151936 47 -> 52 us), eight of short rows
+template <bool BF16, int W, int E>
+__global__ __launch_bounds__(64 * W, E == 8 ? 8 : 5) void k_logp(LogpArgs a, int64_t row0) {
+    constexpr int V = BF16 ? 8 : 4, T = 64 * W, NV = E / V, CH = T * E;
     __shared__ float red[3][W], lane_max[W][64], limit;
     __shared__ int red_n[W], n_cand;
-    __shared__ u64 cand[LOGP_CAND], best_l[W];
+    constexpr int CAND = CH < LOGP_CAND ? CH : LOGP_CAND;
+    __shared__ u64 cand[CAND], best_l[W];
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
     const int64_t row = row0 + blockIdx.y;
     // chunks begin at 16-byte places: `off` values before the row's first are none of its
@@ -73,7 +74,7 @@ __global__ __launch_bounds__(64 * W, 5) void k_logp(LogpArgs a, int64_t row0) {
     const char *row_p = reinterpret_cast<const char *>(a.x) + at * ES;
     const int off = (int)(((uintptr_t)row_p & 15) / ES);
     const int i0 = (int)blockIdx.x * CH - off;
-    float x[LOGP_E];
+    float x[E];
     const float none = -__builtin_inff();
     if (i0 >= 0 && i0 + CH <= a.cols) {
 #pragma unroll
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(64 * W, 5) void k_logp(LogpArgs a, int64_t row0) {
     }
     float tm = none;
 #pragma unroll
-    for (int e = 0; e < LOGP_E; e++) tm = fmaxf(tm, x[e]);
+    for (int e = 0; e < E; e++) tm = fmaxf(tm, x[e]);
     float M = wave_max_f32(tm);
     if (t == 0) n_cand = 0;
     if (W > 1) {
@@ -131,12 +132,12 @@ __global__ __launch_bounds__(64 * W, 5) void k_logp(LogpArgs a, int64_t row0) {
     if (M == none) {
         // nothing above -infinity: NaN if there is one
 #pragma unroll
-        for (int e = 0; e < LOGP_E; e++) s += x[e] != x[e] ? x[e] : 0.0f;
+        for (int e = 0; e < E; e++) s += x[e] != x[e] ? x[e] : 0.0f;
     } else {
         const bool mine = tm == M;
         if (__any(mine)) {
 #pragma unroll
-            for (int e = 0; e < LOGP_E; e++) {
+            for (int e = 0; e < E; e++) {
                 const bool one = x[e] == M;
                 const float d = (x[e] - M) * LOGP_LOG2E, p = __builtin_amdgcn_exp2f(d);
                 h = fmaf(p, fmaxf(d, -200.0f), h);
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(64 * W, 5) void k_logp(LogpArgs a, int64_t row0) {
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < LOGP_E; e++) {
+            for (int e = 0; e < E; e++) {
                 const float d = (x[e] - M) * LOGP_LOG2E, p = __builtin_amdgcn_exp2f(d);
                 h = fmaf(p, fmaxf(d, -200.0f), h);
                 s += p;
@@ -198,7 +199,7 @@ __global__ __launch_bounds__(64 * W, 5) void k_logp(LogpArgs a, int64_t row0) {
                     const int i = i0 + (n * T + t) * V + q + e;
                     if (!(fmaxf(y[e], none) < lim) && i >= 0 && i < a.cols) {
                         const int c = atomicAdd(&n_cand, 1);
-                        if (c < LOGP_CAND) cand[c] = logp_key(y[e], i);
+                        if (c < CAND) cand[c] = logp_key(y[e], i);
                     }
                 }
             }
@@ -206,17 +207,17 @@ __global__ __launch_bounds__(64 * W, 5) void k_logp(LogpArgs a, int64_t row0) {
     __syncthreads();
     int n = n_cand;
     u64 *top = reinterpret_cast<u64 *>(base + 16);
-    if (n > LOGP_CAND) {
+    if (n > CAND) {
         // a value that many share: those above it, then as many of it as are wanted, in order
         __syncthreads();
         if (t == 0) n_cand = 0;
         __syncthreads();
 #pragma unroll
-        for (int e = 0; e < LOGP_E; e++) {
+        for (int e = 0; e < E; e++) {
             const int i = i0 + (e / V * T + t) * V + e % V;
             if (x[e] > lim && i >= 0 && i < a.cols) {
                 const int c = atomicAdd(&n_cand, 1);
-                if (c < LOGP_CAND) cand[c] = logp_key(x[e], i);
+                if (c < CAND) cand[c] = logp_key(x[e], i);
             }
         }
         __syncthreads();
@@ -251,7 +252,7 @@ __global__ __launch_bounds__(64 * W, 5) void k_logp(LogpArgs a, int64_t row0) {
             __syncthreads();
         }
     }
-    if (n <= LOGP_CAND) {
+    if (n <= CAND) {
         for (int i = t; i < n; i += T) {
             const u64 y = cand[i];
             int rank = 0;
@@ -270,7 +271,7 @@ __global__ __launch_bounds__(64 * W, 5) void k_logp(LogpArgs a, int64_t row0) {
     for (int r = 0; r < a.k; r++) {
         u64 best = 0;
 #pragma unroll
-        for (int e = 0; e < LOGP_E; e++) {
+        for (int e = 0; e < E; e++) {
             const int i = i0 + (e / V * T + t) * V + e % V;
             const u64 y = logp_key(x[e], i);
             if (i >= 0 && i < a.cols && y < last && y > best) best = y;
@@ -339,7 +340,7 @@ __global__ __launch_bounds__(256) void k_logp_join(LogpArgs a, int64_t row0) {
     r.h = wave_sum_f32(r.h);
     if (t == 0) logp_row(a, row, r, x_target, has);
     if (a.k == 0) return;
-    // the lists by their first keys, then of the r-th list the k - r first
+    // the lists by their first keys, then of the r-th list the k - r first, if they are not below the k-th list's
     for (int i = t; i < n; i += 256) {
         const u64 y = keys[i * a.k];
         int rank = 0;
@@ -347,11 +348,12 @@ __global__ __launch_bounds__(256) void k_logp_join(LogpArgs a, int64_t row0) {
         if (y != 0 && rank < a.k) list[rank] = i;
     }
     __syncthreads();
+    const u64 least = list[a.k - 1] >= 0 ? keys[list[a.k - 1] * a.k] : 1;      // k first keys are not below it
     for (int i = t; i < a.k * a.k; i += 256) {
         const int r = i / a.k, place = i % a.k;
         if (r + place >= a.k || list[r] < 0) continue;
         const u64 y = keys[list[r] * a.k + place];
-        if (y != 0) cand[atomicAdd(&n_cand, 1)] = y;
+        if (y >= least) cand[atomicAdd(&n_cand, 1)] = y;
     }
     __syncthreads();
     const int found = n_cand;
@@ -363,27 +365,36 @@ __global__ __launch_bounds__(256) void k_logp_join(LogpArgs a, int64_t row0) {
     }
 }
 
-template <bool BF16, int W>
+template <bool BF16, int W, int E>
 static hipError_t go_logp(LogpArgs a, hipStream_t st) {
-    constexpr int CH = 64 * W * LOGP_E, V = BF16 ? 8 : 4;
+    constexpr int CH = 64 * W * E, V = BF16 ? 8 : 4;
     a.chunks = (a.cols + V - 1 + CH - 1) / CH;           // up to V - 1 values before the row's first
     if (a.chunks > 1 && a.cols <= CH && (uintptr_t)a.x % 16 == 0 && a.ld % V == 0) a.chunks = 1;
     const int64_t per_row = a.chunks * logp_part(a.k);
     const int64_t rows = a.chunks == 1 ? 65535 : std::min<int64_t>(65535, QASR_LOGP_PART_BYTES / per_row);
     for (int64_t r = 0; r < a.rows; r += rows) {
         const unsigned n = (unsigned)std::min(rows, a.rows - r);
-        hipLaunchKernelGGL((k_logp<BF16, W>), dim3((unsigned)a.chunks, n), dim3(64 * W), 0, st, a, r);
+        hipLaunchKernelGGL((k_logp<BF16, W, E>), dim3((unsigned)a.chunks, n), dim3(64 * W), 0, st, a, r);
         if (a.chunks > 1) hipLaunchKernelGGL((k_logp_join<BF16>), dim3(n), dim3(256), (size_t)a.chunks * a.k * 8, st, a, r);
     }
     return hipGetLastError();
 }
 
+// the fewest values that hold a row, as those of none cost what others do (4000 x 300 12.5 -> us); longer rows in
+// chunks of four waves (of one, for few rows: 8 x 151936 14.1 -> 16.9 us; 64 values a thread: bf16 375 x 151936 43 -> 47)
+template <bool BF16>
+static hipError_t pick_logp(const LogpArgs &a, hipStream_t st) {
+    const int n = a.cols + (BF16 ? 7 : 3);               // with what a row may begin behind a 16-byte place
+    if (n <= 64 * 8) return go_logp<BF16, 1, 8>(a, st);
+    if (n <= 64 * LOGP_E) return go_logp<BF16, 1, LOGP_E>(a, st);
+    if (n <= 128 * LOGP_E) return go_logp<BF16, 2, LOGP_E>(a, st);
+    if (n <= 192 * LOGP_E) return go_logp<BF16, 3, LOGP_E>(a, st);
+    return go_logp<BF16, 4, LOGP_E>(a, st);
+}
+
 hipError_t launch_token_logprobs(const LogpArgs &a, bool bf16, hipStream_t st) {
     if (a.k > QASR_LOGP_MAX_K || a.cols > QASR_LOGP_MAX_COLS) return hipErrorInvalidValue;
-    // a wave a row where that holds it (as the form for few long rows, more and smaller chunks, it is slower:
-    // 8 x 151936 14.1 -> 16.9 us)
-    if (a.cols + 7 <= 64 * LOGP_E) return bf16 ? go_logp<true, 1>(a, st) : go_logp<false, 1>(a, st);
-    return bf16 ? go_logp<true, 4>(a, st) : go_logp<false, 4>(a, st);
+    return bf16 ? pick_logp<true>(a, st) : pick_logp<false>(a, st);
 }
 
 }  // namespace qasr
