@@ -341,10 +341,10 @@ int qasr_hip_kvp_write(qasr_hip *h, uint16_t *k_pages, uint16_t *v_pages, int64_
  * and those past max_rows, are left as they were.
  * shared (nullable; int32 [ceil(n_seq / group)]): the sequences come in groups of
  * `group` that follow one another (the last may be smaller), and the first shared[g]
- * positions of group g hold the same keys and values for all its members: they are
- * read through its first sequence's table (which has to name them even if that
- * sequence has no rows), once for the rows of all.  Groups of different size are
- * filled up with sequences without rows.
+ * positions of group g hold the same keys and values in all its members' tables (its
+ * first sequence's has to name them even if it sees or has fewer): where that pays, they
+ * are read through the first one's, once for the rows of all.  Groups of different
+ * size are filled up with sequences without rows.
  * What a row does not see does not reach it, whatever its bits; in what it sees,
  * infinities and NaN count as they do in the formula, in f32.  Products and sums
  * are f32; rows of q enter exactly, and a weight is off by f32 rounding of itself

@@ -105,7 +105,7 @@ static int row_args(KvpSeqs &s, const void *kp, const void *vp, int64_t n_pages,
         return bad("kvp: n_rows or max_rows out of range");
     if (!row_start && n_seq * max_rows > n_rows) return bad("kvp: n_seq * max_rows rows need a larger n_rows");
     if ((((uintptr_t)kp) | (uintptr_t)vp) % 16 != 0) return bad("kvp: pages must be 16-byte aligned");
-    s.table = table; s.row_start = row_start; s.pos = pos; s.n_rows = n_rows; s.max_rows = max_rows;
+    s.table = table; s.row_start = row_start; s.pos = pos; s.n_rows = n_rows; s.max_rows = std::min(max_rows, n_rows);
     s.n_seq = (int)n_seq; s.table_ld = (int)table_ld; s.n_pages = (int)n_pages; s.Hkv = (int)n_kv_heads;
     s.hd = (int)head_dim; s.shift = page_shift(page);
     return QASR_OK;

@@ -32,12 +32,6 @@ namespace qasr {
 // a running maximum is moved only when it is passed by 2^8: weights stay below 2^8
 #define KVP_SLACK 8.0f
 
-template <int HD>
-struct KvpDims {
-    static constexpr int KC = HD / 32;       // k chunks of a score product
-    static constexpr int VT = HD / 16;       // products of O, dims of a lane's V row
-};
-
 // one segment of positions: the whole sequence, or a group's shared prefix, or what a
 // sequence has behind it
 struct KvpSegment {
@@ -137,20 +131,16 @@ struct KvpTable {
     const int32_t *table;
     int first, entry;
     __device__ __forceinline__ void load(const AttnKvpArgs &a, int s) {
+        const int at = s + (int)(threadIdx.x & 63);
         first = s;
-        entry = table[min(s + (int)(threadIdx.x & 63), a.s.table_ld - 1)];
+        entry = table[min(at, a.s.table_ld - 1)];
+        if (at >= a.s.table_ld || (unsigned)entry >= (unsigned)a.s.n_pages) entry = -1;
     }
     __device__ __forceinline__ KvpTable(const AttnKvpArgs &a, const int32_t *t, int base) : table(t) { load(a, base >> a.s.shift); }
     __device__ __forceinline__ KvpIds at(const AttnKvpArgs &a, int base) {
         const int s0 = base >> a.s.shift, s1 = (base + 16) >> a.s.shift;
         if (s1 - first > 63) load(a, s0);
-        KvpIds r;
-        r.id[0] = __builtin_amdgcn_readlane(entry, s0 - first);
-        r.id[1] = s1 < a.s.table_ld ? __builtin_amdgcn_readlane(entry, s1 - first) : -1;
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-            if ((unsigned)r.id[h] >= (unsigned)a.s.n_pages) r.id[h] = -1;
-        return r;
+        return {{__builtin_amdgcn_readlane(entry, s0 - first), __builtin_amdgcn_readlane(entry, s1 - first)}};
     }
 };
 // first value of a half's 16 positions of head h
@@ -599,14 +589,17 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
     }
     // the group's tiles; past its last one, that again: nothing sees it
     auto base_of = [&](int it) { return min(from + 32 * (PG * min(it, n_it - 1) + grp), (block_end - 1) & ~31); };
+    const uint32_t page_bytes = (uint32_t)(a.s.Hkv << a.s.shift) * ROW, head_bytes = (uint32_t)(h << a.s.shift) * ROW;
+    const char *const k_head = reinterpret_cast<const char *>(a.kp) + head_bytes, *const v_head = reinterpret_cast<const char *>(a.vp) + head_bytes;
     auto issue = [&](int slot, int base, KvpIds ids) {
         const int half = wid / (RW / 2);
-        const int64_t at = kvp_uniform(kvp_at<HD>(a, half ? ids.id[1] : ids.id[0], h, base + 16 * half));
+        const uint64_t at = (uint64_t)(uint32_t)max(half ? ids.id[1] : ids.id[0], 0) * page_bytes + (uint32_t)(((base + 16 * half) & ((1 << a.s.shift) - 1)) * ROW);
         char *to = ring + slot + 1024 * NL * wid;
+        const char *k_from = k_head + kvp_uniform((int64_t)at), *v_from = v_head + kvp_uniform((int64_t)at);
 #pragma unroll
-        for (int i = 0; i < NL; i++) lds_dma16_s(a.kp + at, src[i], to + 1024 * i);
+        for (int i = 0; i < NL; i++) lds_dma16_s(k_from, src[i], to + 1024 * i);
 #pragma unroll
-        for (int i = 0; i < NL; i++) lds_dma16_s(a.vp + at, src[i], to + TB + 1024 * i);
+        for (int i = 0; i < NL; i++) lds_dma16_s(v_from, src[i], to + TB + 1024 * i);
     };
     KvpTable table(a, sg.table, n_it > 0 ? from : 0);
     KvpIds ids;

@@ -372,6 +372,7 @@ ATTN = [
     ([129, 128], [-20, 333], 1, None, 1, 1, 128, 128),
     ([30, 17] * 10, [3 * j for j in range(20)], 1, None, 8, 2, 64, 16),                   # a tile for each of 160 CUs
     ([33, 50, 20, 41] * 4, [9 * j for j in range(16)], 4, [0] * 4, 8, 1, 128, 32),
+    ([17 + j % 23 for j in range(140)], [j % 50 for j in range(140)], 1, None, 1, 2, 64, 16),    # more sequences than lanes
 ]
 
 
@@ -480,6 +481,15 @@ def test_attention_not_finite_behind_a_shared_prefix(dev, is_bf16):
     got = attention(dev, c, q, counts, pos, 2, 6, [96], is_bf16)
     assert np.isnan(got[[0, 1, 2, 3, 5]]).any(2).all()
     assert np.allclose(got[4], clean[4], rtol=1e-2 if is_bf16 else 1e-4, atol=1e-2 if is_bf16 else 1e-5)
+
+
+def test_attention_bound_of_rows(dev):
+    """max_rows may be far above what there is."""
+    r = rng(23)
+    counts, pos = [3, 1], [20, 900]
+    c = Cache(dev, r, [a + b for a, b in zip(counts, pos)], 32, 2, 64)
+    q = r.normal(0, 1, (4, 4, 64))
+    check_attention(c, attention(dev, c, q, counts, pos, 2, max_rows=1 << 24), q, counts, pos)
 
 
 def test_attention_rows_past_max_rows(dev):
@@ -714,6 +724,7 @@ def test_nothing_to_do(dev):
     K.kvp_write(z, z, 1, z, z, z, 1, z, 0, 1, 0, 1, 64, 16)
     K.attention_kvp(z, z, z, z, 1, z, 1, z, 0, 0, 0, 1, 1, 64, 16, 1.0)
     K.attention_kvp(z, z, z, z, 1, z, 1, z, 4, 0, 4, 1, 1, 64, 16, 1.0, row_start=z)
+    K.kvp_compact(z, At(z, 100), z, z, 0, 1, z, 1, 1, 1, 16, 16)
     assert (z.numpy() == 0).all()
 
 
