@@ -145,7 +145,7 @@ extern "C" int qasr_hip_attention_kvp(qasr_hip *h, void *out, const void *q, int
     if (group < 1) return bad("attention_kvp: group must be positive");
     if (max_len < 0 || max_own < 0) return bad("attention_kvp: max_len and max_own must not be negative");
     if (!std::isfinite(scale)) return bad("attention_kvp: scale must be finite");
-    if (std::min<int64_t>(n_rows, group * max_rows) * (n_heads / n_kv_heads) > (1 << 30) || max_rows * (n_heads / n_kv_heads) > (1 << 30))
+    if (a.s.max_rows * (n_heads / n_kv_heads) > (1 << 30))
         return bad("attention_kvp: rows x heads of a group out of range");
     CHECK_H(h);
     if (n_seq == 0 || n_rows == 0 || max_rows == 0) return QASR_OK;

@@ -380,7 +380,7 @@ static hipError_t go_logp(LogpArgs a, hipStream_t st) {
     return hipGetLastError();
 }
 
-// the fewest values that hold a row, as those of none cost what others do (4000 x 300 12.5 -> us); longer rows in
+// the fewest values that hold a row, as those of none cost what others do (4000 x 300 12.5 -> 9.7 us); longer rows in
 // chunks of four waves (of one, for few rows: 8 x 151936 14.1 -> 16.9 us; 64 values a thread: bf16 375 x 151936 43 -> 47)
 template <bool BF16>
 static hipError_t pick_logp(const LogpArgs &a, hipStream_t st) {

@@ -332,11 +332,11 @@ def attention(dev, c, q, counts, pos, g, group=1, shared=None, is_bf16=False, pa
 
 
 def check_attention(c, got, q, counts, pos, is_bf16=False, scale=None):
-    pools, at = c.floats(), 0
+    pools, at = {x: np.nan_to_num(v) for x, v in c.floats().items()}, 0
     for j, n in enumerate(counts):
         end = min(max(pos[j] + n, 0), c.width * c.page)
-        k, there = refp.gather(np.nan_to_num(pools["k"]), c.table[j], end, c.page)
-        v, _ = refp.gather(np.nan_to_num(pools["v"]), c.table[j], end, c.page)
+        k, there = refp.gather(pools["k"], c.table[j], end, c.page)
+        v, _ = refp.gather(pools["v"], c.table[j], end, c.page)
         seen = (np.arange(end)[None] <= pos[j] + np.arange(n)[:, None]) & there
         want, bound = refp.attend(held(q[at:at + n], is_bf16), k, v, seen, c.dim ** -0.5 if scale is None else scale, 2.0 ** -17 if is_bf16 else U)
         # and the result's own rounding
@@ -490,6 +490,16 @@ def test_attention_bound_of_rows(dev):
     c = Cache(dev, r, [a + b for a, b in zip(counts, pos)], 32, 2, 64)
     q = r.normal(0, 1, (4, 4, 64))
     check_attention(c, attention(dev, c, q, counts, pos, 2, max_rows=1 << 24), q, counts, pos)
+
+
+@pytest.mark.parametrize("n_seq,rows,heads,g,dim", [(2048, 1, 1, 32, 64), (2048, 1, 2, 16, 128), (300, 20, 1, 32, 64)])
+def test_attention_without_room_for_parts(dev, n_seq, rows, heads, g, dim):
+    """So many rows x heads that the scratch area holds one part of each or none: no prefix and no split, whatever the hints."""
+    r = rng(29)
+    counts, pos = [rows] * n_seq, [int(x) for x in r.integers(30, 70, n_seq)]
+    c = Cache(dev, r, [a + b for a, b in zip(counts, pos)], 16, heads, dim, 16, [30] * pages_of(n_seq, 16), width=60)
+    q = r.normal(0, 1, (sum(counts), heads * g, dim))
+    check_attention(c, attention(dev, c, q, counts, pos, g, 16, [30] * pages_of(n_seq, 16)), q, counts, pos)
 
 
 def test_attention_rows_past_max_rows(dev):

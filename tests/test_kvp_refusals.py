@@ -84,7 +84,7 @@ def test_refused(f, kw):
 
 @pytest.mark.parametrize("f,kw", [(fork, {}), (fork, dict(parent=None, n_out=2)), (fork, dict(row_start=None)), (fork, dict(n_out=0)),
                                   (compact, {}), (compact, dict(table_out=AT[4])), (write, {}), (attn, {}), (attn, dict(shared=None)),
-                                  (attn, dict(scale=0.0)), (logp, {}), (logp, dict(logp=None, targets=None)), (logp, dict(k=0)),
+                                  (attn, dict(scale=0.0)), (attn, dict(group=1 << 62)), (logp, {}), (logp, dict(logp=None, targets=None)), (logp, dict(k=0)),
                                   (logp, dict(logits=P + 2, bf16=1))])
 def test_what_is_right_reaches_the_handle(f, kw):
     from qwenasr_amd import _lib
