@@ -58,7 +58,7 @@ __device__ __forceinline__ float logp_at(const LogpArgs &a, int64_t row, int i) 
     return BF16 ? bf16_to_f32(reinterpret_cast<const uint16_t *>(a.x)[at]) : reinterpret_cast<const float *>(a.x)[at];
 }
 
-// W waves with E values a thread; five waves a SIMD (with four, f32 375 x 151936 47 -> 52 us), eight of short rows
+// W waves with E values a thread; five waves a SIMD (with four, f32 375 x 151936 52 us for 47), eight of short rows
 template <bool BF16, int W, int E>
 __global__ __launch_bounds__(64 * W, E == 8 ? 8 : 5) void k_logp(LogpArgs a, int64_t row0) {
     constexpr int V = BF16 ? 8 : 4, T = 64 * W, NV = E / V, CH = T * E;
@@ -118,12 +118,22 @@ __global__ __launch_bounds__(64 * W, E == 8 ? 8 : 5) void k_logp(LogpArgs a, int
         float g = tm;
 #pragma unroll
         for (int i = 1; i < W; i++) g = fmaxf(g, lane_max[i][lane]);
-        int above = 0;
-        if (a.k > 1)
+        float lim = M;
+        // few: one after another, equal ones at once (375 x 151936, k 5: f32 47.2 -> 44.7 us, bf16 43.2 -> 39.2; 2000 x
+        // 28000, k 8: 55.3 -> 53.5); more: by counting (8 x 151936, k 16: 12.9, one after another 13.8)
+        if (a.k <= 8) {
+            for (int n = __popcll(__ballot(g == lim)); n < a.k; n += __popcll(__ballot(g == lim))) {
+                g = g == lim ? none : g;
+                lim = wave_max_f32(g);
+                if (lim == none) break;
+            }
+        } else {
+            int above = 0;
 #pragma unroll 16
             for (int i = 0; i < 64; i++) above += __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), i)) > g;
-        // the least of the maxima that fewer than k pass
-        const float lim = -wave_max_f32(a.k > 1 ? above < a.k ? -g : none : -M);
+            // the least of the maxima that fewer than k pass
+            lim = -wave_max_f32(above < a.k ? -g : none);
+        }
         if (lane == 0) limit = lim;
     }
     // the sums; the terms of the maximum, exactly 1 each, are counted, all but one
@@ -381,7 +391,7 @@ static hipError_t go_logp(LogpArgs a, hipStream_t st) {
 }
 
 // the fewest values that hold a row, as those of none cost what others do (4000 x 300 12.5 -> 9.7 us); longer rows in
-// chunks of four waves (of one, for few rows: 8 x 151936 14.1 -> 16.9 us; 64 values a thread: bf16 375 x 151936 43 -> 47)
+// chunks of four waves (of one, for few rows: 8 x 151936 16.9 us for 14.1; 64 values a thread: bf16 375 x 151936 47 for 43)
 template <bool BF16>
 static hipError_t pick_logp(const LogpArgs &a, hipStream_t st) {
     const int n = a.cols + (BF16 ? 7 : 3);               // with what a row may begin behind a 16-byte place
