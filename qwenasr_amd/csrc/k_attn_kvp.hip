@@ -206,7 +206,7 @@ __device__ __forceinline__ float kvp_sum_groups(float v) { return xhalf_sum(xrow
 template <bool BF16, int HD, int COLS>
 __device__ __forceinline__ void attn_kvp_again(const AttnKvpArgs &a, const KvpSegment &sg, int h, int64_t q_at, bool live, int lim, int first,
                                             int end, int step, float kc, float *om) {
-    constexpr int D = HD * COLS / 64, RUN = COLS == 16 ? D : HD / 8, STRIDE = 64 / COLS * RUN;
+    constexpr int D = HD * COLS / 64, RUN = COLS == 16 ? D : 8, STRIDE = 64 / COLS * RUN;
     const int lane = threadIdx.x & 63, g = lane / COLS * RUN;
     float q[D], o[D], m = KVP_NEG_INF, l = 0.0f;
 #pragma unroll
@@ -536,8 +536,20 @@ __device__ __forceinline__ KvpTile kvp_tile(const AttnKvpArgs &a, int i) {
 // come through a ring of LDS stages, once for its RW waves; the groups' sums are joined at the
 // end.  v_mfma 32x32x16: S^T leaves lane half hf of a
 // column positions 8 (r / 4) + 4 hf + r % 4, and the second product's k is numbered like
-// that, as above.  16-byte piece n of position r stands at n ^ (r & 15) (128 dims) or
-// n ^ ((r / 2) & 7) (64), which spreads the 16 lanes that LDS serves at a time over all banks.
+// that, as above; product t of O has dims 32 t .., a lane of them eight at a time.  V's
+// operand is turned as it is read: of 16 lanes that bring 16 dims of four positions, eight
+// bytes each, every lane gets one dim of the four.  16-byte piece n of position r stands
+// at n ^ kvp_place(r), which spreads over all banks both the 16 positions that K's lanes
+// read a piece of and the four that V's read four pieces of (128 dims; 64: two positions
+// fill the banks).
+template <int HD>
+__device__ __forceinline__ int kvp_place(int r) {
+    return HD == 128 ? (r & 3) << 2 | (r >> 2) : (r & 2) << 1 | (r >> 2);
+}
+__device__ __forceinline__ uint2 kvp_turned(char *p) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p));
+}
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <bool BF16, int HD, int RW, int PG>
 __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a) {
@@ -584,7 +596,7 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
     uint32_t src[NL];
 #pragma unroll
     for (int i = 0; i < NL; i++) {
-        const int r = 32 / RW * wid + RPL * i + lane / PR, n = (lane % PR) ^ (HD == 128 ? r & 15 : (r >> 1) & 7);
+        const int r = 32 / RW * wid + RPL * i + lane / PR, n = (lane % PR) ^ kvp_place<HD>(r & 15);
         src[i] = (uint32_t)((r & 15) * ROW + 16 * n);                // within a half of the tile
     }
     // the group's tiles; past its last one, that again: nothing sees it
@@ -637,16 +649,18 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
     for (int t = 0; t < DV; t++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[t][r] = 0.0f;
-    // where this lane reads in a stage: K's first piece, V's first position
-    const int k_at = c * ROW + 16 * (hf ^ (HD == 128 ? c & 15 : (c >> 1) & 7));
-    const int v_at = TB + 4 * hf * ROW + (HD == 128 ? 16 * ((c >> 1) ^ (4 * hf)) + 8 * (c & 1) : 16 * ((c >> 2) ^ (2 * hf)) + 4 * (c & 3));
+    // where this lane reads in a stage: piece 2 i + hf of position c of K, half of piece 4 t + v_p of V's position 4 hf + v_r
+    const int v_r = (lane >> 2) & 3, v_p = 2 * ((lane >> 4) & 1) + (lane & 1);
+    int k_low = 16 * (hf ^ kvp_place<HD>(c & 15)), v_low = 16 * (v_p ^ kvp_place<HD>(4 * hf + v_r)) + 8 * ((lane >> 1) & 1);
+    const int k_row = (int)(ring - smem) + c * ROW, v_row = (int)(ring - smem) + TB + (4 * hf + v_r) * ROW;
     int stage = 0;
     for (int it = 0; it < n_it; it++) {
         wait_vmcnt<0>();                                         // this wave's loads of the stage have landed
         __syncthreads();                                         // ... and every wave's; the other stage is free
         const KvpIds now = ids;
         ids = table.at(a, base_of(it + 1));
-        const int ks = k_at + stage, vs = v_at + stage;
+        const int ks = k_row + stage, vs = v_row + stage;
+        asm volatile("" : "+v"(k_low), "+v"(v_low));             // kept over the turns the 16 addresses take registers that there are none of
         stage ^= 2 * TB;
         issue(stage, base_of(it + 1), ids);
         const int base = from + 32 * (PG * it + grp);
@@ -654,21 +668,13 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
         // the tile's K first, all of it, and V as early as registers are free: LDS answers late
         bf16x8 k[KC];
 #pragma unroll
-        for (int i = 0; i < KC; i++) k[i] = *reinterpret_cast<const bf16x8 *>(ring + (ks ^ (32 * i)));
-        uint32_t v[2][8][DV / 2];
+        for (int i = 0; i < KC; i++) k[i] = *reinterpret_cast<const bf16x8 *>(smem + ((k_low ^ (32 * i)) + ks));
+        uint2 v[2][DV][2];
         auto load_v = [&](int x) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int n = 8 * (e >> 2) + (e & 3);
-                const char *row = ring + (vs ^ (16 * (HD == 128 ? n : n >> 1))) + (16 * x + n) * ROW;
-                if (HD == 128) {
-                    const uint2 u = *reinterpret_cast<const uint2 *>(row);
-                    v[x][e][0] = u.x;
-                    v[x][e][DV / 2 - 1] = u.y;
-                } else {
-                    v[x][e][0] = *reinterpret_cast<const uint32_t *>(row);
-                }
-            }
+            for (int t = 0; t < DV; t++)
+#pragma unroll
+                for (int y = 0; y < 2; y++) v[x][t][y] = kvp_turned(smem + ((v_low ^ (64 * t + 32 * y)) + vs) + (16 * x + 8 * y) * ROW);
         };
         asm volatile("" ::: "memory");
         f32x16 s;
@@ -711,17 +717,18 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
             if (x == 0) load_v(1);
             if (edge) {
                 // V of positions that no row here sees may hold anything
+                const int left = now.id[x] >= 0 ? end - base - 16 * x - 4 * hf : 0;
 #pragma unroll
-                for (int e = 0; e < 8; e++)
+                for (int y = 0; y < 2; y++) {
+                    const uint32_t m0 = (left > 8 * y ? 0xffffu : 0u) | (left > 8 * y + 1 ? 0xffff0000u : 0u);
+                    const uint32_t m1 = (left > 8 * y + 2 ? 0xffffu : 0u) | (left > 8 * y + 3 ? 0xffff0000u : 0u);
 #pragma unroll
-                    for (int d = 0; d < DV / 2; d++) v[x][e][d] = base + 16 * x + 8 * (e >> 2) + (e & 3) + 4 * hf < end && now.id[x] >= 0 ? v[x][e][d] : 0u;
+                    for (int t = 0; t < DV; t++) v[x][t][y] = make_uint2(v[x][t][y].x & m0, v[x][t][y].y & m1);
+                }
             }
 #pragma unroll
             for (int t = 0; t < DV; t++) {
-                uint32_t d[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) d[e] = __builtin_amdgcn_perm(v[x][2 * e + 1][t >> 1], v[x][2 * e][t >> 1], (t & 1) ? 0x07060302 : 0x05040100);
-                const bf16x8 vt = __builtin_bit_cast(bf16x8, make_uint4(d[0], d[1], d[2], d[3]));
+                const bf16x8 vt = __builtin_bit_cast(bf16x8, make_uint4(v[x][t][0].x, v[x][t][0].y, v[x][t][1].x, v[x][t][1].y));
 #pragma unroll
                 for (int y = PT - 1; y >= 0; y--) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, p[y], o[t], 0, 0, 0);
             }
@@ -741,7 +748,7 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
 #pragma unroll
         for (int t = 0; t < DV; t++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) o[t][r] = om[4 * DV * (r >> 2) + DV * (r & 3) + t];
+            for (int r = 0; r < 16; r++) o[t][r] = om[16 * t + r];
         m = om[HD / 2];
         l = om[HD / 2 + 1];
     }
@@ -783,23 +790,22 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     float *part = a.part + (qi * a.so + split) * kvp_part<HD>;
 #pragma unroll
-    for (int x = 0; x < 4; x++) {
-        float v[4 * DV];
-        const int d = 4 * DV * (2 * x + hf);
+    for (int t = 0; t < DV; t++)
 #pragma unroll
-        for (int r = 0; r < 4; r++)
+        for (int x = 0; x < 2; x++) {
+            const int d = 32 * t + 16 * x + 8 * hf;
+            float v[8];
 #pragma unroll
-            for (int t = 0; t < DV; t++) v[DV * r + t] = o[t][4 * x + r];
-        if (a.so == 1) {
+            for (int e = 0; e < 8; e++) v[e] = o[t][8 * x + e];
+            if (a.so == 1) {
 #pragma unroll
-            for (int e = 0; e < 4 * DV; e++) v[e] *= inv;
+                for (int e = 0; e < 8; e++) v[e] *= inv;
+                kvp_store<BF16, 8>(a.out, qi * HD + d, a.vec_o, v);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 4 * DV; e += 8) kvp_store<BF16, 8>(a.out, qi * HD + d + e, a.vec_o, v + e);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4 * DV; e += 2) *reinterpret_cast<float2 *>(part + d + e) = make_float2(v[e], v[e + 1]);
+                for (int e = 0; e < 8; e += 2) *reinterpret_cast<float2 *>(part + d + e) = make_float2(v[e], v[e + 1]);
+            }
         }
-    }
     if (a.so > 1 && hf == 0) *reinterpret_cast<float2 *>(part + HD) = make_float2(m, l);
 }
 
