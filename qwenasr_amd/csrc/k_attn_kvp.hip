@@ -920,12 +920,15 @@ template <bool BF16, int HD>
 static hipError_t go_attn_kvp(AttnKvpArgs &a, int64_t room, hipStream_t st) {
     const int64_t rows = a.s.max_rows * a.G;
     if (rows <= 32) return go_few<BF16, HD>(a, room, st);
-    // Four groups over the positions where the tiles are one a CU at most, and enough to need no split; else two, and two
-    // blocks a CU.  us, two / four, 8 KV heads x 2 heads of 128, f32: 32 x 20 rows behind 1000 positions 43.2 / 37.9, 2 x
-    // 512 behind 4000 110 / 104, 404 alone 17.4 / 17.9; 6 x 404 20.7 / 29.0, 8 x 512 behind 4000 330 / 372.  (Four side by
-    // side, two groups: 8 x 512 336, but six ragged prompts of 1337 134 against 113.)
+    // Four groups over the positions where the tiles are one a CU at most, and enough to need no split, or a bit more of one
+    // prompt, whose last tiles see twice as much as its middle one; else two, and two blocks a CU.  us, two / four, 8 KV
+    // heads x 2 heads of 128, f32: 32 x 20 rows behind 1000 positions 40.5 / 34.2, 2 x 512 behind 4000 105 / 96, 404 alone
+    // 16.8 / 17.2, 1337 alone 38.7 / 35.2, 1750 alone 50.7 / 49.4; 2 x 900 31.6 / 38.8, 6 x 404 20.2 / 27.7, 4 x 350 behind
+    // 1500 103 / 118, 8 x 512 behind 4000 317 / 338.  (Four side by side, two groups: 8 x 512 2% slower, but six ragged
+    // prompts of 1337 by 18%.)
     const int64_t units = std::min((rows + 63) / 64 * a.s.n_seq, (a.s.n_rows * a.G / 32 + a.s.n_seq) / 2 + 1) * a.s.Hkv;
-    return units >= 128 && units <= 256 ? go_rows<BF16, HD, 2, 4>(a, room, st) : go_rows<BF16, HD, 2, 2>(a, room, st);
+    const bool prompt = a.s.n_seq == 1 && a.max_len <= 2 * a.s.max_rows;
+    return units >= 128 && units <= (prompt ? 400 : 256) ? go_rows<BF16, HD, 2, 4>(a, room, st) : go_rows<BF16, HD, 2, 2>(a, room, st);
 }
 
 hipError_t launch_attention_kvp(const AttnKvpArgs &a0, bool bf16, hipStream_t st) {
