@@ -60,7 +60,7 @@ __device__ __forceinline__ float logp_at(const LogpArgs &a, int64_t row, int i) 
 
 // W waves with E values a thread; five waves a SIMD (with four, f32 375 x 151936 52 us for 47), eight of short rows
 template <bool BF16, int W, int E>
-__global__ __launch_bounds__(64 * W, E == 8 ? 8 : 5) void k_logp(LogpArgs a, int64_t row0) {
+__global__ __launch_bounds__(64 * W, E == 8 ? 8 : W == 16 ? 4 : 5) void k_logp(LogpArgs a, int64_t row0) {
     constexpr int V = BF16 ? 8 : 4, T = 64 * W, NV = E / V, CH = T * E;
     __shared__ float red[3][W], lane_max[W][64], limit;
     __shared__ int red_n[W], n_cand;
@@ -110,13 +110,13 @@ __global__ __launch_bounds__(64 * W, E == 8 ? 8 : 5) void k_logp(LogpArgs a, int
         if (lane == 0) red[0][w] = M;
         lane_max[w][lane] = tm;
         __syncthreads();
-#pragma unroll
+#pragma unroll 4
         for (int i = 0; i < W; i++) M = fmaxf(M, red[0][i]);
     }
     // the k-th largest of the lanes' maxima, by the first wave, while the others go on
     if (a.k > 0 && w == 0) {
         float g = tm;
-#pragma unroll
+#pragma unroll 4
         for (int i = 1; i < W; i++) g = fmaxf(g, lane_max[i][lane]);
         float lim = M;
         // few: one after another, equal ones at once (375 x 151936, k 5: f32 47.2 -> 44.7 us, bf16 43.2 -> 39.2; 2000 x
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(64 * W, E == 8 ? 8 : 5) void k_logp(LogpArgs a, int
     __syncthreads();
     s = h = 0.0f;
     ones = 0;
-#pragma unroll
+#pragma unroll 4
     for (int i = 0; i < W; i++) {
         s += red[1][i];
         h += red[2][i];
@@ -251,7 +251,7 @@ __global__ __launch_bounds__(64 * W, E == 8 ? 8 : 5) void k_logp(LogpArgs a, int
                 if (lane == 63) red_n[w] = before;
                 __syncthreads();
                 before += n - mine;
-#pragma unroll
+#pragma unroll 4
                 for (int u = 0; u < W; u++) {
                     before += u < w ? red_n[u] : 0;
                     n += red_n[u];
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(64 * W, E == 8 ? 8 : 5) void k_logp(LogpArgs a, int
         if (lane == 0) best_l[w] = best;
         __syncthreads();
         last = 0;
-#pragma unroll
+#pragma unroll 4
         for (int i = 0; i < W; i++) last = max(last, best_l[i]);
         __syncthreads();
         if (t == 0) {
@@ -390,8 +390,11 @@ static hipError_t go_logp(LogpArgs a, hipStream_t st) {
     return hipGetLastError();
 }
 
-// the fewest values that hold a row, as those of none cost what others do (4000 x 300 12.5 -> 9.7 us); longer rows in
-// chunks of four waves (of one, for few rows: 8 x 151936 16.9 us for 14.1; 64 values a thread: bf16 375 x 151936 47 for 43)
+// The fewest waves that hold a row, as those of none cost what others do (4000 x 300 12.5 -> 9.7 us): one launch, while
+// blocks of 8 or 16 waves are few enough not to wait for one another (us, chunks / one block: 8 waves, 8 x 12000 bf16 10.7 /
+// 6.9, 2000 x 16000 f32 32.9 / 32.1, 4000 x 16000 55.6 / 56.5; 16 waves, 256 x 30000 f32 15.2 / 10.9, 512 x 20000 17.7 /
+// 17.6, 600 x 20000 19.3 / 23.0).  Longer rows and more of them in chunks of four waves (of one, for few rows: 8 x 151936
+// 16.9 us for 14.1; 64 values a thread: bf16 375 x 151936 47 for 43, and 16 waves of them spill).
 template <bool BF16>
 static hipError_t pick_logp(const LogpArgs &a, hipStream_t st) {
     const int n = a.cols + (BF16 ? 7 : 3);               // with what a row may begin behind a 16-byte place
@@ -399,6 +402,8 @@ static hipError_t pick_logp(const LogpArgs &a, hipStream_t st) {
     if (n <= 64 * LOGP_E) return go_logp<BF16, 1, LOGP_E>(a, st);
     if (n <= 128 * LOGP_E) return go_logp<BF16, 2, LOGP_E>(a, st);
     if (n <= 192 * LOGP_E) return go_logp<BF16, 3, LOGP_E>(a, st);
+    if (n > 256 * LOGP_E && n <= 512 * LOGP_E && a.rows <= 2048) return go_logp<BF16, 8, LOGP_E>(a, st);
+    if (n > 512 * LOGP_E && n <= 1024 * LOGP_E && a.rows <= 512) return go_logp<BF16, 16, LOGP_E>(a, st);
     return go_logp<BF16, 4, LOGP_E>(a, st);
 }
 

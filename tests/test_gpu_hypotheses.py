@@ -610,7 +610,9 @@ def logprobs(dev, x, targets, k, is_bf16, pad=0, off=0):
 @pytest.mark.parametrize("rows,cols,k,pad,off", [(1, 1, 1, 0, 0), (3, 2, 2, 0, 0), (5, 31, 31, 1, 1), (2, 63, 32, 0, 3), (9, 64, 5, 8, 0), (4, 1000, 32, 0, 0),
                                                  (3, 2041, 8, 0, 1), (3, 2048, 8, 0, 0), (2, 2049, 9, 0, 0), (4, 4999, 1, 0, 0), (3, 8185, 32, 2, 1),
                                                  (2, 8192, 32, 0, 0), (2, 8192, 3, 0, 5), (2, 8193, 16, 3, 0), (2, 20011, 32, 1, 2), (3, 151936, 16, 0, 0),
-                                                 (400, 700, 4, 0, 0), (1, 1 << 20, 32, 0, 1)])
+                                                 (400, 700, 4, 0, 0), (1, 1 << 20, 32, 0, 1), (3, 16383, 8, 0, 3), (2, 16384, 5, 0, 0), (3, 24001, 32, 1, 1),
+                                                 (2, 32761, 9, 7, 2), (2, 32768, 4, 0, 0), (2, 32768, 32, 0, 1), (3, 40003, 12, 2, 0), (600, 20001, 3, 0, 0),
+                                                 (2100, 8500, 2, 0, 1)])
 def test_logprobs(dev, rows, cols, k, pad, off, is_bf16):
     print(f"logprobs {rows} x {cols} k={k} pad={pad} off={off} bf16={is_bf16}", flush=True)
     r = rng(cols + rows)
@@ -625,7 +627,7 @@ def test_logprobs(dev, rows, cols, k, pad, off, is_bf16):
 
 
 @pytest.mark.parametrize("is_bf16", [False, True])
-@pytest.mark.parametrize("cols", [40, 2000, 9000, 30000])
+@pytest.mark.parametrize("cols", [40, 2000, 9000, 30000, 40000])
 def test_logprobs_ties_go_to_the_lowest_index(dev, cols, is_bf16):
     r = rng(cols)
     x = np.stack([np.zeros(cols), np.full(cols, -3.5), np.repeat(np.arange(cols // 40 + 1), 40)[:cols] % 2.0, -np.repeat(np.arange(cols // 40 + 1.0), 40)[:cols],
@@ -638,7 +640,7 @@ def test_logprobs_ties_go_to_the_lowest_index(dev, cols, is_bf16):
 
 
 @pytest.mark.parametrize("is_bf16", [False, True])
-@pytest.mark.parametrize("rows,cols", [(12, 3000), (12, 9000), (60, 30000), (5, 151936)])
+@pytest.mark.parametrize("rows,cols", [(12, 3000), (12, 9000), (60, 30000), (5, 151936), (60, 50000)])
 def test_logprobs_masked_vocabularies(dev, rows, cols, is_bf16):
     """Few values left, the others -infinity or the type's lowest; and places of a few lanes that hold all the large ones."""
     r = rng(rows + cols)
@@ -660,7 +662,7 @@ def test_logprobs_masked_vocabularies(dev, rows, cols, is_bf16):
     check_logp(x, targets, 32, logprobs(dev, x, targets, 32, is_bf16))
 
 
-@pytest.mark.parametrize("cols", [50, 9000])
+@pytest.mark.parametrize("cols", [50, 9000, 40000])
 def test_logprobs_next_to_one(dev, cols):
     """A probability of 1 - 1e-9 has a logarithm of -1e-9, not 0; its entropy likewise."""
     x = np.full((3, cols), -60.0, np.float32)
@@ -671,14 +673,14 @@ def test_logprobs_next_to_one(dev, cols):
     assert -3e-9 < lp[0] < -1e-9
     # e^-20: twice 20 half steps, the exponential's and log1p's units.  The last row's entropy is 50 terms of e^-100 = 3.7e-44
     # times 100, 2e-40 at most together with 9000 of them 3e-38: its terms are below 2^-126 = 1.2e-38, f32's smallest normal
-    # number, under which the exponential gives 0
-    tiny = 1e-37 if cols > 50 else 2.0 ** -126
+    # number, under which the exponential gives 0 (40000 of them: 1.5e-37)
+    tiny = max(1e-37, 4e-42 * cols) if cols > 50 else 2.0 ** -126
     assert np.allclose(got[0], lp, rtol=60 * 3 * U, atol=0) and np.allclose(got[1], ent, rtol=60 * 8 * U, atol=tiny)
     assert np.allclose(got[3], top, rtol=60 * 3 * U, atol=2.0 ** -126)       # the last row's: 9000 e^-100 = 3e-40
 
 
 @pytest.mark.parametrize("is_bf16", [False, True])
-@pytest.mark.parametrize("cols", [60, 9000])
+@pytest.mark.parametrize("cols", [60, 9000, 40000])
 def test_logprobs_not_finite(dev, cols, is_bf16):
     """NaN or +infinity: NaN values, ids by value with NaN last; -infinity alone: log 0; targets outside: NaN."""
     x = held(rng(cols).normal(0, 1, (7, cols)), is_bf16).astype(np.float32)
@@ -699,7 +701,7 @@ def test_logprobs_not_finite(dev, cols, is_bf16):
 def test_logprobs_parts(dev):
     """Any of the results alone: the same bits as all of them."""
     from qwenasr_amd import kernels as K
-    for cols in (500, 20000):
+    for cols in (500, 20000, 40000):
         x = rng(3).normal(0, 2, (5, cols)).astype(np.float32)
         d, g = dev.upload(x), ints(dev, [1, 2, 3, 4, 5])
         want = [a.astype(np.float32) if a.dtype == np.float64 else a for a in logprobs(dev, x, [1, 2, 3, 4, 5], 6, False)]
