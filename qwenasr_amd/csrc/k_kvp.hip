@@ -54,8 +54,13 @@ __device__ __forceinline__ void block_scan(int (&v)[N], int (&total)[N], int (*s
 
 __device__ __forceinline__ int kvp_held(int len, int shift) { return (len + (1 << shift) - 1) >> shift; }
 
-// lanes that walk one sequence's entries together: a wave for few sequences, 16 lanes for many
-__device__ __forceinline__ int kvp_lanes(int n) { return n <= KVP_WAVES ? 64 : n <= 2 * KVP_WAVES ? 32 : 16; }
+// lanes that walk one sequence's entries together: a wave for few sequences, and so few for
+// many that all sequences' loads are on their way at once
+__device__ __forceinline__ int kvp_lanes(int n) {
+    int lanes = 64;
+    while (lanes > 4 && KVP_THREADS / lanes < n) lanes >>= 1;
+    return lanes;
+}
 
 // entries [0, held) of a sequence's row, four of a lane on their way at a time
 template <typename F>
@@ -69,6 +74,21 @@ __device__ __forceinline__ void kvp_entries(const int32_t *row, int held, int la
             if (s0 + u * lanes < held) f(s0 + u * lanes, id[u]);
     }
 }
+
+// A thread's part of a bitmap of nw words, in order of the threads: some words, or some bits of one.
+struct KvpBits {
+    int w0, words;
+    uint32_t mask;
+    __device__ __forceinline__ KvpBits(int nw) {
+        const int t = threadIdx.x;
+        int split = 1;                                   // threads a word
+        while (split < 32 && nw * split * 2 <= KVP_THREADS) split *= 2;
+        words = (nw + KVP_THREADS - 1) / KVP_THREADS;
+        w0 = words > 1 ? t * words : t / split;
+        words = w0 < nw ? min(words, nw - w0) : 0;
+        mask = split == 1 ? ~0u : ((1u << 32 / split) - 1) << t % split * (32 / split);
+    }
+};
 
 // bits past n_pages count as used
 __device__ __forceinline__ uint32_t kvp_no_pages(int w, int n_pages) {
@@ -88,12 +108,27 @@ __global__ __launch_bounds__(KVP_THREADS) void k_kvp_fork(KvpForkArgs a, int slo
     const int n_pages = a.pools.n_pages, nw = (n_pages + 31) / 32, shift = a.pools.shift, page = 1 << shift, cap = a.table_ld << shift;
     uint32_t *used = lds, *full = used + nw;
     int *hash_id = reinterpret_cast<int *>(full + nw), *hash_key = hash_id + slots, *pick_l = hash_key + slots;
-    int *len = pick_l + KVP_PICK, *par = len + n, *tail = par + n, *info = tail + n, *base = info + n;
+    int *len = pick_l + KVP_PICK, *par = len + n, *tail = par + n, *info = tail + n, *base = info + n, *rows_l = base + n;
     int *picks = a.work + KVP_PICKS, *copies = a.work + KVP_COPIES;
-    auto rows_of = [&](int j) -> int {
-        if (!a.row_start) return (int)a.max_rows;
-        return (int)min(max((int64_t)a.row_start[j + 1] - a.row_start[j], (int64_t)0), a.max_rows);
-    };
+    // thread t has sequences t, t + 1024, .. until their entries are walked; all that is known of them goes out at once
+    constexpr int PER = KVP_SEQS / KVP_THREADS;
+    int p_of[PER], l_of[PER];
+    int64_t r_of[PER][2];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int j = t + i * KVP_THREADS, jc = min(j, n - 1);
+        p_of[i] = j;
+        l_of[i] = 0;
+        r_of[i][0] = 0;
+        r_of[i][1] = a.max_rows;
+        if (i > 0 && i * KVP_THREADS >= max(n, a.n_seq)) continue;
+        if (n > 0 && a.parent) p_of[i] = a.parent[jc];
+        if (a.n_seq > 0) l_of[i] = a.len[min(j, a.n_seq - 1)];
+        if (n > 0 && a.row_start) {
+            r_of[i][0] = a.row_start[jc];
+            r_of[i][1] = a.row_start[jc + 1];
+        }
+    }
     if (t == 0) over = 0, all_need = 0;
     for (int i = t; i < nw; i += KVP_THREADS) {
         used[i] = kvp_no_pages(i, n_pages);
@@ -103,17 +138,24 @@ __global__ __launch_bounds__(KVP_THREADS) void k_kvp_fork(KvpForkArgs a, int slo
         hash_id[i] = -1;
         hash_key[i] = 0;
     }
+    static_assert(KVP_PICK >= KVP_SEQS, "the parents' lengths, before there are pages to hand out");
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+        if (t + i * KVP_THREADS < a.n_seq) pick_l[t + i * KVP_THREADS] = l_of[i];
     __syncthreads();
-    for (int j = t; j < n; j += KVP_THREADS) {
-        const int p = a.parent ? a.parent[j] : j;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int j = t + i * KVP_THREADS, p = p_of[i], rows = (int)min(max(r_of[i][1] - r_of[i][0], (int64_t)0), a.max_rows);
+        if (j >= n) break;
         const bool ok = (unsigned)p < (unsigned)a.n_seq;
-        const int l = ok ? min(max(a.len[p], 0), cap) : 0, rows = rows_of(j);
+        const int l = ok ? min(max(pick_l[p], 0), cap) : 0;
         const int held = kvp_held(l, shift), fresh = kvp_held(l + rows, shift) - held;
         len[j] = l;
         par[j] = ok ? p : 0;
         tail[j] = -1;
         info[j] = (l & (page - 1)) | (rows > 0 ? 256 : 0);
         base[j] = fresh;
+        rows_l[j] = rows;
         if (held + fresh > a.table_ld) atomicAdd(&over, 1);
     }
     __syncthreads();
@@ -134,7 +176,6 @@ __global__ __launch_bounds__(KVP_THREADS) void k_kvp_fork(KvpForkArgs a, int slo
     }
     __syncthreads();
     // thread t has sequences 2 t and 2 t + 1 from here on
-    constexpr int PER = KVP_SEQS / KVP_THREADS;
     int at_hash[PER], key[PER];
 #pragma unroll
     for (int i = 0; i < PER; i++) {
@@ -154,7 +195,7 @@ __global__ __launch_bounds__(KVP_THREADS) void k_kvp_fork(KvpForkArgs a, int slo
     }
     __syncthreads();
     int v[3] = {0, 0, 0}, total[3];
-    const int per_w = (nw + KVP_THREADS - 1) / KVP_THREADS, w0 = t * per_w;
+    const KvpBits mine(nw);
     long long want = 0;
     int copy[PER];
 #pragma unroll
@@ -170,8 +211,7 @@ __global__ __launch_bounds__(KVP_THREADS) void k_kvp_fork(KvpForkArgs a, int slo
     if (want) atomicAdd(&all_need, (unsigned long long)want);
     // held to what is past any pool, so that the sums stay in 32 bits
     v[0] = (int)min(want, 1LL << 20);
-    for (int i = 0; i < per_w; i++)
-        if (w0 + i < nw) v[2] += __popc(~used[w0 + i]);
+    for (int i = 0; i < mine.words; i++) v[2] += __popc(~used[mine.w0 + i] & mine.mask);
     block_scan(v, total, sums);
     const int n_free = total[2], n_used = n_pages - n_free;
     const bool fail = over > 0 || total[0] > n_free;
@@ -199,10 +239,9 @@ __global__ __launch_bounds__(KVP_THREADS) void k_kvp_fork(KvpForkArgs a, int slo
     // the lowest free pages
     const bool in_lds = total[0] <= KVP_PICK;
     int rank = v[2];
-    for (int i = 0; i < per_w && rank < total[0]; i++) {
-        if (w0 + i >= nw) break;
-        for (uint32_t f = ~used[w0 + i]; f && rank < total[0]; f &= f - 1, rank++) {
-            const int id = (w0 + i) * 32 + __builtin_ctz(f);
+    for (int i = 0; i < mine.words && rank < total[0]; i++) {
+        for (uint32_t f = ~used[mine.w0 + i] & mine.mask; f && rank < total[0]; f &= f - 1, rank++) {
+            const int id = (mine.w0 + i) * 32 + __builtin_ctz(f);
             if (in_lds) pick_l[rank] = id;
             else picks[rank] = id;
         }
@@ -210,7 +249,7 @@ __global__ __launch_bounds__(KVP_THREADS) void k_kvp_fork(KvpForkArgs a, int slo
     __syncthreads();
     auto pick = [&](int r) { return in_lds ? pick_l[r] : picks[r]; };
     for (int j = g; j < n; j += groups) {
-        const int l = len[j], held = kvp_held(l, shift), inf = info[j], c = (inf >> 9) & 1, rows = rows_of(j), last = tail[j];
+        const int l = len[j], held = kvp_held(l, shift), inf = info[j], c = (inf >> 9) & 1, rows = rows_l[j], last = tail[j];
         const int end = kvp_held(l + rows, shift), first = (inf & 255) ? held - 1 : held, b = base[j];
         int32_t *out = a.table_out + (int64_t)j * a.table_ld;
         for (int s = first + lane; s < a.table_ld; s += lanes) {
@@ -245,28 +284,28 @@ __global__ __launch_bounds__(KVP_THREADS) void k_kvp_compact(KvpCompactArgs a) {
             if ((unsigned)id < (unsigned)n_pages) atomicOr(&used[id >> 5], 1u << (id & 31));
         });
     __syncthreads();
-    const int per_w = (nw + KVP_THREADS - 1) / KVP_THREADS, w0 = t * per_w;
+    const KvpBits mine(nw);
+    const int w0 = mine.w0;
     int v1[1] = {0}, t1[1], v[2] = {0, 0}, total[2];
-    for (int i = 0; i < per_w; i++) v1[0] += w0 + i < nw ? __popc(used[w0 + i]) : 0;
+    for (int i = 0; i < mine.words; i++) v1[0] += __popc(used[w0 + i] & mine.mask);
     block_scan(v1, t1, sums);
     const int n_used = t1[0];
     // pages at n_used and behind that are held, and those before that are free: as many
-    auto low = [&](int w) { return ~kvp_no_pages(w, n_used); };
-    for (int i = 0; i < per_w; i++)
-        if (w0 + i < nw) {
-            v[0] += __popc(used[w0 + i] & ~low(w0 + i));
-            v[1] += __popc(~used[w0 + i] & low(w0 + i));
-        }
+    auto from_high = [&](int w) { return used[w] & kvp_no_pages(w, n_used) & mine.mask; };
+    auto to_low = [&](int w) { return ~used[w] & ~kvp_no_pages(w, n_used) & mine.mask; };
+    for (int i = 0; i < mine.words; i++) {
+        v[0] += __popc(from_high(w0 + i));
+        v[1] += __popc(to_low(w0 + i));
+    }
     block_scan(v, total, sums2);
     int src = v[0], dst = v[1];
     const int n_moved = total[0];
-    for (int i = 0; i < per_w; i++) {
-        if (w0 + i >= nw) break;
-        for (uint32_t f = used[w0 + i] & ~low(w0 + i); f; f &= f - 1) {
+    for (int i = 0; i < mine.words; i++) {
+        for (uint32_t f = from_high(w0 + i); f; f &= f - 1) {
             copies[4 * src] = (w0 + i) * 32 + __builtin_ctz(f);
             copies[4 * src++ + 2] = 1 << shift;
         }
-        for (uint32_t f = ~used[w0 + i] & low(w0 + i); f; f &= f - 1) copies[4 * dst++ + 1] = (w0 + i) * 32 + __builtin_ctz(f);
+        for (uint32_t f = to_low(w0 + i); f; f &= f - 1) copies[4 * dst++ + 1] = (w0 + i) * 32 + __builtin_ctz(f);
     }
     if (t == 0) {
         a.status[0] = n_moved;
@@ -329,7 +368,7 @@ hipError_t launch_kvp_fork(const KvpForkArgs &a, hipStream_t st) {
     if (a.pools.n_pages > KVP_PAGES || a.n_out > KVP_SEQS) return hipErrorInvalidValue;
     int slots = 64;
     while (slots < 2 * a.n_out) slots *= 2;
-    const size_t lds = ((size_t)(a.pools.n_pages + 31) / 32 * 2 + 2 * (size_t)slots + 5 * (size_t)a.n_out + KVP_PICK) * 4;
+    const size_t lds = ((size_t)(a.pools.n_pages + 31) / 32 * 2 + 2 * (size_t)slots + 6 * (size_t)a.n_out + KVP_PICK) * 4;
     hipLaunchKernelGGL(k_kvp_fork, dim3(1), dim3(KVP_THREADS), lds, st, a, slots);
     const hipError_t e = hipGetLastError();
     return e != hipSuccess ? e : launch_copies(a.pools, a.work, a.max_rows > 0 ? a.n_out : 0, st);
