@@ -846,7 +846,7 @@ def test_decoding_steps(dev):
 
 def captured(dev, launch):
     from qwenasr_amd._lib import lib
-    hip = C.CDLL("libamdhip64.so")
+    hip = C.CDLL("libamdhip64.so.7")     # the HIP runtime the library already loaded
     stream = C.c_void_p(lib().qasr_hip_stream(dev.h))
     graph, exe = C.c_void_p(), C.c_void_p()
     dev.sync()
