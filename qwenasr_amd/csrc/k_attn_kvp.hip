@@ -883,15 +883,14 @@ static void kvp_split(int64_t units, int64_t len, int64_t most, int blocks, int 
     s = (int)((tiles * 32 + chunk - 1) / chunk);
 }
 
-template <bool BF16, int HD, int RW, int PG>
-static hipError_t go_rows(AttnKvpArgs &a, int64_t room, hipStream_t st) {
-    constexpr int R = 32 * RW;
-    const int64_t tiles = (a.s.max_rows * a.G + R - 1) / R;
-    // sequences shorter than max_rows leave tiles empty: counted are those that n_rows rows fill, half a one a sequence
-    const int64_t units = std::min(tiles * a.s.n_seq, (a.s.n_rows * a.G * 2 / R + a.s.n_seq) / 2 + 1) * a.s.Hkv;
-    kvp_split(units, a.max_len, std::max<int64_t>(1, room), 2048 / (RW * PG), 32 * PG, 4, a.so, a.co);
+#define KVP_ROWS 64                             // rows x heads of a block's tile
+template <bool BF16, int HD, int PG>
+static hipError_t go_rows(AttnKvpArgs &a, int64_t units, int turns, int64_t room, hipStream_t st) {
+    constexpr int RW = KVP_ROWS / 32;
+    const int64_t tiles = (a.s.max_rows * a.G + KVP_ROWS - 1) / KVP_ROWS;
+    kvp_split(units, a.max_len, std::max<int64_t>(1, room), 2048 / (RW * PG), 32 * PG, turns, a.so, a.co);
     a.otiles = (int)tiles;
-    const int64_t blocks = std::min(tiles * a.s.n_seq, a.s.n_rows * a.G / R + a.s.n_seq) * a.so * a.s.Hkv;
+    const int64_t blocks = std::min(tiles * a.s.n_seq, a.s.n_rows * a.G / KVP_ROWS + a.s.n_seq) * a.so * a.s.Hkv;
     if (blocks * 64 * RW * PG > UINT32_MAX) return hipErrorInvalidValue;
     hipLaunchKernelGGL((k_attn_kvp_rows<BF16, HD, RW, PG>), dim3((unsigned)blocks), dim3(64 * RW * PG), 0, st, a);
     return a.so > 1 ? go_merge<BF16, HD>(a, st) : hipGetLastError();
@@ -929,15 +928,24 @@ template <bool BF16, int HD>
 static hipError_t go_attn_kvp(AttnKvpArgs &a, int64_t room, hipStream_t st) {
     const int64_t rows = a.s.max_rows * a.G;
     if (rows <= 32) return go_few<BF16, HD>(a, room, st);
-    // Four groups over the positions where the tiles are one a CU at most, and enough to need no split, or a bit more of one
-    // prompt, whose last tiles see twice as much as its middle one; else two, and two blocks a CU.  us, two / four, 8 KV
-    // heads x 2 heads of 128, f32: 32 x 20 rows behind 1000 positions 40.5 / 34.2, 2 x 512 behind 4000 105 / 96, 404 alone
-    // 16.8 / 17.2, 1337 alone 38.7 / 35.2, 1750 alone 50.7 / 49.4; 2 x 900 31.6 / 38.8, 6 x 404 20.2 / 27.7, 4 x 350 behind
-    // 1500 103 / 118, 8 x 512 behind 4000 317 / 338.  (Four side by side, two groups: 8 x 512 2% slower, but six ragged
-    // prompts of 1337 by 18%.)
-    const int64_t units = std::min((rows + 63) / 64 * a.s.n_seq, (a.s.n_rows * a.G / 32 + a.s.n_seq) / 2 + 1) * a.s.Hkv;
+    // Tiles, by the rows there are: sequences shorter than max_rows leave some empty, counted is half a one a sequence
+    const int64_t tiles = (rows + KVP_ROWS - 1) / KVP_ROWS * a.s.n_seq, full = a.s.n_rows * a.G * 2 / KVP_ROWS;
+    const int64_t units = (a.s.n_rows >= a.s.n_seq * a.s.max_rows ? tiles : std::min(tiles, (full + a.s.n_seq) / 2 + 1)) * a.s.Hkv;
+    // Four groups over the positions, one block a CU, or two and two blocks.  Four are for contexts that two would take long
+    // over, where the tiles are one a CU at most and many enough that the parts of splits cost more; and for one prompt
+    // with a bit more tiles, whose last ones see twice as much as its middle one.  us, two (not split) / four, 8 KV heads
+    // x 2 heads of 128, bf16: 5 x 137 rows of 350 positions 13.7 / 13.8, of 600 17.8 / 16.8; f32: 32 x 20 behind 1000 40.5 /
+    // 34.2, 2 x 512 behind 4000 105 / 96, 404 alone 16.8 / 17.2, 1337 alone 38.7 / 35.2, 1750 alone 50.7 / 49.4; 2 x 900
+    // alone 31.6 / 38.8, 6 x 404 20.2 / 27.7, 4 x 350 behind 1500 103 / 118, 8 x 512 behind 4000 317 / 338.  Fewer tiles, two
+    // (split) / four: bf16 1 x 200 behind 800 18.5 / 19.6, 2 x 137 behind 500 19.2 / 15.9, 3 x 137 behind 8000 58 / 61; f32 2 x
+    // 137 behind 800 23.2 / 26.7, 1 x 400 behind 500 28.7 / 24.8.  A split of many tiles has to save more than one of few (5
+    // x 137 of 450, bf16, two groups: 25.7, not split 15.5; 1 x 67 behind 900: 15.1, not split 18.8).  (Four side by side, two
+    // groups: 8 x 512 2% slower, but six ragged prompts of 1337 by 18%.)
+    const int64_t many = BF16 ? 72 : 96;
     const bool prompt = a.s.n_seq == 1 && a.max_len <= 2 * a.s.max_rows;
-    return units >= 128 && units <= (prompt ? 400 : 256) ? go_rows<BF16, HD, 2, 4>(a, room, st) : go_rows<BF16, HD, 2, 2>(a, room, st);
+    if (units >= many && units <= (prompt ? 400 : 256) && a.max_len > 512 && (units >= 128 || a.max_len <= 4096))
+        return go_rows<BF16, HD, 4>(a, units, 4, room, st);
+    return go_rows<BF16, HD, 2>(a, units, units < many ? 4 : 8, room, st);
 }
 
 hipError_t launch_attention_kvp(const AttnKvpArgs &a0, bool bf16, hipStream_t st) {
