@@ -350,8 +350,9 @@ int qasr_hip_kvp_write(qasr_hip *h, uint16_t *k_pages, uint16_t *v_pages, int64_
  * are f32; rows of q enter exactly, and a weight is off by f32 rounding of itself
  * (bf16 rows: by 2^-17 of itself).  Results are the same bits every time.
  * max_len, max_own (0: unknown): about the longest pos + rows, and the most of it
- * behind the shared positions, by which the work is split; results do not depend on
- * them beyond f32 rounding. */
+ * behind the shared positions, by which the work is split, and a prefix read once if that
+ * saves more than it costs (max_own unknown: it is taken to); results do not depend
+ * on them beyond f32 rounding. */
 int qasr_hip_attention_kvp(qasr_hip *h, void *out, const void *q, int64_t ldq, const uint16_t *k_pages,
                            const uint16_t *v_pages, int64_t n_pages, const int32_t *table, int64_t table_ld,
                            const int32_t *row_start, const int32_t *pos, int64_t n_rows, int64_t n_seq, int64_t max_rows,

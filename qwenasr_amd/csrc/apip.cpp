@@ -155,6 +155,7 @@ extern "C" int qasr_hip_attention_kvp(qasr_hip *h, void *out, const void *q, int
     a.Hq = (int)n_heads; a.G = (int)(n_heads / n_kv_heads);
     a.max_len = max_len > 0 ? std::min(max_len, cap) : cap;
     a.max_own = max_own > 0 ? std::min(max_own, a.max_len) : a.max_len;
+    a.common = max_own > 0 ? a.max_len - a.max_own : -1;
     a.part = reinterpret_cast<float *>(h->scratch);
     LAUNCHCHK(launch_attention_kvp(a, bf16 != 0, h->stream), "attention_kvp");
     return QASR_OK;

@@ -907,8 +907,14 @@ template <bool BF16, int HD>
 static hipError_t go_few(AttnKvpArgs &a, int64_t room, hipStream_t st) {
     constexpr int R = 16;
     const int64_t otiles = (a.s.max_rows * a.G + R - 1) / R, own = (int64_t)a.s.n_seq * a.s.Hkv * otiles;
-    a.prefix = a.prefix && (own > 256 || a.max_len > 640);
-    const int64_t n_groups = a.prefix ? (a.s.n_seq + a.group - 1) / a.group : 0, ptiles = a.prefix ? ((int64_t)a.group * a.s.max_rows * a.G + R - 1) / R : 0;
+    // A prefix read once costs a merge and smaller blocks: it has to save 32 MB (us, once / by every member, 8 KV heads of
+    // 128, bf16: 3 x 5 behind 939, 46 MB saved, 11.0 / 13.2, 2 x 19 of four rows behind 231, 34 MB, 13.5 / 11.7, 2 x 2 behind
+    // 2877, 24 MB, 15.3 / 13.3; 2 x 27 behind 884 and 1011 of their own, 188 MB, 47 / 54), and short ones are in the
+    // L2 for all that have a CU each
+    const int64_t all_groups = (a.s.n_seq + a.group - 1) / a.group;
+    const bool saves = a.common < 0 || (a.s.n_seq - all_groups) * a.common * a.s.Hkv * HD * 4 >= (int64_t)32 << 20;
+    a.prefix = a.prefix && saves && (own > 256 || a.max_len > 640);
+    const int64_t n_groups = a.prefix ? all_groups : 0, ptiles = a.prefix ? ((int64_t)a.group * a.s.max_rows * a.G + R - 1) / R : 0;
     a.otiles = (int)otiles;
     a.ptiles = (int)ptiles;
     a.sp = a.so = 1;

@@ -479,6 +479,7 @@ struct AttnKvpArgs {
     float scale;
     int group, Hq, G;
     int64_t max_len, max_own; // hints; > 0
+    int64_t common;           // positions that a group shares, by the hints; < 0: unknown
     float *part;              // the splits' parts (QASR_KVP_PART_BYTES)
     // set by the launcher
     int vec_q, vec_o, prefix, ptiles, otiles, sp, so, cp, co;

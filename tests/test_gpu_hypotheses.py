@@ -367,6 +367,7 @@ ATTN = [
     ([67, 200], [700, 0], 2, [64], 1, 3, 64, 256),
     ([333], [0], 1, None, 1, 1, 128, 64),
     ([1] * 2, [5000, 7000], 2, [4999], 1, 2, 128, 64),
+    ([1] * 34, [4100 + 3 * (j % 17) for j in range(34)], 17, [4090, 4100], 2, 2, 128, 16),    # read once by the hints, too
     ([300, 1, 131], [10, 600, 0], 3, [0], 2, 3, 128, 64),
     ([45], [2500], 1, None, 1, 1, 64, 32),                                                # splits of one tile
     ([129, 128], [-20, 333], 1, None, 1, 1, 128, 128),
