@@ -264,7 +264,6 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_kvp(AttnKvpArgs a) {
     __shared__ float o_l[W][R][HD + 4];
     __shared__ float ml_l[W][2][R];
     __shared__ bf16x8 q_l[QT][KC][64];
-    static_assert(KC <= W, "a chunk of q a wave");
     __shared__ int64_t qi_l[R];
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -329,17 +328,17 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_kvp(AttnKvpArgs a) {
     const int64_t q_at = (sq.r0 + i_row) * a.ldq + (int64_t)head * HD;
     // a negative scale is the queries', a zero one makes them zero
     const float kc = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.4426950408889634f, sign = a.scale == 0.0f ? 0.0f : a.scale < 0.0f ? -1.0f : 1.0f;
-    if (wid < KC) {
+    for (int i = wid; i < KC; i += W) {
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = 0.0f;
-        if (live) kvp_load_q<BF16, 8>(a.q, q_at + 32 * wid + 8 * g, a.vec_q, x);
+        if (live) kvp_load_q<BF16, 8>(a.q, q_at + 32 * i + 8 * g, a.vec_q, x);
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] *= sign;
         bf16x8 tr[QT];
         kvp_terms<QT>(x, tr);
 #pragma unroll
-        for (int t = 0; t < QT; t++) q_l[t][wid][lane] = tr[t];
+        for (int t = 0; t < QT; t++) q_l[t][i][lane] = tr[t];
     }
     __syncthreads();
 
@@ -907,23 +906,34 @@ template <bool BF16, int HD>
 static hipError_t go_few(AttnKvpArgs &a, int64_t room, hipStream_t st) {
     constexpr int R = 16;
     const int64_t otiles = (a.s.max_rows * a.G + R - 1) / R, own = (int64_t)a.s.n_seq * a.s.Hkv * otiles;
-    // A prefix read once costs a merge and smaller blocks: it has to save 32 MB (us, once / by every member, 8 KV heads of
-    // 128, bf16: 3 x 5 behind 939, 46 MB saved, 11.0 / 13.2, 2 x 19 of four rows behind 231, 34 MB, 13.5 / 11.7, 2 x 2 behind
-    // 2877, 24 MB, 15.3 / 13.3; 2 x 27 behind 884 and 1011 of their own, 188 MB, 47 / 54), and short ones are in the
+    // A prefix read once costs a merge and smaller blocks: it has to save 40 MB (us, once / by every member, 8 KV heads of
+    // 128, bf16: 3 x 5 behind 939, 46 MB saved, 11.1 / 13.2, 2 x 19 of four rows behind 231, 34 MB, 13.4 / 9.1, 2 x 2 behind
+    // 2877, 24 MB, 15.3 / 13.3; 2 x 27 behind 884 and 1011 of their own, 188 MB, 47 / 51), and short ones are in the
     // L2 for all that have a CU each
     const int64_t all_groups = (a.s.n_seq + a.group - 1) / a.group;
-    const bool saves = a.common < 0 || (a.s.n_seq - all_groups) * a.common * a.s.Hkv * HD * 4 >= (int64_t)32 << 20;
+    const bool saves = a.common < 0 || (a.s.n_seq - all_groups) * a.common * a.s.Hkv * HD * 4 >= (int64_t)40 << 20;
     a.prefix = a.prefix && saves && (own > 256 || a.max_len > 640);
     const int64_t n_groups = a.prefix ? all_groups : 0, ptiles = a.prefix ? ((int64_t)a.group * a.s.max_rows * a.G + R - 1) / R : 0;
     a.otiles = (int)otiles;
     a.ptiles = (int)ptiles;
     a.sp = a.so = 1;
     a.cp = a.co = 1 << 30;
-    const int64_t blocks_own = own, blocks_pre = n_groups * ptiles * a.s.Hkv;
+    const int64_t blocks_pre = n_groups * ptiles * a.s.Hkv;
     if (!a.prefix) {
         if (a.max_len > 512) kvp_split(own, a.max_len, room, 256, 256, 1, a.so, a.co);
-        const bool once = otiles == 1 && (int64_t)a.s.n_seq * a.max_len * a.s.Hkv * HD * 4 >= (int64_t)256 << 20;
-        return once ? run_few<BF16, HD, 8, true, false>(a, own * a.so, st) : run_few<BF16, HD, 8, false, true>(a, own * a.so, st);
+        // Eight waves a block where every block has a CU of its own, or long to go; else four, and two of short contexts, as
+        // waves and the LDS of their parts are what blocks wait for.  us, eight / four / two, 8 KV heads x 2 heads of 128, bf16:
+        // 48 sequences of 60 positions 10.3 / 6.8 / -, 250 of 120 46.2 / 25.1 / 24.1, of 500 77 / 67 / 72, 1000 of 32 141 / 53 /
+        // 37, of 250 199 / 141 / 131, 128 of 4000 252 / 266 / 252.  (One wave: 1000 of 32 bf16 37.0, f32 48.5 against 48.0; 250 of
+        // 1000 f32 150 / 144 with two / 132 with four.)
+        const int w = own <= 256 || a.max_len > 2048 ? 8 : own <= 1024 || a.max_len > 384 ? 4 : 2;
+        // K and V past the caches where there is more of them than those hold (250 of 250, 256 MB, two waves 43.2 / 39.7 us;
+        // 64 of 500, 131 MB, 20.9 / 21.2; eight waves, which else ask for a tile ahead, 14 of 3786, 217 MB, 36.0 / 37.5)
+        const bool once = otiles == 1 && (int64_t)a.s.n_seq * a.max_len * a.s.Hkv * HD * 4 >= (int64_t)(w == 8 ? 256 : 192) << 20;
+        const int64_t blocks = own * a.so;
+        if (w == 8) return once ? run_few<BF16, HD, 8, true, false>(a, blocks, st) : run_few<BF16, HD, 8, false, true>(a, blocks, st);
+        if (w == 4) return once ? run_few<BF16, HD, 4, true, false>(a, blocks, st) : run_few<BF16, HD, 4, false, false>(a, blocks, st);
+        return once ? run_few<BF16, HD, 2, true, false>(a, blocks, st) : run_few<BF16, HD, 2, false, false>(a, blocks, st);
     }
     kvp_split(own, a.max_own, room / 2, 768, 128, 1, a.so, a.co);
     kvp_split(blocks_pre, a.max_len, room - a.so, (int)std::max<int64_t>(768 - own * a.so, 256), 128, 1, a.sp, a.cp);

@@ -493,14 +493,19 @@ def test_attention_bound_of_rows(dev):
     check_attention(c, attention(dev, c, q, counts, pos, 2, max_rows=1 << 24), q, counts, pos)
 
 
-@pytest.mark.parametrize("n_seq,rows,heads,g,dim", [(2048, 1, 1, 32, 64), (2048, 1, 2, 16, 128), (300, 20, 1, 32, 64)])
-def test_attention_without_room_for_parts(dev, n_seq, rows, heads, g, dim):
-    """So many rows x heads that the scratch area holds one part of each or none: no prefix and no split, whatever the hints."""
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("n_seq,rows,heads,g,dim,width", [(2048, 1, 1, 32, 64, 60), (2048, 1, 2, 16, 128, 60), (300, 20, 1, 32, 64, 60), (2048, 1, 1, 32, 128, 20),
+                                                          (2048, 1, 2, 16, 64, 20), (700, 1, 2, 2, 128, 10), (400, 1, 1, 3, 64, 150), (700, 2, 2, 8, 128, 24)])
+def test_attention_of_many_sequences(dev, n_seq, rows, heads, g, dim, width, is_bf16):
+    """Up to the most sequences, and so many rows x heads that the scratch area holds one part of each or none: no prefix and
+    no split, whatever the hints."""
     r = rng(29)
     counts, pos = [rows] * n_seq, [int(x) for x in r.integers(30, 70, n_seq)]
-    c = Cache(dev, r, [a + b for a, b in zip(counts, pos)], 16, heads, dim, 16, [30] * pages_of(n_seq, 16), width=60)
+    groups = pages_of(n_seq, 16)
+    c = Cache(dev, r, [a + b for a, b in zip(counts, pos)], 16, heads, dim, 16, [30] * groups, width=width)
     q = r.normal(0, 1, (sum(counts), heads * g, dim))
-    check_attention(c, attention(dev, c, q, counts, pos, g, 16, [30] * pages_of(n_seq, 16)), q, counts, pos)
+    check_attention(c, attention(dev, c, q, counts, pos, g, 16, [30] * groups, is_bf16), q, counts, pos, is_bf16)
+    check_attention(c, attention(dev, c, q, counts, pos, g, is_bf16=is_bf16), q, counts, pos, is_bf16)
 
 
 def test_attention_rows_past_max_rows(dev):
