@@ -24,6 +24,7 @@
 // its rows again one position at a time in f32 (attn_kvp_again), with each row's own mask.
 #include "kernels.h"
 #include "gemm_common.h"
+#include "qasr_hip.h"
 #include <type_traits>
 
 namespace qasr {
@@ -500,37 +501,49 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_kvp(AttnKvpArgs a) {
 // on.  Blocks that have none (there are as many as the host can tell) come last: between
 // the others they leave the CUs' registers in pieces (six prompts of up to 1337 rows: 400 of
 // 512 blocks at a time).
+// Sequences of max_rows rows each need no search, and of more sequences than a wave has
+// lanes the tiles are counted once, into LDS: read again at each step of the search, 500
+// sequences of 40 rows took 226 us.
 struct KvpTile { int j, tile; };
 template <int R>
-__device__ __forceinline__ KvpTile kvp_tile(const AttnKvpArgs &a, int i) {
-    const int lane = threadIdx.x & 63;
-    auto tiles_of = [&](int j) { return j < a.s.n_seq ? (int)(((unsigned)kvp_rows(a.s, j).n * (unsigned)a.G + R - 1) / R) : 0; };
-    if (a.s.n_seq == 1) return {0, tiles_of(0) - 1 - i};
-    const int mine = tiles_of(lane);
+__device__ __forceinline__ KvpTile kvp_tile(const AttnKvpArgs &a, int i, int *tiles_l) {
+    const int lane = threadIdx.x & 63, n_seq = a.s.n_seq;
+    if (a.uniform) return {i % n_seq, a.otiles - 1 - i / n_seq};
+    auto tiles_of = [&](int j) { return j < n_seq ? (int)(((unsigned)kvp_rows(a.s, j).n * (unsigned)a.G + R - 1) / R) : 0; };
+    if (n_seq == 1) return {0, tiles_of(0) - 1 - i};
+    if (n_seq > 64) {
+        for (int j = threadIdx.x; j < ((n_seq + 63) & ~63); j += blockDim.x) tiles_l[j] = tiles_of(j);
+        __syncthreads();
+    }
+    const int mine = n_seq > 64 ? tiles_l[lane] : tiles_of(lane);
     // tiles of index t and more
     auto from = [&](int t) {
         int n = max(0, mine - t);
-        for (int j = 64 + lane; j < a.s.n_seq; j += 64) n += max(0, tiles_of(j) - t);
+        for (int j = 64 + lane; j < n_seq; j += 64) n += max(0, tiles_l[j] - t);
         return wave_sum_i32(n);
     };
-    if (i >= from(0)) return {0, -1};
-    int t = 0, end = a.otiles;                   // from(t) > i >= from(end)
-    while (end - t > 1) {
-        const int mid = (t + end) / 2;
-        if (from(mid) > i) t = mid;
-        else end = mid;
-    }
-    int r = i - from(t + 1);                     // of the sequences that have it
-    for (int j0 = 0; j0 < a.s.n_seq; j0 += 64) {
-        const unsigned long long has = __ballot((j0 == 0 ? mine : tiles_of(j0 + lane)) > t);
-        const int n = __popcll(has);
-        if (r < n) {
-            const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(has >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)has, 0));
-            return {j0 + __ffsll((unsigned long long)__ballot(((has >> lane) & 1) && before == r)) - 1, t};
+    KvpTile at{0, -1};
+    if (i < from(0)) {
+        int t = 0, end = a.otiles;               // from(t) > i >= from(end)
+        while (end - t > 1) {
+            const int mid = (t + end) / 2;
+            if (from(mid) > i) t = mid;
+            else end = mid;
         }
-        r -= n;
+        int r = i - from(t + 1);                 // of the sequences that have it
+        for (int j0 = 0; j0 < n_seq; j0 += 64) {
+            const unsigned long long has = __ballot((j0 == 0 ? mine : tiles_l[j0 + lane]) > t);
+            const int n = __popcll(has);
+            if (r < n) {
+                const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(has >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)has, 0));
+                at = {j0 + __ffsll((unsigned long long)__ballot(((has >> lane) & 1) && before == r)) - 1, t};
+                break;
+            }
+            r -= n;
+        }
     }
-    return {0, -1};
+    if (n_seq > 64) __syncthreads();             // the counts make way for K and V
+    return at;
 }
 
 // Many rows of a sequence: a block of RW x PG waves, RW of them side by side with 32 query
@@ -566,6 +579,7 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
     constexpr int ROW = HD * 2, TB = 32 * ROW, NS = 2, NL = TB / 1024 / RW, PR = ROW / 16, RPL = 64 / PR;
     constexpr int RING = NS * 2 * TB, JOIN = (PG - 1) * RW * (16 * DV + 2) * 256;
     __shared__ __attribute__((aligned(1024))) char smem[PG * RING > JOIN ? PG * RING : JOIN];
+    static_assert(sizeof smem >= 4 * QASR_KVP_MAX_SEQ, "a place for every sequence's count");
     const int lane = threadIdx.x & 63, c = lane & 31, hf = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wid = wave % RW, grp = wave / RW;
     char *const ring = smem + grp * RING;
@@ -575,7 +589,7 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
     const int h = b % a.s.Hkv;
     b /= a.s.Hkv;
     const int split = b % (unsigned)a.so;
-    const KvpTile at_tile = kvp_tile<R>(a, (int)(b / (unsigned)a.so));
+    const KvpTile at_tile = kvp_tile<R>(a, (int)(b / (unsigned)a.so), reinterpret_cast<int *>(smem));
     const int tile = at_tile.tile, j = at_tile.j;
     if (tile < 0) return;
     const int cap = a.s.table_ld << a.s.shift;
@@ -889,6 +903,7 @@ static hipError_t go_rows(AttnKvpArgs &a, int64_t units, int turns, int64_t room
     const int64_t tiles = (a.s.max_rows * a.G + KVP_ROWS - 1) / KVP_ROWS;
     kvp_split(units, a.max_len, std::max<int64_t>(1, room), 2048 / (RW * PG), 32 * PG, turns, a.so, a.co);
     a.otiles = (int)tiles;
+    a.uniform = !a.s.row_start || a.s.n_rows == a.s.n_seq * a.s.max_rows;
     const int64_t blocks = std::min(tiles * a.s.n_seq, a.s.n_rows * a.G / KVP_ROWS + a.s.n_seq) * a.so * a.s.Hkv;
     if (blocks * 64 * RW * PG > UINT32_MAX) return hipErrorInvalidValue;
     hipLaunchKernelGGL((k_attn_kvp_rows<BF16, HD, RW, PG>), dim3((unsigned)blocks), dim3(64 * RW * PG), 0, st, a);

@@ -482,7 +482,7 @@ struct AttnKvpArgs {
     int64_t common;           // positions that a group shares, by the hints; < 0: unknown
     float *part;              // the splits' parts (QASR_KVP_PART_BYTES)
     // set by the launcher
-    int vec_q, vec_o, prefix, ptiles, otiles, sp, so, cp, co;
+    int vec_q, vec_o, prefix, uniform, ptiles, otiles, sp, so, cp, co;
 };
 #define QASR_KVP_PART_BYTES (32u << 20)
 hipError_t launch_attention_kvp(const AttnKvpArgs &a, bool bf16, hipStream_t st);
