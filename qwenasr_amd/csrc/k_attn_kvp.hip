@@ -973,6 +973,13 @@ static hipError_t go_attn_kvp(AttnKvpArgs &a, int64_t room, hipStream_t st) {
     // x 137 of 450, bf16, two groups: 25.7, not split 15.5; 1 x 67 behind 900: 15.1, not split 18.8).  (Four side by side, two
     // groups: 8 x 512 2% slower, but six ragged prompts of 1337 by 18%.)
     const int64_t many = BF16 ? 72 : 96;
+    // One group, and four blocks a CU (128 dims), where tiles are more than two blocks a CU and short, or so many that the longest
+    // is not what all wait for; and of a single tile of positions.  us, two / one: 16 x 32 rows of 32 positions bf16 7.7 / 6.8, of
+    // 130 10.2 / 10.9, 64 x 32 of 32 11.7 / 10.4; bf16 128 x 17 alone 18.7 / 11.9, 500 x 40 alone 147 / 88, 16 x 200 behind
+    // 1000 61.7 / 54.8, 8 x 512 behind 4000 214 / 199, 4 x 700 alone 27.0 / 27.6; f32 16 x 200 behind 100 34.1 / 28.4, 8 x 700
+    // alone 68.0 / 61.3, 12 x 1000 alone 171 / 156, 16 x 512 behind 4000 634 / 644, 4 x 1000 alone 58.0 / 63.5; dim 64, bf16 128 x
+    // 40 behind 1000 79 / 64, 4 x 1000 alone 22.8 / 29.1
+    if (a.max_len <= 32 || (units > 512 && a.max_len <= 320) || units > (BF16 ? 800 : 1200) * (128 / HD)) return go_rows<BF16, HD, 1>(a, units, 8, room, st);
     const bool prompt = a.s.n_seq == 1 && a.max_len <= 2 * a.s.max_rows;
     if (units >= many && units <= (prompt ? 400 : 256) && a.max_len > 512 && (units >= 128 || a.max_len <= 4096))
         return go_rows<BF16, HD, 4>(a, units, 4, room, st);
