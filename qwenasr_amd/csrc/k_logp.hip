@@ -23,6 +23,7 @@ typedef unsigned long long u64;
 // a row's chunks: those of 256 threads, and one more for what its first begins late by
 #define LOGP_CHUNKS (QASR_LOGP_MAX_COLS / (256 * LOGP_E) + 1)
 #define LOGP_CAND 1024                  // values a chunk ranks by counting
+#define LOGP_LANES 64                   // lanes whose values are looked through together
 #define LOGP_LOG2E 1.4426950408889634f
 #define LOGP_LN2 0.6931471805599453f
 
@@ -63,7 +64,9 @@ template <bool BF16, int W, int E>
 __global__ __launch_bounds__(64 * W, E == 8 ? 8 : W == 16 ? 4 : 5) void k_logp(LogpArgs a, int64_t row0) {
     constexpr int V = BF16 ? 8 : 4, T = 64 * W, NV = E / V, CH = T * E;
     __shared__ float red[3][W], lane_max[W][64], limit;
-    __shared__ int red_n[W], n_cand;
+    constexpr bool SHARE = W > 2;                        // (with fewer waves the LDS that it takes holds blocks up)
+    __shared__ int red_n[W], n_cand, n_lanes, lane_of[SHARE ? LOGP_LANES : 1], ranks[SHARE ? 64 : 1];
+    __shared__ __attribute__((aligned(16))) float held[SHARE ? LOGP_LANES : 1][E + 4];
     constexpr int CAND = CH < LOGP_CAND ? CH : LOGP_CAND;
     __shared__ u64 cand[CAND], best_l[W];
     const int t = threadIdx.x, lane = t & 63, w = t >> 6;
@@ -105,7 +108,8 @@ __global__ __launch_bounds__(64 * W, E == 8 ? 8 : W == 16 ? 4 : 5) void k_logp(L
 #pragma unroll
     for (int e = 0; e < E; e++) tm = fmaxf(tm, x[e]);
     float M = wave_max_f32(tm);
-    if (t == 0) n_cand = 0;
+    if (t == 0) n_cand = n_lanes = 0;
+    if (SHARE && t < 64) ranks[t] = 0;
     if (W > 1) {
         if (lane == 0) red[0][w] = M;
         lane_max[w][lane] = tm;
@@ -197,7 +201,32 @@ __global__ __launch_bounds__(64 * W, E == 8 ? 8 : W == 16 ? 4 : 5) void k_logp(L
 
     // ---- the k largest
     const float lim = limit;
-    if (__any(tm >= lim)) {
+    const bool hit = tm >= lim;
+    const u64 hits = __ballot(hit);
+    if (SHARE && hits) {
+        // the values of the lanes that reach T, looked through by all threads: each lane its own is 50 instructions for four
+        // values of which one is wanted (375 x 151936, k 32, bf16 71.7 -> 63.4 us)
+        int slot = 0;
+        if (lane == 0) slot = atomicAdd(&n_lanes, __popcll(hits));
+        slot = __builtin_amdgcn_readfirstlane(slot) + __builtin_amdgcn_mbcnt_hi((unsigned)(hits >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)hits, 0));
+        if (hit && slot < LOGP_LANES) {
+            lane_of[slot] = t;
+#pragma unroll
+            for (int e = 0; e < E; e += 4) *reinterpret_cast<f32x4 *>(&held[slot][e]) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+        }
+    }
+    if (SHARE) __syncthreads();
+    const int lanes = n_lanes;
+    if (SHARE && lanes <= LOGP_LANES) {
+        for (int u = t; u < lanes * E; u += T) {
+            const int e = u % E, i = i0 + (e / V * T + lane_of[u / E]) * V + e % V;
+            const float y = held[u / E][e];
+            if (!(fmaxf(y, none) < lim) && i >= 0 && i < a.cols) {
+                const int c = atomicAdd(&n_cand, 1);
+                if (c < CAND) cand[c] = logp_key(y, i);
+            }
+        }
+    } else if (hits) {
 #pragma unroll
         for (int n = 0; n < NV; n++)
 #pragma unroll
@@ -261,6 +290,24 @@ __global__ __launch_bounds__(64 * W, E == 8 ? 8 : W == 16 ? 4 : 5) void k_logp(L
             n = min(n, a.k);
             __syncthreads();
         }
+    }
+    if (SHARE && n > 8 && n <= 64) {
+        // every wave compares all keys with some of them
+        const u64 y = lane < n ? cand[lane] : ~0ull;
+        int rank = 0;
+        for (int j = w; j < n; j += W) rank += cand[j] > y;
+        if (lane < n) atomicAdd(&ranks[lane], rank);
+        __syncthreads();
+        if (t < n) {
+            const int r = ranks[t];
+            if (r < a.k) {
+                if (only) logp_top(a, row, r, y, part);
+                else top[r] = y;
+            }
+        }
+        if (!only)
+            for (int i = n + t; i < a.k; i += T) top[i] = 0;
+        return;
     }
     if (n <= CAND) {
         for (int i = t; i < n; i += T) {
@@ -350,15 +397,21 @@ __global__ __launch_bounds__(256) void k_logp_join(LogpArgs a, int64_t row0) {
     r.h = wave_sum_f32(r.h);
     if (t == 0) logp_row(a, row, r, x_target, has);
     if (a.k == 0) return;
-    // the lists by their first keys, then of the r-th list the k - r first, if they are not below the k-th list's
+    // the lists by their first keys, then of the r-th list the k - r first, if they are not below a key that k of them reach:
+    // the k-th list's first; of fewer lists the least of those keys of which each has as many above it as make k
+    const int deep = n < a.k ? (a.k - 1) / n : 0;
     for (int i = t; i < n; i += 256) {
         const u64 y = keys[i * a.k];
         int rank = 0;
         for (int j = 0; j < n; j++) rank += keys[j * a.k] > y;
         if (y != 0 && rank < a.k) list[rank] = i;
     }
+    u64 least = ~0ull;
+    if (deep > 0)
+        for (int i = 0; i < n; i++) least = min(least, keys[i * a.k + deep]);
     __syncthreads();
-    const u64 least = list[a.k - 1] >= 0 ? keys[list[a.k - 1] * a.k] : 1;      // k first keys are not below it
+    if (deep == 0) least = list[a.k - 1] >= 0 ? keys[list[a.k - 1] * a.k] : 0;
+    least = max(least, 1ull);                                    // 0: no key
     for (int i = t; i < a.k * a.k; i += 256) {
         const int r = i / a.k, place = i % a.k;
         if (r + place >= a.k || list[r] < 0) continue;
