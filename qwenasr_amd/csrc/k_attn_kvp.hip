@@ -833,7 +833,7 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
 
 // The parts of each row and head, in order; a wave a head.  4.7 us for 64 rows x 16 heads, bound by its chain of loads: a
 // part that has no positions says so by its sum, so that nothing but the rows' places has
-// to be known, and the first eight parts are on their way with the weights.
+// to be known, and the first 24 parts are on their way with the weights.
 template <bool BF16, int HD>
 __global__ __launch_bounds__(256) void k_attn_kvp_merge(AttnKvpArgs a) {
     constexpr int E = HD / 64;
@@ -846,14 +846,16 @@ __global__ __launch_bounds__(256) void k_attn_kvp_merge(AttnKvpArgs a) {
     const int64_t qi = (sq.r0 + i) * a.Hq + head;
     const float *part = a.part + qi * P * kvp_part<HD>;
     const float2 ml = *reinterpret_cast<const float2 *>(part + min(lane, P - 1) * kvp_part<HD> + HD);
-    float p[8][E];
-    auto load = [&](int x0) {
+    float p0[8][E], p1[16][E];
+    auto load = [&](auto &p, int x0, int count) {
 #pragma unroll
-        for (int u = 0; u < 8; u++)
+        for (int u = 0; u < count; u++)
 #pragma unroll
             for (int e = 0; e < E; e++) p[u][e] = part[min(x0 + u, P - 1) * kvp_part<HD> + E * lane + e];
     };
-    load(0);
+    load(p0, 0, 8);
+    if (P > 16) load(p1, 8, 16);
+    else if (P > 8) load(p1, 8, 8);
     const float mx = lane < P ? ml.x : KVP_NEG_INF;
     const float mm = wave_max_f32(mx);
     const float w = mx == KVP_NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(mx - mm);
@@ -861,17 +863,23 @@ __global__ __launch_bounds__(256) void k_attn_kvp_merge(AttnKvpArgs a) {
     float v[E];
 #pragma unroll
     for (int e = 0; e < E; e++) v[e] = 0.0f;
-    for (int x0 = 0; x0 < P; x0 += 8) {
-        if (x0 > 0) load(x0);
+    auto add = [&](const auto &p, int x0, int count) {
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
+        for (int u = 0; u < count; u++) {
             const int x = min(x0 + u, 63);
             const float wx = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), x));
             const bool is = x0 + u < P && __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mx), x)) != KVP_NEG_INF;
 #pragma unroll
             for (int e = 0; e < E; e++) v[e] = is ? fmaf(p[u][e], wx, v[e]) : v[e];
         }
-    }
+    };
+    add(p0, 0, 8);
+    if (P > 16)
+        for (int x0 = 8; x0 < P; x0 += 16) {
+            if (x0 > 8) load(p1, x0, 16);
+            add(p1, x0, 16);
+        }
+    else if (P > 8) add(p1, 8, 8);
     const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll
     for (int e = 0; e < E; e++) {
@@ -951,7 +959,8 @@ static hipError_t go_few(AttnKvpArgs &a, int64_t room, hipStream_t st) {
         return once ? run_few<BF16, HD, 2, true, false>(a, blocks, st) : run_few<BF16, HD, 2, false, false>(a, blocks, st);
     }
     kvp_split(own, a.max_own, room / 2, 768, 128, 1, a.so, a.co);
-    kvp_split(blocks_pre, a.max_len, room - a.so, (int)std::max<int64_t>(768 - own * a.so, 256), 128, 1, a.sp, a.cp);
+    // 128 positions a part at least, of long prefixes 256: parts cost the merge (5 behind 5204, 8 heads of 64, 21.4 -> 15.9 us)
+    kvp_split(blocks_pre, a.max_len, room - a.so, (int)std::max<int64_t>(768 - own * a.so, 256), 128, a.max_len > 1024 ? 2 : 1, a.sp, a.cp);
     return run_few<BF16, HD, 4, false, false>(a, blocks_pre * a.sp + own * a.so, st);
 }
 
