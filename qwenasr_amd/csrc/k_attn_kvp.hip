@@ -256,8 +256,8 @@ constexpr int kvp_part = HD + 2;                 // floats of a query's part: O,
 // Blocks: h fastest, then the tile of rows, the split, the group or sequence; the
 // prefixes' first.  What bounds short ones is the chain rows -> table -> K -> products ->
 // merge, so each load goes out as soon as its address is known: 8 hypotheses of 404 to 440
-// positions 9.6 us (the first form 15.3).  Long ones are bound by memory: 32 sequences of 4000
-// 73 us, 5.6 TB/s (four waves a block 81); four groups of 16 behind 4000 33.9 us (63), of
+// positions 9.6 us (the first form 15.3).  Long ones are bound by memory: 32 sequences of up to 4000
+// 74 us, 5.6 TB/s (four waves a block 81); four groups of 16 behind 4000 33.9 us (63), of
 // which the merge is 4.7.
 template <bool BF16, int HD, int W, bool ONCE, bool AHEAD>
 __global__ __launch_bounds__(64 * W, 2) void k_attn_kvp(AttnKvpArgs a) {
@@ -560,9 +560,9 @@ __device__ __forceinline__ KvpTile kvp_tile(const AttnKvpArgs &a, int i, int *ti
 //
 // Bound by the matrix instructions, three terms each of q and of the weights for f32 rows,
 // and the chain between the two products that two waves a SIMD do not cover: 8 x 512 rows
-// behind 4000 positions, 16 heads, f32 318 us (1.35 PFLOP/s, every term counted; the library's
-// bf16 product of 8192^3 reaches 1.41), bf16 212; six prompts of up to 1337 rows, f32, 107.5 us
-// (K and V straight into registers 272, turned in registers 109.5).
+// behind 2262 to 4000 positions, 16 heads, f32 318 us (1.05 PFLOP/s, every term counted; the
+// library's bf16 product of 8192^3 reaches 1.41), bf16 199 (0.83); six prompts of up to 1337 rows, f32, 109 us
+// (K and V straight into registers 272, V turned there 2% more).
 template <int HD>
 __device__ __forceinline__ int kvp_place(int r) {
     return HD == 128 ? (r & 3) << 2 | (r >> 2) : (r & 2) << 1 | (r >> 2);
@@ -945,7 +945,8 @@ static hipError_t go_few(AttnKvpArgs &a, int64_t room, hipStream_t st) {
     if (!a.prefix) {
         if (a.max_len > 512) kvp_split(own, a.max_len, room, 256, 256, 1, a.so, a.co);
         // Eight waves a block where every block has a CU of its own, or long to go; else four, and two of short contexts, as
-        // waves and the LDS of their parts are what blocks wait for.  us, eight / four / two, 8 KV heads x 2 heads of 128, bf16:
+        // waves and the LDS of their parts are what blocks wait for.  us, eight / four / two, 8 KV heads x 2 heads of 128, bf16,
+        // sequences of half to all of the positions named:
         // 48 sequences of 60 positions 10.3 / 6.8 / -, 250 of 120 46.2 / 25.1 / 24.1, of 500 77 / 67 / 72, 1000 of 32 141 / 53 /
         // 37, of 250 199 / 141 / 131, 128 of 4000 252 / 266 / 252.  (One wave: 1000 of 32 bf16 37.0, f32 48.5 against 48.0; 250 of
         // 1000 f32 150 / 144 with two / 132 with four.)
@@ -974,13 +975,13 @@ static hipError_t go_attn_kvp(AttnKvpArgs &a, int64_t room, hipStream_t st) {
     // Four groups over the positions, one block a CU, or two and two blocks.  Four are for contexts that two would take long
     // over, where the tiles are one a CU at most and many enough that the parts of splits cost more; and for one prompt
     // with a bit more tiles, whose last ones see twice as much as its middle one.  us, two (not split) / four, 8 KV heads
-    // x 2 heads of 128, bf16: 5 x 137 rows of 350 positions 13.7 / 13.8, of 600 17.8 / 16.8; f32: 32 x 20 behind 1000 40.5 /
-    // 34.2, 2 x 512 behind 4000 105 / 96, 404 alone 16.8 / 17.2, 1337 alone 38.7 / 35.2, 1750 alone 50.7 / 49.4; 2 x 900
-    // alone 31.6 / 38.8, 6 x 404 20.2 / 27.7, 4 x 350 behind 1500 103 / 118, 8 x 512 behind 4000 317 / 338.  Fewer tiles, two
-    // (split) / four: bf16 1 x 200 behind 800 18.5 / 19.6, 2 x 137 behind 500 19.2 / 15.9, 3 x 137 behind 8000 58 / 61; f32 2 x
-    // 137 behind 800 23.2 / 26.7, 1 x 400 behind 500 28.7 / 24.8.  A split of many tiles has to save more than one of few (5
-    // x 137 of 450, bf16, two groups: 25.7, not split 15.5; 1 x 67 behind 900: 15.1, not split 18.8).  (Four side by side, two
-    // groups: 8 x 512 2% slower, but six ragged prompts of 1337 by 18%.)
+    // x 2 heads of 128, behind half to all of what is named, bf16: 5 x 137 rows of 350 positions 13.7 / 13.8, of 600 17.8 /
+    // 16.8; f32: 32 x 20 behind 1000 40.5 / 34.2, 2 x 512 behind 4000 105 / 96, 404 alone 16.8 / 17.2, 1337 alone 38.7 /
+    // 35.2, 1750 alone 50.7 / 49.4; 2 x 900 alone 31.6 / 38.8, 6 x 404 20.2 / 27.7, 4 x 350 behind 1500 103 / 118, 8 x 512
+    // behind 4000 317 / 338.  Fewer tiles, two (split) / four: bf16 1 x 200 behind 800 18.5 / 19.6, 2 x 137 behind 500 19.2 /
+    // 15.9, 3 x 137 behind 8000 58 / 61; f32 2 x 137 behind 800 23.2 / 26.7, 1 x 400 behind 500 28.7 / 24.8.  A split of many
+    // tiles has to save more than one of few (5 x 137 of 450, bf16, two groups: 25.7, not split 15.5; 1 x 67 behind 900: 15.1,
+    // not split 18.8).  (Four side by side, two groups: 8 x 512 2% slower, but six ragged prompts of 1337 by 18%.)
     const int64_t many = BF16 ? 72 : 96;
     // One group, and four blocks a CU (128 dims), where tiles are more than two blocks a CU and short, or so many that the longest
     // is not what all wait for; and of a single tile of positions.  us, two / one: 16 x 32 rows of 32 positions bf16 7.7 / 6.8, of
