@@ -255,7 +255,7 @@ constexpr int kvp_part = HD + 2;                 // floats of a query's part: O,
 // wave every W-th 32 positions straight into registers, as no second tile shares them.
 // Blocks: h fastest, then the tile of rows, the split, the group or sequence; the
 // prefixes' first.  What bounds short ones is the chain rows -> table -> K -> products ->
-// merge, so each load goes out as soon as its address is known: 8 hypotheses of 404 to 440
+// merge, so each load goes out as soon as its address is known: 8 hypotheses of 410 to 435
 // positions 9.6 us (the first form 15.3).  Long ones are bound by memory: 32 sequences of up to 4000
 // 74 us, 5.6 TB/s (four waves a block 81); four groups of 16 behind 4000 33.9 us (63), of
 // which the merge is 4.7.
