@@ -236,7 +236,7 @@ __device__ __forceinline__ void attn_kvp_again(const AttnKvpArgs &a, const KvpSe
             for (int d = 0; d < D; d++) o[d] = fmaf(w, bf16_to_f32(a.vp[at + d / RUN * STRIDE + d % RUN]), o[d] * al);
         }
     }
-    if (m == __builtin_inff()) {                 // an infinite score: NaN, in every part
+    if (m == __builtin_inff() || l != l) {       // an infinite score, or one of NaN (no maximum knows of it): NaN, and a part that the merge takes
         m = 0.0f;
         l = __builtin_nanf("");
 #pragma unroll
@@ -832,8 +832,9 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
 }
 
 // The parts of each row and head, in order; a wave a head.  4.7 us for 64 rows x 16 heads, bound by its chain of loads: a
-// part that has no positions says so by its sum, so that nothing but the rows' places has
-// to be known, and the first 24 parts are on their way with the weights.
+// part that has no positions says so by its maximum, -infinity (a part that is NaN has 0), so
+// that nothing but the rows' places has to be known, and the first 24 parts are on their way
+// with the weights.
 template <bool BF16, int HD>
 __global__ __launch_bounds__(256) void k_attn_kvp_merge(AttnKvpArgs a) {
     constexpr int E = HD / 64;

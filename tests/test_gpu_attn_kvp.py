@@ -1,0 +1,140 @@
+"""Attention over pages where its parts are joined: rows, keys and whole parts that are not finite, against the formula in
+float64, with the work split, behind a shared prefix, and in one piece."""
+import numpy as np
+import pytest
+
+import refp
+from conftest import rng
+from refp import U
+from test_gpu_hypotheses import BF16, Cache, attention, held
+
+pytestmark = pytest.mark.gpu
+
+NAN, INF, NEG = 0x7FC0, 0x7F80, 0xFF80
+
+
+def formula(c, q, counts, pos, is_bf16):
+    """softmax(scale q k) v and its bound; NaN where the formula has it, zeros for rows that see nothing."""
+    pools, at = c.floats(), 0
+    want, bound = np.zeros(q.shape), np.zeros(q.shape)
+    q, scale = held(q, is_bf16), c.dim ** -0.5
+    for j, n in enumerate(counts):
+        end = min(max(pos[j] + n, 0), c.width * c.page)
+        k, there = refp.gather(pools["k"], c.table[j], end, c.page)
+        v, _ = refp.gather(pools["v"], c.table[j], end, c.page)
+        for i in range(n):
+            see = (np.arange(end) <= pos[j] + i) & there
+            for h in range(q.shape[1]):
+                with np.errstate(invalid="ignore"):
+                    s = scale * (k[see, h // (q.shape[1] // c.heads)] @ q[at + i, h])
+                if see.any() and not (np.isfinite(s).any() and (np.isfinite(s) | np.isneginf(s)).all()):
+                    want[at + i, h] = np.nan                 # NaN, +infinity, or -infinity alone
+                    continue
+                use = np.flatnonzero(see)[np.isfinite(s)]    # a score of -infinity: weight 0
+                g = h // (q.shape[1] // c.heads)
+                o, b = refp.attend(q[at + i:at + i + 1, h:h + 1], k[use, g:g + 1], v[use, g:g + 1], np.ones((1, len(use)), bool), scale,
+                                   2.0 ** -17 if is_bf16 else U)
+                want[at + i, h], bound[at + i, h] = o[0, 0], b[0, 0]
+        at += n
+    return want, bound * (1 + BF16) + (BF16 if is_bf16 else U) * np.abs(want)
+
+
+def check(c, q, counts, pos, g, is_bf16, forms):
+    want, bound = formula(c, q, counts, pos, is_bf16)
+    for group, shared, more in forms:
+        got = attention(c.dev, c, q, counts, pos, g, group, shared, is_bf16, **more)
+        assert (np.isnan(got) == np.isnan(want)).all(), (group, shared, more, np.argwhere(np.isnan(got) != np.isnan(want))[:4])
+        ok = ~np.isnan(want)
+        assert (np.abs(got - want)[ok] <= bound[ok]).all(), (group, shared, more)
+    return want
+
+
+def put(c, x, j, positions, heads, dims, bits):
+    for p in positions:
+        c.bits[x][c.table[j, p // c.page], heads, p % c.page, dims] = bits
+
+
+# rows a sequence x heads a KV head: few rows, and tiles of many; capacities of 1024 and more, which are split if no hint says
+# that less of them is in use
+FORMS = [(1, 2), (3, 5), (40, 2)]
+PIECES = [(1, None, {}), (1, None, dict(max_len=64)), (1, None, dict(max_len=300)), (1, None, dict(max_len=1000))]
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows,g", FORMS)
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64)])
+def test_a_row_of_nan_is_nan_in_every_part(dev, rows, g, dim, page, is_bf16):
+    print(f"row of NaN rows={rows} g={g} dim={dim} page={page} bf16={is_bf16}", flush=True)
+    r = rng(50 + dim)
+    counts, pos = [rows] * 3, [700, 20, 330]
+    c = Cache(dev, r, [a + b for a, b in zip(counts, pos)], page, 2, dim, 3, [20], width=1024 // page)
+    q = r.normal(0, 1, (3 * rows, 2 * g, dim))
+    q[0, 0, 5] = q[2 * rows, 2 * g - 1, 0] = q[3 * rows - 1, 1, dim - 1] = np.nan
+    want = check(c, q, counts, pos, g, is_bf16, PIECES + [(3, [20], {}), (3, [20], dict(max_len=1000, max_own=900)), (2, [3, 20], {})])
+    assert np.isnan(want).any(2).sum() == 3
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows,g", FORMS)
+def test_a_part_of_nan_keys(dev, rows, g, is_bf16):
+    """Keys of NaN in one stretch, of which a whole part is made (a table of 1024 positions is split into parts of 288), or the
+    last one: the rows that see it are NaN, those before it are not."""
+    r = rng(51)
+    counts, pos = [rows] * 3, [800, 310, 250]
+    c = Cache(dev, r, [a + b for a, b in zip(counts, pos)], 16, 2, 128, width=64)
+    put(c, "k", 0, range(288, 576), 1, slice(None), NAN)
+    put(c, "k", 1, range(300, 310 + rows), 0, 7, NAN)
+    put(c, "k", 2, range(max(1, 250 + rows // 2), 250 + rows), slice(None), 3, NAN)
+    c.upload()
+    q = r.normal(0, 1, (3 * rows, 2 * g, 128))
+    want = check(c, q, counts, pos, g, is_bf16, PIECES)
+    assert np.isnan(want[:rows, g:]).all() and np.isnan(want[rows:2 * rows, :g]).all() and np.isfinite(want[:rows, :g]).all()
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("dim,page", [(64, 32), (128, 16)])
+def test_nan_in_the_only_position_behind_a_prefix(dev, dim, page, is_bf16):
+    """A finite prefix, and one position of its own a member: NaN in that of two members, and in nobody else's."""
+    r = rng(52)
+    counts, pos = [1] * 6, [96] * 6
+    c = Cache(dev, r, [97] * 6, page, 2, dim, 6, [96], width=1024 // page)
+    put(c, "k", 2, [96], 1, 3, NAN)
+    put(c, "v", 4, [96], 0, 9, NAN)
+    c.upload()
+    q = r.normal(0, 1, (6, 4, dim))
+    want = check_members(c, q, counts, pos, is_bf16, [(6, [96], {}), (6, [96], dict(max_len=97, max_own=1)), (1, None, {}), (1, None, dict(max_len=97))])
+    assert np.isnan(want[2, 2:]).all() and np.isnan(want[4, :2, 9]).all() and np.isnan(want).sum() == 2 * dim + 2
+
+
+def check_members(c, q, counts, pos, is_bf16, forms):
+    """As check, where a value of V is NaN: that dim of the rows that see it."""
+    bits = c.bits["v"].copy()
+    v = c.floats()["v"]
+    nan = [np.isnan(refp.gather(v, c.table[j], pos[j] + n, c.page)[0]).any(0) for j, n in enumerate(counts)]
+    c.bits["v"] = np.where((bits & 0x7FFF) > 0x7F80, 0, bits).astype(np.uint16)
+    want, bound = formula(c, q, counts, pos, is_bf16)
+    c.bits["v"] = bits
+    g = q.shape[1] // c.heads
+    for j in range(len(counts)):
+        want[j][np.repeat(nan[j], g, 0)] = np.nan
+    for group, shared, more in forms:
+        got = attention(c.dev, c, q, counts, pos, g, group, shared, is_bf16, **more)
+        assert (np.isnan(got) == np.isnan(want)).all(), (group, shared, more, np.argwhere(np.isnan(got) != np.isnan(want))[:4])
+        ok = ~np.isnan(want)
+        assert (np.abs(got - want)[ok] <= bound[ok]).all(), (group, shared, more)
+    return want
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+def test_every_part_of_a_prefix_of_nan_keys(dev, is_bf16):
+    """A prefix of NaN keys for one head, and finite positions behind it."""
+    r = rng(53)
+    counts, pos = [1, 2, 1, 1], [700, 710, 705, 690]
+    c = Cache(dev, r, [a + b for a, b in zip(counts, pos)], 16, 2, 64, 4, [690], width=80)
+    put(c, "k", 0, range(690), 1, 11, NAN)
+    for j in (1, 2, 3):                                      # the copies of the part of a page
+        put(c, "k", j, range(688, 690), 1, 11, NAN)
+    c.upload()
+    q = r.normal(0, 1, (5, 6, 64))
+    want = check(c, q, counts, pos, 3, is_bf16, [(4, [690], {}), (4, [690], dict(max_len=720, max_own=40)), (1, None, {}), (1, None, dict(max_len=100))])
+    assert np.isnan(want[:, 3:]).all() and np.isfinite(want[:, :3]).all()
