@@ -346,7 +346,8 @@ int qasr_hip_kvp_write(qasr_hip *h, uint16_t *k_pages, uint16_t *v_pages, int64_
  * are read through the first one's, once for the rows of all.  Groups of different
  * size are filled up with sequences without rows.
  * What a row does not see does not reach it, whatever its bits; in what it sees,
- * infinities and NaN count as they do in the formula, in f32.  Products and sums
+ * infinities and NaN count as they do in the formula, in f32 (scores of -infinity
+ * alone: NaN).  Products and sums
  * are f32; rows of q enter exactly, and a weight is off by f32 rounding of itself
  * (bf16 rows: by 2^-17 of itself).  Results are the same bits every time.
  * max_len, max_own (0: unknown): about the longest pos + rows, and the most of it

@@ -22,6 +22,8 @@
 // not finite can still stand where one row sees it and another does not, and a weight's
 // term of zero times infinity is NaN: a wave whose sums do not come out finite computes
 // its rows again one position at a time in f32 (attn_kvp_again), with each row's own mask.
+// So does one with a row that sees positions and found no score above -infinity: the tiles
+// do not tell those from positions that it does not see.
 #include "kernels.h"
 #include "gemm_common.h"
 #include "qasr_hip.h"
@@ -30,6 +32,9 @@
 namespace qasr {
 
 #define KVP_NEG_INF (-__builtin_inff())
+// the maximum where positions are seen whose scores are all -infinity, with a sum of 0: -infinity is where none is seen.
+// The first gives 0 / 0, as the formula does, unless other positions join it, the second zeros
+#define KVP_LOWEST (-__FLT_MAX__)
 // a running maximum is moved only when it is passed by 2^8: weights stay below 2^8
 #define KVP_SLACK 8.0f
 
@@ -203,7 +208,7 @@ __device__ __forceinline__ float kvp_sum_groups(float v) { return xhalf_sum(xrow
 
 // The rows of one tile of queries over the wave's positions again, one at a time: a
 // lane holds the dims of its column's query that it holds in o, a quarter (16 columns) or
-// a half (32) of them, RUN consecutive ones at a time.
+// a half (32) of them, RUN consecutive ones at a time.  first < end.
 template <bool BF16, int HD, int COLS>
 __device__ __forceinline__ void attn_kvp_again(const AttnKvpArgs &a, const KvpSegment &sg, int h, int64_t q_at, bool live, int lim, int first,
                                             int end, int step, float kc, float *om) {
@@ -215,7 +220,6 @@ __device__ __forceinline__ void attn_kvp_again(const AttnKvpArgs &a, const KvpSe
     if (live)
 #pragma unroll
         for (int d = 0; d < D; d += RUN) kvp_load_q<BF16, RUN>(a.q, q_at + g + d / RUN * STRIDE, false, q + d);
-    if (first >= end) return;
     KvpTable table(a, sg.table, first);
     for (int base = first; base < end; base += step) {
         const KvpIds ids = table.at(a, base);
@@ -228,8 +232,8 @@ __device__ __forceinline__ void attn_kvp_again(const AttnKvpArgs &a, const KvpSe
             for (int d = 0; d < D; d++) s = fmaf(q[d], bf16_to_f32(a.kp[at + d / RUN * STRIDE + d % RUN]), s);
             s = (COLS == 16 ? kvp_sum_groups(s) : xhalf_sum(s)) * kc;
             if (!live || p > lim) continue;
-            const float mn = fmaxf(m, s), ref = mn == KVP_NEG_INF ? 0.0f : mn;
-            const float al = __builtin_amdgcn_exp2f(m - ref), w = __builtin_amdgcn_exp2f(s - ref);
+            const float mn = fmaxf(m, fmaxf(s, KVP_LOWEST));
+            const float al = __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(s - mn);
             m = mn;
             l = l * al + w;
 #pragma unroll
@@ -432,7 +436,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_kvp(AttnKvpArgs a) {
                 id0 = id1;
             }
         }
-        // sums that are not finite: again, row by row
+        // sums that are not finite, or no score where positions are seen (or would be, on pages that are none): again, row by row
         float z4[4] = {l * 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int t = 0; t < VT; t++)
@@ -440,7 +444,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_kvp(AttnKvpArgs a) {
             for (int r = 0; r < 4; r++) z4[r] = fmaf(o[t][r], 0.0f, z4[r]);
         const float z = (z4[0] + z4[1]) + (z4[2] + z4[3]);
         l = kvp_sum_groups(l);
-        if (__any(live && z != 0.0f)) {
+        if (__any(live && (z != 0.0f || (m == KVP_NEG_INF && lim >= max(first, sg.lo))))) {
             float om[HD / 4 + 2];
             attn_kvp_again<BF16, HD, 16>(a, sg, h, q_at, live, lim, first, end, STEP, a.scale * 1.4426950408889634f, om);
 #pragma unroll
@@ -483,7 +487,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_attn_kvp(AttnKvpArgs a) {
             for (int r = 0; r < 4; r++) r4[r] = fmaf(ow[r], e, r4[r]);
         }
         if (whole) {
-            const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+            const float inv = mm == KVP_NEG_INF ? 0.0f : 1.0f / ll;
 #pragma unroll
             for (int r = 0; r < 4; r++) r4[r] *= inv;
             kvp_store<BF16, 4>(a.out, to * HD + d, a.vec_o, r4);
@@ -757,16 +761,17 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
         }
     }
     wait_vmcnt<0>();                                             // no load may land in LDS after the block ends
-    // sums that are not finite: again, row by row
+    // sums that are not finite, or no score where positions are seen (or would be, on pages that are none): again, row by row
     float z = l * 0.0f;
 #pragma unroll
     for (int t = 0; t < DV; t++)
 #pragma unroll
         for (int r = 0; r < 16; r++) z = fmaf(o[t][r], 0.0f, z);
     l = xhalf_sum(l);
-    if (__any(live && z != 0.0f)) {
+    const int first = from + 32 * grp;
+    if (first < end && __any(live && (z != 0.0f || (m == KVP_NEG_INF && lim >= first)))) {
         float om[HD / 2 + 2];
-        attn_kvp_again<BF16, HD, 32>(a, sg, h, q_at, live, lim, from + 32 * grp, end, 32 * PG, a.scale * 1.4426950408889634f, om);
+        attn_kvp_again<BF16, HD, 32>(a, sg, h, q_at, live, lim, first, end, 32 * PG, a.scale * 1.4426950408889634f, om);
 #pragma unroll
         for (int t = 0; t < DV; t++)
 #pragma unroll
@@ -809,7 +814,7 @@ __global__ __launch_bounds__(64 * RW * PG, 2) void k_attn_kvp_rows(AttnKvpArgs a
         }
         m = mm;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = m == KVP_NEG_INF ? 0.0f : 1.0f / l;
     float *part = a.part + (qi * a.so + split) * kvp_part<HD>;
 #pragma unroll
     for (int t = 0; t < DV; t++)
@@ -881,7 +886,7 @@ __global__ __launch_bounds__(256) void k_attn_kvp_merge(AttnKvpArgs a) {
             add(p1, x0, 16);
         }
     else if (P > 8) add(p1, 8, 8);
-    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+    const float inv = mm == KVP_NEG_INF ? 0.0f : 1.0f / ll;
 #pragma unroll
     for (int e = 0; e < E; e++) {
         const int64_t at = qi * HD + E * lane + e;

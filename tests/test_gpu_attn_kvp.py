@@ -138,3 +138,61 @@ def test_every_part_of_a_prefix_of_nan_keys(dev, is_bf16):
     q = r.normal(0, 1, (5, 6, 64))
     want = check(c, q, counts, pos, 3, is_bf16, [(4, [690], {}), (4, [690], dict(max_len=720, max_own=40)), (1, None, {}), (1, None, dict(max_len=100))])
     assert np.isnan(want[:, 3:]).all() and np.isfinite(want[:, :3]).all()
+
+
+# a dim of q that is 1 and of K that is -infinity: a score of -infinity
+def low(c, j, positions, heads=slice(None)):
+    put(c, "k", j, positions, heads, 2, NEG)
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows,g", FORMS)
+@pytest.mark.parametrize("dim,page", [(64, 64), (128, 16)])
+def test_scores_of_minus_infinity_alone(dev, rows, g, dim, page, is_bf16):
+    """What a row sees has scores of -infinity: 0 / 0, as the formula has it.  Where one score is finite, the others weigh
+    nothing; a row that sees nothing gives zeros."""
+    print(f"-infinity rows={rows} g={g} dim={dim} page={page} bf16={is_bf16}", flush=True)
+    r = rng(54 + dim)
+    counts, pos = [rows] * 6, [800, 0, 700, 30, -5, 40]
+    c = Cache(dev, r, [max(a + b, 1) for a, b in zip(counts, pos)], page, 2, dim, width=1024 // page)
+    low(c, 0, range(288, 576))                               # a whole part; the others are finite
+    low(c, 1, range(0, rows), 0)                             # all there is, of one head
+    low(c, 2, range(0, 700 + rows - 1))                      # all but what the last row sees last
+    low(c, 3, range(30 + rows // 2, 30 + rows), 1)
+    if rows > 5:
+        low(c, 4, range(0, rows - 6))                        # rows that see nothing, -infinity alone, and (the last) something
+    low(c, 5, range(page, 40 + rows))
+    c.table[5, 0] = -1                                       # no page, and -infinity behind it
+    c.upload()
+    q = r.normal(0, 1, (6 * rows, 2 * g, dim))
+    q[:, :, 2] = 1.0
+    if rows == 1:
+        q[2, 1, 2] = -1.0                                    # +infinity
+    want = check(c, q, counts, pos, g, is_bf16, PIECES)
+    assert np.isfinite(want[:rows]).all() and np.isnan(want[rows:2 * rows, :g]).all() and np.isnan(want[2 * rows:3 * rows - 1]).all()
+    assert (want[4 * rows:4 * rows + min(rows, 5)] == 0).all()
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows", [1, 4])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scores_of_minus_infinity_behind_a_prefix(dev, rows, dim, is_bf16):
+    """-infinity in the prefix, in what a member has behind it, and in both."""
+    r = rng(55 + dim)
+    counts, pos = [rows] * 8, [331, 340, 350, 331, 120, 130, 121, 5]
+    c = Cache(dev, r, [a + b for a, b in zip(counts, pos)], 16, 2, dim, 4, [331, 120], width=64)
+    low(c, 0, range(331), 1)                                 # the first group's prefix for one head, with the copies of its last page
+    for j in (1, 2, 3):
+        low(c, j, range(320, 331), 1)
+    low(c, 1, range(331, 340 + rows))                        # with what the second member has behind it
+    low(c, 2, range(331, 345))                               # with a part of that
+    low(c, 5, range(120, 130 + rows))                        # behind a finite prefix
+    low(c, 4, range(0, 6))                                   # what the last member sees of the second prefix
+    c.upload()
+    q = r.normal(0, 1, (8 * rows, 4, dim))
+    q[:, :, 2] = 1.0
+    forms = [(4, [331, 120], {}), (4, [331, 120], dict(max_len=360, max_own=30)), (4, [331, 120], dict(max_len=1000, max_own=60)), (1, None, {}),
+             (1, None, dict(max_len=200))]
+    want = check(c, q, counts, pos, 2, is_bf16, forms)
+    assert np.isnan(want[rows:2 * rows, 2:]).all() and np.isfinite(want[:rows]).all() and np.isfinite(want[5 * rows:6 * rows]).all()
+    assert np.isnan(want[7 * rows]).all()
