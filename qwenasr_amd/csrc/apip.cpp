@@ -27,7 +27,7 @@ static int seq_args(int64_t n_seq, int64_t table_ld, int64_t n_pages, int64_t pa
     if (page_shift(page) < 0) return bad("kvp: page must be 16, 32, 64, 128 or 256");
     if (n_pages <= 0 || n_pages > QASR_KVP_MAX_PAGES) return bad("kvp: n_pages must be in [1, 2^18]");
     if (n_seq < 0 || n_seq > QASR_KVP_MAX_SEQ) return bad("kvp: at most 2048 sequences");
-    if (table_ld <= 0 || table_ld * page > (1 << 30)) return bad("kvp: table_ld x page must be in [1, 2^30]");
+    if (table_ld <= 0 || table_ld > (1 << 30) / page) return bad("kvp: table_ld x page must be in [1, 2^30]");
     return QASR_OK;
 }
 
