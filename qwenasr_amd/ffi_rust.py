@@ -9,6 +9,8 @@ header's field order, and one `extern "C"` declaration per entry point, with
 the header's argument names.  The integration notes embed this output, and
 tests/test_abi.py checks that the embedded copy is current.
 """
+import ast
+import operator
 import os
 import re
 import sys
@@ -66,9 +68,37 @@ def rust_type(ctype, structs):
     return out
 
 
+OPERATORS = {ast.Add: operator.add, ast.Sub: operator.sub, ast.Mult: operator.mul, ast.LShift: operator.lshift,
+             ast.RShift: operator.rshift, ast.BitOr: operator.or_, ast.BitAnd: operator.and_}
+
+
+def constant(name, body, known):
+    """The value of a macro: whole numbers, constants defined before it, and the operators that are the same in C and here."""
+    def value(n):
+        if isinstance(n, ast.Constant) and type(n.value) is int:
+            return n.value
+        if isinstance(n, ast.Name) and n.id in known:
+            return known[n.id]
+        if isinstance(n, ast.UnaryOp) and isinstance(n.op, ast.USub):
+            return -value(n.operand)
+        if isinstance(n, ast.BinOp) and type(n.op) in OPERATORS:
+            return OPERATORS[type(n.op)](value(n.left), value(n.right))
+        raise ValueError(f"cannot tell the value of {name}: {body!r}")
+    try:
+        v = value(ast.parse(re.sub(r"\b(0[xX][0-9a-fA-F]+|[1-9]\d*|0)[uUlL]+\b", r"\1", body).strip(), mode="eval").body)
+    except SyntaxError:
+        raise ValueError(f"cannot tell the value of {name}: {body!r}") from None
+    if not -1 << 31 <= v < 1 << 31:
+        raise ValueError(f"{name} does not fit a c_int: {v}")
+    return v
+
+
 def parse(src):
     text = strip_comments(src)
-    consts = re.findall(r"#define\s+(QASR_[A-Z0-9_]+)\s+\(?(-?\d+)\)?", text)
+    known = {}
+    for name, body in re.findall(r"^[ \t]*#[ \t]*define[ \t]+(QASR_\w+)[ \t]+(\S.*)$", text, re.M):
+        known[name] = constant(name, body, known)
+    consts = [(name, str(v)) for name, v in known.items()]
     opaque = re.findall(r"typedef\s+struct\s+(\w+)\s+\1\s*;", text)
     structs_raw = re.findall(r"typedef\s+struct\s*\{(.*?)\}\s*(\w+)\s*;", text, flags=re.S)
     names = set(opaque) | {n for _, n in structs_raw}
