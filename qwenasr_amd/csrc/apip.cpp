@@ -16,6 +16,8 @@ static bool overlap(const void *a, int64_t na, const void *b, int64_t nb) {
     return a && b && na > 0 && nb > 0 && x < y + nb && y < x + na;
 }
 
+static bool off_type(const void *p, int bf16) { return (uintptr_t)p % (bf16 ? 2 : 4) != 0; }
+
 // log2 of a page's positions, -1 for a size that is none
 static int page_shift(int64_t page) {
     for (int s = 4; s <= 8; s++)
@@ -120,6 +122,7 @@ extern "C" int qasr_hip_kvp_write(qasr_hip *h, uint16_t *k_pages, uint16_t *v_pa
                           n_kv_heads, head_dim, page))
         return rc;
     if (!k || !v) return bad("kvp_write: null pointer");
+    if (off_type(k, bf16) || off_type(v, bf16)) return bad("kvp_write: k or v is not aligned to its type");
     if (ld < n_kv_heads * head_dim || ld > INT32_MAX) return bad("kvp_write: row stride out of range");
     CHECK_H(h);
     if (n_seq == 0 || n_rows == 0 || max_rows == 0) return QASR_OK;
@@ -139,6 +142,7 @@ extern "C" int qasr_hip_attention_kvp(qasr_hip *h, void *out, const void *q, int
                           n_kv_heads, head_dim, page))
         return rc;
     if (!out || !q) return bad("attention_kvp: null pointer");
+    if (off_type(out, bf16) || off_type(q, bf16)) return bad("attention_kvp: q or out is not aligned to its type");
     if (n_heads <= 0 || n_heads % n_kv_heads != 0 || n_heads > 65536)
         return bad("attention_kvp: n_heads must be a positive multiple of n_kv_heads");
     if (ldq < n_heads * head_dim || ldq > INT32_MAX) return bad("attention_kvp: row stride out of range");
@@ -169,7 +173,7 @@ extern "C" int qasr_hip_token_logprobs(qasr_hip *h, float *logp, float *entropy,
     if (cols <= 0 || cols > QASR_LOGP_MAX_COLS || ld < cols || ld > INT32_MAX) return bad("token_logprobs: cols must be in [1, 2^20], ld at least cols");
     if (rows < 0 || rows > (1 << 24)) return bad("token_logprobs: rows must be in [0, 2^24]");
     if (k < 0 || k > QASR_LOGP_MAX_K || k > cols) return bad("token_logprobs: k must be in [0, 32], at most cols");
-    if (((uintptr_t)logits) % (bf16 ? 2 : 4) != 0) return bad("token_logprobs: logits are not aligned to their type");
+    if (off_type(logits, bf16)) return bad("token_logprobs: logits are not aligned to their type");
     CHECK_H(h);
     if (k == 0) { top_ids = nullptr; top_logp = nullptr; }
     if (!top_ids && !top_logp) k = 0;

@@ -2,7 +2,7 @@
 the device are looked at (no GPU: a null handle comes last)."""
 import pytest
 
-from test_kvp_refusals import attn, compact, fork, write
+from test_kvp_refusals import P, attn, compact, fork, write
 
 INT64 = (1 << 63) - 1
 
@@ -15,3 +15,11 @@ def test_a_table_longer_than_positions_count(f, page, table_ld):
     from qwenasr_amd import _lib
     rc, msg = f(page=page, table_ld=table_ld)
     assert rc == _lib.QASR_ERR_INVALID and "table_ld" in msg, (rc, msg)
+
+
+@pytest.mark.parametrize("f,name", [(write, "k"), (write, "v"), (attn, "q"), (attn, "out")], ids=lambda v: getattr(v, "__name__", v))
+@pytest.mark.parametrize("bf16,off,taken", [(0, 1, False), (0, 2, False), (0, 3, False), (0, 4, True), (1, 1, False), (1, 2, True), (1, 3, False), (1, 6, True)])
+def test_rows_that_are_not_aligned_to_their_type(f, name, bf16, off, taken):
+    from qwenasr_amd import _lib
+    rc, msg = f(**{name: P + off, "bf16": bf16})
+    assert rc == _lib.QASR_ERR_INVALID and ("handle is null" == msg if taken else "aligned" in msg), (rc, msg)
