@@ -21,6 +21,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 #define KVP_COPIES 16
 #define KVP_PICKS (KVP_COPIES + 4 * (KVP_PAGES / 2))
 #define KVP_MAP (KVP_PICKS + KVP_PAGES)
+static_assert(KVP_MAP + KVP_PAGES == KVP_WORK_INTS && KVP_SEQS <= KVP_PAGES / 2, "a place for every copy, id and page");
 
 // sums over the wave's lanes up to and with each
 __device__ __forceinline__ int wave_scan(int v) {

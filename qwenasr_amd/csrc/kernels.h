@@ -429,8 +429,10 @@ struct KvpCompactArgs {
     int32_t *table_out, *status;
     const int32_t *table, *len;
     int n_seq, table_ld;
-    int *work;
+    int *work;                // scratch: KVP_WORK_INTS
 };
+// a fork's or compaction's lists: the copies' count, up to half the pages moved, the ids handed out, where pages go
+#define KVP_WORK_INTS (16 + 4 * (QASR_KVP_MAX_PAGES / 2) + 2 * QASR_KVP_MAX_PAGES)
 hipError_t launch_kvp_fork(const KvpForkArgs &a, hipStream_t st);
 hipError_t launch_kvp_compact(const KvpCompactArgs &a, hipStream_t st);
 

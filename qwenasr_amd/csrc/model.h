@@ -15,7 +15,7 @@
 #define QASR_CTR_ATTN 64
 #define QASR_CTR_ATTN_N 256
 static_assert(QASR_KV8_PART_BYTES <= QASR_SCRATCH_BYTES && QASR_KVP_PART_BYTES <= QASR_SCRATCH_BYTES &&
-                  QASR_LOGP_PART_BYTES <= QASR_SCRATCH_BYTES, "scratch");
+                  QASR_LOGP_PART_BYTES <= QASR_SCRATCH_BYTES && KVP_WORK_INTS * 4 <= QASR_SCRATCH_BYTES, "scratch");
 // kernel kinds of qasr_hip_decoder_profile
 #define QASR_PROFILE_KINDS 8
 
