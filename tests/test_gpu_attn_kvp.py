@@ -6,7 +6,7 @@ import pytest
 import refp
 from conftest import rng
 from refp import U
-from test_gpu_hypotheses import BF16, Cache, attention, held
+from test_gpu_hypotheses import BF16, Cache, attention, check_attention, held
 
 pytestmark = pytest.mark.gpu
 
@@ -196,3 +196,70 @@ def test_scores_of_minus_infinity_behind_a_prefix(dev, rows, dim, is_bf16):
     want = check(c, q, counts, pos, 2, is_bf16, forms)
     assert np.isnan(want[rows:2 * rows, 2:]).all() and np.isfinite(want[:rows]).all() and np.isfinite(want[5 * rows:6 * rows]).all()
     assert np.isnan(want[7 * rows]).all()
+
+
+# The forms that the work's size picks, reached with small caches: which one runs goes by the hints and the table's width.
+# sequences, rows, lengths (of the first ones, and at most of the others), heads, g, dim, page, width, group, shared, hints
+PICKED = [
+    # eight waves a block, K and V past the caches: in one piece, and split
+    (34, 1, [700, 1, 257, 256, 64], 150, 8, 2, 128, 64, 40, 1, None, dict(max_len=2200)),
+    (34, 2, [600, 2, 520, 33], 150, 8, 3, 64, 16, 270, 1, None, dict(max_len=4300)),
+    (34, 1, [500], 90, 8, 16, 128, 16, 140, 1, None, {}),
+    (12, 1, [3000, 2817, 2816, 2815, 1], 300, 8, 2, 128, 64, 90, 1, None, dict(max_len=5600)),
+    (16, 3, [4400, 4193, 4191, 3], 200, 8, 2, 64, 256, 33, 1, None, dict(max_len=8300)),
+    # four waves, in the caches and past them; two
+    (40, 1, [600, 513, 128, 129, 1], 200, 8, 2, 128, 32, 20, 1, None, {}),
+    (40, 2, [400, 129, 2], 100, 8, 5, 128, 16, 32, 1, None, dict(max_len=450)),
+    (100, 1, [600, 129, 128, 1], 120, 8, 2, 64, 16, 64, 1, None, dict(max_len=1000)),
+    (60, 1, [400], 120, 8, 3, 128, 128, 7, 1, None, dict(max_len=880)),
+    (140, 1, [300, 65, 64, 63, 1], 80, 8, 2, 64, 16, 20, 1, None, {}),
+    (140, 2, [250, 2], 60, 8, 4, 64, 64, 4, 1, None, dict(max_len=200)),
+    # a prefix read once: prefixes and what is behind them in one part or several
+    (130, 1, [450], 330, 8, 2, 64, 16, 45, 10, [300, 0, 17, 256, 300, 31, 1, 300, 299, 64, 128, 300, 300], {}),
+    (40, 1, [700, 650], 500, 8, 16, 64, 16, 48, 10, [290, 300, 0, 100], {}),
+    (40, 1, [700, 650], 400, 8, 16, 128, 64, 12, 10, [290, 300, 0, 100], {}),
+    (12, 2, [1500, 900], 300, 1, 4, 64, 32, 50, 6, [640, 280], {}),
+    # many rows: four groups over the positions, in one piece and split
+    (3, 65, [1090, 1000, 641], 0, 16, 1, 128, 64, 18, 1, None, dict(max_len=1100)),
+    (3, 65, [1090, 1025, 66], 0, 16, 1, 64, 16, 70, 1, None, dict(max_len=1100)),
+    (4, 70, [570, 513, 512, 100], 0, 16, 1, 128, 16, 36, 1, None, {}),
+    (4, 70, [570, 513, 512, 100], 0, 16, 1, 64, 32, 18, 1, None, {}),
+]
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("n_seq,rows,first,most,heads,g,dim,page,width,group,shared,hints", PICKED)
+def test_forms_that_sizes_pick(dev, n_seq, rows, first, most, heads, g, dim, page, width, group, shared, hints, is_bf16):
+    print(f"form {n_seq} x {rows} of {first[:3]} {most} heads={heads} x {g} dim={dim} page={page} width={width} group={group} {hints} bf16={is_bf16}", flush=True)
+    r = rng(n_seq + rows + dim)
+    lengths = (first + [int(x) for x in r.integers(rows, max(most, rows + 1), n_seq)])[:n_seq]
+    if shared:                                               # members hold the prefix, but for some that end inside it
+        lengths = [m if j % 7 == 5 else max(m, shared[j // group] + rows) for j, m in enumerate(lengths)]
+    counts, pos = [rows] * n_seq, [m - rows for m in lengths]
+    c = Cache(dev, r, lengths, page, heads, dim, group, shared, width=width)
+    q = r.normal(0, 1, (sum(counts), heads * g, dim))
+    got = attention(dev, c, q, counts, pos, g, group, shared, is_bf16, **hints)
+    check_attention(c, got, q, counts, pos, is_bf16)
+    assert (attention(dev, c, q, counts, pos, g, group, shared, is_bf16, **hints) == got).all()
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("dim,page", [(64, 32), (128, 64)])
+def test_not_finite_in_groups_over_the_positions(dev, dim, page, is_bf16):
+    """The same with one, two and four groups of a block over the positions, split and in one piece."""
+    r = rng(56 + dim)
+    counts, pos = [65] * 3, [1000, 0, 440]
+    c = Cache(dev, r, [a + b for a, b in zip(counts, pos)], page, 16, dim, width=1120 // page)
+    put(c, "k", 0, range(0, 576), 1, 7, NAN)                 # the first part, and every group's first positions
+    put(c, "k", 0, range(1030, 1065), 2, 0, NAN)
+    low(c, 0, range(0, 1064), 3)                             # all but the last position
+    low(c, 1, range(0, 65), 0)                               # all
+    low(c, 1, range(0, 32), 1)                               # what one group has
+    low(c, 2, range(32, 500), 5)                             # what the others have, and all of it in the first rows but one group's
+    c.upload()
+    q = r.normal(0, 1, (195, 16, dim))
+    q[:, :, 2] = 1.0
+    q[70, 4, 9] = q[194, 15, 0] = q[3, 15, dim - 1] = np.nan
+    want = check(c, q, counts, pos, 1, is_bf16, [(1, None, m) for m in ({}, dict(max_len=600), dict(max_len=200), dict(max_len=32))])
+    assert np.isnan(want[:65, 1]).all() and np.isnan(want[:64, 3]).all() and np.isfinite(want[64, 3]).all() and np.isnan(want[65:130, 0]).all()
+    assert np.isnan(want[65:97, 1]).all() and np.isfinite(want[97:130, 1]).all() and np.isfinite(want[130:, 5]).all()
