@@ -338,7 +338,7 @@ int qasr_hip_kvp_write(qasr_hip *h, uint16_t *k_pages, uint16_t *v_pages, int64_
  * over bf16 pages: out [n_rows][n_heads * head_dim] of q's type = softmax(scale *
  * q . k) v.  Rows as for the write; row i of sequence j sees the positions up to
  * pos[j] + i.  A row that sees nothing gives zeros; rows behind the last sequence,
- * and those past max_rows, are left as they were.
+ * and those past max_rows, are left as they were.  scale is at most 2.3e38 in size.
  * shared (nullable; int32 [ceil(n_seq / group)]): the sequences come in groups of
  * `group` that follow one another (the last may be smaller), and the first shared[g]
  * positions of group g hold the same keys and values in all its members' tables (its

@@ -148,7 +148,7 @@ extern "C" int qasr_hip_attention_kvp(qasr_hip *h, void *out, const void *q, int
     if (ldq < n_heads * head_dim || ldq > INT32_MAX) return bad("attention_kvp: row stride out of range");
     if (group < 1) return bad("attention_kvp: group must be positive");
     if (max_len < 0 || max_own < 0) return bad("attention_kvp: max_len and max_own must not be negative");
-    if (!std::isfinite(scale)) return bad("attention_kvp: scale must be finite");
+    if (!std::isfinite(scale * 1.4426950408889634f)) return bad("attention_kvp: scale x log2 e must be finite");
     if (a.s.max_rows * (n_heads / n_kv_heads) > (1 << 30))
         return bad("attention_kvp: rows x heads of a group out of range");
     CHECK_H(h);

@@ -23,3 +23,11 @@ def test_rows_that_are_not_aligned_to_their_type(f, name, bf16, off, taken):
     from qwenasr_amd import _lib
     rc, msg = f(**{name: P + off, "bf16": bf16})
     assert rc == _lib.QASR_ERR_INVALID and ("handle is null" == msg if taken else "aligned" in msg), (rc, msg)
+
+
+@pytest.mark.parametrize("scale,taken", [(2.3e38, True), (-2.3e38, True), (2.4e38, False), (-3.4e38, False), (float("inf"), False)])
+def test_a_scale_whose_product_with_log2_e_is_not_finite(scale, taken):
+    """Scores are taken in base 2: 2.4e38 x log2 e is no f32, and 0 times it no score of 0."""
+    from qwenasr_amd import _lib
+    rc, msg = attn(scale=scale)
+    assert rc == _lib.QASR_ERR_INVALID and ("handle is null" == msg if taken else "scale" in msg), (rc, msg)
