@@ -339,6 +339,7 @@ int qasr_hip_kvp_write(qasr_hip *h, uint16_t *k_pages, uint16_t *v_pages, int64_
  * q . k) v.  Rows as for the write; row i of sequence j sees the positions up to
  * pos[j] + i.  A row that sees nothing gives zeros; rows behind the last sequence,
  * and those past max_rows, are left as they were.  scale is at most 2.3e38 in size.
+ * out may be q itself, if ldq = n_heads * head_dim, and else does not overlap it.
  * shared (nullable; int32 [ceil(n_seq / group)]): the sequences come in groups of
  * `group` that follow one another (the last may be smaller), and the first shared[g]
  * positions of group g hold the same keys and values in all its members' tables (its

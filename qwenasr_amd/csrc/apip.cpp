@@ -146,6 +146,9 @@ extern "C" int qasr_hip_attention_kvp(qasr_hip *h, void *out, const void *q, int
     if (n_heads <= 0 || n_heads % n_kv_heads != 0 || n_heads > 65536)
         return bad("attention_kvp: n_heads must be a positive multiple of n_kv_heads");
     if (ldq < n_heads * head_dim || ldq > INT32_MAX) return bad("attention_kvp: row stride out of range");
+    const int64_t es = bf16 ? 2 : 4, row = n_heads * head_dim;
+    if ((out != q || ldq != row) && overlap(out, n_rows * row * es, q, n_rows > 0 ? ((n_rows - 1) * ldq + row) * es : 0))
+        return bad("attention_kvp: out overlaps q and is not q");
     if (group < 1) return bad("attention_kvp: group must be positive");
     if (max_len < 0 || max_own < 0) return bad("attention_kvp: max_len and max_own must not be negative");
     if (!std::isfinite(scale * 1.4426950408889634f)) return bad("attention_kvp: scale x log2 e must be finite");

@@ -263,3 +263,22 @@ def test_not_finite_in_groups_over_the_positions(dev, dim, page, is_bf16):
     want = check(c, q, counts, pos, 1, is_bf16, [(1, None, m) for m in ({}, dict(max_len=600), dict(max_len=200), dict(max_len=32))])
     assert np.isnan(want[:65, 1]).all() and np.isnan(want[:64, 3]).all() and np.isfinite(want[64, 3]).all() and np.isnan(want[65:130, 0]).all()
     assert np.isnan(want[65:97, 1]).all() and np.isfinite(want[97:130, 1]).all() and np.isfinite(want[130:, 5]).all()
+
+
+@pytest.mark.parametrize("is_bf16", [False, True])
+@pytest.mark.parametrize("rows,group,shared,hints", [(1, 1, None, dict(max_len=64)), (1, 1, None, {}), (2, 4, [300], {}), (50, 1, None, {}), (50, 1, None, dict(max_len=100)),
+                                                      (50, 1, None, dict(max_len=30))])
+def test_results_in_the_rows_of_q(dev, rows, group, shared, hints, is_bf16):
+    """out may be q: the same bits."""
+    from qwenasr_amd import kernels as K
+    from test_gpu_hypotheses import ints, prefix, up
+    r = rng(57)
+    counts, pos = [rows] * 4, [900, 310, 320, 305]
+    c = Cache(dev, r, [a + b for a, b in zip(counts, pos)], 16, 2, 128, group, shared, width=64)
+    q = r.normal(0, 1, (4 * rows, 6, 128))
+    a, b = up(dev, q, is_bf16), up(dev, q, is_bf16)
+    out = up(dev, np.zeros((4 * rows, 768)), is_bf16)
+    more = dict(row_start=ints(dev, prefix(counts)), group=group, shared=None if shared is None else ints(dev, shared), bf16=is_bf16, **hints)
+    for o, x in ((out, a), (b, b)):
+        K.attention_kvp(o, x, c.k, c.v, c.n_pages, c.t, c.width, ints(dev, pos), 4 * rows, 4, rows, 6, 2, 128, 16, 128 ** -0.5, **more)
+    assert (out.numpy().reshape(-1) == b.numpy().reshape(-1)).all() and (a.numpy() == up(dev, q, is_bf16).numpy()).all()
