@@ -343,18 +343,22 @@ int qasr_hip_kvp_write(qasr_hip *h, uint16_t *k_pages, uint16_t *v_pages, int64_
  * shared (nullable; int32 [ceil(n_seq / group)]): the sequences come in groups of
  * `group` that follow one another (the last may be smaller), and the first shared[g]
  * positions of group g hold the same keys and values in all its members' tables (its
- * first sequence's has to name them even if it sees or has fewer): where that pays, they
- * are read through the first one's, once for the rows of all.  Groups of different
- * size are filled up with sequences without rows.
+ * first sequence's has to name them even if it sees or has fewer): where that pays, for
+ * up to 32 rows x heads of a KV head a sequence, they are read through the first one's,
+ * once for every 16 rows x heads of the members together instead of by each member.
+ * Groups of different size are filled up with sequences without rows.
  * What a row does not see does not reach it, whatever its bits; in what it sees,
  * infinities and NaN count as they do in the formula, in f32 (scores of -infinity
- * alone: NaN).  Products and sums
- * are f32; rows of q enter exactly, and a weight is off by f32 rounding of itself
- * (bf16 rows: by 2^-17 of itself).  Results are the same bits every time.
+ * alone: NaN).  Products and sums are f32, of values times weights of at most 1 (V of
+ * 1e29 and more may leave its range); rows of q enter exactly (f32: from 2^-110 on),
+ * and a weight is off by f32 rounding of itself (bf16 rows: by 2^-17 of itself), down to
+ * 2^-100 of its row's largest.  Results are the same bits every time.
  * max_len, max_own (0: unknown): about the longest pos + rows, and the most of it
- * behind the shared positions, by which the work is split, and a prefix read once if that
- * saves more than it costs (max_own unknown: it is taken to); results do not depend
- * on them beyond f32 rounding. */
+ * behind the shared positions, by which the work is split, and a prefix read for all if
+ * that saves more than it costs (max_own unknown: it is taken to); results do not depend
+ * on them beyond f32 rounding.  Without max_len the split is over the whole table, and
+ * past it the last part takes what there is: both cost time where the table is several
+ * times as long, or max_len a fraction.  A captured call keeps its hints. */
 int qasr_hip_attention_kvp(qasr_hip *h, void *out, const void *q, int64_t ldq, const uint16_t *k_pages,
                            const uint16_t *v_pages, int64_t n_pages, const int32_t *table, int64_t table_ld,
                            const int32_t *row_start, const int32_t *pos, int64_t n_rows, int64_t n_seq, int64_t max_rows,

@@ -1,5 +1,5 @@
 // Attention over a KV cache in pages, a prefix that a group of sequences shares read
-// once for all of them.
+// for 16 rows x heads of theirs at a time.
 //
 // A wave takes 16 (or 32) query rows x heads of a group against 32 positions at a
 // time, everything in registers: S^T = K Q^T leaves a lane (column c = its query, lane
@@ -935,7 +935,8 @@ template <bool BF16, int HD>
 static hipError_t go_few(AttnKvpArgs &a, int64_t room, hipStream_t st) {
     constexpr int R = 16;
     const int64_t otiles = (a.s.max_rows * a.G + R - 1) / R, own = (int64_t)a.s.n_seq * a.s.Hkv * otiles;
-    // A prefix read once costs a merge and smaller blocks: it has to save 40 MB (us, once / by every member, 8 KV heads of
+    // A prefix read for all members costs a merge and smaller blocks: it has to save 40 MB, counted as if one read were all
+    // (every 16 rows x heads read it, most of them from the L2) (us, for all / by every member, 8 KV heads of
     // 128, bf16: 3 x 5 behind 939, 46 MB saved, 11.1 / 13.2, 2 x 19 of four rows behind 231, 34 MB, 13.4 / 9.1, 2 x 2 behind
     // 2877, 24 MB, 15.3 / 13.3; 2 x 27 behind 884 and 1011 of their own, 188 MB, 47 / 51), and short ones are in the
     // L2 for all that have a CU each

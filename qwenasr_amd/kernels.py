@@ -234,7 +234,7 @@ def attention_kvp(out, q, k_pages, v_pages, n_pages, table, table_ld, pos, n_row
     """softmax(scale q k) v over bf16 pages: row i of sequence j sees the positions up to pos[j] + i.
 
     shared (int32, one a group of `group` sequences that follow one another): the
-    first positions that the members have in common, read once for all of them.
+    first positions that the members have in common, read for 16 rows x heads of theirs at a time.
     max_len, max_own: hints (the longest sequence, the most of it not shared)."""
     check(lib().qasr_hip_attention_kvp(_h(q), out.ptr, q.ptr, n_heads * head_dim if ldq is None else ldq, k_pages.ptr,
                                        v_pages.ptr, n_pages, table.ptr, table_ld, _p(row_start), pos.ptr, n_rows, n_seq,
