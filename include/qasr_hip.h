@@ -351,8 +351,9 @@ int qasr_hip_kvp_write(qasr_hip *h, uint16_t *k_pages, uint16_t *v_pages, int64_
  * infinities and NaN count as they do in the formula, in f32 (scores of -infinity
  * alone: NaN).  Products and sums are f32, of values times weights of at most 1 (V of
  * 1e29 and more may leave its range); rows of q enter exactly (f32: from 2^-110 on),
- * and a weight is off by f32 rounding of itself (bf16 rows: by 2^-17 of itself), down to
- * 2^-100 of its row's largest.  Results are the same bits every time.
+ * and a weight is off by f32 rounding of itself (bf16 rows, more than 32 rows x heads of
+ * a KV head a sequence: by 2^-17 of itself), down to 2^-100 of its row's largest.
+ * Results are the same bits every time.
  * max_len, max_own (0: unknown): about the longest pos + rows, and the most of it
  * behind the shared positions, by which the work is split, and a prefix read for all if
  * that saves more than it costs (max_own unknown: it is taken to); results do not depend

@@ -13,9 +13,12 @@
 // 8 consecutive dims a register, and running maximum and sum are one value a lane.
 //
 // All products take operands that lose nothing: K, V and bf16 rows of q are bf16,
-// f32 rows of q three bf16 terms; weights are three terms for f32 rows (2^-24 of
-// themselves) and two for bf16 rows (2^-17: with one term, 2^-9, the results' error was
-// 1.4 times that of their own rounding).
+// f32 rows of q three bf16 terms; weights are three terms (2^-24 of themselves), but two
+// (2^-17) in tiles of many bf16 rows: the third costs 10 to 20% there (8 x 512 rows behind
+// 3400 180 us, with three 217), and 0.2 to 2.7% of few rows (32 x 4000 73.6 / 73.9, 8
+// hypotheses 9.1 / 9.3).  With two, results come out one step off the nearest bf16 value
+// about twice as often as an f32 form's (2-norm of the difference 1.0e-4 of the results',
+// with three 4e-5); with one, 2^-9, their error was 1.4 times that of their own rounding.
 //
 // Positions that a row does not see: scores become -infinity by selection, and V of
 // positions that no row of the wave sees is not read into a product.  A value that is
@@ -265,7 +268,7 @@ constexpr int kvp_part = HD + 2;                 // floats of a query's part: O,
 // which the merge is 4.7.
 template <bool BF16, int HD, int W, bool ONCE, bool AHEAD>
 __global__ __launch_bounds__(64 * W, 2) void k_attn_kvp(AttnKvpArgs a) {
-    constexpr int KC = HD / 32, VT = HD / 16, QT = BF16 ? 1 : 3, PT = BF16 ? 2 : 3, R = 16, STEP = 32 * W;
+    constexpr int KC = HD / 32, VT = HD / 16, QT = BF16 ? 1 : 3, PT = 3, R = 16, STEP = 32 * W;
     __shared__ float o_l[W][R][HD + 4];
     __shared__ float ml_l[W][2][R];
     __shared__ bf16x8 q_l[QT][KC][64];

@@ -78,6 +78,35 @@ def tolerance_w(want, is_bf16):
     return (8 * U if not is_bf16 else 2.0 ** -17 + 8 * U) + (2.0 ** -8 if is_bf16 else 4 * U) * np.abs(want)
 
 
+# ---- weights of bf16 rows: 1, e^x, e^y, and values whose sum with them is next to nothing, as the result is rounded to bf16
+
+def rows_v(r, n, dim):
+    """x, y [n] and values [n][3][dim] of at most 1 in size: the best of 512 pairs for each dim, the third the bf16 value that
+    comes nearest to taking the sum away."""
+    x, y = (bf16f(bf16(-r.uniform(0.05, 0.69, n))).astype(np.float64) for _ in range(2))
+    v = np.empty((n, 3, dim))
+    for i in range(n):
+        a, b = (bf16f(bf16(s * r.uniform(0.5, 1.0, (512, dim)))).astype(np.float64) for s in (1, -1))
+        c = bf16f(bf16(-(a + b * np.exp(x[i])) / np.exp(y[i]))).astype(np.float64)
+        left = np.where(np.abs(c) <= 1, np.abs(a + b * np.exp(x[i]) + c * np.exp(y[i])), np.inf)
+        best = left.argmin(0), np.arange(dim)
+        v[i] = a[best], b[best], c[best]
+    return x, y, v
+
+
+def out_v(x, y, v, terms=None):
+    w = np.stack([np.ones(len(x)), np.exp(x), np.exp(y)], 1)
+    p = w if terms is None else split(w.astype(np.float32), terms)
+    return (p[:, None] @ v)[:, 0] / w.sum(1)[:, None]
+
+
+def tolerance_v(want):
+    """Scores as above: 6 U of a weight, of values of at most 1 the same of the result.  Sums of at most 3, the last one's
+    three additions and the one to the lower terms' of U x 3 each, over weights of 2 and more together (1 + 2 x 0.5): 6 U.
+    Quotient, product and result relative to what is left."""
+    return 12 * U + (2.0 ** -8 + 4 * U) * np.abs(want)
+
+
 # ---------------------------------------------------------------------------
 # the tolerances themselves
 # ---------------------------------------------------------------------------
@@ -95,6 +124,10 @@ def test_the_tolerances_tell_a_term():
     x = rows_w(r, (2000, 1), True, 0)[:, 0]
     off = lambda n: np.abs(bf16f(bf16(out_w(x, n))) - out_w(x)) > tolerance_w(out_w(x), True)  # noqa: E731
     assert not off(2).any() and off(1).mean() > 0.1
+    x, y, v = rows_v(r, 100, 64)
+    want = out_v(x, y, v)
+    off = lambda n: np.abs(bf16f(bf16(out_v(x, y, v, n))) - want) > tolerance_v(want)  # noqa: E731
+    assert np.abs(want).max() < 2.0 ** -12 and not off(3).any() and off(2).mean() > 0.1
 
 
 # ---------------------------------------------------------------------------
@@ -161,3 +194,26 @@ def test_every_bit_of_small_and_large_q(dev, n_seq, heads, g, dim, power):
     q = rows_q(r, (n_seq, heads * g, dim), (2, 9))
     got = attention(dev, c, q * 2.0 ** power, [1] * n_seq, [len(KEYS) - 1] * n_seq, g, scale=SCALE_Q)
     assert (np.abs(got - out_q(q[..., 2] - q[..., 9], v)) <= tolerance_q(v)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hints", [dict(max_len=48), dict(max_len=3000), {}])
+@pytest.mark.parametrize("n_seq,dim", [(60, 64), (24, 128)])
+def test_every_bit_of_a_weight_of_few_bf16_rows(dev, n_seq, dim, hints):
+    """Of up to 32 rows x heads; 2^-17 of a weight would show."""
+    from test_gpu_hypotheses import Cache, attention
+    r, heads = rng(64 + dim), 8
+    x, y, v = rows_v(r, n_seq * heads, dim)
+    c = Cache(dev, rng(1), [3] * n_seq, 16, heads, dim, fill=False, width=200)
+    k, val = np.zeros((n_seq, heads, 16, dim)), np.zeros((n_seq, heads, 16, dim))
+    k[:, :, 1, 5] = k[:, :, 2, 6] = 1.0
+    val[:, :, :3] = v.reshape(n_seq, heads, 3, dim)
+    for j in range(n_seq):
+        c.bits["k"][c.table[j, 0]], c.bits["v"][c.table[j, 0]] = bf16(k[j]), bf16(val[j])
+    c.upload()
+    q = np.zeros((n_seq, heads, dim))
+    q[..., 5], q[..., 6] = x.reshape(n_seq, heads), y.reshape(n_seq, heads)
+    got = attention(dev, c, q, [1] * n_seq, [2] * n_seq, 1, is_bf16=True, scale=1.0, **hints).reshape(-1, dim)
+    want = out_v(x, y, v)
+    off = np.abs(got - want)
+    assert (off <= tolerance_v(want)).all(), np.max(off / tolerance_v(want))
