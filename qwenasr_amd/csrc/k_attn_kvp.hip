@@ -17,8 +17,8 @@
 // (2^-17) in tiles of many bf16 rows: the third costs 10 to 20% there (8 x 512 rows behind
 // 3400 180 us, with three 217), and 0.2 to 2.7% of few rows (32 x 4000 73.6 / 73.9, 8
 // hypotheses 9.1 / 9.3).  With two, results come out one step off the nearest bf16 value
-// about twice as often as an f32 form's (2-norm of the difference 1.0e-4 of the results',
-// with three 4e-5); with one, 2^-9, their error was 1.4 times that of their own rounding.
+// more often (2-norm of the difference 1.0e-4 of the results', with three 4e-5, of an f32
+// form 5e-5); with one, 2^-9, their error was 1.4 times that of their own rounding.
 //
 // Positions that a row does not see: scores become -infinity by selection, and V of
 // positions that no row of the wave sees is not read into a product.  A value that is
@@ -263,8 +263,8 @@ constexpr int kvp_part = HD + 2;                 // floats of a query's part: O,
 // Blocks: h fastest, then the tile of rows, the split, the group or sequence; the
 // prefixes' first.  What bounds short ones is the chain rows -> table -> K -> products ->
 // merge, so each load goes out as soon as its address is known: 8 hypotheses of 410 to 435
-// positions 9.6 us (the first form 15.3).  Long ones are bound by memory: 32 sequences of up to 4000
-// 74 us, 5.6 TB/s (four waves a block 81); four groups of 16 behind 4000 33.9 us (63), of
+// positions 9.7 us (the first form 15.3).  Long ones are bound by memory: 32 sequences of up to 4000
+// 74 us, 5.6 TB/s (four waves a block 81); four groups of 16 behind 4000 34.1 us (63), of
 // which the merge is 4.7.
 template <bool BF16, int HD, int W, bool ONCE, bool AHEAD>
 __global__ __launch_bounds__(64 * W, 2) void k_attn_kvp(AttnKvpArgs a) {
@@ -956,7 +956,7 @@ static hipError_t go_few(AttnKvpArgs &a, int64_t room, hipStream_t st) {
         if (a.max_len > 512) kvp_split(own, a.max_len, room, 256, 256, 1, a.so, a.co);
         // Eight waves a block where every block has a CU of its own, or long to go; else four, and two of short contexts, as
         // waves and the LDS of their parts are what blocks wait for.  us, eight / four / two, 8 KV heads x 2 heads of 128, bf16,
-        // sequences of half to all of the positions named:
+        // sequences of half to all of the positions named (with weights of two terms; three add at most 0.4 us):
         // 48 sequences of 60 positions 10.3 / 6.8 / -, 250 of 120 46.2 / 25.1 / 24.1, of 500 77 / 67 / 72, 1000 of 32 141 / 53 /
         // 37, of 250 199 / 141 / 131, 128 of 4000 252 / 266 / 252.  (One wave: 1000 of 32 bf16 37.0, f32 48.5 against 48.0; 250 of
         // 1000 f32 150 / 144 with two / 132 with four.)
